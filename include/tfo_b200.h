@@ -283,6 +283,68 @@ TFO_API int tfo_gated_mlp_quantize(const void* x, const void* w_gate, const void
                                    float* scale_out, int code_dtype, void* workspace, size_t workspace_bytes,
                                    void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The query/key path: rotary tables, rotation of query and key heads, and the
+ * per-head RMSNorm with the rotation. No counterpart in the reference (its
+ * RoPE is the half layout over a whole hidden row, inside fused_rmsnorm_rope).
+ * ------------------------------------------------------------------------- */
+
+/* dtype of a positions array */
+#define TFO_POS_NONE 0 /* no array: the token's index in its sequence */
+#define TFO_POS_I32 1
+#define TFO_POS_I64 2
+
+/* cos and sin rows [n, 2 * half] of rotary positions:
+ *   cos[p, i] = cos[p, half + i] = gain * cos(2 pi * position[p] * turns[i])
+ * positions: n integers on the device, or NULL with TFO_POS_NONE (0 .. n - 1).
+ * turns: `half` (<= 256) doubles in HOST memory, read before the call returns.
+ * Angles are formed and reduced in fp64. */
+TFO_API int tfo_rope_tables(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half,
+                            double gain, void* cos, void* sin, int out_dtype, void* stream);
+
+/* Rotates query and key heads x [batch, seq, heads, head_dim] (innermost
+ * stride 1; q_strides / k_strides: element strides of batch, seq and heads, in
+ * host memory) into contiguous q_out / k_out, in fp32 with one rounding:
+ *   (y1, y2) = (x1 c - x2 s, x1 s + x2 c)
+ * for the pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0,
+ * c, s = cos/sin[position * table_stride + i], i < rotary_dim / 2; the columns
+ * from rotary_dim on are copied. inverse != 0 rotates by -s (the gradient).
+ * positions: TFO_POS_NONE (token index), or integers at [b * pos_stride_batch +
+ * s * pos_stride_seq]. A position outside 0 .. table_rows - 1 reads no table
+ * row: the token's rotated columns become NaN and the device error word gets
+ * bit 6 (tfo_device_error_flags). k_heads may be 0 (k, k_out NULL). */
+TFO_API int tfo_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* cos,
+                     const void* sin, int64_t table_stride, int64_t table_rows, const void* positions, int pos_dtype,
+                     int64_t pos_stride_batch, int64_t pos_stride_seq, void* q_out, void* k_out, int64_t batch,
+                     int64_t seq, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim,
+                     int interleaved, int inverse, int dtype, int table_dtype, void* stream);
+
+/* tfo_rope of x / sqrt(mean(x^2) + eps) * weight, the mean over each head's
+ * head_dim columns; weights [head_dim] or NULL (ones). */
+TFO_API int tfo_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                             const void* q_weight, const void* k_weight, const void* cos, const void* sin,
+                             int64_t table_stride, int64_t table_rows, const void* positions, int pos_dtype,
+                             int64_t pos_stride_batch, int64_t pos_stride_seq, void* q_out, void* k_out, int64_t batch,
+                             int64_t seq, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim,
+                             int interleaved, double eps, int dtype, int q_w_dtype, int k_w_dtype, int table_dtype,
+                             void* stream);
+
+/* Gradients of tfo_qk_norm_rope: dq / dk contiguous, dq_weight / dk_weight
+ * [head_dim] in the weight's dtype (NULL: not wanted; then the workspace may be
+ * NULL too when neither is). dq_out / dk_out: the outputs' gradients, strided
+ * like q and k. Sums are fp32 in a fixed order (no atomics). */
+TFO_API size_t tfo_qk_norm_rope_backward_workspace_bytes(int64_t head_dim);
+TFO_API int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides, const void* dk_out,
+                                      const int64_t* dk_out_strides, const void* q, const int64_t* q_strides,
+                                      const void* k, const int64_t* k_strides, const void* q_weight,
+                                      const void* k_weight, const void* cos, const void* sin, int64_t table_stride,
+                                      int64_t table_rows, const void* positions, int pos_dtype,
+                                      int64_t pos_stride_batch, int64_t pos_stride_seq, void* dq, void* dk,
+                                      void* dq_weight, void* dk_weight, int64_t batch, int64_t seq, int64_t q_heads,
+                                      int64_t k_heads, int64_t head_dim, int64_t rotary_dim, int interleaved,
+                                      double eps, int dtype, int q_w_dtype, int k_w_dtype, int table_dtype,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

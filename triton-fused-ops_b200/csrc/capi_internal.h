@@ -214,4 +214,60 @@ cudaError_t gated_mlp_launch(const GatedMlpArgs& g, cudaStream_t st);
 bool gated_mlp_tensor_path(const GatedMlpArgs& g);
 // Upper bound on the CTAs of the tcgen05 kernel (amax partials: 4 per CTA).
 int gated_mlp_max_ctas();
+
+// Rotary tables (rope_tables.cu): cos/sin [n, 2 * half] of gain * (cos, sin)(2 pi * position * turns[i]).
+constexpr int kMaxRopeHalf = 256;
+enum PosDType : int { POS_NONE = 0, POS_I32 = 1, POS_I64 = 2 };
+struct RopeTablesArgs {
+  const void* positions;  // n integers, or NULL: 0, 1, ..., n - 1
+  int pos_dtype;
+  int64_t n;
+  const double* turns;  // host, `half` values: turns per position of each pair
+  int half;
+  double gain;
+  void* cos;
+  void* sin;
+  int out_dtype;
+};
+cudaError_t rope_tables_launch(const RopeTablesArgs& a, cudaStream_t st);
+
+// Rotation of query and key heads, alone or after an RMSNorm of each head
+// (qk_rope.cu), and the gradients (qk_rope_backward.cu; the rotation's own
+// gradient is the rotation with `inverse`).
+struct HeadTables {
+  const void* cos;
+  const void* sin;
+  int64_t row_stride;  // elements between table rows
+  int64_t rows;        // positions 0 .. rows - 1
+  int dtype;
+  const void* positions;  // per token, or NULL: the token's index in its sequence
+  int pos_dtype;
+  int64_t pos_stride_batch, pos_stride_seq;
+};
+struct HeadSide {  // the queries or the keys
+  const void* x;   // [batch, seq, heads, head_dim]
+  int64_t stride_batch, stride_seq, stride_head;
+  void* out;       // contiguous
+  const void* weight;  // [head_dim], or NULL: ones
+  int w_dtype;
+  int heads;
+  // backward only: dy with strides, out receives dx, dweight the weight's gradient (or NULL)
+  const void* dy;
+  int64_t dy_stride_batch, dy_stride_seq, dy_stride_head;
+  void* dweight;
+};
+struct HeadArgs {
+  HeadSide q, k;
+  HeadTables t;
+  int64_t batch, seq;
+  int head_dim, rotary_dim;
+  bool pairs, inverse, norm;
+  float eps;
+  int dtype;
+};
+cudaError_t qk_rope_launch(const HeadArgs& a, cudaStream_t st);
+size_t qk_norm_rope_backward_workspace_bytes(int head_dim);
+cudaError_t qk_norm_rope_backward_launch(const HeadArgs& a, void* ws, cudaStream_t st);
+// Elements per vector with which the vector kernels can take these heads (0: they cannot).
+int head_vector_elems(const HeadArgs& a, bool backward);
 }  // namespace tfo

@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <array>
 #include <mutex>
 #include <stdexcept>
 #include <string>
@@ -153,11 +154,250 @@ py::object linear_prepared(const at::Tensor& x, const at::Tensor& w_s8, const at
   return py::cast(out);
 }
 
+// ---------------------------------------------------------------------------
+// The query/key path: rotary tables, rotation of heads, per-head norm with the
+// rotation, with their gradients as autograd nodes (the Python wrappers carry
+// the same for inputs outside the common case).
+// ---------------------------------------------------------------------------
+using OptTensor = c10::optional<at::Tensor>;
+using Strides3 = std::array<int64_t, 3>;
+
+int pos_code(at::ScalarType t) {
+  return t == at::kInt ? TFO_POS_I32 : t == at::kLong ? TFO_POS_I64 : -1;
+}
+
+// (batch, seq, head) strides of [batch, seq, heads, dim] or [tokens, heads, dim].
+Strides3 strides_of(const at::Tensor& t) {
+  if (t.dim() == 4) return {t.stride(0), t.stride(1), t.stride(2)};
+  return {0, t.stride(0), t.stride(1)};
+}
+
+bool heads_ok(const at::Tensor& t) {
+  return t.is_cuda() && is_float(t.scalar_type()) && (t.dim() == 3 || t.dim() == 4) && t.numel() > 0 &&
+         t.stride(-1) == 1;
+}
+
+bool weight_ok(const OptTensor& w, const at::Tensor& q) {
+  return !w.has_value() || (w->device() == q.device() && is_float(w->scalar_type()) && w->dim() == 1 &&
+                            w->size(0) == q.size(-1) && w->is_contiguous());
+}
+
+// Everything the shared arguments of the head functions must satisfy here.
+bool heads_common(const at::Tensor& q, const OptTensor& k, const at::Tensor& cos, const at::Tensor& sin,
+                  const OptTensor& positions) {
+  if (!heads_ok(q)) return false;
+  if (k.has_value()) {
+    if (!heads_ok(*k) || k->device() != q.device() || k->scalar_type() != q.scalar_type() || k->dim() != q.dim() ||
+        k->size(-1) != q.size(-1))
+      return false;
+    for (int64_t i = 0; i < q.dim() - 2; ++i)
+      if (k->size(i) != q.size(i)) return false;
+  }
+  if (cos.device() != q.device() || sin.device() != q.device() || cos.dim() != 2 || sin.dim() != 2 ||
+      !is_float(cos.scalar_type()) || sin.scalar_type() != cos.scalar_type() || cos.sizes() != sin.sizes() ||
+      cos.strides() != sin.strides() || cos.stride(1) != 1 || cos.requires_grad() || sin.requires_grad())
+    return false;
+  const int64_t dim = q.size(-1), rot = cos.size(1);
+  if (dim < 2 || dim > 1024 || rot < 2 || rot % 2 != 0 || rot > dim || cos.size(0) == 0) return false;
+  if (!positions.has_value()) return cos.size(0) >= q.size(-3);
+  if (positions->device() != q.device() || pos_code(positions->scalar_type()) < 0 || positions->dim() != q.dim() - 2)
+    return false;
+  for (int64_t i = 0; i < q.dim() - 2; ++i)
+    if (positions->size(i) != q.size(i)) return false;
+  return true;
+}
+
+struct HeadsCall {  // the C ABI's shared arguments
+  const at::Tensor* positions;
+  int pos_dtype = TFO_POS_NONE;
+  int64_t pos_sb = 0, pos_ss = 0, batch, seq, q_heads, k_heads, dim, rot;
+  HeadsCall(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos, const at::Tensor& pos) : positions(&pos) {
+    if (pos.defined()) {
+      pos_dtype = pos_code(pos.scalar_type());
+      pos_sb = q.dim() == 4 ? pos.stride(0) : 0;
+      pos_ss = pos.stride(-1);
+    }
+    batch = q.dim() == 4 ? q.size(0) : 1;
+    seq = q.size(-3);
+    q_heads = q.size(-2);
+    k_heads = k.defined() ? k.size(-2) : 0;
+    dim = q.size(-1);
+    rot = cos.size(1);
+  }
+  const void* pos_ptr() const { return positions->defined() ? positions->data_ptr() : nullptr; }
+};
+
+const void* ptr_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* out_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+at::Tensor empty_heads(const at::Tensor& t) {
+  return t.defined() ? at::empty(t.sizes(), t.options().requires_grad(false)) : at::Tensor();
+}
+at::Tensor dense_heads(const at::Tensor& t) {
+  return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+int weight_code(const at::Tensor& w) { return w.defined() ? dtype_code(w.scalar_type()) : TFO_DTYPE_F32; }
+
+std::array<at::Tensor, 2> rope_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos,
+                                    const at::Tensor& sin, const at::Tensor& positions, bool interleaved, bool inverse) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  const HeadsCall h(q, k, cos, positions);
+  std::array<at::Tensor, 2> out{empty_heads(q), empty_heads(k)};
+  const Strides3 qs = strides_of(q), ks = k.defined() ? strides_of(k) : Strides3{};
+  check(tfo_rope(q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(), cos.data_ptr(), sin.data_ptr(), cos.stride(0),
+                 cos.size(0), h.pos_ptr(), h.pos_dtype, h.pos_sb, h.pos_ss, out[0].data_ptr(), out_or_null(out[1]),
+                 h.batch, h.seq, h.q_heads, h.k_heads, h.dim, h.rot, interleaved, inverse,
+                 dtype_code(q.scalar_type()), dtype_code(cos.scalar_type()),
+                 at::cuda::getCurrentCUDAStream(q.device().index()).stream()),
+        "tfo_rope");
+  return out;
+}
+
+std::array<at::Tensor, 2> qk_norm_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw,
+                                       const at::Tensor& kw, const at::Tensor& cos, const at::Tensor& sin,
+                                       const at::Tensor& positions, double eps, bool interleaved) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  const HeadsCall h(q, k, cos, positions);
+  std::array<at::Tensor, 2> out{empty_heads(q), empty_heads(k)};
+  const Strides3 qs = strides_of(q), ks = k.defined() ? strides_of(k) : Strides3{};
+  check(tfo_qk_norm_rope(q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(), ptr_or_null(qw), ptr_or_null(kw),
+                         cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.size(0), h.pos_ptr(), h.pos_dtype, h.pos_sb,
+                         h.pos_ss, out[0].data_ptr(), out_or_null(out[1]), h.batch, h.seq, h.q_heads, h.k_heads, h.dim,
+                         h.rot, interleaved, eps, dtype_code(q.scalar_type()), weight_code(qw), weight_code(kw),
+                         dtype_code(cos.scalar_type()), at::cuda::getCurrentCUDAStream(q.device().index()).stream()),
+        "tfo_qk_norm_rope");
+  return out;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+variable_list outputs_of(const std::array<at::Tensor, 2>& out) {
+  return out[1].defined() ? variable_list{out[0], out[1]} : variable_list{out[0]};
+}
+
+// The gradient of a rotation is the rotation by the opposite angle, itself differentiable.
+struct RopeNode : public torch::autograd::Function<RopeNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k, const at::Tensor& cos,
+                               const at::Tensor& sin, const OptTensor& positions, bool interleaved, bool inverse) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor pos = positions.value_or(at::Tensor()), kt = k.value_or(at::Tensor());
+    ctx->save_for_backward({cos, sin, pos});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    return outputs_of(rope_call(q, kt, cos, sin, pos, interleaved, inverse));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor dq = dense_heads(grads[0]);
+    OptTensor dk, pos;
+    if (grads.size() > 1) dk = dense_heads(grads[1]);
+    if (saved[2].defined()) pos = saved[2];
+    const variable_list d = RopeNode::apply(dq, dk, saved[0], saved[1], pos, ctx->saved_data["interleaved"].toBool(),
+                                            !ctx->saved_data["inverse"].toBool());
+    return {d[0], d.size() > 1 ? d[1] : at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor()};
+  }
+};
+
+struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k, const OptTensor& qw,
+                               const OptTensor& kw, const at::Tensor& cos, const at::Tensor& sin,
+                               const OptTensor& positions, double eps, bool interleaved) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor kt = k.value_or(at::Tensor()), qwt = qw.value_or(at::Tensor()), kwt = kw.value_or(at::Tensor()),
+                     pos = positions.value_or(at::Tensor());
+    ctx->save_for_backward({q, kt, qwt, kwt, cos, sin, pos});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["dqw"] = qwt.defined() && qwt.requires_grad();
+    ctx->saved_data["dkw"] = kwt.defined() && kwt.requires_grad();
+    return outputs_of(qk_norm_call(q, kt, qwt, kwt, cos, sin, pos, eps, interleaved));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (at::GradMode::is_enabled())
+      throw std::runtime_error("fused_qk_norm_rope is differentiable once: its gradients cannot be differentiated");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3], &cos = saved[4], &sin = saved[5];
+    const c10::cuda::CUDAGuard guard(q.device());
+    const auto st = at::cuda::getCurrentCUDAStream(q.device().index()).stream();
+    const HeadsCall h(q, k, cos, saved[6]);
+    const at::Tensor gq = dense_heads(grads[0]), gk = k.defined() ? dense_heads(grads[1]) : at::Tensor();
+    const at::Tensor dq = empty_heads(q), dk = empty_heads(k);
+    at::Tensor dqw, dkw, ws;
+    if (ctx->saved_data["dqw"].toBool()) dqw = at::empty(qw.sizes(), qw.options().requires_grad(false));
+    if (ctx->saved_data["dkw"].toBool()) dkw = at::empty(kw.sizes(), kw.options().requires_grad(false));
+    if (dqw.defined() || dkw.defined())
+      ws = workspace(tfo_qk_norm_rope_backward_workspace_bytes(h.dim), q.device(), st);
+    const Strides3 qs = strides_of(q), gqs = strides_of(gq), ks = k.defined() ? strides_of(k) : Strides3{},
+                   gks = k.defined() ? strides_of(gk) : Strides3{};
+    check(tfo_qk_norm_rope_backward(
+              gq.data_ptr(), gqs.data(), ptr_or_null(gk), gks.data(), q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(),
+              ptr_or_null(qw), ptr_or_null(kw), cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.size(0), h.pos_ptr(),
+              h.pos_dtype, h.pos_sb, h.pos_ss, dq.data_ptr(), out_or_null(dk), out_or_null(dqw), out_or_null(dkw),
+              h.batch, h.seq, h.q_heads, h.k_heads, h.dim, h.rot, ctx->saved_data["interleaved"].toBool(),
+              ctx->saved_data["eps"].toDouble(), dtype_code(q.scalar_type()), weight_code(qw), weight_code(kw),
+              dtype_code(cos.scalar_type()), out_or_null(ws), ws.defined() ? static_cast<size_t>(ws.numel()) : 0, st),
+          "tfo_qk_norm_rope_backward");
+    return {dq, dk, dqw, dkw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
+
+py::object pair_of(const variable_list& out) {
+  if (out.size() > 1) return py::make_tuple(out[0], out[1]);
+  return py::make_tuple(out[0], py::none());
+}
+
+// fused_rope: (q, k or None) rotated, or None outside the common case.
+py::object rope(const at::Tensor& q, const OptTensor& k, const at::Tensor& cos, const at::Tensor& sin,
+                const OptTensor& positions, bool interleaved) {
+  if (!heads_common(q, k, cos, sin, positions)) return py::none();
+  if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k)))
+    return pair_of(RopeNode::apply(q, k, cos, sin, positions, interleaved, false));
+  return pair_of(outputs_of(rope_call(q, k.value_or(at::Tensor()), cos, sin, positions.value_or(at::Tensor()),
+                                      interleaved, false)));
+}
+
+// fused_qk_norm_rope: (q, k or None) normed and rotated, or None outside the common case.
+py::object qk_norm_rope(const at::Tensor& q, const OptTensor& k, const OptTensor& qw, const OptTensor& kw,
+                        const at::Tensor& cos, const at::Tensor& sin, const OptTensor& positions, double eps,
+                        bool interleaved) {
+  if (!heads_common(q, k, cos, sin, positions) || !weight_ok(qw, q) || (k.has_value() ? !weight_ok(kw, q) : kw.has_value()))
+    return py::none();
+  if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k) || wants_grad(qw) || wants_grad(kw)))
+    return pair_of(QKNormRopeNode::apply(q, k, qw, kw, cos, sin, positions, eps, interleaved));
+  return pair_of(outputs_of(qk_norm_call(q, k.value_or(at::Tensor()), qw.value_or(at::Tensor()),
+                                         kw.value_or(at::Tensor()), cos, sin, positions.value_or(at::Tensor()), eps,
+                                         interleaved)));
+}
+
+// rope_tables of given positions: (cos, sin), or None outside the common case.
+py::object rope_tables(const at::Tensor& positions, const at::Tensor& turns, double gain, int64_t out_code) {
+  if (!positions.is_cuda() || !positions.is_contiguous() || pos_code(positions.scalar_type()) < 0) return py::none();
+  const c10::cuda::CUDAGuard guard(positions.device());
+  const int64_t half = turns.numel();
+  std::vector<int64_t> shape(positions.sizes().begin(), positions.sizes().end());
+  shape.push_back(2 * half);
+  const auto type = out_code == TFO_DTYPE_F16 ? at::kHalf : out_code == TFO_DTYPE_BF16 ? at::kBFloat16 : at::kFloat;
+  at::Tensor cos = at::empty(shape, positions.options().dtype(type));
+  at::Tensor sin = at::empty(shape, positions.options().dtype(type));
+  check(tfo_rope_tables(positions.data_ptr(), pos_code(positions.scalar_type()), positions.numel(),
+                        turns.data_ptr<double>(), half, gain, cos.data_ptr(), sin.data_ptr(),
+                        static_cast<int>(out_code),
+                        at::cuda::getCurrentCUDAStream(positions.device().index()).stream()),
+        "tfo_rope_tables");
+  return py::make_tuple(cos, sin);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tfo_ext, m) {
   m.doc() = "PyTorch entry points over the tfo_b200 C ABI for launch-latency-bound calls";
   m.def("quantize_dynamic", &quantize_dynamic, "dynamic-scale quantize (codes, scale) or None");
   m.def("linear_prepared", &linear_prepared, "FP8Linear forward with a prepared weight, or None");
+  m.def("rope", &rope, "fused_rope, or None");
+  m.def("qk_norm_rope", &qk_norm_rope, "fused_qk_norm_rope, or None");
+  m.def("rope_tables", &rope_tables, "rope_tables of given positions, or None");
   m.def("clear_workspaces", &clear_workspaces, "releases the cached scratch buffers");
 }

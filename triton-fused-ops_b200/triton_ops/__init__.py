@@ -5,6 +5,8 @@ Ops (each one launches hand-written sm_100a CUDA kernels through the C ABI in
 
 * ``fused_rmsnorm_rope`` / ``FusedRMSNormRoPE``
 * ``fused_gated_mlp`` / ``FusedGatedMLP``
+* ``rope_tables`` / ``RoPEScaling``, ``fused_rope``
+* ``fused_qk_norm_rope`` / ``FusedQKNormRoPE``
 * ``fp8_gemm`` / ``FP8Linear``
 * ``quantize_fp8`` / ``dequantize_fp8``
 
@@ -40,7 +42,9 @@ from triton_ops.exceptions import (
 from triton_ops.kernels.fp8_gemm import FP8Linear, fp8_gemm
 from triton_ops.kernels.fp8_quantize import dequantize_fp8, quantize_fp8, quantize_fp8_per_token
 from triton_ops.kernels.gated_mlp import FusedGatedMLP, fused_gated_mlp, fused_gated_mlp_quantize
+from triton_ops.kernels.qk_norm_rope import FusedQKNormRoPE, fused_qk_norm_rope
 from triton_ops.kernels.rmsnorm_rope import FusedRMSNormRoPE, fused_rmsnorm_rope, fused_rmsnorm_rope_quantize
+from triton_ops.kernels.rope import RoPEScaling, fused_rope, rope_tables
 from triton_ops.models import (
     FP8Format,
     FP8GEMMInput,
@@ -55,6 +59,11 @@ __all__ = [
     "fused_rmsnorm_rope",
     "fused_rmsnorm_rope_quantize",
     "FusedRMSNormRoPE",
+    "rope_tables",
+    "RoPEScaling",
+    "fused_rope",
+    "fused_qk_norm_rope",
+    "FusedQKNormRoPE",
     "fused_gated_mlp",
     "fused_gated_mlp_quantize",
     "FusedGatedMLP",

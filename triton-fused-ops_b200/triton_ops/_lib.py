@@ -13,6 +13,7 @@ import ctypes
 import os
 import threading
 from collections import OrderedDict
+from contextlib import nullcontext
 from pathlib import Path
 
 import torch
@@ -41,10 +42,20 @@ ACT_CODE = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 # layout of fp8_gemm's B operand
 B_KN, B_NK = 0, 1
 
+# dtype codes of a positions array
+POS_NONE, POS_I32, POS_I64 = 0, 1, 2
+
+# bit of the device error word: a token's position lies outside the rotary table
+ERR_BAD_POSITION = 1 << 6
+
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
 _c_vp = ctypes.c_void_p
 _c_size = ctypes.c_size_t
+_c_strides = ctypes.POINTER(ctypes.c_int64)
+# the arguments that the query/key entry points share
+_HEADS_TABLE = [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_int, _c_i64, _c_i64]
+_HEADS_SIZES = [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int]
 
 # name -> (restype, argtypes)
 _SIGNATURES = {
@@ -102,6 +113,26 @@ _SIGNATURES = {
         _c_int,
         [_c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp,
          _c_size, _c_vp],
+    ),
+    "tfo_rope_tables": (
+        _c_int,
+        [_c_vp, _c_int, _c_i64, ctypes.POINTER(ctypes.c_double), _c_i64, ctypes.c_double, _c_vp, _c_vp, _c_int, _c_vp],
+    ),
+    "tfo_rope": (
+        _c_int,
+        [_c_vp, _c_strides, _c_vp, _c_strides, *_HEADS_TABLE, _c_vp, _c_vp, *_HEADS_SIZES, _c_int, _c_int, _c_int, _c_vp],
+    ),
+    "tfo_qk_norm_rope": (
+        _c_int,
+        [_c_vp, _c_strides, _c_vp, _c_strides, _c_vp, _c_vp, *_HEADS_TABLE, _c_vp, _c_vp, *_HEADS_SIZES,
+         ctypes.c_double, _c_int, _c_int, _c_int, _c_int, _c_vp],
+    ),
+    "tfo_qk_norm_rope_backward_workspace_bytes": (_c_size, [_c_i64]),
+    "tfo_qk_norm_rope_backward": (
+        _c_int,
+        [_c_vp, _c_strides, _c_vp, _c_strides, _c_vp, _c_strides, _c_vp, _c_strides, _c_vp, _c_vp, *_HEADS_TABLE,
+         _c_vp, _c_vp, _c_vp, _c_vp, *_HEADS_SIZES, ctypes.c_double, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_size,
+         _c_vp],
     ),
     "tfo_gated_mlp_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_int, _c_int]),
     "tfo_gated_mlp": (
@@ -211,6 +242,16 @@ def stream_of(t: torch.Tensor) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def on_device(t: torch.Tensor):
+    """Context in which t's device is the current one (kernels launch on the current device)."""
+    if t.get_device() == torch.cuda.current_device():
+        return _NO_SWITCH
+    return torch.cuda.device(t.device)
+
+
+_NO_SWITCH = nullcontext()
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

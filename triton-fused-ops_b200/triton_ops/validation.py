@@ -254,3 +254,114 @@ def validate_fp8_quantize_inputs(tensor: torch.Tensor, scale: Optional[torch.Ten
     _check_contiguous(tensor, "tensor")
     if scale is not None:
         _check_cuda(scale, "scale")
+
+
+def check_rope_table(ref: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Checks cos/sin ([rows, rotary_dim] or [1, rows, 1, rotary_dim]) and returns them as 2-D rows of stride 1."""
+    for t, n in ((cos, "cos"), (sin, "sin")):
+        _check_cuda(t, n)
+        _check_dtype(t, n, SUPPORTED_DTYPES_FLOAT)
+        _check_same_device(ref, t, n)
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{n} must not require a gradient: the rotary tables have none")
+    if cos.dim() == 4 and cos.shape[0] == 1 and cos.shape[2] == 1:
+        cos = cos[0, :, 0]
+    elif cos.dim() != 2:
+        raise ShapeMismatchError(
+            f"cos must be [rows, rotary_dim] or [1, rows, 1, rotary_dim], got {tuple(cos.shape)}",
+            actual=cos.shape, tensor_name="cos",
+        )
+    if sin.dim() == 4 and sin.shape[0] == 1 and sin.shape[2] == 1:
+        sin = sin[0, :, 0]
+    if sin.shape != cos.shape:
+        raise ShapeMismatchError(
+            f"sin shape {tuple(sin.shape)} doesn't match cos shape {tuple(cos.shape)}",
+            expected=cos.shape, actual=sin.shape, tensor_name="sin",
+        )
+    if sin.dtype != cos.dtype:
+        cos, sin = cos.float(), sin.float()
+    if cos.stride(1) != 1 or sin.stride() != cos.stride():
+        cos, sin = cos.contiguous(), sin.contiguous()
+    return cos, sin
+
+
+def _check_heads(t: torch.Tensor, name: str) -> None:
+    _check_cuda(t, name)
+    _check_dtype(t, name, SUPPORTED_DTYPES_FLOAT)
+    if t.dim() not in (3, 4):
+        raise ShapeMismatchError(
+            f"{name} must be [batch, seq_len, heads, head_dim] or [tokens, heads, head_dim], got {t.dim()}D",
+            actual=t.shape, tensor_name=name,
+        )
+    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have contiguous heads (innermost stride 1), got strides {t.stride()}")
+
+
+def validate_rope_heads(
+    q: torch.Tensor,
+    k: Optional[torch.Tensor],
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: Optional[torch.Tensor],
+) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """Checks query/key heads with their rotary tables and positions.
+
+    Returns (cos, sin, positions) with 2-D tables of stride 1 and positions
+    (int32 or int64, or None) expanded to q's token dimensions.
+    """
+    _check_heads(q, "q")
+    if k is not None:
+        _check_heads(k, "k")
+        _check_same_device(q, k, "k")
+        if k.dtype != q.dtype:
+            raise UnsupportedDtypeError(f"k has dtype {k.dtype} but q has {q.dtype}", dtype=k.dtype,
+                                        supported_dtypes=[q.dtype], tensor_name="k")
+        if k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+            raise ShapeMismatchError(
+                f"k shape {tuple(k.shape)} doesn't match q shape {tuple(q.shape)} (all but the heads must agree)",
+                expected=q.shape, actual=k.shape, tensor_name="k",
+            )
+    cos, sin = check_rope_table(q, cos, sin)
+    head_dim, rotary_dim = q.shape[-1], cos.shape[1]
+    if head_dim < 2 or head_dim > 1024:
+        raise ShapeMismatchError(f"head_dim must be in 2..1024, got {head_dim}", tensor_name="q")
+    if rotary_dim < 2 or rotary_dim % 2 != 0 or rotary_dim > head_dim:
+        raise ShapeMismatchError(
+            f"rotary_dim (the tables' width) must be even and at most head_dim {head_dim}, got {rotary_dim}",
+            tensor_name="cos",
+        )
+    if positions is None:
+        if cos.shape[0] < q.shape[-3]:
+            raise ShapeMismatchError(
+                f"the tables have {cos.shape[0]} rows for sequences of {q.shape[-3]} tokens",
+                expected=(q.shape[-3], rotary_dim), actual=cos.shape, tensor_name="cos",
+            )
+        return cos, sin, None
+    _check_cuda(positions, "positions")
+    _check_dtype(positions, "positions", [torch.int32, torch.int64])
+    _check_same_device(q, positions, "positions")
+    try:
+        positions = positions.expand(q.shape[:-2])
+    except RuntimeError:
+        raise ShapeMismatchError(
+            f"positions shape {tuple(positions.shape)} doesn't fit the tokens {tuple(q.shape[:-2])}",
+            expected=tuple(q.shape[:-2]), actual=positions.shape, tensor_name="positions",
+        ) from None
+    if cos.shape[0] == 0 and positions.numel():
+        raise ShapeMismatchError("the tables have no rows", actual=cos.shape, tensor_name="cos")
+    return cos, sin, positions
+
+
+def validate_head_weight(q: torch.Tensor, weight: Optional[torch.Tensor], name: str) -> None:
+    """Checks a per-head norm weight [head_dim] (None: ones)."""
+    if weight is None:
+        return
+    _check_cuda(weight, name)
+    _check_dtype(weight, name, SUPPORTED_DTYPES_FLOAT)
+    _check_same_device(q, weight, name)
+    if weight.shape != (q.shape[-1],):
+        raise ShapeMismatchError(
+            f"{name} shape {tuple(weight.shape)} doesn't match head_dim {q.shape[-1]}",
+            expected=(q.shape[-1],), actual=weight.shape, tensor_name=name,
+        )
+    _check_contiguous(weight, name)
