@@ -109,8 +109,16 @@ CASES = [
     (1, 3, 2, 1, 256, 256, False, "f32", "f32", None),
     (1, 3, 2, 1, 512, 512, False, "bf16", "f32", None),
     (1, 2, 1, 1, 1024, 1000, True, "f16", "f32", None),   # wider than a warp's vectors
-    (4, 700, 8, 2, 64, 64, False, "bf16", "f32", None),   # four heads per group
+    (4, 700, 8, 2, 64, 64, False, "bf16", "f32", None),
     (1, 1500, 7, 3, 32, 16, True, "f32", "f32", "given"),
+    # enough tokens for four heads per group, then for the streaming kernel
+    (1, 2500, 8, 2, 128, 128, False, "bf16", "f32", "given"),
+    (3, 901, 5, 1, 128, 64, True, "f16", "f16", "shared"),
+    (2, 3001, 8, 3, 128, 128, False, "bf16", "bf16", "given"),
+    (1, 6100, 13, 3, 80, 80, False, "f16", "f32", None),   # five lanes a head, six heads a warp
+    (1, 6100, 9, 5, 64, 24, True, "f16", "f32", "given"),
+    (2, 3500, 6, 2, 80, 40, False, "bf16", "f32", None),   # ten lanes of 8-byte vectors
+    (1, 4100, 4, 1, 256, 64, False, "f32", "f32", "given"),
 ]
 
 

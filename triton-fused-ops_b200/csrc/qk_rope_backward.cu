@@ -6,11 +6,18 @@
 //   dw = sum over tokens and heads of b * x * r
 //
 // Both means come from one read of x and dy; nothing of the forward pass is
-// stored. Bound by HBM (x and dy read, dx written). CTAs are persistent, split
-// between queries and keys by their work; a lane keeps fp32 sums of dw for its
-// columns over all its rows, a CTA joins its lanes' sums through shared memory
-// into one partial row, and a second kernel adds the partial rows in order, so
-// the result does not depend on scheduling (no atomics).
+// stored. CTAs are persistent, split between queries and keys by their work,
+// and stream both tensors through shared memory (HeadStream); a lane keeps
+// fp32 sums of dw for its columns over all its heads, a CTA joins its lanes'
+// sums through shared memory into one partial row, and a second kernel adds
+// the partial rows in order, so the result does not depend on scheduling (no
+// atomics).
+//
+// Floor: HBM (x and dy read, dx written). Measured at 32768 tokens of 32 + 8
+// heads of 128 columns, bf16: 188 us with the weights' gradients, 82 % of the
+// measured copy rate; 8192 tokens 55 us (70 %). The two sums over a head's
+// lanes and 128 registers a thread (16 warps an SM) bound it: the schedulers
+// issue in 49 % of the cycles and the rest is latency within a warp.
 #include "heads.cuh"
 
 namespace tfo {
@@ -19,111 +26,138 @@ constexpr int kBwdThreads = 256;
 constexpr int kBwdWarps = kBwdThreads / 32;
 constexpr int kBwdCtasPerSm = 4;
 
-struct SideSplit {  // CTAs [0, q_ctas) take the queries, the rest the keys
-  int q_ctas, k_ctas;
-};
-
-template <typename T, int E, bool PAIRS, int NH>
-__global__ void __launch_bounds__(kBwdThreads) qk_norm_rope_backward_kernel(const HeadArgs a, int lane_shift,
-                                                                            SideSplit split, float* __restrict__ partials,
-                                                                            uint32_t* err) {
+template <typename T, int E, bool PAIRS, int NH, int STAGES, bool FULL>
+__global__ void __launch_bounds__(kBwdThreads, 2) qk_norm_rope_backward_kernel(
+    const HeadArgs a, int lanes, SideSplit split, FastDiv by_seq, FastDiv by_q_chunks, FastDiv by_k_chunks,
+    float* __restrict__ partials, uint32_t* err) {
   using V = HeadVec<T, E>;
-  extern __shared__ float red[];  // [kBwdWarps][head_dim]
+  extern __shared__ __align__(16) uint8_t smem[];
   griddep_launch_dependents();
   griddep_wait();
   const bool is_q = blockIdx.x < static_cast<unsigned>(split.q_ctas);
   const HeadSide& side = is_q ? a.q : a.k;
   const uint32_t cta = is_q ? blockIdx.x : blockIdx.x - split.q_ctas;
-  const uint32_t ctas = is_q ? split.q_ctas : split.k_ctas;
+  const uint32_t per_warp = 32 / lanes;
+  const uint32_t groups = static_cast<uint32_t>(is_q ? split.q_ctas : split.k_ctas) * kBwdWarps * per_warp;
+  const LaneGroup group(lanes);
   const int D = a.head_dim, heads = side.heads;
-  const int lanes = 1 << lane_shift;
-  const int p = threadIdx.x & (lanes - 1);
-  const uint32_t per_cta = kBwdThreads >> lane_shift;
-  const uint32_t chunks = (heads + NH - 1) / NH;
-  const uint32_t groups = static_cast<uint32_t>(a.batch * a.seq) * chunks;
-  const LaneCols col = lane_cols<PAIRS>(p, D / E, a.rotary_dim / E);
-  const float inv_d = 1.f / static_cast<float>(D);
+  const LaneCols col = lane_cols<PAIRS>(group.p, lanes, D / E, a.rotary_dim / E);
+  const int column = max(0, col.va) * E;
 
-  float wa[E], wb[E], acc_a[E], acc_b[E];
+  HeadStream<T, E, NH, STAGES, 2, FULL> st;
+  st.in[0] = {static_cast<const T*>(side.x) + column, side.stride_batch, side.stride_seq, side.stride_head};
+  st.in[1] = {static_cast<const T*>(side.dy) + column, side.dy_stride_batch, side.dy_stride_seq, side.dy_stride_head};
+  st.vb_offset = col.vb * E - column;
+  st.has_a = col.va >= 0 && !group.spare;
+  st.has_b = col.vb >= 0 && !group.spare;
+  st.by_seq = by_seq;
+  st.by_chunks = is_q ? by_q_chunks : by_k_chunks;
+  st.seq = static_cast<uint32_t>(a.seq);
+  st.chunks = (heads + NH - 1) / NH;
+  st.units = static_cast<uint32_t>(a.batch * a.seq) * st.chunks;
+  st.heads = heads;
+  // the warp's groups walk in step: the first one's unit decides the end
+  uint32_t lead = (cta * kBwdWarps + (threadIdx.x >> 5)) * per_warp;
+  st.start(smem, lead + group.group, groups);
+
+  F2 wa[E / 2], wb[E / 2], acc_a[E / 2], acc_b[E / 2];
+  {
+    float fa[E], fb[E];
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    wa[j] = wb[j] = 1.f;
-    acc_a[j] = acc_b[j] = 0.f;
-  }
-  if (side.weight != nullptr) {
-    if (col.va >= 0) load_floats<E>(side.weight, col.va * E, side.w_dtype, wa);
-    if (col.vb >= 0) load_floats<E>(side.weight, col.vb * E, side.w_dtype, wb);
-  }
-  for (uint32_t base = cta * per_cta; base < groups; base += ctas * per_cta) {
-    const uint32_t want = base + (threadIdx.x >> lane_shift);
-    const bool live = want < groups;
-    const uint32_t gid = live ? want : groups - 1;
-    const uint32_t token = gid / chunks;
-    const int h0 = static_cast<int>(gid - token * chunks) * NH;
-    const uint32_t b = token / static_cast<uint32_t>(a.seq);
-    const uint32_t sq = token - b * static_cast<uint32_t>(a.seq);
-    const T* x = static_cast<const T*>(side.x) + b * side.stride_batch + sq * side.stride_seq;
-    const T* dy = static_cast<const T*>(side.dy) + b * side.dy_stride_batch + sq * side.dy_stride_seq;
-    typename V::Raw xa[NH], xb[NH], ga[NH], gb[NH];
-#pragma unroll
-    for (int i = 0; i < NH; ++i) {
-      const bool in = live && h0 + i < heads;
-      const T* xr = x + (h0 + i) * side.stride_head;
-      const T* gr = dy + (h0 + i) * side.dy_stride_head;
-      xa[i] = in && col.va >= 0 ? V::load(xr + col.va * E) : V::zero();
-      xb[i] = in && col.vb >= 0 ? V::load(xr + col.vb * E) : V::zero();
-      ga[i] = in && col.va >= 0 ? V::load(gr + col.va * E) : V::zero();
-      gb[i] = in && col.vb >= 0 ? V::load(gr + col.vb * E) : V::zero();
+    for (int j = 0; j < E; ++j) fa[j] = fb[j] = 1.f;
+    if (side.weight != nullptr) {
+      if (col.va >= 0) load_floats<E>(side.weight, col.va * E, side.w_dtype, fa);
+      if (col.vb >= 0) load_floats<E>(side.weight, col.vb * E, side.w_dtype, fb);
     }
-    const int64_t pos = token_position(a.t, b, sq, err, p == 0);
-    float c[E], s[E];
-    lane_table<E>(a.t, pos, p, col.rotated, true, c, s);
-    T* out = static_cast<T*>(side.out) + (static_cast<int64_t>(token) * heads + h0) * D;
+#pragma unroll
+    for (int j = 0; j < E / 2; ++j) {
+      wa[j] = f2(fa[2 * j], fa[2 * j + 1]);
+      wb[j] = f2(fb[2 * j], fb[2 * j + 1]);
+      acc_a[j] = acc_b[j] = f2(0.f, 0.f);
+    }
+  }
+  const float inv_d = 1.f / static_cast<float>(D);
+  const int most = min(NH, heads);
+  int stage = 0;
+  for (; lead < st.units; lead += groups) {
+    const uint32_t unit = min(lead + group.group, st.units - 1);
+    const uint32_t token = st.by_chunks.div(unit);
+    const int h0 = static_cast<int>(unit - token * st.chunks) * NH;
+    const int mine = lead + group.group < st.units ? heads - h0 : 0;  // heads of this unit
+    const uint32_t b = by_seq.div(token);
+    const int64_t pos = token_position(a.t, b, token - b * st.seq, err, group.p == 0);
+    PlainRotation<E, PAIRS> rot;  // the inverse rotation
+    {
+      float c[E], s[E];
+      lane_table<E, PAIRS>(a.t, pos, col, true, c, s);
+      rot.set(c, s);
+    }
+    T* out = static_cast<T*>(side.out) + (static_cast<int64_t>(token) * heads + h0) * D + column;
+    st.wait();
 #pragma unroll
     for (int i = 0; i < NH; ++i) {
-      float ua[E], ub[E], fa[E], fb[E];
-      V::unpack(xa[i], ua);
-      V::unpack(xb[i], ub);
-      V::unpack(ga[i], fa);
-      V::unpack(gb[i], fb);
-      rotate_lane<E, PAIRS>(fa, fb, c, s, col.rotated);
-      float ss = 0.f, dot = 0.f;
+      if (i >= most) break;
+      F2 ua[E / 2], ub[E / 2], fa[E / 2], fb[E / 2];
+      V::unpack(*st.slot(stage, 0, i, 0), ua);
+      V::unpack(*st.slot(stage, 0, i, 1), ub);
+      V::unpack(*st.slot(stage, 1, i, 0), fa);
+      V::unpack(*st.slot(stage, 1, i, 1), fb);
+      rot.apply(fa, fb, col);
+      F2 ss = f2(0.f, 0.f), dot = ss, ta[E / 2], tb[E / 2];
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        ss += ua[j] * ua[j] + ub[j] * ub[j];
-        dot += fa[j] * wa[j] * ua[j] + fb[j] * wb[j] * ub[j];
+      for (int j = 0; j < E / 2; ++j) {
+        ss = fma2(ub[j], ub[j], fma2(ua[j], ua[j], ss));
+        ta[j] = mul2(fa[j], ua[j]);
+        tb[j] = mul2(fb[j], ub[j]);
+        dot = fma2(tb[j], wb[j], fma2(ta[j], wa[j], dot));
       }
-      ss = group_sum(ss, lanes);
-      dot = group_sum(dot, lanes);
-      const float r = rsqrtf(ss * inv_d + a.eps);
-      const float k = dot * inv_d * r * r * r;  // in this order: r^3 alone can overflow
-      if (live && h0 + i < heads) {
+      const float r = rsqrtf(group.sum(ss.x + ss.y) * inv_d + a.eps);
+      const float k = group.sum(dot.x + dot.y) * inv_d * r * r * r;  // in this order: r^3 alone can overflow
+      if (i < mine) {
+        const F2 r2 = f2(r, r), k2 = f2(-k, -k);
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          acc_a[j] += fa[j] * (ua[j] * r);
-          acc_b[j] += fb[j] * (ub[j] * r);
-          ua[j] = r * (fa[j] * wa[j]) - ua[j] * k;
-          ub[j] = r * (fb[j] * wb[j]) - ub[j] * k;
+        for (int j = 0; j < E / 2; ++j) {
+          acc_a[j] = fma2(ta[j], r2, acc_a[j]);
+          acc_b[j] = fma2(tb[j], r2, acc_b[j]);
+          fa[j] = fma2(mul2(fa[j], wa[j]), r2, mul2(ua[j], k2));
+          fb[j] = fma2(mul2(fb[j], wb[j]), r2, mul2(ub[j], k2));
         }
-        if (col.va >= 0) V::store(out + i * D + col.va * E, ua);
-        if (col.vb >= 0) V::store(out + i * D + col.vb * E, ub);
+        if (FULL || st.has_a) V::store(out + i * D, fa);
+        if (FULL || st.has_b) V::store(out + i * D + st.vb_offset, fb);
       }
     }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    st.load();  // into the stage that the unit before this one has left
   }
   if (side.dweight == nullptr) return;
+  // the warp's groups, then the CTA's warps (the ring is done with: no load is in flight past the last unit)
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    for (int o = lanes; o < 32; o <<= 1) {
-      acc_a[j] += __shfl_xor_sync(0xffffffffu, acc_a[j], o);
-      acc_b[j] += __shfl_xor_sync(0xffffffffu, acc_b[j], o);
+  for (int j = 0; j < E / 2; ++j) {
+    const F2 own_a = acc_a[j], own_b = acc_b[j];
+    for (uint32_t g = 1; g < per_warp; ++g) {
+      const int from = min(31, lane + static_cast<int>(g) * lanes);
+      acc_a[j].x += __shfl_sync(0xffffffffu, own_a.x, from);
+      acc_a[j].y += __shfl_sync(0xffffffffu, own_a.y, from);
+      acc_b[j].x += __shfl_sync(0xffffffffu, own_b.x, from);
+      acc_b[j].y += __shfl_sync(0xffffffffu, own_b.y, from);
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);  // [warps][head_dim]
   float* mine = red + (threadIdx.x >> 5) * D;
-  if ((threadIdx.x & 31) < lanes) {
+  if (lane < lanes) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      if (col.va >= 0) mine[col.va * E + j] = acc_a[j];
-      if (col.vb >= 0) mine[col.vb * E + j] = acc_b[j];
+    for (int j = 0; j < E / 2; ++j) {
+      if (col.va >= 0) {
+        mine[col.va * E + 2 * j] = acc_a[j].x;
+        mine[col.va * E + 2 * j + 1] = acc_a[j].y;
+      }
+      if (col.vb >= 0) {
+        mine[col.vb * E + 2 * j] = acc_b[j].x;
+        mine[col.vb * E + 2 * j + 1] = acc_b[j].y;
+      }
     }
   }
   __syncthreads();
@@ -237,33 +271,41 @@ __global__ void __launch_bounds__(1024) qk_weight_grad_kernel(const HeadArgs a, 
 }
 
 namespace {
-// CTAs of each side in proportion to its heads, at most one wave and no more than `units(heads)` CTAs of work.
-template <typename F> SideSplit split_ctas(const HeadArgs& a, F units) {
-  const int64_t all = static_cast<int64_t>(num_sms()) * kBwdCtasPerSm;
-  const int heads = a.q.heads + a.k.heads;
-  auto share = [&](int h) -> int {
-    if (h == 0) return 0;
-    return static_cast<int>(std::min<int64_t>(units(h), std::max<int64_t>(1, all * h / heads)));
+// One wave of resident CTAs (at most kBwdCtasPerSm on an SM), shared between
+// the sides by their units of work, at most one CTA for `per_cta` units.
+SideSplit split_ctas(const void* kernel, size_t smem, int64_t q_units, int64_t k_units, int64_t per_cta) {
+  const int64_t all =
+      static_cast<int64_t>(num_sms()) * std::min(kBwdCtasPerSm, cached_occupancy(kernel, kBwdThreads, smem));
+  auto share = [&](int64_t u) {
+    if (u == 0) return 0;
+    const double part = static_cast<double>(u) / static_cast<double>(q_units + k_units);
+    return static_cast<int>(std::min((u + per_cta - 1) / per_cta, std::max<int64_t>(1, static_cast<int64_t>(all * part))));
   };
-  return SideSplit{share(a.q.heads), share(a.k.heads)};
-}
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch_smem(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t st, Args&&... args) {
-  return launch_gemm_grid(kernel, block, grid, 1, smem, st, std::forward<Args>(args)...);
+  return SideSplit{share(q_units), share(k_units)};
 }
 
 template <typename T, int E, bool PAIRS>
 cudaError_t launch_vec(const HeadArgs& a, SideSplit* split, float* partials, cudaStream_t st) {
-  constexpr int NH = 2;
+  // 16-byte slots: 3 heads x 2 tensors x 2 stages = 96 KB a CTA, two CTAs an SM.
+  // Measured, us at 8192 / 32768 tokens of 32 + 8 heads of 128 columns, bf16:
+  // 3 heads, 2 stages 55 / 188; 2 heads, 3 stages 59 / 215; 1 head, 5 stages
+  // 71 / 255; 4 heads, 2 stages (one CTA of 416 threads) 65 / 232.
+  constexpr int NH = 3, STAGES = 2;
   const int lanes = (a.head_dim / E + 1) / 2;
-  int shift = 0;
-  while ((1 << shift) < lanes) ++shift;
-  const int64_t per_cta = kBwdThreads >> shift;
-  *split = split_ctas(a, [&](int h) { return (a.batch * a.seq * ((h + NH - 1) / NH) + per_cta - 1) / per_cta; });
+  const bool full = a.head_dim == 2 * E * lanes && 32 % lanes == 0;
+  auto* kernel = full ? qk_norm_rope_backward_kernel<T, E, PAIRS, NH, STAGES, true>
+                      : qk_norm_rope_backward_kernel<T, E, PAIRS, NH, STAGES, false>;
+  constexpr size_t smem = HeadStream<T, E, NH, STAGES, 2, true>::kSmemBytes;
+  static_assert(smem >= sizeof(float) * kBwdWarps * 64 * E, "the weight sums fit into the ring");
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  if (const cudaError_t e = ensure_smem_attr(fn, smem); e != cudaSuccess) return e;
+  const uint32_t qc = (a.q.heads + NH - 1) / NH, kc = (a.k.heads + NH - 1) / NH;
+  const int64_t tokens = a.batch * a.seq;
+  *split = split_ctas(fn, smem, tokens * qc, tokens * kc, kBwdWarps * (32 / lanes));
   note_launch();
-  return launch_smem(qk_norm_rope_backward_kernel<T, E, PAIRS, NH>, split->q_ctas + split->k_ctas, kBwdThreads,
-                     sizeof(float) * kBwdWarps * a.head_dim, st, a, shift, *split, partials, error_word_ptr());
+  return launch_gemm_grid(kernel, kBwdThreads, split->q_ctas + split->k_ctas, 1, smem, st, a, lanes, *split,
+                          FastDiv::make(static_cast<uint32_t>(a.seq)), FastDiv::make(std::max(1u, qc)),
+                          FastDiv::make(std::max(1u, kc)), partials, error_word_ptr());
 }
 
 template <typename T>
@@ -275,10 +317,13 @@ cudaError_t launch_type(const HeadArgs& a, SideSplit* split, float* partials, cu
   if (e == E / 2)
     return a.pairs ? launch_vec<T, E / 2, true>(a, split, partials, st)
                    : launch_vec<T, E / 2, false>(a, split, partials, st);
-  *split = split_ctas(a, [&](int h) { return (a.batch * a.seq * h + kBwdWarps - 1) / kBwdWarps; });
+  auto* kernel = qk_norm_rope_backward_any_kernel<T>;
+  const size_t smem = sizeof(float) * kBwdWarps * a.head_dim;
+  const int64_t tokens = a.batch * a.seq;
+  *split = split_ctas(reinterpret_cast<const void*>(kernel), smem, tokens * a.q.heads, tokens * a.k.heads, kBwdWarps);
   note_launch();
-  return launch_smem(qk_norm_rope_backward_any_kernel<T>, split->q_ctas + split->k_ctas, kBwdThreads,
-                     sizeof(float) * kBwdWarps * a.head_dim, st, a, *split, partials, error_word_ptr());
+  return launch_gemm_grid(kernel, kBwdThreads, split->q_ctas + split->k_ctas, 1, smem, st, a, *split, partials,
+                          error_word_ptr());
 }
 }  // namespace
 

@@ -292,8 +292,11 @@ struct RopeNode : public torch::autograd::Function<RopeNode> {
     OptTensor dk, pos;
     if (grads.size() > 1) dk = dense_heads(grads[1]);
     if (saved[2].defined()) pos = saved[2];
-    const variable_list d = RopeNode::apply(dq, dk, saved[0], saved[1], pos, ctx->saved_data["interleaved"].toBool(),
-                                            !ctx->saved_data["inverse"].toBool());
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
+    const variable_list d =
+        at::GradMode::is_enabled()
+            ? RopeNode::apply(dq, dk, saved[0], saved[1], pos, interleaved, inverse)
+            : outputs_of(rope_call(dq, dk.value_or(at::Tensor()), saved[0], saved[1], saved[2], interleaved, inverse));
     return {d[0], d.size() > 1 ? d[1] : at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
             at::Tensor()};
   }
