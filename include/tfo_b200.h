@@ -345,6 +345,22 @@ TFO_API int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_
                                       double eps, int dtype, int q_w_dtype, int k_w_dtype, int table_dtype,
                                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* Low-rank adapters of many requests beside a shared projection:
+ *   out[t, :] = base[t, :] + scaling[i] * b[i] . (a[i] . x[t, :]),  i = ids[t]
+ * x [tokens, k] (rows x_stride elements apart, innermost stride 1), a
+ * [adapters, rank, k] and b [adapters, n, rank] contiguous, ids [tokens]
+ * (TFO_POS_I32 or _I64), scaling [adapters] fp32 or NULL (ones), base and out
+ * [tokens, n] with their row strides; base may be NULL (zeros) or out itself,
+ * out must overlap neither x, a nor b. ids < 0: no adapter, out = base (left
+ * untouched when base == out). An id >= adapters reads nothing: its row becomes
+ * NaN and the device error word gets bit 7. rank <= 256, adapters <= 16384.
+ * fp32 sums; one rounding of the result. No counterpart in the reference. */
+TFO_API size_t tfo_lora_workspace_bytes(int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int dtype);
+TFO_API int tfo_lora(const void* x, int64_t x_stride, const void* a, const void* b, const void* ids, int ids_dtype,
+                     const float* scaling, const void* base, int64_t base_stride, void* out, int64_t out_stride,
+                     int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int64_t n, int dtype, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -135,3 +135,44 @@ def test_entry_points_report_bad_arguments():
     assert backward(wd=3) == _lib.ERR_DTYPE
     assert lib.tfo_qk_norm_rope_backward_workspace_bytes(128) >= 4 * 128
     assert lib.tfo_qk_norm_rope_backward_workspace_bytes(0) == 0
+
+
+def test_lora_argument_checks(monkeypatch):
+    from triton_ops import fused_lora
+
+    x, a, b, ids = torch.zeros(3, 8), torch.zeros(2, 4, 8), torch.zeros(2, 6, 4), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(DeviceError):
+        fused_lora(x, a, b, ids)
+    monkeypatch.setattr(validation, "_check_cuda", lambda t, n: None)
+    check = validation.validate_lora_inputs
+    assert check(x, a, b, ids, None, None, None) == (3, 2, 4, 8, 6)
+    for args, error in (
+        ((x, a.half(), b, ids, None, None, None), UnsupportedDtypeError),
+        ((x, a, b, ids.float(), None, None, None), UnsupportedDtypeError),
+        ((x, a[:, :, :7], b, ids, None, None, None), ShapeMismatchError),
+        ((x, a, b[:1], ids, None, None, None), ShapeMismatchError),
+        ((x, a, b, ids[:2], None, None, None), ShapeMismatchError),
+        ((x, a, b, ids, torch.ones(3), None, None), ShapeMismatchError),
+        ((x, a, b, ids, None, torch.zeros(3, 5), None), ShapeMismatchError),
+        ((x, a, b, ids, None, None, torch.zeros(2, 6)), ShapeMismatchError),
+        ((x, torch.zeros(2, 257, 8), torch.zeros(2, 6, 257), ids, None, None, None), ShapeMismatchError),
+        ((x.clone().requires_grad_(), a, b, ids, None, None, None), ValueError),
+    ):
+        with pytest.raises(error):
+            check(*args)
+
+
+def test_lora_entry_point_reports_bad_arguments():
+    lib = _lib.load()
+
+    def lora(tokens=2, adapters=1, rank=4, k=8, n=8, dtype=2, ids_dtype=2, x=16, ws=None, bytes_=0):
+        return lib.tfo_lora(x, 8, 16, 16, 16, ids_dtype, None, None, 0, 16, 8, tokens, adapters, rank, k, n, dtype, ws,
+                            bytes_, None)
+
+    assert lora(tokens=0) == _lib.OK and lora(n=0) == _lib.OK
+    assert lora(dtype=3) == _lib.ERR_DTYPE and lora(ids_dtype=0) == _lib.ERR_DTYPE
+    for bad in ({"rank": 257}, {"rank": 0}, {"k": 0}, {"adapters": 0}, {"adapters": 16385}, {"tokens": -1}, {"x": None}, {},
+                {"ws": 8, "bytes_": 1 << 40}):
+        assert lora(**bad) == _lib.ERR_INVALID, bad
+    assert lib.tfo_lora_workspace_bytes(300, 4, 16, 64, 0) >= 300 * 32 * 4
+    assert lib.tfo_lora_workspace_bytes(300, 4, 257, 64, 0) == 0

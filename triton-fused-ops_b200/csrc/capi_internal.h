@@ -270,4 +270,24 @@ size_t qk_norm_rope_backward_workspace_bytes(int head_dim);
 cudaError_t qk_norm_rope_backward_launch(const HeadArgs& a, void* ws, cudaStream_t st);
 // Elements per vector with which the vector kernels can take these heads (0: they cannot).
 int head_vector_elems(const HeadArgs& a, bool backward);
+
+// Low-rank adapters of many requests (lora.cu):
+//   out[t] = base[t] + scaling[id] * B[id] (A[id] x[t]),  id = ids[t]
+struct LoraArgs {
+  const void* x;  // [tokens, k]
+  int64_t x_stride;
+  const void* a;  // [adapters, rank, k]
+  const void* b;  // [adapters, n, rank]
+  const void* ids;
+  int ids_dtype;         // POS_I32 or POS_I64
+  const float* scaling;  // [adapters], or NULL: ones
+  const void* base;      // [tokens, n], or NULL: zeros; may be out itself
+  int64_t base_stride;
+  void* out;
+  int64_t out_stride;
+  int64_t tokens, adapters, rank, k, n;
+  int dtype;
+};
+size_t lora_workspace_bytes(int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int dtype);
+cudaError_t lora_launch(const LoraArgs& a, void* ws, cudaStream_t st);
 }  // namespace tfo

@@ -32,6 +32,7 @@ enum : uint32_t {
   ERR_WAIT_TIMEOUT_OTHER = 1u << 3,
   ERR_BAD_LAUNCH = 1u << 4,
   ERR_GRID_BARRIER = 1u << 5,
+  ERR_BAD_ADAPTER = 1u << 7,   // an adapter id at or past the number of adapters
   ERR_BAD_POSITION = 1u << 6,  // a token's position lies outside the rotary table
 };
 

@@ -393,6 +393,45 @@ py::object rope_tables(const at::Tensor& positions, const at::Tensor& turns, dou
   return py::make_tuple(cos, sin);
 }
 
+// fused_lora on 2-D operands: the result, or None outside the common case.
+py::object lora(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, const at::Tensor& ids,
+                const OptTensor& scaling, const OptTensor& base, const OptTensor& out) {
+  if (!x.is_cuda() || !is_float(x.scalar_type()) || x.dim() != 2 || x.stride(1) != 1 || a.dim() != 3 || b.dim() != 3)
+    return py::none();
+  const int64_t tokens = x.size(0), k = x.size(1), adapters = a.size(0), rank = a.size(1), n = b.size(1);
+  auto same = [&](const at::Tensor& t) { return t.device() == x.device() && t.scalar_type() == x.scalar_type(); };
+  if (!same(a) || !same(b) || !a.is_contiguous() || !b.is_contiguous() || a.size(2) != k || b.size(0) != adapters ||
+      b.size(2) != rank || adapters < 1 || adapters > 16384 || rank < 1 || rank > 256 || k < 1 || n < 1 || tokens < 1)
+    return py::none();
+  if (ids.device() != x.device() || pos_code(ids.scalar_type()) < 0 || ids.dim() != 1 || ids.size(0) != tokens ||
+      !ids.is_contiguous())
+    return py::none();
+  if (scaling.has_value() && (scaling->device() != x.device() || scaling->scalar_type() != at::kFloat ||
+                              scaling->dim() != 1 || scaling->size(0) != adapters || !scaling->is_contiguous()))
+    return py::none();
+  for (const OptTensor* t : {&base, &out}) {
+    if (t->has_value() && (!same(**t) || (*t)->dim() != 2 || (*t)->size(0) != tokens || (*t)->size(1) != n ||
+                           (*t)->stride(1) != 1))
+      return py::none();
+  }
+  if (at::GradMode::is_enabled() && (x.requires_grad() || a.requires_grad() || b.requires_grad() ||
+                                     wants_grad(scaling) || wants_grad(base) || wants_grad(out)))
+    return py::none();
+  // rows of one output may not share memory
+  if (out.has_value() && tokens > 1 && out->stride(0) < n) return py::none();
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto st = at::cuda::getCurrentCUDAStream(x.device().index()).stream();
+  at::Tensor y = out.has_value() ? *out : at::empty({tokens, n}, x.options().requires_grad(false));
+  const int dtype = dtype_code(x.scalar_type());
+  at::Tensor ws = workspace(tfo_lora_workspace_bytes(tokens, adapters, rank, k, dtype), x.device(), st);
+  check(tfo_lora(x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ids.data_ptr(), pos_code(ids.scalar_type()),
+                 scaling.has_value() ? scaling->data_ptr<float>() : nullptr,
+                 base.has_value() ? base->data_ptr() : nullptr, base.has_value() ? base->stride(0) : 0, y.data_ptr(),
+                 y.stride(0), tokens, adapters, rank, k, n, dtype, ws.data_ptr(), static_cast<size_t>(ws.numel()), st),
+        "tfo_lora");
+  return py::cast(y);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tfo_ext, m) {
@@ -402,5 +441,6 @@ PYBIND11_MODULE(_tfo_ext, m) {
   m.def("rope", &rope, "fused_rope, or None");
   m.def("qk_norm_rope", &qk_norm_rope, "fused_qk_norm_rope, or None");
   m.def("rope_tables", &rope_tables, "rope_tables of given positions, or None");
+  m.def("lora", &lora, "fused_lora on 2-D operands, or None");
   m.def("clear_workspaces", &clear_workspaces, "releases the cached scratch buffers");
 }

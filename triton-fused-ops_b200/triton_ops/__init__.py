@@ -8,6 +8,7 @@ Ops (each one launches hand-written sm_100a CUDA kernels through the C ABI in
 * ``rope_tables`` / ``RoPEScaling``, ``fused_rope``
 * ``fused_qk_norm_rope`` / ``FusedQKNormRoPE``
 * ``fp8_gemm`` / ``FP8Linear``
+* ``fused_lora`` / ``FP8LoRALinear``
 * ``quantize_fp8`` / ``dequantize_fp8``
 
 Example::
@@ -42,6 +43,7 @@ from triton_ops.exceptions import (
 from triton_ops.kernels.fp8_gemm import FP8Linear, fp8_gemm
 from triton_ops.kernels.fp8_quantize import dequantize_fp8, quantize_fp8, quantize_fp8_per_token
 from triton_ops.kernels.gated_mlp import FusedGatedMLP, fused_gated_mlp, fused_gated_mlp_quantize
+from triton_ops.kernels.lora import FP8LoRALinear, fused_lora
 from triton_ops.kernels.qk_norm_rope import FusedQKNormRoPE, fused_qk_norm_rope
 from triton_ops.kernels.rmsnorm_rope import FusedRMSNormRoPE, fused_rmsnorm_rope, fused_rmsnorm_rope_quantize
 from triton_ops.kernels.rope import RoPEScaling, fused_rope, rope_tables
@@ -69,6 +71,8 @@ __all__ = [
     "FusedGatedMLP",
     "fp8_gemm",
     "FP8Linear",
+    "fused_lora",
+    "FP8LoRALinear",
     "quantize_fp8",
     "quantize_fp8_per_token",
     "dequantize_fp8",

@@ -47,6 +47,8 @@ POS_NONE, POS_I32, POS_I64 = 0, 1, 2
 
 # bit of the device error word: a token's position lies outside the rotary table
 ERR_BAD_POSITION = 1 << 6
+# bit of the device error word: an adapter id at or past the number of adapters
+ERR_BAD_ADAPTER = 1 << 7
 
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
@@ -133,6 +135,12 @@ _SIGNATURES = {
         [_c_vp, _c_strides, _c_vp, _c_strides, _c_vp, _c_strides, _c_vp, _c_strides, _c_vp, _c_vp, *_HEADS_TABLE,
          _c_vp, _c_vp, _c_vp, _c_vp, *_HEADS_SIZES, ctypes.c_double, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_size,
          _c_vp],
+    ),
+    "tfo_lora_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64, _c_int]),
+    "tfo_lora": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_int, _c_vp, _c_size, _c_vp],
     ),
     "tfo_gated_mlp_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_int, _c_int]),
     "tfo_gated_mlp": (

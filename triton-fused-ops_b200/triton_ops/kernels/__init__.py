@@ -8,6 +8,7 @@ from triton_ops.kernels.fp8_quantize import (
     quantize_fp8_kernel,
 )
 from triton_ops.kernels.gated_mlp import FusedGatedMLP, fused_gated_mlp, fused_gated_mlp_kernel
+from triton_ops.kernels.lora import FP8LoRALinear, fused_lora, fused_lora_kernel
 from triton_ops.kernels.qk_norm_rope import (
     FusedQKNormRoPE,
     fused_qk_norm_rope,
@@ -50,6 +51,9 @@ __all__ = [
     "fp8_gemm",
     "FP8Linear",
     "fp8_gemm_kernel",
+    "fused_lora",
+    "FP8LoRALinear",
+    "fused_lora_kernel",
     "quantize_fp8",
     "dequantize_fp8",
     "quantize_fp8_kernel",

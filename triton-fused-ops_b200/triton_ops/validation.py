@@ -365,3 +365,61 @@ def validate_head_weight(q: torch.Tensor, weight: Optional[torch.Tensor], name: 
             expected=(q.shape[-1],), actual=weight.shape, tensor_name=name,
         )
     _check_contiguous(weight, name)
+
+
+def validate_lora_inputs(
+    x: torch.Tensor,
+    lora_a: torch.Tensor,
+    lora_b: torch.Tensor,
+    adapter_ids: torch.Tensor,
+    scaling: Optional[torch.Tensor],
+    base: Optional[torch.Tensor],
+    out: Optional[torch.Tensor],
+) -> Tuple[int, int, int, int, int]:
+    """Checks the adapters' inputs; returns (tokens, adapters, rank, in_features, out_features)."""
+    named = [(x, "x"), (lora_a, "lora_a"), (lora_b, "lora_b")]
+    named += [(t, n) for t, n in ((base, "base"), (out, "out")) if t is not None]
+    for t, n in named:
+        _check_cuda(t, n)
+    for t, n in named:
+        _check_dtype(t, n, SUPPORTED_DTYPES_FLOAT if t is x else [x.dtype])
+        _check_same_device(x, t, n)
+    _check_cuda(adapter_ids, "adapter_ids")
+    _check_dtype(adapter_ids, "adapter_ids", [torch.int32, torch.int64])
+    _check_same_device(x, adapter_ids, "adapter_ids")
+    if x.dim() < 1:
+        raise ShapeMismatchError("x must be [..., in_features]", actual=x.shape, tensor_name="x")
+    if lora_a.dim() != 3:
+        raise ShapeMismatchError(f"lora_a must be 3D [adapters, rank, in_features], got {lora_a.dim()}D",
+                                 actual=lora_a.shape, tensor_name="lora_a")
+    adapters, rank, k = lora_a.shape
+    if x.shape[-1] != k:
+        raise ShapeMismatchError(f"lora_a in_features {k} doesn't match x {x.shape[-1]}",
+                                 expected=(adapters, rank, x.shape[-1]), actual=lora_a.shape, tensor_name="lora_a")
+    if lora_b.dim() != 3 or lora_b.shape[0] != adapters or lora_b.shape[2] != rank:
+        raise ShapeMismatchError(f"lora_b must be [{adapters}, out_features, {rank}], got {tuple(lora_b.shape)}",
+                                 expected=(adapters, None, rank), actual=lora_b.shape, tensor_name="lora_b")
+    n = lora_b.shape[1]
+    if not (0 < adapters <= 16384 and 0 < rank <= 256 and k > 0):
+        raise ShapeMismatchError(f"need 1..16384 adapters of rank 1..256 and in_features > 0, got {tuple(lora_a.shape)}",
+                                 actual=lora_a.shape, tensor_name="lora_a")
+    _check_contiguous(lora_a, "lora_a")
+    _check_contiguous(lora_b, "lora_b")
+    if adapter_ids.shape != x.shape[:-1]:
+        raise ShapeMismatchError(f"adapter_ids shape {tuple(adapter_ids.shape)} doesn't match x's rows {tuple(x.shape[:-1])}",
+                                 expected=tuple(x.shape[:-1]), actual=adapter_ids.shape, tensor_name="adapter_ids")
+    for t, name in ((base, "base"), (out, "out")):
+        if t is not None and t.shape != (*x.shape[:-1], n):
+            raise ShapeMismatchError(f"{name} shape {tuple(t.shape)} doesn't match {(*x.shape[:-1], n)}",
+                                     expected=(*x.shape[:-1], n), actual=t.shape, tensor_name=name)
+    if scaling is not None:
+        _check_cuda(scaling, "scaling")
+        _check_dtype(scaling, "scaling", [torch.float32])
+        _check_same_device(x, scaling, "scaling")
+        if scaling.shape != (adapters,):
+            raise ShapeMismatchError(f"scaling must be [{adapters}], got {tuple(scaling.shape)}", expected=(adapters,),
+                                     actual=scaling.shape, tensor_name="scaling")
+        _check_contiguous(scaling, "scaling")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, lora_a, lora_b, scaling, base, out)):
+        raise ValueError("the adapters of many requests serve and have no gradient: call under torch.no_grad()")
+    return x.numel() // k, adapters, rank, k, n
