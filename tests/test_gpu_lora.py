@@ -85,6 +85,15 @@ CASES = [
     (2100, 9, 128, 256, 200, "bf16"),
     (300, 3, 256, 512, 72, "f16"),
     (70, 3, 256, 100, 72, "f32"),
+    # each width of the streaming kernels, whole vectors
+    (700, 6, 32, 1024, 512, "bf16"),
+    (400, 3, 96, 256, 136, "f16"),
+    (600, 5, 16, 192, 96, "f32"),
+    (320, 2, 64, 128, 200, "f32"),
+    (300, 2, 200, 128, 64, "f32"),
+    (300, 2, 200, 128, 64, "f16"),
+    (90, 3, 100, 256, 96, "bf16"),
+    (3, 2, 16, 8192, 2048, "bf16"),    # eight CTAs a tile
 ]
 
 

@@ -38,8 +38,8 @@ int tfo_lora(const void* x, int64_t x_stride, const void* a, const void* b, cons
     return fail(TFO_ERR_INVALID, std::string(fn) + ": rank must be in 1..256 and k positive");
   if (tokens == 0 || n == 0) return TFO_OK;
   if (!x || !a || !b || !ids || !out) return fail(TFO_ERR_INVALID, std::string(fn) + ": NULL pointer");
-  if (!workspace || workspace_bytes < lora_workspace_bytes(tokens, adapters, rank, k, dtype) ||
-      reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+  const size_t need = lora_workspace_bytes(tokens, adapters, rank, k, dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
     return fail(TFO_ERR_INVALID, std::string(fn) + ": workspace too small or not 16-byte aligned");
   const LoraArgs args{x,   x_stride,   a,      b,        ids,  ids_dtype, scaling, base, base_stride,
                       out, out_stride, tokens, adapters, rank, k,         n,       dtype};
