@@ -355,7 +355,7 @@ TFO_API int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_
  * untouched when base == out). An id >= adapters reads nothing: its row becomes
  * NaN and the device error word gets bit 7. rank <= 256, adapters <= 16384.
  * fp32 sums; one rounding of the result. No counterpart in the reference. */
-TFO_API size_t tfo_lora_workspace_bytes(int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int dtype);
+TFO_API size_t tfo_lora_workspace_bytes(int64_t tokens, int64_t adapters);
 TFO_API int tfo_lora(const void* x, int64_t x_stride, const void* a, const void* b, const void* ids, int ids_dtype,
                      const float* scaling, const void* base, int64_t base_stride, void* out, int64_t out_stride,
                      int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int64_t n, int dtype, void* workspace,

@@ -85,6 +85,7 @@ CASES = [
     (2100, 9, 128, 256, 200, "bf16"),
     (300, 3, 256, 512, 72, "f16"),
     (70, 3, 256, 100, 72, "f32"),
+    (9000, 20, 8, 64, 64, "bf16"),     # more rows than the sort holds at once
     # each width of the streaming kernels, whole vectors
     (700, 6, 32, 1024, 512, "bf16"),
     (400, 3, 96, 256, 136, "f16"),

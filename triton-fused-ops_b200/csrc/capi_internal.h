@@ -288,6 +288,6 @@ struct LoraArgs {
   int64_t tokens, adapters, rank, k, n;
   int dtype;
 };
-size_t lora_workspace_bytes(int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int dtype);
+size_t lora_workspace_bytes(int64_t tokens, int64_t adapters);
 cudaError_t lora_launch(const LoraArgs& a, void* ws, cudaStream_t st);
 }  // namespace tfo

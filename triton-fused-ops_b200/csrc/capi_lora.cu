@@ -17,9 +17,9 @@ using namespace tfo;
 
 extern "C" {
 
-size_t tfo_lora_workspace_bytes(int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int dtype) {
-  if (tokens <= 0 || adapters <= 0 || rank <= 0 || rank > kMaxRank || k <= 0) return 0;
-  return lora_workspace_bytes(tokens, adapters, rank, k, dtype);
+size_t tfo_lora_workspace_bytes(int64_t tokens, int64_t adapters) {
+  if (tokens <= 0 || adapters <= 0) return 0;
+  return lora_workspace_bytes(tokens, adapters);
 }
 
 int tfo_lora(const void* x, int64_t x_stride, const void* a, const void* b, const void* ids, int ids_dtype,
@@ -38,7 +38,7 @@ int tfo_lora(const void* x, int64_t x_stride, const void* a, const void* b, cons
     return fail(TFO_ERR_INVALID, std::string(fn) + ": rank must be in 1..256 and k positive");
   if (tokens == 0 || n == 0) return TFO_OK;
   if (!x || !a || !b || !ids || !out) return fail(TFO_ERR_INVALID, std::string(fn) + ": NULL pointer");
-  const size_t need = lora_workspace_bytes(tokens, adapters, rank, k, dtype);
+  const size_t need = lora_workspace_bytes(tokens, adapters);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
     return fail(TFO_ERR_INVALID, std::string(fn) + ": workspace too small or not 16-byte aligned");
   const LoraArgs args{x,   x_stride,   a,      b,        ids,  ids_dtype, scaling, base, base_stride,

@@ -7,15 +7,16 @@
 // Two steps with the low-rank values v = A x in fp32 between them:
 //   shrink: v = the sum over K, cut into parts that are added in a fixed order
 //   expand: out = base + B (scaling * v)
+// both in one kernel, v never leaves the SMs.
 // Rows that use the same adapter are grouped into tiles, so that an adapter's
 // matrices are read once per tile and not once per row:
-//   up to 256 tokens, one launch (lora_small_kernel): row i leads a tile if 0,
-//     16, 32, ... rows before it use the same adapter, which every CTA finds
-//     out from the ids; a cluster of CTAs shares a tile, each shrinks a part of
-//     K, reads the others' sums through distributed shared memory and expands a
-//     part of the columns;
-//   more: a one-CTA kernel sorts the rows by adapter into tiles of 64, then two
-//     kernels stream x and A, and base and B, through shared memory.
+//   up to 256 tokens, one launch (lora_small_kernel): every CTA finds its tile
+//     of up to 16 rows from the ids; a cluster of CTAs shares a tile, each
+//     shrinks a part of K, sends its sums to the others' shared memory and
+//     expands a part of the columns;
+//   more: a one-CTA kernel sorts the rows by adapter into tiles of 64, then a
+//     cluster of CTAs takes a tile in the same way, streaming x and A, then
+//     base and B, through shared memory (lora_large_kernel).
 // A row's result does not depend on the rows beside it in its tile.
 //
 // Both products run on m16n8 tensor instructions with rows of a tile as M.
@@ -38,7 +39,7 @@ namespace tfo {
 
 constexpr int kSmallTokens = 256;  // at most: each CTA reads all ids (one per thread)
 constexpr int kSmallRows = 16, kSmallWarps = 8, kMaxCluster = 8;
-constexpr int kLargeRows = 64, kLargeThreads = 128;
+constexpr int kLargeRows = 64, kLargeThreads = 256;
 
 __host__ __device__ constexpr int chunk_elems(int esize) { return 64 / esize; }  // summed elements per 64-byte chunk
 // Ranks as the expand step holds them: a power of two of chunks.
@@ -151,33 +152,48 @@ struct Tile {
   int group, count;  // count 0: nothing to do
 };
 
-// The tile that row `lead` leads, by the whole CTA (256 threads, tokens <= 256); rows gets its rows.
-__device__ __forceinline__ Tile find_tile(const LoraArgs& a, int lead, int* rows, int* scratch) {
-  const int t = threadIdx.x;
+// Tile `index` of at most 256 rows, by the whole CTA (256 threads); rows gets
+// its rows. A row leads a tile if 0, 16, 32, ... rows before it are of its
+// group; tiles are counted in the order of their leaders.
+__device__ __forceinline__ Tile find_tile(const LoraArgs& a, int index, int* rows, int* groups, int* scratch) {
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int tokens = static_cast<int>(a.tokens);
   const int group = t < tokens ? row_group(a, t) : -1;
-  if (t == lead) scratch[8] = group;
+  groups[t] = group;
   __syncthreads();
-  const int want = scratch[8];
-  const bool same = group == want;
-  if (__syncthreads_count(same && t < lead) % kSmallRows != 0) return Tile{want, 0};
-  const uint32_t votes = __ballot_sync(0xffffffffu, same && t >= lead);
-  if ((t & 31) == 0) scratch[t >> 5] = __popc(votes);
-  __syncthreads();
-  int before = __popc(votes & ((1u << (t & 31)) - 1)), all = 0;
-  for (int w = 0; w < kSmallWarps; ++w) {
-    if (w < t >> 5) before += scratch[w];
-    all += scratch[w];
+  int rank = 0;  // rows of the group before this one
+  const int end = t < tokens ? t : 0;
+#pragma unroll 8
+  for (int i = 0; i + 4 <= end; i += 4) {
+    const int4 g = *reinterpret_cast<const int4*>(groups + i);
+    rank += (g.x == group) + (g.y == group) + (g.z == group) + (g.w == group);
   }
-  if (same && t >= lead && before < kSmallRows) rows[before] = t;
+  for (int i = end & ~3; i < end; ++i) rank += groups[i] == group;
+  const bool leads = group >= 0 && rank % kSmallRows == 0;
+  const uint32_t votes = __ballot_sync(0xffffffffu, leads);
+  if (lane == 0) scratch[warp] = __popc(votes);
+  if (t == 0) scratch[8] = -1;
   __syncthreads();
-  return Tile{want, min(all, kSmallRows)};
+  int before = __popc(votes & ((1u << lane) - 1));
+  for (int w = 0; w < warp; ++w) before += scratch[w];
+  if (leads && before == index) {
+    scratch[8] = t;
+    scratch[9] = rank;
+  }
+  __syncthreads();
+  const int lead = scratch[8];
+  if (lead < 0) return Tile{0, 0};
+  const int want = groups[lead], place = rank - scratch[9];
+  const bool mine = group == want && place >= 0 && place < kSmallRows;
+  if (mine) rows[place] = t;
+  const int count = __syncthreads_count(mine);
+  return Tile{want, count};
 }
 
 // A tile of the sorted rows, by the whole CTA.
-__device__ __forceinline__ Tile planned_tile(const LoraPlan& plan, int* rows) {
-  if (static_cast<int>(blockIdx.x) >= *plan.num_tiles) return Tile{0, 0};
-  const int4 t = plan.tiles[blockIdx.x];
+__device__ __forceinline__ Tile planned_tile(const LoraPlan& plan, int index, int* rows) {
+  const int4 t = plan.tiles[index];  // past the last tile: anything, not used
+  if (index >= *plan.num_tiles) return Tile{0, 0};
   if (threadIdx.x < t.z) rows[threadIdx.x] = plan.perm[t.y + threadIdx.x];
   __syncthreads();
   return Tile{t.x, t.z};
@@ -185,90 +201,102 @@ __device__ __forceinline__ Tile planned_tile(const LoraPlan& plan, int* rows) {
 
 // Sorts the rows by group (the order inside a group is free) and cuts the
 // groups into tiles. One CTA, whose threads hold kHeld ids each: their loads
-// are in flight together, and up to 8192 rows are read once.
+// are in flight together, and up to 8192 rows are read and counted once.
 constexpr int kHeld = 8, kPlanThreads = 1024;
+
+// Inclusive prefix sums over a warp.
+__device__ __forceinline__ int warp_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int p = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += p;
+  }
+  return v;
+}
+
 __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs a, LoraPlan plan) {
-  extern __shared__ int bins[];  // [groups] rows of each, then the next free place
+  extern __shared__ int bins[];  // [groups] rows of each, then its first place
   __shared__ int carry[2], sum_rows[32], sum_tiles[32];
   griddep_launch_dependents();
   griddep_wait();
   const int groups = static_cast<int>(a.adapters) + 2;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int tokens = static_cast<int>(a.tokens);
-  int held[kHeld];
-  auto load = [&](int first) {
+  constexpr int kStep = kHeld * kPlanThreads;
+  int group[kHeld], place[kHeld];
+  auto load = [&](int64_t first) {
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
-      const int64_t i = static_cast<int64_t>(first) + j * kPlanThreads + t;
-      held[j] = i < tokens ? row_group(a, i) : -1;
+      const int64_t i = first + j * kPlanThreads + t;
+      group[j] = i < tokens ? row_group(a, i) : -1;
     }
   };
-  constexpr int kStep = kHeld * kPlanThreads;
+  // adds the held rows to the bins; place: where the row comes in its bin
+  auto count = [&](int64_t first) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      if (first + j * kPlanThreads + (t & ~31) >= tokens) break;
+      // requests' rows mostly lie together: a whole warp of one group needs no match
+      const bool one = __all_sync(0xffffffffu, group[j] == __shfl_sync(0xffffffffu, group[j], 0));
+      const uint32_t peers = one ? 0xffffffffu : __match_any_sync(0xffffffffu, group[j]);
+      const int leader = __ffs(peers) - 1;
+      int at = 0;
+      if (group[j] >= 0 && lane == leader) at = atomicAdd(&bins[group[j]], __popc(peers));
+      place[j] = __shfl_sync(0xffffffffu, at, leader) + __popc(peers & ((1u << lane) - 1));
+    }
+  };
   load(0);
   for (int i = t; i < groups; i += kPlanThreads) bins[i] = 0;
   if (t < 2) carry[t] = 0;
   __syncthreads();
-  for (int64_t first = 0; first < tokens; first += kStep) {
-    if (first > 0) load(static_cast<int>(first));
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      if (first + j * kPlanThreads + (t & ~31) >= tokens) break;
-      const uint32_t peers = __match_any_sync(0xffffffffu, held[j]);
-      if (held[j] >= 0 && lane == __ffs(peers) - 1) atomicAdd(&bins[held[j]], __popc(peers));
-    }
+  count(0);
+  for (int64_t first = kStep; first < tokens; first += kStep) {
+    load(first);
+    count(first);
   }
   __syncthreads();
   // exclusive prefix sums of rows and tiles over the groups
   for (int first = 0; first < groups; first += kPlanThreads) {
     const int g = first + t;
-    const int count = g < groups ? bins[g] : 0;
-    const int ntiles = (count + kLargeRows - 1) / kLargeRows;
-    int r = count, n = ntiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int pr = __shfl_up_sync(0xffffffffu, r, o), pn = __shfl_up_sync(0xffffffffu, n, o);
-      if (lane >= o) {
-        r += pr;
-        n += pn;
-      }
-    }
+    const int rows = g < groups ? bins[g] : 0;
+    const int tiles = (rows + kLargeRows - 1) / kLargeRows;
+    const int r = warp_scan(rows, lane), n = warp_scan(tiles, lane);
     if (lane == 31) {
       sum_rows[warp] = r;
       sum_tiles[warp] = n;
     }
     __syncthreads();
-    int before_r = carry[0], before_n = carry[1];
-    for (int w = 0; w < warp; ++w) {
-      before_r += sum_rows[w];
-      before_n += sum_tiles[w];
-    }
-    const int row0 = before_r + r - count, tile0 = before_n + n - ntiles;
-    if (g < groups) {
-      bins[g] = row0;
-      for (int i = 0; i < ntiles; ++i)
-        plan.tiles[tile0 + i] = make_int4(g, row0 + i * kLargeRows, min(kLargeRows, count - i * kLargeRows), 0);
+    if (warp == 0) {
+      const int sr = warp_scan(sum_rows[lane], lane), sn = warp_scan(sum_tiles[lane], lane);
+      sum_rows[lane] = sr;
+      sum_tiles[lane] = sn;
     }
     __syncthreads();
-    if (t == kPlanThreads - 1) {
-      carry[0] = before_r + r;
-      carry[1] = before_n + n;
+    const int row0 = carry[0] + (warp > 0 ? sum_rows[warp - 1] : 0) + r - rows;
+    const int tile0 = carry[1] + (warp > 0 ? sum_tiles[warp - 1] : 0) + n - tiles;
+    if (g < groups) {
+      bins[g] = row0;
+      for (int i = 0; i < tiles; ++i)
+        plan.tiles[tile0 + i] = make_int4(g, row0 + i * kLargeRows, min(kLargeRows, rows - i * kLargeRows), 0);
+    }
+    __syncthreads();
+    if (t == 0) {
+      carry[0] += sum_rows[31];
+      carry[1] += sum_tiles[31];
     }
     __syncthreads();
   }
   if (t == 0) *plan.num_tiles = carry[1];
+  // the rows' places; past kStep rows the bins go on counting from their first place
   for (int64_t first = 0; first < tokens; first += kStep) {
-    if (tokens > kStep) load(static_cast<int>(first));
+    if (tokens > kStep) {
+      load(first);
+      count(first);
+    }
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
       const int64_t i = first + j * kPlanThreads + t;
-      if (i - lane >= tokens) break;
-      const int g = held[j];
-      const uint32_t peers = __match_any_sync(0xffffffffu, g);
-      const int leader = __ffs(peers) - 1;
-      int at = 0;
-      if (g >= 0 && lane == leader) at = atomicAdd(&bins[g], __popc(peers));
-      at = __shfl_sync(0xffffffffu, at, leader);
-      if (g >= 0) plan.perm[at + __popc(peers & ((1u << lane) - 1))] = static_cast<int>(i);
+      if (i < tokens) plan.perm[tokens > kStep ? place[j] : bins[group[j]] + place[j]] = static_cast<int>(i);
     }
   }
 }
@@ -281,137 +309,19 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int nch, int chunk, int
   const int c = (nch & 1) ? chunk : chunk ^ (row & 1);
   return static_cast<uint32_t>((row * nch + c) * 64 + quarter * 16);
 }
-// 16 bytes from global to shared memory, or zeros.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+// `bytes` (16 or 0) from global to shared memory, the rest of 16 as zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
-// ---- shrink: v = A x ---------------------------------------------------------------
-// grid: (tiles, splits of K, blocks of 8 NT ranks); a warp has 16 rows.
-__device__ __forceinline__ void split_range(int64_t units, int splits, int split, int* first, int* last) {
-  *first = static_cast<int>(units * split / splits);
-  *last = static_cast<int>(units * (split + 1) / splits);
+// Part `part` of `parts` of a range.
+__device__ __forceinline__ void split_range(int64_t units, int parts, int part, int* first, int* last) {
+  *first = static_cast<int>(units * part / parts);
+  *last = static_cast<int>(units * (part + 1) / parts);
 }
 
-template <int NT>
-__device__ __forceinline__ void store_v(const Tile& tile, const int* rows, float* v, int64_t v_rank, int r0, int m0, int g,
-                                        int q, const float (&acc)[NT][4]) {
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int r = r0 + j * 8 + 2 * q;
-    if (r >= v_rank) continue;  // v_rank is a multiple of 16
-    if (m0 + g < tile.count)
-      *reinterpret_cast<float2*>(v + static_cast<int64_t>(rows[m0 + g]) * v_rank + r) = make_float2(acc[j][0], acc[j][1]);
-    if (m0 + g + 8 < tile.count)
-      *reinterpret_cast<float2*>(v + static_cast<int64_t>(rows[m0 + g + 8]) * v_rank + r) = make_float2(acc[j][2], acc[j][3]);
-  }
-}
-
-// x and A in steps of 128 bytes of K, STAGES deep.
-template <typename T, int NT, int STAGES>
-__global__ void __launch_bounds__(kLargeThreads) lora_shrink_kernel(const LoraArgs a, LoraPlan plan, float* __restrict__ v,
-                                                                    int splits, int64_t v_rank) {
-  constexpr int E = 16 / sizeof(T), KS = 128 / sizeof(T);
-  constexpr int kXBytes = kLargeRows * 128, kStage = kXBytes + 8 * NT * 128;
-  __shared__ int rows[kLargeRows];
-  extern __shared__ __align__(128) uint8_t smem[];
-  griddep_launch_dependents();
-  griddep_wait();
-  const Tile tile = planned_tile(plan, rows);
-  if (tile.count == 0 || tile.group >= a.adapters) return;
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  int k0, k1;
-  split_range((a.k + KS - 1) / KS, splits, blockIdx.y, &k0, &k1);
-  // this thread's copies: 16 bytes `vec` of every sixteenth row
-  const int vec = t & 7, row0 = t >> 3;
-  const int r0 = blockIdx.z * 8 * NT;
-  const T* x = static_cast<const T*>(a.x) + vec * E;
-  const T* w = static_cast<const T*>(a.a) + (static_cast<int64_t>(tile.group) * a.rank + r0) * a.k + vec * E;
-  const T* xp[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) xp[i] = x + static_cast<int64_t>(rows[min(row0 + 16 * i, tile.count - 1)]) * a.x_stride;
-  const uint32_t base = smem_u32(smem);
-  auto load = [&](int step, int stage) {
-    if (step < k1) {
-      const int64_t at = static_cast<int64_t>(step) * KS;
-      const bool in = at + vec * E < a.k;
-      const uint32_t dst = base + stage * kStage;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = row0 + 16 * i;
-        copy16(dst + tile_offset(r, 2, vec >> 2, vec & 3), in ? xp[i] + at : a.x, in && r < tile.count);
-      }
-#pragma unroll
-      for (int i = 0; i < NT / 2; ++i) {
-        const int r = row0 + 16 * i;
-        const bool ok = in && r0 + r < a.rank;
-        copy16(dst + kXBytes + tile_offset(r, 2, vec >> 2, vec & 3), ok ? w + r * a.k + at : a.a, ok);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) load(k0 + i, i);
-  const int g = lane >> 2, q = lane & 3, m0 = warp * 16;
-  float acc[NT][4] = {};
-  int stage = 0;
-  for (int step = k0; step < k1; ++step) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-    __syncthreads();  // the step's bytes are there, and the stage before it is free
-    load(step + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-    if (m0 < tile.count) {
-      const uint8_t* xs = smem + stage * kStage;
-      const uint8_t* as = xs + kXBytes;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint4 a0 = lds16(xs + tile_offset(m0 + g, 2, c, q)), a1 = lds16(xs + tile_offset(m0 + g + 8, 2, c, q));
-#pragma unroll
-        for (int j = 0; j < NT; ++j) Chunk<T>::mma(acc[j], a0, a1, lds16(as + tile_offset(j * 8 + g, 2, c, q)));
-      }
-    }
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
-  }
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  store_v<NT>(tile, rows, v + static_cast<int64_t>(blockIdx.y) * a.tokens * v_rank, v_rank, r0, m0, g, q, acc);
-}
-
-// Any alignment of x and A: elements straight into fragments.
-template <typename T, int NT>
-__global__ void __launch_bounds__(kLargeThreads) lora_shrink_any_kernel(const LoraArgs a, LoraPlan plan,
-                                                                        float* __restrict__ v, int splits, int64_t v_rank) {
-  constexpr int E = 16 / sizeof(T), C = chunk_elems(sizeof(T));
-  __shared__ int rows[kLargeRows];
-  griddep_launch_dependents();
-  griddep_wait();
-  const Tile tile = planned_tile(plan, rows);
-  if (tile.count == 0 || tile.group >= a.adapters) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, q = lane & 3, m0 = warp * 16;
-  if (m0 >= tile.count) return;
-  const T* x = static_cast<const T*>(a.x);
-  const T* x0 = m0 + g < tile.count ? x + static_cast<int64_t>(rows[m0 + g]) * a.x_stride : nullptr;
-  const T* x1 = m0 + g + 8 < tile.count ? x + static_cast<int64_t>(rows[m0 + g + 8]) * a.x_stride : nullptr;
-  const int r0 = blockIdx.z * 8 * NT;
-  const T* w[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int r = r0 + j * 8 + g;
-    w[j] = r < a.rank ? static_cast<const T*>(a.a) + (static_cast<int64_t>(tile.group) * a.rank + r) * a.k : nullptr;
-  }
-  int c0, c1;
-  split_range((a.k + C - 1) / C, splits, blockIdx.y, &c0, &c1);
-  float acc[NT][4] = {};
-  for (int c = c0; c < c1; ++c) {
-    const int64_t i = static_cast<int64_t>(c) * C + q * E;
-    const uint4 a0 = load_chunk<T>(x0, i, a.k, 1), a1 = load_chunk<T>(x1, i, a.k, 1);
-#pragma unroll
-    for (int j = 0; j < NT; ++j) Chunk<T>::mma(acc[j], a0, a1, load_chunk<T>(w[j], i, a.k, 1));
-  }
-  store_v<NT>(tile, rows, v + static_cast<int64_t>(blockIdx.y) * a.tokens * v_rank, v_rank, r0, m0, g, q, acc);
-}
-
-// ---- expand: out = base + B v ------------------------------------------------------
+// ---- the expand step -----------------------------------------------------------------
 // Eight neighbouring values of a row, as raw 16-byte vectors.
 template <typename T> struct Eight {
   static constexpr int W = 8 * sizeof(T) / 16;
@@ -475,11 +385,12 @@ __device__ __forceinline__ void fill_rows(const LoraArgs& a, const Tile& tile, c
 // Stages the tile's v as operands in shared memory: hi and lo (16-bit types;
 // fp32 as it is), [M][stride] elements. sum(m, r) gives four neighbouring
 // values of row m, summed and scaled. fp16 rows are scaled by a power of two
-// to below 2 (row_scale takes it back; `sums` holds them meanwhile); rows past
-// the tile and ranks past the end are zero.
+// to below 2 (row_scale takes it back; `sums`, [M][sums_stride], holds them meanwhile
+// and may be what sum(m, r) reads); rows past the tile and ranks past the end
+// are zero.
 template <typename T, int M, typename Sum>
 __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int stride, T* hi, T* lo, float* sums,
-                                        float* row_scale, unsigned* row_max, Sum sum) {
+                                        int sums_stride, float* row_scale, unsigned* row_max, Sum sum) {
   constexpr bool SPLIT = sizeof(T) == 2;
   constexpr bool SCALED = std::is_same<T, __half>::value;
   const int quads = vr / 4, threads = blockDim.x;
@@ -511,7 +422,7 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int 
       t[3] = r + 3 < rank ? u.w : 0.f;
     }
     if constexpr (SCALED) {
-      *reinterpret_cast<float4*>(sums + m * vr + r) = make_float4(t[0], t[1], t[2], t[3]);
+      if (r < sums_stride) *reinterpret_cast<float4*>(sums + m * sums_stride + r) = make_float4(t[0], t[1], t[2], t[3]);
       float most = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) most = !(fabsf(t[j]) <= most) ? fabsf(t[j]) : most;  // NaN stays
@@ -529,7 +440,8 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int 
     __syncthreads();
     for (int i = threadIdx.x; i < M * quads; i += threads) {
       const int m = i / quads, r = i % quads * 4;
-      const float4 u = *reinterpret_cast<const float4*>(sums + m * vr + r);
+      float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < sums_stride) u = *reinterpret_cast<const float4*>(sums + m * sums_stride + r);
       const float t[4] = {u.x, u.y, u.z, u.w};
       put(m, r, t, 1.f / row_scale[m]);
     }
@@ -537,19 +449,15 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int 
   }
 }
 
-// v of a sorted tile's row from the splits' parts, in order.
-struct SumParts {
-  const float* v;
-  const int* rows;
-  int64_t part;  // elements from one split's part to the next
-  int splits, vr;
+// The parts of v that a cluster's CTAs have sent, [cluster][M][stride], added in order.
+template <int M> struct SumParts {
+  const float* parts;
+  int cluster, stride;
   float scale;
   __device__ float4 operator()(int m, int r) const {
-    const float* p = v + static_cast<int64_t>(rows[m]) * vr + r;
-    float4 u = *reinterpret_cast<const float4*>(p);
-#pragma unroll 4
-    for (int k = 1; k < splits; ++k) {
-      const float4 w = *reinterpret_cast<const float4*>(p + k * part);
+    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < cluster; ++k) {
+      const float4 w = *reinterpret_cast<const float4*>(parts + (k * M + m) * stride + r);
       u.x += w.x;
       u.y += w.y;
       u.z += w.z;
@@ -619,190 +527,7 @@ __device__ __forceinline__ void block_values(const float (&acc)[4][4], float s0,
 // instruction j: 2 j further.
 __device__ __forceinline__ int block_column(int g) { return (g >> 1) * 8 + (g & 1); }
 
-// base and B in steps of 128 bytes of a row (64 or 32 columns), STAGES deep;
-// NCH: 64-byte chunks of a row of B (up to two: v stays in registers).
-// grid: (tiles, ranges of `range` columns); a warp has 16 rows.
-template <typename T, int NCH, int STAGES>
-__global__ void __launch_bounds__(kLargeThreads) lora_expand_kernel(const LoraArgs a, LoraPlan plan,
-                                                                    const float* __restrict__ v, int splits,
-                                                                    int64_t v_rank, int64_t range, uint32_t* err) {
-  constexpr int E = 16 / sizeof(T), C = chunk_elems(sizeof(T));
-  constexpr int NS = 128 / sizeof(T);  // columns of a step
-  constexpr int M = kLargeRows;
-  constexpr bool SCALED = std::is_same<T, __half>::value;
-  __shared__ int rows[M];
-  __shared__ float row_scale[M];
-  __shared__ unsigned row_max[M];
-  extern __shared__ __align__(128) uint8_t smem[];
-  griddep_launch_dependents();
-  griddep_wait();
-  const Tile tile = planned_tile(plan, rows);
-  if (tile.count == 0) return;
-  const int64_t col0 = blockIdx.y * range, col1 = min(a.n, col0 + range);
-  if (tile.group >= a.adapters) {
-    fill_rows<T>(a, tile, rows, col0, col1, true, err);
-    return;
-  }
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  constexpr int vr = NCH * C, stride = vr + E;
-  constexpr int kBase = M * 128, kStage = kBase + NS * NCH * 64;
-  T* hi = reinterpret_cast<T*>(smem + STAGES * kStage);
-  T* lo = hi + M * stride;
-
-  // this thread's copies of a step: 16 bytes `vec` of every sixteenth row of
-  // base, and of every kBStep-th row of B
-  const int vec = t & 7, row0 = t >> 3;
-  constexpr int kBVecs = NCH * 4, kBStep = kBVecs > kLargeThreads ? 1 : kLargeThreads / kBVecs;
-  static_assert(kBVecs <= kLargeThreads, "a row of B has at most one vector for each thread");
-  const int b_vec = t % kBVecs, b_row0 = t / kBVecs;
-  const bool with_base = a.base != nullptr;
-  const T* bp[4];
-  bool has_row[4];
-  uint32_t base_dst[4];
-  const uint32_t ring = smem_u32(smem);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = row0 + 16 * i;
-    has_row[i] = r < tile.count;
-    bp[i] = static_cast<const T*>(a.base) + static_cast<int64_t>(rows[has_row[i] ? r : 0]) * a.base_stride + col0 + vec * E;
-    base_dst[i] = ring + tile_offset(r, 2, vec >> 2, vec & 3);
-  }
-  const T* b = static_cast<const T*>(a.b) + (static_cast<int64_t>(tile.group) * a.n + col0 + b_row0) * a.rank + b_vec * E;
-  const bool b_in = b_vec * E < a.rank;
-  const int64_t b_step = static_cast<int64_t>(kBStep) * a.rank;
-  const int cols = static_cast<int>(col1 - col0);
-  const int steps = (cols + NS - 1) / NS;
-  auto load = [&](int step, int stage) {
-    if (step < steps) {
-      const int col = step * NS;
-      const uint32_t at = stage * kStage;
-      if (with_base) {
-        const bool in = col + vec * E < cols;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool ok = in && has_row[i];
-          copy16(base_dst[i] + at, ok ? bp[i] + col : a.base, ok);
-        }
-      }
-      const T* src = b + static_cast<int64_t>(col) * a.rank;
-#pragma unroll
-      for (int r = 0; r < NS; r += kBStep, src += b_step) {
-        const bool ok = b_in && col + r + b_row0 < cols;
-        copy16(ring + at + kBase + tile_offset(r + b_row0, NCH, b_vec >> 2, b_vec & 3), ok ? src : a.b, ok);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) load(i, i);
-  const SumParts sum{v, rows, a.tokens * v_rank, splits, vr, a.scaling != nullptr ? a.scaling[tile.group] : 1.f};
-  stage_v<T, M>(tile, static_cast<int>(a.rank), vr, stride, hi, lo, reinterpret_cast<float*>(lo + M * stride), row_scale,
-                row_max, sum);
-  const int g = lane >> 2, q = lane & 3, m0 = warp * 16;
-  const bool in0 = m0 + g < tile.count, in1 = m0 + g + 8 < tile.count;
-  const float s0 = SCALED ? row_scale[m0 + g] : 1.f, s1 = SCALED ? row_scale[m0 + g + 8] : 1.f;
-  const T* hi0 = hi + (m0 + g) * stride + q * E;
-  const T* lo0 = lo + (m0 + g) * stride + q * E;
-  T* out0 = static_cast<T*>(a.out) + static_cast<int64_t>(rows[in0 ? m0 + g : 0]) * a.out_stride + col0 + q * 8;
-  T* out1 = static_cast<T*>(a.out) + static_cast<int64_t>(rows[in1 ? m0 + g + 8 : 0]) * a.out_stride + col0 + q * 8;
-  constexpr bool HELD = NCH <= 2 && sizeof(T) == 2;
-  StagedRows<T, HELD ? NCH : 1> held;
-  if constexpr (HELD) held.load(hi0, lo0, stride);
-  int stage = 0;
-  for (int step = 0; step < steps; ++step, out0 += NS, out1 += NS) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-    __syncthreads();  // the step's bytes are there, and the stage before it is free
-    load(step + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-    const uint8_t* es = smem + stage * kStage;
-    const uint8_t* bs = es + kBase;
-    if (m0 < tile.count) {
-#pragma unroll
-      for (int blk = 0; blk < NS / 32; ++blk) {
-        float acc[4][4] = {};
-        auto bf = [&](int j, int c) { return lds16(bs + tile_offset(blk * 32 + block_column(g) + 2 * j, NCH, c, q)); };
-        if constexpr (HELD) {
-          held.expand(acc, bf);
-        } else {
-#pragma unroll 2
-          for (int c = 0; c < NCH; ++c) expand_chunk<T>(acc, hi0, lo0, stride, c, bf);
-        }
-        float f0[8], f1[8];
-        block_values(acc, s0, s1, f0, f1);
-        if (step * NS + blk * 32 + q * 8 < cols) {
-          Eight<T> e0, e1;
-#pragma unroll
-          for (int i = 0; i < Eight<T>::W; ++i) {
-            const int w = (blk * 4 + q) * Eight<T>::W + i;  // 16-byte vector of the row
-            e0.u[i] = lds16(es + tile_offset(m0 + g, 2, w >> 2, w & 3));
-            e1.u[i] = lds16(es + tile_offset(m0 + g + 8, 2, w >> 2, w & 3));
-          }
-          if (in0) store_sum<T>(out0 + blk * 32, e0, with_base, f0);
-          if (in1) store_sum<T>(out1 + blk * 32, e1, with_base, f1);
-        }
-      }
-    }
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
-  }
-  asm volatile("cp.async.wait_all;" ::: "memory");
-}
-
-// Any alignment: B, base and out element by element. Grid as above.
-template <typename T>
-__global__ void __launch_bounds__(kLargeThreads) lora_expand_any_kernel(const LoraArgs a, LoraPlan plan,
-                                                                        const float* __restrict__ v, int splits,
-                                                                        int64_t v_rank, int64_t range, int b_width,
-                                                                        uint32_t* err) {
-  constexpr int E = 16 / sizeof(T), C = chunk_elems(sizeof(T));
-  constexpr int M = kLargeRows;
-  constexpr bool SCALED = std::is_same<T, __half>::value;
-  __shared__ int rows[M];
-  __shared__ float row_scale[M];
-  __shared__ unsigned row_max[M];
-  extern __shared__ __align__(128) uint8_t smem[];
-  griddep_launch_dependents();
-  griddep_wait();
-  const Tile tile = planned_tile(plan, rows);
-  if (tile.count == 0) return;
-  const int64_t col0 = blockIdx.y * range, col1 = min(a.n, col0 + range);
-  if (tile.group >= a.adapters) {
-    fill_rows<T>(a, tile, rows, col0, col1, false, err);
-    return;
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int vr = static_cast<int>(v_rank);
-  const int stride = vr + E;
-  T* hi = reinterpret_cast<T*>(smem);
-  T* lo = hi + M * stride;
-  const SumParts sum{v, rows, a.tokens * v_rank, splits, vr, a.scaling != nullptr ? a.scaling[tile.group] : 1.f};
-  stage_v<T, M>(tile, static_cast<int>(a.rank), vr, stride, hi, lo, reinterpret_cast<float*>(lo + M * stride), row_scale,
-                row_max, sum);
-  const int g = lane >> 2, q = lane & 3, m0 = warp * 16;
-  if (m0 >= tile.count) return;
-  const bool in0 = m0 + g < tile.count, in1 = m0 + g + 8 < tile.count;
-  const int64_t t0 = rows[in0 ? m0 + g : 0], t1 = rows[in1 ? m0 + g + 8 : 0];
-  const float s0 = SCALED ? row_scale[m0 + g] : 1.f, s1 = SCALED ? row_scale[m0 + g + 8] : 1.f;
-  const T* hi0 = hi + (m0 + g) * stride + q * E;
-  const T* lo0 = lo + (m0 + g) * stride + q * E;
-  const T* b = static_cast<const T*>(a.b) + static_cast<int64_t>(tile.group) * a.n * a.rank;
-  const T* base = static_cast<const T*>(a.base);
-  T* out = static_cast<T*>(a.out);
-  for (int64_t n0 = col0; n0 < col1; n0 += 32) {
-    float acc[4][4] = {};
-    for (int c = 0; c < vr / C; ++c) {
-      expand_chunk<T>(acc, hi0, lo0, stride, c, [&](int j, int k) {
-        const int64_t col = n0 + block_column(g) + 2 * j;
-        return load_chunk<T>(col < a.n ? b + col * a.rank : nullptr, k * C + q * E, a.rank, b_width);
-      });
-    }
-    float f0[8], f1[8];
-    block_values(acc, s0, s1, f0, f1);
-    const int64_t at = n0 + q * 8, left = a.n - at;
-    if (in0) store_each<T>(out + t0 * a.out_stride + at, base ? base + t0 * a.base_stride + at : nullptr, left, f0);
-    if (in1) store_each<T>(out + t1 * a.out_stride + at, base ? base + t1 * a.base_stride + at : nullptr, left, f1);
-  }
-}
-
-// ---- few tokens: one launch ------------------------------------------------------------
+// ---- clusters ----------------------------------------------------------------------------
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // 16 bytes to a cluster address; their arrival is counted by the mbarrier at `bar` in the same CTA.
@@ -813,13 +538,13 @@ __device__ __forceinline__ void push16(uint32_t addr, float4 v, uint32_t bar) {
                : "memory");
 }
 
+// ---- few tokens ----------------------------------------------------------------------------
 struct SmallWidths {  // elements that rows are aligned to: of x and A, of B; whole vectors of out and base
   int k, b;
   bool n;
 };
 
-// A cluster of CTAs (grid.x / tokens of them) takes the tile that row
-// blockIdx.x / cluster leads. Its CTA c shrinks part c of K (a warp a part of
+// A cluster of CTAs takes tile blockIdx.x / cluster. Its CTA c shrinks part c of K (a warp a part of
 // that), sends its sums to all CTAs of the cluster, and expands part c of the
 // columns. What such a launch takes is a chain of memory latencies (ids, x and
 // A, the exchange), so every load is issued as early as its address is known:
@@ -834,7 +559,8 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
   constexpr int M = kSmallRows, RB = 8 * NT;  // ranks of a pass
   constexpr int BATCH = NT == 2 ? 4 : NT == 4 ? 2 : 1;
   constexpr bool SCALED = std::is_same<T, __half>::value;
-  __shared__ int rows[M], scratch[9];
+  __shared__ int rows[M], scratch[10];
+  __shared__ __align__(16) int groups[kSmallTokens];
   __shared__ float row_scale[M];
   __shared__ unsigned row_max[M];
   __shared__ uint64_t received;
@@ -848,8 +574,8 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
   cluster_arrive();  // the barriers of the cluster's CTAs exist when all have arrived
   griddep_launch_dependents();
   griddep_wait();
-  const int lead = static_cast<int>(blockIdx.x) / cluster, part = static_cast<int>(blockIdx.x) % cluster;
-  const Tile tile = find_tile(a, lead, rows, scratch);
+  const int part = static_cast<int>(blockIdx.x) % cluster;
+  const Tile tile = find_tile(a, static_cast<int>(blockIdx.x) / cluster, rows, groups, scratch);
   if (tile.count == 0) {  // of the whole cluster
     cluster_wait();
     return;
@@ -868,8 +594,7 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
   float* parts = reinterpret_cast<float*>(smem);  // [cluster][M][vr]: the CTAs' parts of v
   T* hi = reinterpret_cast<T*>(smem + sizeof(float) * cluster * M * vr);
   T* lo = hi + M * stride;
-  float* staged = reinterpret_cast<float*>(lo + (sizeof(T) == 2 ? M * stride : 0));  // [M][vr] for fp16
-  auto* red = reinterpret_cast<float(*)[M][RB + 4]>(staged + (SCALED ? M * vr : 0));  // [kSmallWarps]
+  auto* red = reinterpret_cast<float(*)[M][RB + 4]>(lo + (sizeof(T) == 2 ? M * stride : 0));  // [kSmallWarps]
   if (t == 0) mbar_arrive_expect_tx(&received, static_cast<uint32_t>(cluster * tile.count * quads * 16));
   const bool in0 = g < tile.count, in1 = g + 8 < tile.count;
   const int64_t t0 = rows[in0 ? g : 0], t1 = rows[in1 ? g + 8 : 0];
@@ -951,19 +676,9 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
   Block next{};
   load_block(next, first);
   const float scale = a.scaling != nullptr ? a.scaling[tile.group] : 1.f;
-  if (!mbar_wait(&received, 0, err, ERR_WAIT_TIMEOUT_OTHER)) return;
-  // v: the parts of the cluster's CTAs in order
-  stage_v<T, M>(tile, rank, vr, stride, hi, lo, staged, row_scale, row_max, [&](int m, int r) {
-    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < cluster; ++k) {
-      const float4 w = *reinterpret_cast<const float4*>(parts + (k * M + m) * vr + r);
-      u.x += w.x;
-      u.y += w.y;
-      u.z += w.z;
-      u.w += w.w;
-    }
-    return make_float4(u.x * scale, u.y * scale, u.z * scale, u.w * scale);
-  });
+  const bool arrived = mbar_wait(&received, 0, err, ERR_WAIT_TIMEOUT_OTHER);
+  if (__syncthreads_or(!arrived)) return;
+  stage_v<T, M>(tile, rank, vr, stride, hi, lo, parts, vr, row_scale, row_max, SumParts<M>{parts, cluster, vr, scale});
   const float s0 = SCALED ? row_scale[g] : 1.f, s1 = SCALED ? row_scale[g + 8] : 1.f;
   const T* hi0 = hi + g * stride + q * E;
   const T* lo0 = lo + g * stride + q * E;
@@ -988,6 +703,303 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
   }
 }
 
+// ---- many tokens ---------------------------------------------------------------------------
+// A cluster of CTAs takes a tile of 64 rows that use the same adapter; CTA c of
+// it shrinks part c of K and expands part c of the columns. Both steps stream
+// through a ring of STAGES stages in shared memory: 128 bytes of K of x's rows
+// and A's (RANKS of them at a time), then 128 bytes of columns of base with
+// their rows of B. The first columns are on their way while the cluster's CTAs
+// exchange their parts of v. Warp w has rows 16 (w % 4) .. + 15; the two halves
+// of the warps share the 64-byte chunks of K and the blocks of 32 columns.
+// VR: ranks held by the expand step (a power of two of chunks). VEC: x, A, B,
+// base and out are whole aligned vectors; else elements are copied one by one.
+template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
+struct LargeShape {
+  static constexpr int E = 16 / sizeof(T), C = chunk_elems(sizeof(T));
+  static constexpr int M = kLargeRows;
+  static constexpr int SB = STEP;         // bytes of a row in a step
+  static constexpr int KS = SB / sizeof(T);    // elements of K, and columns, of a step
+  static constexpr int NCH = VR / C;           // chunks of a row of B
+  static constexpr int kRows = M * SB;         // bytes of the tile's rows in a stage
+  static constexpr int kShrink = kRows + RANKS * SB, kExpand = kRows + KS * NCH * 64;
+  static constexpr int kStage = kShrink > kExpand ? kShrink : kExpand;
+  static constexpr int stride = VR + E;
+  static constexpr size_t kStaged = static_cast<size_t>(sizeof(T) == 2 ? 2 : 1) * sizeof(T) * M * stride;
+  static_assert(kStaged >= sizeof(float) * M * (RANKS + 4), "the halves' sums fit where v is staged later");
+  static constexpr int PR = VR > RANKS && RANKS < 128 ? RANKS : VR;  // ranks of a row of an exchanged part
+  static size_t smem(int cluster) { return STAGES * kStage + kStaged + sizeof(float) * cluster * M * PR; }
+};
+
+template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
+__global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArgs a, LoraPlan plan, int cluster,
+                                                                   uint32_t* err) {
+  using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
+  constexpr int E = S::E, M = S::M, KS = S::KS, NCH = S::NCH, NT = RANKS / 8, stride = S::stride;
+  constexpr bool SCALED = std::is_same<T, __half>::value;
+  __shared__ int rows[M];
+  __shared__ float row_scale[M];
+  __shared__ unsigned row_max[M];
+  __shared__ uint64_t received;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  if (t == 0) {
+    mbar_init(&received, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  cluster_arrive();  // the barriers of the cluster's CTAs exist when all have arrived
+  griddep_launch_dependents();
+  griddep_wait();
+  const int part = static_cast<int>(blockIdx.x) % cluster;
+  const Tile tile = planned_tile(plan, static_cast<int>(blockIdx.x) / cluster, rows);
+  const int64_t col_steps = (a.n + KS - 1) / KS;
+  int s0i, s1i;
+  split_range(col_steps, cluster, part, &s0i, &s1i);
+  const int64_t col0 = static_cast<int64_t>(s0i) * KS, col1 = min(a.n, static_cast<int64_t>(s1i) * KS);
+  if (tile.count == 0 || tile.group >= a.adapters) {  // of the whole cluster
+    if (tile.count > 0) fill_rows<T>(a, tile, rows, col0, col1, VEC, err);
+    __syncwarp();
+    cluster_wait();
+    return;
+  }
+  const int rank = static_cast<int>(a.rank), quads = (rank + 3) / 4;
+  uint8_t* ring = smem;
+  T* hi = reinterpret_cast<T*>(smem + STAGES * S::kStage);
+  T* lo = hi + M * stride;
+  auto* halves = reinterpret_cast<float(*)[RANKS + 4]>(hi);  // until v is staged
+  float* parts = reinterpret_cast<float*>(smem + STAGES * S::kStage + S::kStaged);  // [cluster][M][PR]
+  if (t == 0) mbar_arrive_expect_tx(&received, static_cast<uint32_t>(cluster * tile.count * quads * 16));
+  const int g = lane >> 2, q = lane & 3;
+  const int m0 = (warp & 3) * 16, half = warp >> 2;
+  const bool busy = m0 < tile.count;
+  const uint32_t ring_at = smem_u32(ring);
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  // This thread's copies of a step: 16 bytes `vec` of every kRowStep-th row.
+  // Where they go does not change but for the stage, and the sources move on by
+  // a step's bytes: a copy costs a few instructions.
+  constexpr int kVecs = S::SB / 16, kRowStep = kLargeThreads / kVecs, kCopies = M / kRowStep, kChunks = S::SB / 64;
+  const int vec = t % kVecs, row0 = t / kVecs;
+  const uint32_t copy_at = tile_offset(row0, kChunks, vec >> 2, vec & 3);  // rows kRowStep apart have the same parity
+  static_assert(kRowStep % 2 == 0, "rows of a thread have one parity");
+  auto put = [&](uint32_t at, const T* from, int left) {  // `left` elements exist (none: zeros)
+    if constexpr (VEC) {
+      copy16(ring_at + at, from, left > 0 ? 16 : 0);
+    } else {
+      *reinterpret_cast<uint4*>(ring + at) = load_chunk<T>(left > 0 ? from : nullptr, 0, left, 1);
+    }
+  };
+
+  // ---- shrink
+  int k0, k1;
+  split_range((a.k + KS - 1) / KS, cluster, part, &k0, &k1);
+  const uint32_t my_part = smem_u32(parts + part * M * S::PR), bar = smem_u32(&received);
+  // a lane's operands in a stage: row m0 + g (and 8 further) of x, row g (and 8, 16, ... further) of A
+  constexpr int kHalfChunks = kChunks / 2;
+  const uint32_t x_at = tile_offset(m0 + g, kChunks, half * kHalfChunks, q), a_at = S::kRows + tile_offset(g, kChunks, half * kHalfChunks, q);
+  for (int r0 = 0; r0 < rank; r0 += RANKS) {
+    constexpr int kACopies = (RANKS + kRowStep - 1) / kRowStep;
+    const int64_t start = static_cast<int64_t>(k0) * KS + vec * E;
+    const T *xp[kCopies], *ap[kACopies];
+    bool x_ok[kCopies], a_ok[kACopies];
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const int r = row0 + kRowStep * i;
+      x_ok[i] = r < tile.count;
+      xp[i] = static_cast<const T*>(a.x) + static_cast<int64_t>(rows[x_ok[i] ? r : 0]) * a.x_stride + start;
+    }
+#pragma unroll
+    for (int i = 0; i < kACopies; ++i) {
+      const int r = r0 + row0 + kRowStep * i;
+      a_ok[i] = r < rank && row0 + kRowStep * i < RANKS;
+      ap[i] = static_cast<const T*>(a.a) + (static_cast<int64_t>(tile.group) * rank + (a_ok[i] ? r : 0)) * a.k + start;
+    }
+    int left = static_cast<int>(a.k - start), to_load = k1 - k0;
+    auto load = [&](uint32_t at) {
+      if (to_load > 0) {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          put(at + copy_at + i * kRowStep * S::SB, xp[i], x_ok[i] ? left : 0);
+          xp[i] += KS;
+        }
+#pragma unroll
+        for (int i = 0; i < kACopies; ++i) {
+          if (RANKS % kRowStep == 0 || row0 + kRowStep * i < RANKS)
+            put(at + S::kRows + copy_at + i * kRowStep * S::SB, ap[i], a_ok[i] ? left : 0);
+          ap[i] += KS;
+        }
+        left -= KS;
+      }
+      --to_load;
+      commit();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) load(i * S::kStage);
+    float acc[NT][4] = {};
+    uint32_t now = 0, free = (STAGES - 1) * S::kStage;  // the stage at hand, and the one before it
+    for (int step = k0; step < k1; ++step) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+      __syncthreads();  // the step's bytes are there, and the stage before it is free
+      load(free);
+      if (busy) {
+        const uint8_t* xs = ring + now + x_at;
+        const uint8_t* as = ring + now + a_at;
+#pragma unroll
+        for (int h = 0; h < kHalfChunks; ++h) {
+          // the next chunk: 64 bytes on, or where the swap of odd rows puts it
+          const int on = h == 0 ? 0 : static_cast<int>(tile_offset(g, kChunks, half * kHalfChunks + h, q)) -
+                                          static_cast<int>(tile_offset(g, kChunks, half * kHalfChunks, q));
+          const uint4 a0 = lds16(xs + on), a1 = lds16(xs + on + 8 * S::SB);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) Chunk<T>::mma(acc[j], a0, a1, lds16(as + on + j * 8 * S::SB));
+        }
+      }
+      free = now;
+      now = now + S::kStage == STAGES * S::kStage ? 0 : now + S::kStage;
+    }
+    // the two halves' sums, then this CTA's part to all CTAs of the cluster
+    auto each = [&](auto f) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        f(reinterpret_cast<float2*>(&halves[m0 + g][j * 8 + 2 * q]), acc[j][0], acc[j][1]);
+        f(reinterpret_cast<float2*>(&halves[m0 + g + 8][j * 8 + 2 * q]), acc[j][2], acc[j][3]);
+      }
+    };
+    if (busy && half == 1) each([](float2* p, float x, float y) { *p = make_float2(x, y); });
+    __syncthreads();
+    if (busy && half == 0) {
+      each([](float2* p, float x, float y) {
+        const float2 o = *p;
+        *p = make_float2(x + o.x, y + o.y);
+      });
+    }
+    if (r0 == 0) cluster_wait();
+    __syncthreads();
+    const int here = min(RANKS / 4, quads - r0 / 4);  // quads of this pass
+    for (int i = t; i < tile.count * here; i += kLargeThreads) {
+      const int m = i / here, r = i % here * 4;
+      const float4 u = *reinterpret_cast<const float4*>(&halves[m][r]);
+      const uint32_t dst = my_part + (m * S::PR + r0 + r) * 4;
+      for (int k = 0; k < cluster; ++k) push16(mapa_shared(dst, k), u, mapa_shared(bar, k));
+    }
+    __syncthreads();  // before the halves' sums and the ring are written again
+  }
+
+  // ---- expand
+  const bool with_base = a.base != nullptr;
+  const int cols = static_cast<int>(col1 - col0);
+  const T* bp[kCopies];
+  bool b_row_ok[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const int r = row0 + kRowStep * i;
+    b_row_ok[i] = r < tile.count;
+    bp[i] = static_cast<const T*>(a.base) + static_cast<int64_t>(rows[b_row_ok[i] ? r : 0]) * a.base_stride + col0 + vec * E;
+  }
+  // of B: 16 bytes w_vec of every kWStep-th row
+  constexpr int kWVecs = NCH * 4, kWStep = kLargeThreads / kWVecs, kWCopies = (KS + kWStep - 1) / kWStep;
+  static_assert(kWVecs <= kLargeThreads && kWStep % 2 == 0, "a row of B has at most one vector for each thread");
+  const int w_vec = t % kWVecs, w_row0 = t / kWVecs;
+  const T* wp = static_cast<const T*>(a.b) + (static_cast<int64_t>(tile.group) * a.n + col0 + w_row0) * rank + w_vec * E;
+  const uint32_t w_at = S::kRows + tile_offset(w_row0, NCH, w_vec >> 2, w_vec & 3);
+  const int w_left = rank - w_vec * E;
+  const int64_t w_step = static_cast<int64_t>(kWStep) * rank, w_on = static_cast<int64_t>(KS) * rank;
+  int cols_left = cols;
+  auto load = [&](uint32_t at) {
+    if (cols_left > 0) {
+      if (VEC && with_base) {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          put(at + copy_at + i * kRowStep * S::SB, bp[i], b_row_ok[i] ? cols_left - vec * E : 0);
+          bp[i] += KS;
+        }
+      }
+      const T* from = wp;
+#pragma unroll
+      for (int i = 0; i < kWCopies; ++i, from += w_step) {
+        const int r = w_row0 + kWStep * i;
+        if (KS % kWStep == 0 || r < KS) put(at + w_at + i * kWStep * NCH * 64, from, r < cols_left ? w_left : 0);
+      }
+      wp += w_on;
+    }
+    cols_left -= KS;
+    commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) load(i * S::kStage);
+  const float scale = a.scaling != nullptr ? a.scaling[tile.group] : 1.f;
+  const bool arrived = mbar_wait(&received, 0, err, ERR_WAIT_TIMEOUT_OTHER);
+  if (__syncthreads_or(!arrived)) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
+  stage_v<T, M>(tile, rank, VR, stride, hi, lo, parts, S::PR, row_scale, row_max, SumParts<M>{parts, cluster, S::PR, scale});
+  const bool in0 = m0 + g < tile.count, in1 = m0 + g + 8 < tile.count;
+  const float f0s = SCALED ? row_scale[m0 + g] : 1.f, f1s = SCALED ? row_scale[m0 + g + 8] : 1.f;
+  const T* hi0 = hi + (m0 + g) * stride + q * E;
+  const T* lo0 = lo + (m0 + g) * stride + q * E;
+  const int64_t t0 = rows[in0 ? m0 + g : 0], t1 = rows[in1 ? m0 + g + 8 : 0];
+  T* out0 = static_cast<T*>(a.out) + t0 * a.out_stride + col0 + q * 8;
+  T* out1 = static_cast<T*>(a.out) + t1 * a.out_stride + col0 + q * 8;
+  constexpr bool HELD = NCH <= 2 && sizeof(T) == 2;
+  StagedRows<T, HELD ? NCH : 1> held;
+  if constexpr (HELD) held.load(hi0, lo0, stride);
+  constexpr int BLOCKS = KS / 32;  // of a step: the halves of the warps share them, or take turns
+  const uint32_t b_at = S::kRows + tile_offset(block_column(g), NCH, 0, q);
+  const uint32_t e_at = (m0 + g) * S::SB;
+  uint32_t now = 0, free = (STAGES - 1) * S::kStage;
+  const int steps = s1i - s0i;
+  for (int step = 0; step < steps; ++step, out0 += KS, out1 += KS) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncthreads();  // the step's bytes are there, and the stage before it is free
+    load(free);
+    if (busy && (BLOCKS > 1 || (step & 1) == half)) {
+      constexpr int MINE = BLOCKS > 1 ? BLOCKS / 2 : 1;
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const int blk = BLOCKS > 1 ? half * MINE + i : 0;
+        const uint8_t* es = ring + now + e_at;
+        const uint8_t* bs = ring + now + b_at + blk * 32 * NCH * 64;
+        float acc[4][4] = {};
+        auto bf = [&](int j, int c) {  // chunk c of an odd row may be swapped
+          const int on = (NCH & 1) ? c * 64 : ((c ^ (g & 1)) - (g & 1)) * 64;
+          return lds16(bs + j * 2 * NCH * 64 + on);
+        };
+        if constexpr (HELD) {
+          held.expand(acc, bf);
+        } else {
+#pragma unroll 2
+          for (int c = 0; c < NCH; ++c) expand_chunk<T>(acc, hi0, lo0, stride, c, bf);
+        }
+        float f0[8], f1[8];
+        block_values(acc, f0s, f1s, f0, f1);
+        const int left = cols - step * KS - blk * 32 - q * 8;
+        if constexpr (VEC) {
+          if (left > 0) {
+            Eight<T> e0, e1;
+#pragma unroll
+            for (int k = 0; k < Eight<T>::W; ++k) {
+              const int w = (blk * 4 + q) * Eight<T>::W + k;  // 16-byte vector of the row; odd rows' chunks are swapped
+              const uint32_t off = ((w >> 2) ^ (g & 1)) * 64 + (w & 3) * 16;
+              e0.u[k] = lds16(es + off);
+              e1.u[k] = lds16(es + off + 8 * S::SB);
+            }
+            if (in0) store_sum<T>(out0 + blk * 32, e0, with_base, f0);
+            if (in1) store_sum<T>(out1 + blk * 32, e1, with_base, f1);
+          }
+        } else {
+          const T* base = static_cast<const T*>(a.base);
+          const int64_t at = col0 + step * KS + blk * 32 + q * 8;
+          if (in0) store_each<T>(out0 + blk * 32, with_base ? base + t0 * a.base_stride + at : nullptr, left, f0);
+          if (in1) store_each<T>(out1 + blk * 32, with_base ? base + t1 * a.base_stride + at : nullptr, left, f1);
+        }
+      }
+    }
+    free = now;
+    now = now + S::kStage == STAGES * S::kStage ? 0 : now + S::kStage;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 // ---- host ----------------------------------------------------------------------------
 namespace {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -995,29 +1007,17 @@ size_t round256(size_t v) { return (v + 255) / 256 * 256; }
 
 bool small_call(int64_t tokens) { return tokens <= kSmallTokens; }
 
-struct Launch {  // of many tokens
-  int64_t tiles;   // upper bound
-  int64_t likely;  // tiles to expect
-  int splits;
-  int64_t v_rank;
-  size_t v_bytes, perm_bytes, tile_bytes;
-  size_t total() const { return v_bytes + perm_bytes + tile_bytes + 256; }
+struct PlanBytes {  // of many tokens
+  int64_t tiles;  // upper bound
+  size_t perm, list;
+  size_t total() const { return perm + list + 256; }
 };
-
-Launch plan_launch(int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int dtype) {
-  const int esize = dtype == F32 ? 4 : 2;
-  Launch l{};
-  l.tiles = tokens / kLargeRows + std::min(tokens, adapters + 2);
-  l.likely = (tokens + kLargeRows - 1) / kLargeRows;
-  l.v_rank = padded_rank(rank, esize);
-  // about four CTAs for every SM, and at least four steps of 128 bytes for a CTA
-  const int64_t steps = (k * esize + 127) / 128;
-  const int64_t ctas = static_cast<int64_t>(num_sms()) * 4;
-  l.splits = static_cast<int>(std::min<int64_t>({16, std::max<int64_t>(1, steps / 4), std::max<int64_t>(1, ctas / l.likely)}));
-  l.v_bytes = round256(sizeof(float) * l.splits * tokens * l.v_rank);
-  l.perm_bytes = round256(sizeof(int) * tokens);
-  l.tile_bytes = round256(sizeof(int4) * l.tiles);
-  return l;
+PlanBytes plan_bytes(int64_t tokens, int64_t adapters) {
+  PlanBytes p{};
+  p.tiles = tokens / kLargeRows + std::min(tokens, adapters + 2);
+  p.perm = round256(sizeof(int) * tokens);
+  p.list = round256(sizeof(int4) * p.tiles);
+  return p;
 }
 
 template <typename... KArgs, typename... Args>
@@ -1066,17 +1066,19 @@ cudaError_t launch_small(const LoraArgs& a, cudaStream_t st) {
   const int64_t v_rank = padded_rank(a.rank, sizeof(T));
   const int kw = std::min(row_width<T>(a.x, a.k, a.tokens == 1 ? 0 : a.x_stride), row_width<T>(a.a, a.k, 0));
   const SmallWidths width{kw, row_width<T>(a.b, a.rank, 0), output_vectors<T>(a)};
-  // enough CTAs that a warp has about two chunks of K and two blocks of columns
+  // at most so many tiles, most of them there when the adapters are mixed
+  const int64_t tiles = std::min(a.tokens, a.tokens / kSmallRows + a.adapters + 2);
+  // enough CTAs that a warp has about two chunks of K and two blocks of
+  // columns, about one wave of them, and 16 KB of exchanged sums at most
   const int64_t chunks = (a.k + chunk_elems(sizeof(T)) - 1) / chunk_elems(sizeof(T));
   const int64_t want = std::max(chunks / (2 * kSmallWarps), a.n / (2 * 32 * kSmallWarps));
   int cluster = 1;
-  while (cluster < kMaxCluster && cluster < want && 2 * cluster * a.tokens <= 2 * num_sms() && 2 * cluster * v_rank <= 512)
+  while (cluster < kMaxCluster && cluster < want && 2 * cluster * tiles <= 4 * num_sms() && 2 * cluster * v_rank <= 512)
     cluster *= 2;
-  const size_t smem = kSmallRows * (sizeof(float) * v_rank * cluster + (sizeof(T) == 2 ? 2 : 1) * sizeof(T) * (v_rank + E) +
-                                    (std::is_same<T, __half>::value ? sizeof(float) * v_rank : 0));
+  const size_t smem = kSmallRows * (sizeof(float) * v_rank * cluster + (sizeof(T) == 2 ? 2 : 1) * sizeof(T) * (v_rank + E));
   auto launch = [&](auto* kernel, int nt) {
     const size_t red = sizeof(float) * kSmallWarps * kSmallRows * (8 * nt + 4);
-    return launch_grid(kernel, dim3(static_cast<unsigned>(a.tokens * cluster)), 256, cluster, smem + red, st, a, cluster,
+    return launch_grid(kernel, dim3(static_cast<unsigned>(tiles * cluster)), 256, cluster, smem + red, st, a, cluster,
                        width, v_rank, error_word_ptr());
   };
   const bool vec = width.k == E && width.b == E && width.n;
@@ -1085,63 +1087,57 @@ cudaError_t launch_small(const LoraArgs& a, cudaStream_t st) {
   return vec ? launch(lora_small_kernel<T, 8, true>, 8) : launch(lora_small_kernel<T, 8, false>, 8);
 }
 
+template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
+cudaError_t launch_shape(const LoraArgs& a, const PlanBytes& p, const LoraPlan& plan, cudaStream_t st) {
+  using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
+  // As many CTAs a tile as are resident at once with the tiles to expect (more
+  // of them only queue: 8192 tokens, 136 tiles, rank 32: 62 / 50 / 84 us for
+  // one, two, four), each with four steps of K at least.
+  auto* kernel = lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>;
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  const int64_t groups = std::min(a.tokens, a.adapters + 1);
+  const int64_t likely = std::max(groups, a.tokens / kLargeRows + groups / 2);
+  const int64_t steps = (a.k + S::KS - 1) / S::KS;
+  int cluster = 1;
+  while (cluster < kMaxCluster && 8 * cluster <= steps && S::smem(2 * cluster) <= 216 * 1024) {
+    const size_t smem = S::smem(2 * cluster);
+    if (const cudaError_t e = ensure_smem_attr(fn, smem + 4096); e != cudaSuccess) return e;
+    if (likely * 2 * cluster > static_cast<int64_t>(num_sms()) * cached_occupancy(fn, kLargeThreads, smem)) break;
+    cluster *= 2;
+  }
+  return launch_grid(lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>, dim3(static_cast<unsigned>(p.tiles * cluster)),
+                     kLargeThreads, cluster, S::smem(cluster), st, a, plan, cluster, error_word_ptr());
+}
+
 template <typename T>
 cudaError_t launch_large(const LoraArgs& a, void* ws, cudaStream_t st) {
-  constexpr int E = 16 / sizeof(T), STAGES = 4;
-  const Launch l = plan_launch(a.tokens, a.adapters, a.rank, a.k, a.dtype);
-  char* p = static_cast<char*>(ws);
-  float* v = reinterpret_cast<float*>(p);
-  LoraPlan plan{};
-  plan.perm = reinterpret_cast<int*>(p + l.v_bytes);
-  plan.tiles = reinterpret_cast<int4*>(p + l.v_bytes + l.perm_bytes);
-  plan.num_tiles = reinterpret_cast<int*>(p + l.v_bytes + l.perm_bytes + l.tile_bytes);
-  cudaError_t e = launch_grid(lora_plan_kernel, dim3(1), kPlanThreads, 0, sizeof(int) * static_cast<size_t>(a.adapters + 2),
-                              st, a, plan);
+  constexpr int E = 16 / sizeof(T), C = chunk_elems(sizeof(T));
+  const PlanBytes p = plan_bytes(a.tokens, a.adapters);
+  char* at = static_cast<char*>(ws);
+  const LoraPlan plan{reinterpret_cast<int*>(at), reinterpret_cast<int4*>(at + p.perm),
+                      reinterpret_cast<int*>(at + p.perm + p.list)};
+  const cudaError_t e = launch_grid(lora_plan_kernel, dim3(1), kPlanThreads, 0,
+                                    sizeof(int) * static_cast<size_t>(a.adapters + 2), st, a, plan);
   if (e != cudaSuccess) return e;
-
-  const bool vec_k = row_width<T>(a.x, a.k, a.x_stride) == E && row_width<T>(a.a, a.k, 0) == E;
-  auto shrink = [&](auto* kernel, auto* any, int nt, int stages) {
-    const dim3 grid(static_cast<unsigned>(l.tiles), static_cast<unsigned>(l.splits),
-                    static_cast<unsigned>((a.rank + 8 * nt - 1) / (8 * nt)));
-    return vec_k ? launch_grid(kernel, grid, kLargeThreads, 0, static_cast<size_t>(stages) * (kLargeRows + 8 * nt) * 128, st,
-                               a, plan, v, l.splits, l.v_rank)
-                 : launch_grid(any, grid, kLargeThreads, 0, 0, st, a, plan, v, l.splits, l.v_rank);
-  };
-  if (a.rank <= 16) {
-    e = shrink(lora_shrink_kernel<T, 2, STAGES>, lora_shrink_any_kernel<T, 2>, 2, STAGES);
-  } else if (a.rank <= 32) {
-    e = shrink(lora_shrink_kernel<T, 4, STAGES>, lora_shrink_any_kernel<T, 4>, 4, STAGES);
-  } else {
-    e = shrink(lora_shrink_kernel<T, 8, STAGES>, lora_shrink_any_kernel<T, 8>, 8, STAGES);
-  }
-  if (e != cudaSuccess) return e;
-
-  const int b_width = row_width<T>(a.b, a.rank, 0);
-  const int64_t unit = 128 / sizeof(T);  // columns of a step
-  const int64_t units = (a.n + unit - 1) / unit;
-  const int64_t ranges = std::min<int64_t>(units, std::max<int64_t>(1, num_sms() * 4 / l.likely));
-  const int64_t range = (units + ranges - 1) / ranges * unit;
-  const dim3 grid(static_cast<unsigned>(l.tiles), static_cast<unsigned>((a.n + range - 1) / range));
-  // hi and lo, and for fp16 the fp32 sums that they are made from
-  const size_t staged = kLargeRows * ((sizeof(T) == 2 ? 2 : 1) * sizeof(T) * (l.v_rank + E) +
-                                      (std::is_same<T, __half>::value ? sizeof(float) * l.v_rank : 0));
-  if (b_width == E && output_vectors<T>(a)) {
-    auto expand = [&](auto* kernel, int stages) {
-      const size_t stage = kLargeRows * 128 + unit * l.v_rank * sizeof(T);
-      return launch_grid(kernel, grid, kLargeThreads, 0, stages * stage + staged, st, a, plan, static_cast<const float*>(v),
-                         l.splits, l.v_rank, range, error_word_ptr());
-    };
-    const int64_t chunks = l.v_rank * static_cast<int64_t>(sizeof(T)) / 64;
-    if (chunks == 1) return expand(lora_expand_kernel<T, 1, 3>, 3);
-    if (chunks == 2) return expand(lora_expand_kernel<T, 2, 3>, 3);
-    if (chunks == 4) return expand(lora_expand_kernel<T, 4, 3>, 3);
-    if constexpr (sizeof(T) == 4) {
-      if (chunks == 16) return expand(lora_expand_kernel<T, 16, 2>, 2);
-    }
-    return expand(lora_expand_kernel<T, 8, 2>, 2);  // fp16: 217 KB with two stages
-  }
-  return launch_grid(lora_expand_any_kernel<T>, grid, kLargeThreads, 0, staged, st, a, plan, static_cast<const float*>(v),
-                     l.splits, l.v_rank, range, b_width, error_word_ptr());
+  const bool vec = row_width<T>(a.x, a.k, a.x_stride) == E && row_width<T>(a.a, a.k, 0) == E &&
+                   row_width<T>(a.b, a.rank, 0) == E && output_vectors<T>(a);
+#define TFO_LORA(RANKS, VR, STEP, STAGES)                                        \
+  (vec ? launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, true>(a, p, plan, st) \
+       : launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, false>(a, p, plan, st))
+  // 256 bytes of a row a step: fewer barriers, one or two CTAs on an SM. 8192
+  // tokens (136 tiles) 61 -> 50 us; 1024 tokens over 32 adapters (33 tiles, four
+  // CTAs each instead of two) 19 -> 24 us.
+  const int64_t groups = std::min(a.tokens, a.adapters + 1);
+  const bool wide = std::max(groups, a.tokens / kLargeRows + groups / 2) * 3 >= num_sms() * 2;
+  if (a.rank <= 16 && wide) return TFO_LORA(16, 16, 256, 3);
+  if (a.rank <= 32 && wide) return TFO_LORA(32, 32, 256, 3);
+  if (a.rank <= 64 && wide) return TFO_LORA(64, 64, 256, 3);
+  if (a.rank <= 16) return TFO_LORA(16, 16, 128, 4);
+  if (a.rank <= 32) return TFO_LORA(32, 32, 128, 4);
+  if (a.rank <= 64) return TFO_LORA(64, 64, 128, 4);
+  if (a.rank <= 128) return TFO_LORA(128, 128, 128, 3);
+  return TFO_LORA(128, 256, 128, 2);
+#undef TFO_LORA
 }
 
 template <typename T>
@@ -1150,8 +1146,8 @@ cudaError_t launch_type(const LoraArgs& a, void* ws, cudaStream_t st) {
 }
 }  // namespace
 
-size_t lora_workspace_bytes(int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int dtype) {
-  return small_call(tokens) ? 0 : plan_launch(tokens, adapters, rank, k, dtype).total();
+size_t lora_workspace_bytes(int64_t tokens, int64_t adapters) {
+  return small_call(tokens) ? 0 : plan_bytes(tokens, adapters).total();
 }
 
 cudaError_t lora_launch(const LoraArgs& a, void* ws, cudaStream_t st) {

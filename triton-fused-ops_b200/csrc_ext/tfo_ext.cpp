@@ -423,7 +423,7 @@ py::object lora(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, c
   const auto st = at::cuda::getCurrentCUDAStream(x.device().index()).stream();
   at::Tensor y = out.has_value() ? *out : at::empty({tokens, n}, x.options().requires_grad(false));
   const int dtype = dtype_code(x.scalar_type());
-  at::Tensor ws = workspace(tfo_lora_workspace_bytes(tokens, adapters, rank, k, dtype), x.device(), st);
+  at::Tensor ws = workspace(tfo_lora_workspace_bytes(tokens, adapters), x.device(), st);
   check(tfo_lora(x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ids.data_ptr(), pos_code(ids.scalar_type()),
                  scaling.has_value() ? scaling->data_ptr<float>() : nullptr,
                  base.has_value() ? base->data_ptr() : nullptr, base.has_value() ? base->stride(0) : 0, y.data_ptr(),

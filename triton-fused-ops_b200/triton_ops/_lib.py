@@ -136,7 +136,7 @@ _SIGNATURES = {
          _c_vp, _c_vp, _c_vp, _c_vp, *_HEADS_SIZES, ctypes.c_double, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_size,
          _c_vp],
     ),
-    "tfo_lora_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i64, _c_int]),
+    "tfo_lora_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
     "tfo_lora": (
         _c_int,
         [_c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64,
