@@ -138,7 +138,6 @@ struct LoraPlan {  // of many tokens, in the workspace
   int* perm;       // rows, by group
   int4* tiles;     // {group, first, count, 0}; first indexes perm
   int* num_tiles;
-  int tile_rows;
 };
 
 // Group of a row: its adapter, `adapters` for none, `adapters` + 1 for an id past the end.
@@ -260,7 +259,7 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs 
   for (int first = 0; first < groups; first += kPlanThreads) {
     const int g = first + t;
     const int rows = g < groups ? bins[g] : 0;
-    const int tiles = (rows + plan.tile_rows - 1) / plan.tile_rows;
+    const int tiles = (rows + kLargeRows - 1) / kLargeRows;
     const int r = warp_scan(rows, lane), n = warp_scan(tiles, lane);
     if (lane == 31) {
       sum_rows[warp] = r;
@@ -278,7 +277,7 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const LoraArgs 
     if (g < groups) {
       bins[g] = row0;
       for (int i = 0; i < tiles; ++i)
-        plan.tiles[tile0 + i] = make_int4(g, row0 + i * plan.tile_rows, min(plan.tile_rows, rows - i * plan.tile_rows), 0);
+        plan.tiles[tile0 + i] = make_int4(g, row0 + i * kLargeRows, min(kLargeRows, rows - i * kLargeRows), 0);
     }
     __syncthreads();
     if (t == 0) {
@@ -383,15 +382,15 @@ __device__ __forceinline__ void fill_rows(const LoraArgs& a, const Tile& tile, c
   }
 }
 
-// Stages the tile's v as operands in shared memory: at(m, r, false) gets the
-// four values of row m from rank r on in T, at(m, r, true) (16-bit types) what
-// is left of them. sum(m, r) gives the four, summed and scaled. fp16 rows are
-// scaled by a power of two to below 2 (row_scale takes it back; `sums`,
-// [M][sums_stride], holds them meanwhile and may be what sum reads); rows past
-// the tile and ranks past the end are zero.
-template <typename T, int M, typename At, typename Sum>
-__device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, At at, float* sums, int sums_stride,
-                                        float* row_scale, unsigned* row_max, Sum sum) {
+// Stages the tile's v as operands in shared memory: hi and lo (16-bit types;
+// fp32 as it is), [M][stride] elements. sum(m, r) gives four neighbouring
+// values of row m, summed and scaled. fp16 rows are scaled by a power of two
+// to below 2 (row_scale takes it back; `sums`, [M][sums_stride], holds them meanwhile
+// and may be what sum(m, r) reads); rows past the tile and ranks past the end
+// are zero.
+template <typename T, int M, typename Sum>
+__device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int stride, T* hi, T* lo, float* sums,
+                                        int sums_stride, float* row_scale, unsigned* row_max, Sum sum) {
   constexpr bool SPLIT = sizeof(T) == 2;
   constexpr bool SCALED = std::is_same<T, __half>::value;
   const int quads = vr / 4, threads = blockDim.x;
@@ -400,19 +399,15 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, At a
     __syncthreads();
   }
   auto put = [&](int m, int r, const float (&t)[4], float down) {
-    alignas(16) T h[4], l[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float x = SCALED ? t[j] * down : t[j];
-      h[j] = Ty<T>::from_f(x);
-      const float hf = Ty<T>::to_f(h[j]);
-      l[j] = Ty<T>::from_f(fabsf(hf) <= 3.402823466e38f ? x - hf : 0.f);  // infinities are all in hi
-    }
-    if constexpr (SPLIT) {
-      *reinterpret_cast<uint2*>(at(m, r, false)) = *reinterpret_cast<const uint2*>(h);
-      *reinterpret_cast<uint2*>(at(m, r, true)) = *reinterpret_cast<const uint2*>(l);
-    } else {
-      *reinterpret_cast<uint4*>(at(m, r, false)) = *reinterpret_cast<const uint4*>(h);
+      const T h = Ty<T>::from_f(x);
+      hi[m * stride + r + j] = h;
+      if constexpr (SPLIT) {
+        const float hf = Ty<T>::to_f(h);
+        lo[m * stride + r + j] = Ty<T>::from_f(fabsf(hf) <= 3.402823466e38f ? x - hf : 0.f);  // infinities are all in hi
+      }
     }
   };
 #pragma unroll 2
@@ -453,12 +448,6 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, At a
     __syncthreads();
   }
 }
-// Staged rows one after the other, `stride` elements apart, hi and lo.
-template <typename T> struct PlainRows {
-  T *hi, *lo;
-  int stride;
-  __device__ T* operator()(int m, int r, bool low) const { return (low ? lo : hi) + m * stride + r; }
-};
 
 // The parts of v that a cluster's CTAs have sent, [cluster][M][stride], added in order.
 template <int M> struct SumParts {
@@ -689,7 +678,7 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
   const float scale = a.scaling != nullptr ? a.scaling[tile.group] : 1.f;
   const bool arrived = mbar_wait(&received, 0, err, ERR_WAIT_TIMEOUT_OTHER);
   if (__syncthreads_or(!arrived)) return;
-  stage_v<T, M>(tile, rank, vr, PlainRows<T>{hi, lo, stride}, parts, vr, row_scale, row_max, SumParts<M>{parts, cluster, vr, scale});
+  stage_v<T, M>(tile, rank, vr, stride, hi, lo, parts, vr, row_scale, row_max, SumParts<M>{parts, cluster, vr, scale});
   const float s0 = SCALED ? row_scale[g] : 1.f, s1 = SCALED ? row_scale[g + 8] : 1.f;
   const T* hi0 = hi + g * stride + q * E;
   const T* lo0 = lo + g * stride + q * E;
@@ -943,7 +932,7 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
     asm volatile("cp.async.wait_all;" ::: "memory");
     return;
   }
-  stage_v<T, M>(tile, rank, VR, PlainRows<T>{hi, lo, stride}, parts, S::PR, row_scale, row_max, SumParts<M>{parts, cluster, S::PR, scale});
+  stage_v<T, M>(tile, rank, VR, stride, hi, lo, parts, S::PR, row_scale, row_max, SumParts<M>{parts, cluster, S::PR, scale});
   const bool in0 = m0 + g < tile.count, in1 = m0 + g + 8 < tile.count;
   const float f0s = SCALED ? row_scale[m0 + g] : 1.f, f1s = SCALED ? row_scale[m0 + g + 8] : 1.f;
   const T* hi0 = hi + (m0 + g) * stride + q * E;
@@ -1011,301 +1000,6 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// ---- many tokens, 16-bit types: tcgen05 --------------------------------------------------
-// The same division of work with tiles of 128 rows on the 5th-generation tensor
-// cores: x and A (then B) are copied into 128-byte-swizzled K-major tiles, one
-// thread issues the products, v and the outputs' products accumulate in tensor
-// memory. There a row is a lane: thread (quarter of the warp, lane) has one row
-// and half of the step's 64 columns, adds base (loaded a step ahead) and stores.
-// v is staged as the operand [hi | lo]: its products with B are two accumulating
-// series on the same tile of B.
-template <typename T, int RANKS, int STAGES>
-struct TensorShape {
-  static constexpr int M = 128, NS = 64;             // rows of a tile, columns of an expand step
-  static constexpr int kX = M * 128;                 // bytes of x in a stage
-  static constexpr int kShrink = kX + RANKS * 128;
-  static constexpr int kBlocks = (RANKS + 63) / 64;  // 128-byte blocks of a row of B
-  static constexpr int kExpand = kBlocks * NS * 128;
-  static constexpr int kStage = ((kShrink > kExpand ? kShrink : kExpand) + 1023) / 1024 * 1024;
-  static constexpr bool kShared = RANKS <= 32;       // hi and lo share one 128-byte block
-  static constexpr int kV = (kShared ? 1 : 2 * kBlocks) * M * 128;
-  static size_t smem(int cluster) { return 1024 + STAGES * kStage + kV + sizeof(float) * cluster * M * RANKS; }
-  static constexpr int kTmemCols = 128;              // v (up to 128 ranks), then two accumulators of 64 columns
-};
-
-// 16-byte vector `vec` of row `row` in a tile of 128-byte rows with the 128-byte swizzle.
-__device__ __forceinline__ uint32_t swizzled(int row, int vec) {
-  return static_cast<uint32_t>(row * 128 + ((vec ^ (row & 7)) << 4));
-}
-
-template <typename T, int RANKS, int STAGES>
-__global__ void __launch_bounds__(256) lora_tensor_kernel(const LoraArgs a, LoraPlan plan, int cluster, uint32_t* err) {
-  using S = TensorShape<T, RANKS, STAGES>;
-  constexpr int E = 8, M = S::M, NS = S::NS, KS = 64;
-  constexpr bool SCALED = std::is_same<T, __half>::value;
-  constexpr int FMT = SCALED ? 0 : 1;
-  __shared__ int rows[M];
-  __shared__ float row_scale[M];
-  __shared__ unsigned row_max[M];
-  __shared__ uint64_t received, used[STAGES], full[2];
-  __shared__ uint32_t tmem_slot;
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  if (t == 0) {
-    mbar_init(&received, 1);
-    for (int i = 0; i < STAGES; ++i) mbar_init(&used[i], 1);
-    mbar_init(&full[0], 1);
-    mbar_init(&full[1], 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
-  cluster_arrive();  // the barriers of the cluster's CTAs exist when all have arrived
-  griddep_launch_dependents();
-  griddep_wait();
-  const int part = static_cast<int>(blockIdx.x) % cluster;
-  const Tile tile = planned_tile(plan, static_cast<int>(blockIdx.x) / cluster, rows);
-  int n0i, n1i;
-  split_range((a.n + NS - 1) / NS, cluster, part, &n0i, &n1i);
-  const int64_t col0 = static_cast<int64_t>(n0i) * NS, col1 = min(a.n, static_cast<int64_t>(n1i) * NS);
-  if (tile.count == 0 || tile.group >= a.adapters) {  // of the whole cluster
-    if (tile.count > 0) fill_rows<T>(a, tile, rows, col0, col1, true, err);
-    __syncwarp();
-    cluster_wait();
-    return;
-  }
-  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // the same place in every CTA
-  uint8_t* v_op = smem + STAGES * S::kStage;
-  float* parts = reinterpret_cast<float*>(v_op + S::kV);  // [cluster][M][RANKS]
-  const int rank = static_cast<int>(a.rank), quads = (rank + 3) / 4;
-  if (t == 0) mbar_arrive_expect_tx(&received, static_cast<uint32_t>(cluster * tile.count * quads * 16));
-  __syncwarp();
-  if (warp == 0) {
-    tmem_alloc(&tmem_slot, S::kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  const uint32_t ring = smem_u32(smem);
-  auto commit_copies = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-  bool ok = true;  // a wait that runs out: the CTA goes through its loops without further waits and leaves
-  auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t bit) {
-    ok = ok && mbar_wait(bar, parity, err, bit);
-    __syncwarp();
-  };
-
-  // ---- shrink: v[128, RANKS] in tensor memory
-  int k0, k1;
-  split_range((a.k + KS - 1) / KS, cluster, part, &k0, &k1);
-  const int vec = t & 7, row0 = t >> 3;  // this thread's 16 bytes of every 32nd row
-  constexpr int kACopies = (RANKS + 31) / 32;
-  {
-    const int64_t start = static_cast<int64_t>(k0) * KS + vec * E;
-    const T *xp[4], *ap[kACopies];
-    bool x_ok[4], a_ok[kACopies];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = row0 + 32 * i;
-      x_ok[i] = r < tile.count;
-      xp[i] = static_cast<const T*>(a.x) + static_cast<int64_t>(rows[x_ok[i] ? r : 0]) * a.x_stride + start;
-    }
-#pragma unroll
-    for (int i = 0; i < kACopies; ++i) {
-      const int r = row0 + 32 * i;
-      a_ok[i] = r < rank;
-      ap[i] = static_cast<const T*>(a.a) + (static_cast<int64_t>(tile.group) * rank + (a_ok[i] ? r : 0)) * a.k + start;
-    }
-    const uint32_t copy_at = ring + swizzled(row0, vec);  // rows 32 apart are swizzled alike
-    int left = static_cast<int>(a.k - start), to_load = k1 - k0;
-    auto load = [&](int stage) {
-      if (to_load > 0) {
-        const uint32_t at = copy_at + stage * S::kStage;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          copy16(at + i * 32 * 128, xp[i], x_ok[i] && left > 0 ? 16 : 0);
-          xp[i] += KS;
-        }
-#pragma unroll
-        for (int i = 0; i < kACopies; ++i) {
-          if (RANKS % 32 == 0 || row0 < RANKS) copy16(at + S::kX + i * 32 * 128, ap[i], a_ok[i] && left > 0 ? 16 : 0);
-          ap[i] += KS;
-        }
-        left -= KS;
-      }
-      --to_load;
-      commit_copies();
-    };
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) load(i);
-    constexpr uint32_t idesc = make_idesc(1, FMT, FMT, false, false, M, RANKS);
-    int stage = 0, prev = STAGES - 1;
-    uint32_t prev_parity = 1;  // of the use of stage `prev` by the step before
-    const int steps = k1 - k0;
-    for (int i = 0; i < steps; ++i) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-      fence_proxy_async_smem();
-      __syncthreads();
-      if (t == 0) {
-        tc_fence_after();
-        const uint32_t at = ring + stage * S::kStage;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma<MmaKind::F16>(tmem, smem_desc_kmajor_sw128(at + k * 32), smem_desc_kmajor_sw128(at + S::kX + k * 32), idesc,
-                             i > 0 || k > 0);
-        umma_commit(&used[stage]);
-      }
-      if (i > 0) wait(&used[prev], prev_parity, ERR_WAIT_TIMEOUT_MMA);
-      load(prev);
-      prev = stage;
-      if (stage == 0) prev_parity ^= 1;
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
-    }
-    wait(&used[prev], prev_parity, ERR_WAIT_TIMEOUT_MMA);
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    tc_fence_after();
-  }
-  const int quarter = warp & 3, half = warp >> 2;
-  const int m = quarter * 32 + lane;  // this thread's row
-  const bool row_ok = m < tile.count;
-  const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  cluster_wait();
-  {
-    // this CTA's part of v to all CTAs of the cluster: 16 ranks at a time, the halves in turn
-    const uint32_t dst = smem_u32(parts + (part * M + m) * RANKS), bar = smem_u32(&received);
-#pragma unroll
-    for (int c = 0; c < RANKS / 16; ++c) {
-      if ((c & 1) != half) continue;
-      uint32_t r[16];
-      tmem_ld16(lanes + c * 16, r);
-      tmem_ld_wait();
-      tmem_ld_fence(r);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (row_ok && c * 4 + j < quads) {
-          const float4 u = make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
-                                       __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
-          for (int k = 0; k < cluster; ++k) push16(mapa_shared(dst + (c * 4 + j) * 16, k), u, mapa_shared(bar, k));
-        }
-      }
-    }
-    tc_fence_before();
-  }
-
-  // ---- expand
-  const int cols = static_cast<int>(col1 - col0), steps = n1i - n0i;
-  constexpr int kVecs = RANKS / 8, kRowsAtOnce = 256 / kVecs, kBCopies = (NS + kRowsAtOnce - 1) / kRowsAtOnce;
-  const int b_vec = t % kVecs, b_row0 = t / kVecs;
-  const T* bp = static_cast<const T*>(a.b) + (static_cast<int64_t>(tile.group) * a.n + col0 + b_row0) * rank + b_vec * E;
-  const bool b_in = b_vec * E < rank;
-  const int64_t b_skip = static_cast<int64_t>(kRowsAtOnce) * rank, b_on = static_cast<int64_t>(NS) * rank;
-  int cols_left = cols;
-  auto load = [&](int stage) {
-    if (cols_left > 0) {
-      const uint32_t at = ring + stage * S::kStage + (b_vec >> 3) * NS * 128;
-      const T* from = bp;
-#pragma unroll
-      for (int i = 0; i < kBCopies; ++i, from += b_skip) {
-        const int r = b_row0 + kRowsAtOnce * i;
-        if (NS % kRowsAtOnce == 0 || r < NS) copy16(at + swizzled(r, b_vec & 7), from, b_in && r < cols_left ? 16 : 0);
-      }
-      bp += b_on;
-    }
-    cols_left -= NS;
-    commit_copies();
-  };
-  __syncthreads();  // v has been read, and no copy is on its way into the ring
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) load(i);
-  const float scale = a.scaling != nullptr ? a.scaling[tile.group] : 1.f;
-  const bool with_base = a.base != nullptr;
-  const int64_t token = rows[row_ok ? m : 0];
-  const T* base = static_cast<const T*>(a.base) + token * a.base_stride + col0 + half * 32;
-  T* out = static_cast<T*>(a.out) + token * a.out_stride + col0 + half * 32;
-  Eight<T> ahead[4];
-  int to_base = cols - half * 32;  // columns left from this thread's first on, for the next load of base
-  auto load_base = [&] {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (with_base && row_ok && to_base > j * 8) load_eight(ahead[j], base + j * 8);
-    }
-    base += NS;
-    to_base -= NS;
-  };
-  wait(&received, 0, ERR_WAIT_TIMEOUT_OTHER);
-  stage_v<T, M>(
-      tile, rank, RANKS,
-      [&](int row, int r, bool low) {
-        const int block = (r >> 6) + (low && !S::kShared ? S::kBlocks : 0);
-        const int v16 = ((r & 63) >> 3) + (low && S::kShared ? 4 : 0);
-        return reinterpret_cast<T*>(v_op + block * M * 128 + swizzled(row, v16)) + (r & 7);
-      },
-      parts, RANKS, row_scale, row_max, SumParts<M>{parts, cluster, RANKS, scale});
-  fence_proxy_async_smem();
-  const float up = SCALED ? row_scale[m] : 1.f;
-  constexpr uint32_t idesc = make_idesc(1, FMT, FMT, false, false, M, NS);
-  const int k16 = (rank + 15) / 16;
-  int left = cols - half * 32;  // columns of this thread's row that are still to be stored
-  int stage = 0;
-  for (int i = 0; i <= steps; ++i) {
-    if (i < steps) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-      fence_proxy_async_smem();
-    }
-    __syncthreads();
-    if (i < steps && t == 0) {
-      tc_fence_after();
-      const uint32_t b_at = ring + stage * S::kStage, v_at = smem_u32(v_op), d = tmem + (i & 1) * NS;
-      for (int low = 0; low < 2; ++low) {
-        for (int k = 0; k < k16; ++k) {
-          const int block = (k >> 2) + (low && !S::kShared ? S::kBlocks : 0);
-          const int in = (k & 3) * 32 + (low && S::kShared ? 64 : 0);
-          umma<MmaKind::F16>(d, smem_desc_kmajor_sw128(v_at + block * M * 128 + in),
-                             smem_desc_kmajor_sw128(b_at + (k >> 2) * NS * 128 + (k & 3) * 32), idesc, low > 0 || k > 0);
-        }
-      }
-      umma_commit(&full[i & 1]);
-    }
-    Eight<T> now[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) now[j] = ahead[j];
-    if (i < steps) load_base();
-    if (i > 0) {
-      const int p = i - 1;
-      wait(&full[p & 1], (p >> 1) & 1, ERR_WAIT_TIMEOUT_EPILOGUE);
-      tc_fence_after();
-      if (quarter * 32 < tile.count) {
-        uint32_t r[2][16];
-        tmem_ld16(lanes + (p & 1) * NS + half * 32, r[0]);
-        tmem_ld16(lanes + (p & 1) * NS + half * 32 + 16, r[1]);
-        tmem_ld_wait();
-        tmem_ld_fence(r[0]);
-        tmem_ld_fence(r[1]);
-        if (row_ok) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float f[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(r[j >> 1][(j & 1) * 8 + k]) * up;
-            if (left > j * 8) store_sum<T>(out + j * 8, now[j], with_base, f);
-          }
-        }
-        tc_fence_before();
-      }
-      out += NS;
-      left -= NS;
-    }
-    load(stage == 0 ? STAGES - 1 : stage - 1);
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
-  }
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncthreads();
-  if (warp == 0) {
-    tc_fence_after();
-    tmem_dealloc(tmem, S::kTmemCols);
-  }
-}
-
 // ---- host ----------------------------------------------------------------------------
 namespace {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -1318,7 +1012,7 @@ struct PlanBytes {  // of many tokens
   size_t perm, list;
   size_t total() const { return perm + list + 256; }
 };
-PlanBytes plan_bytes(int64_t tokens, int64_t adapters) {  // for the lower tiles, of which there are more
+PlanBytes plan_bytes(int64_t tokens, int64_t adapters) {
   PlanBytes p{};
   p.tiles = tokens / kLargeRows + std::min(tokens, adapters + 2);
   p.perm = round256(sizeof(int) * tokens);
@@ -1393,41 +1087,26 @@ cudaError_t launch_small(const LoraArgs& a, cudaStream_t st) {
   return vec ? launch(lora_small_kernel<T, 8, true>, 8) : launch(lora_small_kernel<T, 8, false>, 8);
 }
 
-// Tiles to expect: one for each group at least, and half a tile of each is empty.
-int64_t likely_tiles(const LoraArgs& a, int tile_rows) {
-  const int64_t groups = std::min(a.tokens, a.adapters + 1);
-  return std::max(groups, a.tokens / tile_rows + groups / 2);
-}
-
-// As many CTAs a tile as are resident at once with the tiles to expect (more of
-// them only queue: 8192 tokens, 136 tiles of 64, rank 32: 62 / 50 / 84 us for
-// one, two, four), each with four of the `steps` of K at least.
-template <typename Smem>
-cudaError_t launch_tiles(void (*kernel)(LoraArgs, LoraPlan, int, uint32_t*), Smem smem, int64_t steps, int64_t bound,
-                         const LoraArgs& a, const LoraPlan& plan, cudaStream_t st) {
+template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
+cudaError_t launch_shape(const LoraArgs& a, const PlanBytes& p, const LoraPlan& plan, cudaStream_t st) {
+  using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
+  // As many CTAs a tile as are resident at once with the tiles to expect (more
+  // of them only queue: 8192 tokens, 136 tiles, rank 32: 62 / 50 / 84 us for
+  // one, two, four), each with four steps of K at least.
+  auto* kernel = lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>;
   const void* fn = reinterpret_cast<const void*>(kernel);
-  const int64_t likely = likely_tiles(a, plan.tile_rows);
+  const int64_t groups = std::min(a.tokens, a.adapters + 1);
+  const int64_t likely = std::max(groups, a.tokens / kLargeRows + groups / 2);
+  const int64_t steps = (a.k + S::KS - 1) / S::KS;
   int cluster = 1;
-  while (cluster < kMaxCluster && 8 * cluster <= steps && smem(2 * cluster) <= 216 * 1024) {
-    const size_t bytes = smem(2 * cluster);
-    if (const cudaError_t e = ensure_smem_attr(fn, bytes + 4096); e != cudaSuccess) return e;
-    if (likely * 2 * cluster > static_cast<int64_t>(num_sms()) * cached_occupancy(fn, kLargeThreads, bytes)) break;
+  while (cluster < kMaxCluster && 8 * cluster <= steps && S::smem(2 * cluster) <= 216 * 1024) {
+    const size_t smem = S::smem(2 * cluster);
+    if (const cudaError_t e = ensure_smem_attr(fn, smem + 4096); e != cudaSuccess) return e;
+    if (likely * 2 * cluster > static_cast<int64_t>(num_sms()) * cached_occupancy(fn, kLargeThreads, smem)) break;
     cluster *= 2;
   }
-  return launch_grid(kernel, dim3(static_cast<unsigned>(bound * cluster)), kLargeThreads, cluster, smem(cluster), st, a, plan,
-                     cluster, error_word_ptr());
-}
-
-template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
-cudaError_t launch_shape(const LoraArgs& a, int64_t bound, const LoraPlan& plan, cudaStream_t st) {
-  using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
-  return launch_tiles(lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>, S::smem, (a.k + S::KS - 1) / S::KS, bound, a, plan, st);
-}
-
-template <typename T, int RANKS, int STAGES>
-cudaError_t launch_tensor(const LoraArgs& a, int64_t bound, const LoraPlan& plan, cudaStream_t st) {
-  using S = TensorShape<T, RANKS, STAGES>;
-  return launch_tiles(lora_tensor_kernel<T, RANKS, STAGES>, S::smem, (a.k + 63) / 64, bound, a, plan, st);
+  return launch_grid(lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>, dim3(static_cast<unsigned>(p.tiles * cluster)),
+                     kLargeThreads, cluster, S::smem(cluster), st, a, plan, cluster, error_word_ptr());
 }
 
 template <typename T>
@@ -1435,31 +1114,21 @@ cudaError_t launch_large(const LoraArgs& a, void* ws, cudaStream_t st) {
   constexpr int E = 16 / sizeof(T), C = chunk_elems(sizeof(T));
   const PlanBytes p = plan_bytes(a.tokens, a.adapters);
   char* at = static_cast<char*>(ws);
-  const bool vec = row_width<T>(a.x, a.k, a.x_stride) == E && row_width<T>(a.a, a.k, 0) == E &&
-                   row_width<T>(a.b, a.rank, 0) == E && output_vectors<T>(a);
-  static const int w_ = getenv("TFO_W") ? atoi(getenv("TFO_W")) : 0;
-  const bool tensor = sizeof(T) == 2 && vec && a.rank <= 128 && w_ == 0;
   const LoraPlan plan{reinterpret_cast<int*>(at), reinterpret_cast<int4*>(at + p.perm),
-                      reinterpret_cast<int*>(at + p.perm + p.list), tensor ? 128 : kLargeRows};
-  const int64_t bound = a.tokens / plan.tile_rows + std::min(a.tokens, a.adapters + 2);
+                      reinterpret_cast<int*>(at + p.perm + p.list)};
   const cudaError_t e = launch_grid(lora_plan_kernel, dim3(1), kPlanThreads, 0,
                                     sizeof(int) * static_cast<size_t>(a.adapters + 2), st, a, plan);
   if (e != cudaSuccess) return e;
-  if constexpr (sizeof(T) == 2) {
-    if (tensor) {
-      if (a.rank <= 16) return launch_tensor<T, 16, 3>(a, bound, plan, st);
-      if (a.rank <= 32) return launch_tensor<T, 32, 3>(a, bound, plan, st);
-      if (a.rank <= 64) return launch_tensor<T, 64, 3>(a, bound, plan, st);
-      return launch_tensor<T, 128, 2>(a, bound, plan, st);
-    }
-  }
+  const bool vec = row_width<T>(a.x, a.k, a.x_stride) == E && row_width<T>(a.a, a.k, 0) == E &&
+                   row_width<T>(a.b, a.rank, 0) == E && output_vectors<T>(a);
 #define TFO_LORA(RANKS, VR, STEP, STAGES)                                        \
-  (vec ? launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, true>(a, bound, plan, st) \
-       : launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, false>(a, bound, plan, st))
+  (vec ? launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, true>(a, p, plan, st) \
+       : launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, false>(a, p, plan, st))
   // 256 bytes of a row a step: fewer barriers, one or two CTAs on an SM. 8192
   // tokens (136 tiles) 61 -> 50 us; 1024 tokens over 32 adapters (33 tiles, four
   // CTAs each instead of two) 19 -> 24 us.
-  const bool wide = likely_tiles(a, kLargeRows) * 3 >= num_sms() * 2;
+  const int64_t groups = std::min(a.tokens, a.adapters + 1);
+  const bool wide = std::max(groups, a.tokens / kLargeRows + groups / 2) * 3 >= num_sms() * 2;
   if (a.rank <= 16 && wide) return TFO_LORA(16, 16, 256, 3);
   if (a.rank <= 32 && wide) return TFO_LORA(32, 32, 256, 3);
   if (a.rank <= 64 && wide) return TFO_LORA(64, 64, 256, 3);
