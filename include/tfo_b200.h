@@ -297,8 +297,8 @@ TFO_API int tfo_gated_mlp_quantize(const void* x, const void* w_gate, const void
 /* cos and sin rows [n, 2 * half] of rotary positions:
  *   cos[p, i] = cos[p, half + i] = gain * cos(2 pi * position[p] * turns[i])
  * positions: n integers on the device, or NULL with TFO_POS_NONE (0 .. n - 1).
- * turns: `half` (<= 256) doubles in HOST memory, read before the call returns.
- * Angles are formed and reduced in fp64. */
+ * turns: `half` (<= 256) finite doubles in HOST memory, read before the call
+ * returns. Angles are reduced exactly (integer arithmetic modulo a turn). */
 TFO_API int tfo_rope_tables(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half,
                             double gain, void* cos, void* sin, int out_dtype, void* stream);
 

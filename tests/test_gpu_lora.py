@@ -86,6 +86,14 @@ CASES = [
     (300, 3, 256, 512, 72, "f16"),
     (70, 3, 256, 100, 72, "f32"),
     (9000, 20, 8, 64, 64, "bf16"),     # more rows than the sort holds at once
+    (5000, 3, 48, 640, 328, "bf16"),   # full tiles, a last one, columns that end inside a step
+    (1500, 40, 128, 512, 264, "f16"),
+    (600, 2, 64, 4096, 512, "bf16"),   # a cluster for each tile
+    (300, 1, 72, 1000, 64, "f16"),
+    (900, 4, 8, 72, 8, "bf16"),
+    (7000, 2, 20, 64, 72, "f32"),      # steps of 256 bytes
+    (6500, 3, 60, 200, 136, "bf16"),
+    (6500, 3, 7, 33, 17, "f16"),
     # each width of the streaming kernels, whole vectors
     (700, 6, 32, 1024, 512, "bf16"),
     (400, 3, 96, 256, 136, "f16"),
@@ -101,12 +109,13 @@ CASES = [
 @pytest.mark.parametrize("case", CASES, ids=str)
 @pytest.mark.parametrize("order", ["mixed", "requests"])
 def test_against_64_bits(cuda, case, order):
-    from triton_ops import fused_lora
+    from triton_ops import _lib, fused_lora
 
     x, a, b, ids, scaling, base = make(*case, seed=sum(case[:5]), order=order)
     keep = base.clone()
     got = fused_lora(x, a, b, ids, scaling, base=base)
     check(got, x, a, b, ids, scaling, base)
+    assert _lib.device_error_flags(clear=True) == 0  # no wait ran out
     assert torch.equal(base, keep)
     assert torch.equal(got[ids < 0], base[ids < 0])  # copied bit for bit
     assert torch.equal(got, fused_lora(x, a, b, ids, scaling, base=base))

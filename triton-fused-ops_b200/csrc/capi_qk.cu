@@ -83,6 +83,9 @@ int tfo_rope_tables(const void* positions, int pos_dtype, int64_t n, const doubl
   if (n == 0) return TFO_OK;
   if (!turns || !cos || !sin || (pos_dtype != TFO_POS_NONE && !positions))
     return fail(TFO_ERR_INVALID, std::string(fn) + ": NULL pointer");
+  for (int64_t i = 0; i < half; ++i) {
+    if (!(turns[i] - turns[i] == 0.0)) return fail(TFO_ERR_INVALID, std::string(fn) + ": turns must be finite");
+  }
   const RopeTablesArgs a{positions, pos_dtype, n, turns, static_cast<int>(half), gain, cos, sin, out_dtype};
   const cudaError_t e = rope_tables_launch(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? TFO_OK : cuda_fail(e, fn);

@@ -27,7 +27,7 @@ from triton_ops.kernels._native import NativeKernel
 from triton_ops.validation import SUPPORTED_DTYPES_FLOAT, validate_rope_heads
 
 rope_tables_kernel = NativeKernel(
-    "rope_tables_kernel", "tfo_rope_tables", "cos/sin rows of rotary positions, angles reduced in fp64"
+    "rope_tables_kernel", "tfo_rope_tables", "cos/sin rows of rotary positions, angles reduced exactly"
 )
 fused_rope_kernel = NativeKernel(
     "fused_rope_kernel", "tfo_rope", "rotation of query and key heads in one pass over both"
