@@ -20,13 +20,21 @@
 // A row's result does not depend on the rows beside it in its tile.
 //
 // Both products run on m16n8 tensor instructions with rows of a tile as M.
-// They are far from the tensor rate (2 * rank flops for each byte of x); what
-// bounds them is reading x, A and B once and the output traffic, so operands
-// go from global memory straight into fragments: the order of the summed index
-// inside a product is free, and with thread q of four taking the 16 bytes
-// [16 q, 16 q + 16) of a 64-byte chunk on both sides, every load is a whole
-// vector. Likewise the output columns of four instructions are dealt out so
-// that a thread ends up with eight neighbouring ones.
+// Their floor is memory (x, base and out once, A and B of the adapters that are
+// there): a rank of 16 makes 16 flops for each byte. The order of the summed
+// index inside a product is free, so thread q of four takes the 16 bytes
+// [16 q, 16 q + 16) of a 64-byte chunk on both sides: every operand load, from
+// global or shared memory, is a whole vector. Likewise the output columns of
+// four instructions are dealt out so that a thread ends up with eight
+// neighbouring ones.
+//
+// Measured (us; 4096 x 4096, bf16): one token of rank 16 5.5; 64 tokens over 32
+// adapters 8.4; 256: 12.6; 512: 15.8; 8192 tokens of 16 adapters of rank 32 50,
+// 64 % of the measured copy rate (rank 64 74, rank 128 138: the legacy tensor
+// path's 530 TFLOP/s bounds those). A form of the large kernel on tcgen05
+// (128-row tiles copied into swizzled shared memory, v and the outputs in
+// tensor memory) took 67 us at rank 32, 98 at 64 and 152 at 128: its steps'
+// waits, proxy fences and barriers ran 750 cycles with one CTA on an SM.
 //
 // Rounding: products and sums are fp32. v enters the second product as the sum
 // of two values of x's type, hi + lo (16 bits of bf16, 22 of fp16 relative to
@@ -544,12 +552,14 @@ struct SmallWidths {  // elements that rows are aligned to: of x and A, of B; wh
   bool n;
 };
 
-// A cluster of CTAs takes tile blockIdx.x / cluster. Its CTA c shrinks part c of K (a warp a part of
-// that), sends its sums to all CTAs of the cluster, and expands part c of the
-// columns. What such a launch takes is a chain of memory latencies (ids, x and
-// A, the exchange), so every load is issued as early as its address is known:
-// BATCH chunks of x and A at a time, the first B rows and base values before
-// the exchange, and each next block's before the one at hand is computed.
+// A cluster of CTAs takes tile blockIdx.x / cluster. Its CTA c shrinks part c
+// of K (a warp a part of that), sends its sums to all CTAs of the cluster, and
+// expands part c of the columns. What such a launch takes is a chain of memory
+// latencies (ids, x and A, the exchange), so every load is issued as early as
+// its address is known: BATCH chunks of x and A at a time, the first B rows and
+// base values before the exchange, and each next block's before the one at hand
+// is computed. One token, 4096 x 4096, rank 16, bf16: 5.5 us, of which the
+// launch is 1.5 (two launches with v in global memory took 6.3).
 template <typename T, int NT, bool VEC>
 __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int cluster, SmallWidths given, int64_t v_rank,
                                                          uint32_t* err) {
@@ -706,8 +716,8 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
 // ---- many tokens ---------------------------------------------------------------------------
 // A cluster of CTAs takes a tile of 64 rows that use the same adapter; CTA c of
 // it shrinks part c of K and expands part c of the columns. Both steps stream
-// through a ring of STAGES stages in shared memory: 128 bytes of K of x's rows
-// and A's (RANKS of them at a time), then 128 bytes of columns of base with
+// through a ring of STAGES stages in shared memory: STEP bytes of K of x's rows
+// and A's (RANKS of them at a time), then STEP bytes of columns of base with
 // their rows of B. The first columns are on their way while the cluster's CTAs
 // exchange their parts of v. Warp w has rows 16 (w % 4) .. + 15; the two halves
 // of the warps share the 64-byte chunks of K and the blocks of 32 columns.

@@ -241,7 +241,7 @@ bool rows_aligned(const void* x, const HeadArgs& a, int heads, int64_t sb, int64
 int head_vector_elems(const HeadArgs& a, bool backward) {
   const int esz = a.dtype == F32 ? 4 : 2;
   const int64_t tokens = a.batch * a.seq;
-  if (tokens * (a.q.heads + a.k.heads) >= (1ll << 26)) return 0;
+  if (tokens * (a.q.heads + a.k.heads) >= (1ll << 31) - (1 << 20)) return 0;  // units are counted in 32 bits
   for (int bytes = 16; bytes >= 8; bytes /= 2) {
     const int e = bytes / esz;
     if (a.head_dim % e != 0 || a.head_dim / e > 64) continue;

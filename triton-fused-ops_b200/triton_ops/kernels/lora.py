@@ -1,8 +1,9 @@
 """Low-rank adapters of many requests beside a shared projection.
 
 ``fused_lora`` adds ``scaling[i] * B[i] (A[i] x[t])`` of each row's own adapter
-``i`` to the shared projection's output in two launches (``tfo_lora``,
-csrc/lora.cu), whatever the order of the requests. ``FP8LoRALinear`` is
+``i`` to the shared projection's output (``tfo_lora``, csrc/lora.cu: one launch
+for up to 256 rows, a sort and one launch for more), whatever the order of the
+requests. ``FP8LoRALinear`` is
 :class:`~triton_ops.kernels.fp8_gemm.FP8Linear` with such adapters.
 
 ``lora_reference`` is the same in plain PyTorch, for tests; the op never calls it.
@@ -58,7 +59,7 @@ def fused_lora(
             (the shared projection's output), or None for zeros
         out: where to write, or None for a new tensor. It may be `base` itself
             (rows without an adapter are then left as they are) and must not
-            overlap x or the adapters. Rows may be strided, for example the
+            otherwise overlap base, x or the adapters. Rows may be strided, for example the
             query columns of a fused projection's output
 
     Returns:
