@@ -45,6 +45,16 @@ def test_scaling_refusals(args):
         RoPEScaling(*args)
 
 
+def test_scaling_is_a_checked_value():
+    s = RoPEScaling("yarn", 8.0, original_max_position=4096)
+    assert s == RoPEScaling("yarn", 8.0, 4096) and hash(s) == hash(RoPEScaling("yarn", 8.0, 4096))
+    assert s.factor == 8.0 and s._replace(factor=2.0) == RoPEScaling("yarn", 2.0, 4096)
+    with pytest.raises(ValueError):
+        s._replace(factor=-1.0)
+    with pytest.raises(AttributeError):
+        s.factor = 3.0
+
+
 def test_frequency_refusals():
     for rot in (0, 3, 514):
         with pytest.raises(ShapeMismatchError):

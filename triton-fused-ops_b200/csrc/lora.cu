@@ -28,8 +28,8 @@
 // four instructions are dealt out so that a thread ends up with eight
 // neighbouring ones.
 //
-// Measured (us; 4096 x 4096, bf16): one token of rank 16 5.5; 64 tokens over 32
-// adapters 8.4; 256: 12.6; 512: 15.8; 8192 tokens of 16 adapters of rank 32 50,
+// Measured (us; 4096 x 4096, bf16): one token of rank 16 4.8; 64 tokens over 32
+// adapters 7.3; 256: 11.7; 512: 15.1; 8192 tokens of 16 adapters of rank 32 50,
 // 64 % of the measured copy rate (rank 64 74, rank 128 138: the legacy tensor
 // path's 530 TFLOP/s bounds those). A form of the large kernel on tcgen05
 // (128-row tiles copied into swizzled shared memory, v and the outputs in
@@ -323,10 +323,10 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
 }
 __device__ __forceinline__ uint4 lds16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
 
-// Part `part` of `parts` of a range.
-__device__ __forceinline__ void split_range(int64_t units, int parts, int part, int* first, int* last) {
-  *first = static_cast<int>(units * part / parts);
-  *last = static_cast<int>(units * (part + 1) / parts);
+// Part `part` of 2^log_parts of a range.
+__device__ __forceinline__ void split_range(int64_t units, int log_parts, int part, int* first, int* last) {
+  *first = static_cast<int>((units * part) >> log_parts);
+  *last = static_cast<int>((units * (part + 1)) >> log_parts);
 }
 
 // ---- the expand step -----------------------------------------------------------------
@@ -374,18 +374,29 @@ __device__ __forceinline__ void fill_rows(const LoraArgs& a, const Tile& tile, c
   if (bad && threadIdx.x == 0) set_error(err, ERR_BAD_ADAPTER);
   if (col0 >= col1 || (!bad && a.base == a.out)) return;  // left as they are
   const T fill = Ty<T>::from_f(bad ? __int_as_float(0x7fffffff) : 0.f);
-  const int per_row = static_cast<int>((col1 - col0 + 7) / 8);
-  for (int i = threadIdx.x; i < per_row * tile.count; i += blockDim.x) {
-    const int64_t row = rows[i / per_row], col = col0 + i % per_row * 8;
-    const T* base = a.base != nullptr && !bad ? static_cast<const T*>(a.base) + row * a.base_stride + col : nullptr;
-    T* out = static_cast<T*>(a.out) + row * a.out_stride + col;
+  const int lane = threadIdx.x & 31, cols = static_cast<int>(col1 - col0);
+  constexpr int AHEAD = 4;  // vectors of a lane in flight: one at a time, a CTA of these was the last to end
+  for (int m = threadIdx.x >> 5; m < tile.count; m += blockDim.x >> 5) {  // a warp for a row
+    const int64_t row = rows[m];
+    const T* base = a.base != nullptr && !bad ? static_cast<const T*>(a.base) + row * a.base_stride + col0 : nullptr;
+    T* out = static_cast<T*>(a.out) + row * a.out_stride + col0;
     if (vec && base != nullptr) {
-      Eight<T> e;
-      load_eight(e, base);
+      for (int c = lane * 8; c < cols; c += AHEAD * 256) {
+        Eight<T> e[AHEAD];
 #pragma unroll
-      for (int j = 0; j < Eight<T>::W; ++j) reinterpret_cast<uint4*>(out)[j] = e.u[j];
+        for (int j = 0; j < AHEAD; ++j) {
+          if (c + j * 256 < cols) load_eight(e[j], base + c + j * 256);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+          if (c + j * 256 < cols) {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::W; ++i) reinterpret_cast<uint4*>(out + c + j * 256)[i] = e[j].u[i];
+          }
+        }
+      }
     } else {
-      for (int j = 0; j < 8 && col + j < col1; ++j) out[j] = base != nullptr ? base[j] : fill;
+      for (int c = lane; c < cols; c += 32) out[c] = base != nullptr ? base[c] : fill;
     }
   }
 }
@@ -401,7 +412,7 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int 
                                         int sums_stride, float* row_scale, unsigned* row_max, Sum sum) {
   constexpr bool SPLIT = sizeof(T) == 2;
   constexpr bool SCALED = std::is_same<T, __half>::value;
-  const int quads = vr / 4, threads = blockDim.x;
+  const int shift = 31 - __clz(vr / 4), quads = 1 << shift, threads = blockDim.x;  // vr is a power of two
   if constexpr (SCALED) {
     for (int m = threadIdx.x; m < M; m += threads) row_max[m] = 0;
     __syncthreads();
@@ -420,7 +431,7 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int 
   };
 #pragma unroll 2
   for (int i = threadIdx.x; i < M * quads; i += threads) {
-    const int m = i / quads, r = i % quads * 4;
+    const int m = i >> shift, r = (i & (quads - 1)) * 4;
     float t[4] = {};
     if (m < tile.count && r < rank) {
       const float4 u = sum(m, r);
@@ -447,7 +458,7 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int 
     }
     __syncthreads();
     for (int i = threadIdx.x; i < M * quads; i += threads) {
-      const int m = i / quads, r = i % quads * 4;
+      const int m = i >> shift, r = (i & (quads - 1)) * 4;
       float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < sums_stride) u = *reinterpret_cast<const float4*>(sums + m * sums_stride + r);
       const float t[4] = {u.x, u.y, u.z, u.w};
@@ -552,22 +563,24 @@ struct SmallWidths {  // elements that rows are aligned to: of x and A, of B; wh
   bool n;
 };
 
-// A cluster of CTAs takes tile blockIdx.x / cluster. Its CTA c shrinks part c
-// of K (a warp a part of that), sends its sums to all CTAs of the cluster, and
-// expands part c of the columns. What such a launch takes is a chain of memory
-// latencies (ids, x and A, the exchange), so every load is issued as early as
-// its address is known: BATCH chunks of x and A at a time, the first B rows and
+// A cluster of CTAs takes a tile. Its CTA c shrinks part c of K (a warp a part
+// of that), sends its sums to all CTAs of the cluster, and expands part c of
+// the columns. What such a launch takes is a chain of memory latencies (ids, x
+// and A, the exchange, B and base), so loads are issued as early as their
+// addresses are known: BATCH chunks of x and A at a time, the first B rows and
 // base values before the exchange, and each next block's before the one at hand
-// is computed. One token, 4096 x 4096, rank 16, bf16: 5.5 us, of which the
-// launch is 1.5 (two launches with v in global memory took 6.3).
+// is computed. Its instructions are fetched once, too, so the kernel is kept
+// short: four chunks or two blocks in flight were 0.2 and 0.3 us slower. One
+// token, 4096 x 4096, rank 16, bf16: 4.8 us, of which the launch is 1.5 (two
+// launches with v in global memory took 6.3).
 template <typename T, int NT, bool VEC>
-__global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int cluster, SmallWidths given, int64_t v_rank,
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) lora_small_kernel(const LoraArgs a, int log_cluster, SmallWidths given, int64_t v_rank,
                                                          uint32_t* err) {
   // aligned calls (VEC) are compiled without the other widths: a launch this short waits for its instructions too
   const SmallWidths width = VEC ? SmallWidths{16 / sizeof(T), 16 / sizeof(T), true} : given;
   constexpr int E = 16 / sizeof(T), C = chunk_elems(sizeof(T));
   constexpr int M = kSmallRows, RB = 8 * NT;  // ranks of a pass
-  constexpr int BATCH = NT == 2 ? 4 : NT == 4 ? 2 : 1;
+  constexpr int BATCH = NT == 8 ? 1 : 2;
   constexpr bool SCALED = std::is_same<T, __half>::value;
   __shared__ int rows[M], scratch[10];
   __shared__ __align__(16) int groups[kSmallTokens];
@@ -584,14 +597,15 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
   cluster_arrive();  // the barriers of the cluster's CTAs exist when all have arrived
   griddep_launch_dependents();
   griddep_wait();
-  const int part = static_cast<int>(blockIdx.x) % cluster;
-  const Tile tile = find_tile(a, static_cast<int>(blockIdx.x) / cluster, rows, groups, scratch);
+  const int cluster = 1 << log_cluster, part = static_cast<int>(blockIdx.x) & (cluster - 1);
+  const Tile tile = find_tile(a, static_cast<int>(blockIdx.x) >> log_cluster, rows, groups, scratch);
   if (tile.count == 0) {  // of the whole cluster
     cluster_wait();
     return;
   }
-  const int64_t blocks = (a.n + 31) / 32;
-  const int64_t col0 = blocks * part / cluster * 32, col1 = min(a.n, blocks * (part + 1) / cluster * 32);
+  int block0, block1;
+  split_range((a.n + 31) / 32, log_cluster, part, &block0, &block1);
+  const int64_t col0 = static_cast<int64_t>(block0) * 32, col1 = min(a.n, static_cast<int64_t>(block1) * 32);
   if (tile.group >= a.adapters) {
     fill_rows<T>(a, tile, rows, col0, col1, width.n, err);
     __syncwarp();
@@ -612,7 +626,8 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
   const T* x0 = in0 ? static_cast<const T*>(a.x) + t0 * a.x_stride : nullptr;
   const T* x1 = in1 ? static_cast<const T*>(a.x) + t1 * a.x_stride : nullptr;
   int c0, c1;
-  split_range((a.k + C - 1) / C, cluster * kSmallWarps, part * kSmallWarps + warp, &c0, &c1);
+  static_assert(kSmallWarps == 8, "a power of two");
+  split_range((a.k + C - 1) / C, log_cluster + 3, part * kSmallWarps + warp, &c0, &c1);
   const uint32_t my_part = smem_u32(parts + part * M * vr), bar = smem_u32(&received);
   for (int r0 = 0; r0 < rank; r0 += RB) {
     const T* w[NT];
@@ -646,9 +661,9 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
     }
     __syncthreads();
     if (r0 == 0) cluster_wait();
-    const int here = min(RB / 4, quads - r0 / 4);  // quads of this pass
-    for (int i = t; i < tile.count * here; i += 256) {
-      const int m = i / here, r = i % here * 4;
+    for (int i = t; i < tile.count * (RB / 4); i += 256) {
+      const int m = i / (RB / 4), r = i % (RB / 4) * 4;
+      if (r0 + r >= rank) continue;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < kSmallWarps; ++k) {
@@ -683,6 +698,7 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
     }
   };
   const int64_t first = col0 + warp * 32;
+  constexpr int kStride = kSmallWarps * 32;
   Block next{};
   load_block(next, first);
   const float scale = a.scaling != nullptr ? a.scaling[tile.group] : 1.f;
@@ -694,9 +710,9 @@ __global__ void __launch_bounds__(256) lora_small_kernel(const LoraArgs a, int c
   const T* lo0 = lo + g * stride + q * E;
   T* out0 = static_cast<T*>(a.out) + t0 * a.out_stride + q * 8;
   T* out1 = static_cast<T*>(a.out) + t1 * a.out_stride + q * 8;
-  for (int64_t n0 = first; n0 < col1; n0 += kSmallWarps * 32) {
+  for (int64_t n0 = first; n0 < col1; n0 += kStride) {
     const Block now = next;
-    if (n0 + kSmallWarps * 32 < col1) load_block(next, n0 + kSmallWarps * 32);
+    if (n0 + kStride < col1) load_block(next, n0 + kStride);
     float acc[4][4] = {};
     expand_chunk<T>(acc, hi0, lo0, stride, 0, [&](int j, int) { return now.b[j]; });
     for (int c = 1; c < vr / C; ++c) expand_chunk<T>(acc, hi0, lo0, stride, c, [&](int j, int k) { return b_chunk(n0, j, k); });
@@ -741,7 +757,7 @@ struct LargeShape {
 };
 
 template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
-__global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArgs a, LoraPlan plan, int cluster,
+__global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArgs a, LoraPlan plan, int log_cluster,
                                                                    uint32_t* err) {
   using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
   constexpr int E = S::E, M = S::M, KS = S::KS, NCH = S::NCH, NT = RANKS / 8, stride = S::stride;
@@ -760,11 +776,11 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
   cluster_arrive();  // the barriers of the cluster's CTAs exist when all have arrived
   griddep_launch_dependents();
   griddep_wait();
-  const int part = static_cast<int>(blockIdx.x) % cluster;
-  const Tile tile = planned_tile(plan, static_cast<int>(blockIdx.x) / cluster, rows);
+  const int cluster = 1 << log_cluster, part = static_cast<int>(blockIdx.x) & (cluster - 1);
+  const Tile tile = planned_tile(plan, static_cast<int>(blockIdx.x) >> log_cluster, rows);
   const int64_t col_steps = (a.n + KS - 1) / KS;
   int s0i, s1i;
-  split_range(col_steps, cluster, part, &s0i, &s1i);
+  split_range(col_steps, log_cluster, part, &s0i, &s1i);
   const int64_t col0 = static_cast<int64_t>(s0i) * KS, col1 = min(a.n, static_cast<int64_t>(s1i) * KS);
   if (tile.count == 0 || tile.group >= a.adapters) {  // of the whole cluster
     if (tile.count > 0) fill_rows<T>(a, tile, rows, col0, col1, VEC, err);
@@ -801,7 +817,7 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
 
   // ---- shrink
   int k0, k1;
-  split_range((a.k + KS - 1) / KS, cluster, part, &k0, &k1);
+  split_range((a.k + KS - 1) / KS, log_cluster, part, &k0, &k1);
   const uint32_t my_part = smem_u32(parts + part * M * S::PR), bar = smem_u32(&received);
   // a lane's operands in a stage: row m0 + g (and 8 further) of x, row g (and 8, 16, ... further) of A
   constexpr int kHalfChunks = kChunks / 2;
@@ -884,9 +900,9 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
     }
     if (r0 == 0) cluster_wait();
     __syncthreads();
-    const int here = min(RANKS / 4, quads - r0 / 4);  // quads of this pass
-    for (int i = t; i < tile.count * here; i += kLargeThreads) {
-      const int m = i / here, r = i % here * 4;
+    for (int i = t; i < tile.count * (RANKS / 4); i += kLargeThreads) {
+      const int m = i / (RANKS / 4), r = i % (RANKS / 4) * 4;
+      if (r0 + r >= rank) continue;
       const float4 u = *reinterpret_cast<const float4*>(&halves[m][r]);
       const uint32_t dst = my_part + (m * S::PR + r0 + r) * 4;
       for (int k = 0; k < cluster; ++k) push16(mapa_shared(dst, k), u, mapa_shared(bar, k));
@@ -1015,6 +1031,8 @@ namespace {
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 size_t round256(size_t v) { return (v + 255) / 256 * 256; }
 
+int log2_of(int cluster) { return cluster == 8 ? 3 : cluster == 4 ? 2 : cluster - 1; }
+
 bool small_call(int64_t tokens) { return tokens <= kSmallTokens; }
 
 struct PlanBytes {  // of many tokens
@@ -1088,7 +1106,7 @@ cudaError_t launch_small(const LoraArgs& a, cudaStream_t st) {
   const size_t smem = kSmallRows * (sizeof(float) * v_rank * cluster + (sizeof(T) == 2 ? 2 : 1) * sizeof(T) * (v_rank + E));
   auto launch = [&](auto* kernel, int nt) {
     const size_t red = sizeof(float) * kSmallWarps * kSmallRows * (8 * nt + 4);
-    return launch_grid(kernel, dim3(static_cast<unsigned>(tiles * cluster)), 256, cluster, smem + red, st, a, cluster,
+    return launch_grid(kernel, dim3(static_cast<unsigned>(tiles * cluster)), 256, cluster, smem + red, st, a, log2_of(cluster),
                        width, v_rank, error_word_ptr());
   };
   const bool vec = width.k == E && width.b == E && width.n;
@@ -1116,7 +1134,7 @@ cudaError_t launch_shape(const LoraArgs& a, const PlanBytes& p, const LoraPlan& 
     cluster *= 2;
   }
   return launch_grid(lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>, dim3(static_cast<unsigned>(p.tiles * cluster)),
-                     kLargeThreads, cluster, S::smem(cluster), st, a, plan, cluster, error_word_ptr());
+                     kLargeThreads, cluster, S::smem(cluster), st, a, plan, log2_of(cluster), error_word_ptr());
 }
 
 template <typename T>

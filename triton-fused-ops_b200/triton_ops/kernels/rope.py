@@ -15,9 +15,8 @@ from __future__ import annotations
 
 import ctypes
 import math
-from dataclasses import dataclass
 from functools import lru_cache
-from typing import Optional, Tuple, Union
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -37,8 +36,18 @@ _SCALING_KINDS = ("linear", "ntk", "yarn", "wavelength")
 _POS_CODE = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64}
 
 
-@dataclass(frozen=True)
-class RoPEScaling:
+class _Scaling(NamedTuple):
+    kind: str
+    factor: float
+    original_max_position: Optional[int]
+    beta_fast: float
+    beta_slow: float
+    low_freq_factor: float
+    high_freq_factor: float
+    attention_factor: Optional[float]
+
+
+class RoPEScaling(_Scaling):
     """How the rotary frequencies ``f_i = base^(-2i / rotary_dim)`` change for a context `factor` times as long.
 
     Kinds:
@@ -58,26 +67,28 @@ class RoPEScaling:
     `attention_factor` multiplies cos and sin for every kind when it is given.
     """
 
-    kind: str
-    factor: float = 1.0
-    original_max_position: Optional[int] = None
-    beta_fast: float = 32.0
-    beta_slow: float = 1.0
-    low_freq_factor: float = 1.0
-    high_freq_factor: float = 4.0
-    attention_factor: Optional[float] = None
+    __slots__ = ()
 
-    def __post_init__(self):
-        if self.kind not in _SCALING_KINDS:
-            raise ValueError(f"kind must be one of {_SCALING_KINDS}, got '{self.kind}'")
-        if not (self.factor > 0 and math.isfinite(self.factor)):
-            raise ValueError(f"factor must be positive and finite, got {self.factor}")
-        if self.kind in ("yarn", "wavelength") and not (self.original_max_position and self.original_max_position > 0):
-            raise ValueError(f"kind '{self.kind}' needs original_max_position")
-        if self.kind == "yarn" and not self.beta_fast > self.beta_slow > 0:
+    def __new__(cls, kind: str, factor: float = 1.0, original_max_position: Optional[int] = None, beta_fast: float = 32.0,
+                beta_slow: float = 1.0, low_freq_factor: float = 1.0, high_freq_factor: float = 4.0,
+                attention_factor: Optional[float] = None):
+        if kind not in _SCALING_KINDS:
+            raise ValueError(f"kind must be one of {_SCALING_KINDS}, got '{kind}'")
+        if not 0 < factor < math.inf:
+            raise ValueError(f"factor must be positive and finite, got {factor}")
+        if kind in ("yarn", "wavelength") and not (original_max_position and original_max_position > 0):
+            raise ValueError(f"kind '{kind}' needs original_max_position")
+        if kind == "yarn" and not beta_fast > beta_slow > 0:
             raise ValueError("yarn needs beta_fast > beta_slow > 0")
-        if self.kind == "wavelength" and not self.high_freq_factor > self.low_freq_factor > 0:
+        if kind == "wavelength" and not high_freq_factor > low_freq_factor > 0:
             raise ValueError("wavelength needs high_freq_factor > low_freq_factor > 0")
+        return _Scaling.__new__(cls, kind, factor, original_max_position, beta_fast, beta_slow, low_freq_factor,
+                                high_freq_factor, attention_factor)
+
+    @classmethod
+    def _make(cls, values):
+        """Checked too, so that ``_replace`` is."""
+        return cls(*values)
 
 
 @lru_cache(maxsize=64)
