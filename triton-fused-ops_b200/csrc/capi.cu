@@ -32,7 +32,6 @@ bool is_float_dtype(int d) { return d == F16 || d == BF16 || d == F32; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 std::mutex g_cache_mu;
-std::map<int, int> g_sm_count;
 std::map<std::tuple<const void*, int, size_t, int>, int> g_occ;
 }  // namespace
 
@@ -41,29 +40,33 @@ int report_error(int code, const char* msg) { return fail(code, msg); }
 static std::atomic<unsigned long long> g_launches{0};
 void note_launch(int n) { g_launches.fetch_add(static_cast<unsigned long long>(n), std::memory_order_relaxed); }
 
+// Both are asked for by every launch: their answers are kept per device
+// without a lock (racing first calls find the same answer).
+constexpr int kMaxDevices = 64;
+
 uint32_t* error_word_ptr() {
   int dev = 0;
   cudaGetDevice(&dev);
-  static std::mutex mu;
-  static std::map<int, uint32_t*> ptrs;
-  std::lock_guard<std::mutex> lk(mu);
-  auto it = ptrs.find(dev);
-  if (it != ptrs.end()) return it->second;
+  static std::atomic<uint32_t*> ptrs[kMaxDevices];
+  if (dev >= 0 && dev < kMaxDevices) {
+    if (uint32_t* p = ptrs[dev].load(std::memory_order_relaxed)) return p;
+  }
   void* p = nullptr;
-  if (cudaGetSymbolAddress(&p, g_error_word) != cudaSuccess) p = nullptr;
-  ptrs[dev] = static_cast<uint32_t*>(p);
+  if (cudaGetSymbolAddress(&p, g_error_word) != cudaSuccess) return nullptr;
+  if (dev >= 0 && dev < kMaxDevices) ptrs[dev].store(static_cast<uint32_t*>(p), std::memory_order_relaxed);
   return static_cast<uint32_t*>(p);
 }
 
 int num_sms() {
   int dev = 0;
   cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> lk(g_cache_mu);
-  auto it = g_sm_count.find(dev);
-  if (it != g_sm_count.end()) return it->second;
+  static std::atomic<int> counts[kMaxDevices];
+  if (dev >= 0 && dev < kMaxDevices) {
+    if (const int n = counts[dev].load(std::memory_order_relaxed)) return n;
+  }
   int n = 0;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-  g_sm_count[dev] = n;
+  if (dev >= 0 && dev < kMaxDevices) counts[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
