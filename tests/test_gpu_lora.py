@@ -86,6 +86,8 @@ CASES = [
     (300, 3, 256, 512, 72, "f16"),
     (70, 3, 256, 100, 72, "f32"),
     (9000, 20, 8, 64, 64, "bf16"),     # more rows than the sort holds at once
+    (20, 16384, 1, 8, 8, "bf16"),      # the most adapters
+    (300, 16384, 1, 8, 8, "bf16"),
     (5000, 3, 48, 640, 328, "bf16"),   # full tiles, a last one, columns that end inside a step
     (1500, 40, 128, 512, 264, "f16"),
     (600, 2, 64, 4096, 512, "bf16"),   # a cluster for each tile
@@ -176,6 +178,39 @@ def test_large_low_rank_values_in_fp16(cuda):
         b[0] /= 64
         check(fused_lora(x, a, b, ids, scaling, base=base), x, a, b, ids, scaling, base)
         check(fused_lora(x, a, b, ids, scaling), x, a, b, ids, scaling, None)
+
+
+@pytest.mark.parametrize("t", [3, 300])
+@pytest.mark.parametrize("where", ["x", "a"])
+def test_infinity_beside_values_past_the_fp16_range(cuda, t, where):
+    """Low-rank values 6e7 and 1e6 beside an infinite one, in fp16.
+
+    An infinity in x multiplies the zeros of A too (NaN): all of that row is NaN. One in A makes one low-rank value of
+    every row infinite: where B is one for it the row is +inf (the others stay finite, so nothing cancels it), where B
+    is zero it is NaN."""
+    from triton_ops import fused_lora
+
+    x = torch.zeros(t, 64, device="cuda", dtype=torch.float16)
+    x[:, 0], x[:, 1] = 60000.0, 1000.0
+    a = torch.zeros(1, 16, 64, device="cuda", dtype=torch.float16)
+    a[0, 0, 0], a[0, 1, 1], a[0, 2, 2] = 1000.0, 1000.0, 1.0
+    if where == "x":
+        x[1, 2] = float("inf")
+    else:
+        x[:, 2] = 1.0
+        a[0, 2, 2] = float("inf")
+    b = torch.zeros(1, 32, 16, device="cuda", dtype=torch.float16)
+    b[0, :, 0], b[0, :, 1] = 2.0**-14, -(2.0**-14)
+    b[0, :8, 2] = 1.0
+    got = fused_lora(x, a, b, torch.zeros(t, dtype=torch.int64, device="cuda")).double()
+    if where == "a":
+        assert (got[:, :8] == float("inf")).all()
+        assert torch.isnan(got[:, 8:]).all()
+        return
+    want = (6e7 - 1e6) * 2.0**-14
+    keep = torch.arange(t, device="cuda") != 1
+    assert ((got[keep] - want).abs() <= want * 2.0**-10).all()
+    assert torch.isnan(got[1]).all()
 
 
 def test_bad_ids(cuda):

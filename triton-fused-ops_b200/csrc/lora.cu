@@ -444,8 +444,11 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int 
       if (r < sums_stride) *reinterpret_cast<float4*>(sums + m * sums_stride + r) = make_float4(t[0], t[1], t[2], t[3]);
       float most = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) most = !(fabsf(t[j]) <= most) ? fabsf(t[j]) : most;  // NaN stays
-      if (most != 0.f) atomicMax(row_max + m, __float_as_uint(most));  // ordered like the floats; NaN above all
+      for (int j = 0; j < 4; ++j) {
+        const float x = fabsf(t[j]);
+        if (x <= 3.402823466e38f) most = fmaxf(most, x);  // infinities and NaN need no scale
+      }
+      if (most != 0.f) atomicMax(row_max + m, __float_as_uint(most));  // ordered like the floats
     } else {
       put(m, r, t, 1.f);
     }
@@ -454,7 +457,7 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int 
   if constexpr (SCALED) {
     for (int m = threadIdx.x; m < M; m += threads) {
       const float most = __uint_as_float(row_max[m]);
-      row_scale[m] = most > 0.f && most <= 1.7e38f ? ldexpf(1.f, min(126, max(-126, ilogbf(most)))) : 1.f;
+      row_scale[m] = most > 0.f ? ldexpf(1.f, min(126, max(-126, ilogbf(most)))) : 1.f;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < M * quads; i += threads) {
