@@ -172,8 +172,9 @@ int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides,
   if (empty) return TFO_OK;
   if ((q_heads > 0 && (!dq_out || !dq_out_strides)) || (k_heads > 0 && (!dk_out || !dk_out_strides)))
     return fail(TFO_ERR_INVALID, std::string(fn) + ": NULL pointer");
-  if ((dq_weight || dk_weight) && (!workspace || workspace_bytes < tfo_qk_norm_rope_backward_workspace_bytes(head_dim)))
-    return fail(TFO_ERR_INVALID, std::string(fn) + ": workspace too small");
+  if ((dq_weight || dk_weight) && (!workspace || workspace_bytes < tfo_qk_norm_rope_backward_workspace_bytes(head_dim) ||
+                                   reinterpret_cast<uintptr_t>(workspace) % sizeof(float) != 0))
+    return fail(TFO_ERR_INVALID, std::string(fn) + ": workspace too small or not aligned");
   a.norm = true;
   a.eps = static_cast<float>(eps);
   auto grads = [](HeadSide* side, const void* w, int w_dtype, const void* dy, const int64_t* strides, void* dw) {
