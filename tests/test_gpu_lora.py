@@ -327,6 +327,35 @@ def test_streams_and_graphs(cuda):
                 assert torch.equal(out, ref[seed])
 
 
+@pytest.mark.parametrize("extension", [True, False])
+def test_threads_on_one_stream(cuda, monkeypatch, extension):
+    """Calls of several threads may alternate their launches on the stream: each keeps its own plan."""
+    import threading
+
+    from triton_ops import _lib, fused_lora
+
+    if not extension:
+        monkeypatch.setattr(_lib, "ext", lambda: None)
+    jobs = [make(t, 4, 16, 128, 128, "bf16", seed=t) for t in (300, 700, 40, 1300)]
+    ref = [fused_lora(x, a, b, ids, scaling, base=base) for x, a, b, ids, scaling, base in jobs]
+    wrong, done, start = [], [], threading.Barrier(len(jobs))
+
+    def work(i):
+        x, a, b, ids, scaling, base = jobs[i]
+        start.wait(60)
+        for _ in range(50):
+            if not torch.equal(fused_lora(x, a, b, ids, scaling, base=base), ref[i]):
+                wrong.append(i)
+        done.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and len(done) == len(threads)
+
+
 def test_without_the_extension(cuda, monkeypatch):
     from triton_ops import _lib, fused_lora
 

@@ -515,6 +515,51 @@ def test_streams_and_graphs(cuda):
             assert all(torch.equal(x, y) for x, y in zip(out, plain[seed]))
 
 
+@pytest.mark.parametrize("extension", [True, False])
+def test_gradients_of_threads_on_one_stream(cuda, monkeypatch, extension):
+    """Gradients of two threads and calls that use scratch memory beside them, all on one stream."""
+    import threading
+
+    from triton_ops import _lib, fused_lora, fused_qk_norm_rope
+
+    cos, sin = table(600, 64, torch.float32)
+    cases = [(1, 600, 4, 64), (2, 37, 3, 64), (1, 300, 8, 64)]
+    tensors = [(heads(s, "bf16", i), 1 + 0.1 * heads((64,), "f32", i + 9), heads(s, "bf16", i + 20))
+               for i, s in enumerate(cases)]
+    lora = (heads((400, 64), "bf16", 1), heads((3, 8, 64), "bf16", 2), heads((3, 64, 8), "bf16", 3),
+            torch.arange(400, device="cuda") % 4 - 1)
+
+    def grads(i):
+        q, w, g = tensors[i]
+        leaves = [q.clone().requires_grad_(), w.clone().requires_grad_()]
+        out, _ = fused_qk_norm_rope(leaves[0], None, leaves[1], None, cos, sin)
+        return torch.autograd.grad(out, leaves, g)
+
+    if not extension:
+        monkeypatch.setattr(_lib, "ext", lambda: None)
+    ref = [grads(i) for i in range(len(cases))]
+    lora_ref = fused_lora(*lora)
+    wrong, done, start = [], [], threading.Barrier(len(cases) + 1)
+
+    def work(i):
+        start.wait(60)
+        for _ in range(40):
+            if i == len(cases):
+                same = torch.equal(fused_lora(*lora), lora_ref)
+            else:
+                same = all(torch.equal(x, y) for x, y in zip(grads(i), ref[i]))
+            if not same:
+                wrong.append(i)
+        done.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases) + 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and len(done) == len(threads)
+
+
 def test_without_the_extension(cuda, monkeypatch):
     """The same kernels through ctypes: the same bits, forward and backward."""
     from triton_ops import _lib, fused_qk_norm_rope, fused_rope, rope_tables

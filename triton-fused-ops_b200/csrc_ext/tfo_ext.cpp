@@ -168,6 +168,13 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Device& d
   return at::detail::empty_cuda(sizes, type, dev, c10::nullopt);
 }
 
+// Scratch of one call of several launches (undefined for none). Not kept
+// between calls: gradients run on a thread of their own and two threads may
+// call on one stream, so that launches of two calls may alternate there.
+at::Tensor scratch(size_t bytes, const at::Device& dev) {
+  return bytes == 0 ? at::Tensor() : fresh({static_cast<int64_t>(bytes)}, at::kByte, dev);
+}
+
 using Strides3 = std::array<int64_t, 3>;
 
 int pos_code(at::ScalarType t) {
@@ -337,8 +344,7 @@ struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
     at::Tensor dqw, dkw, ws;
     if (ctx->saved_data["dqw"].toBool()) dqw = fresh(qw.sizes(), qw.scalar_type(), qw.device());
     if (ctx->saved_data["dkw"].toBool()) dkw = fresh(kw.sizes(), kw.scalar_type(), kw.device());
-    if (dqw.defined() || dkw.defined())
-      ws = workspace(tfo_qk_norm_rope_backward_workspace_bytes(h.dim), q.device(), st);
+    if (dqw.defined() || dkw.defined()) ws = scratch(tfo_qk_norm_rope_backward_workspace_bytes(h.dim), q.device());
     const Strides3 qs = strides_of(q), gqs = strides_of(gq), ks = k.defined() ? strides_of(k) : Strides3{},
                    gks = k.defined() ? strides_of(gk) : Strides3{};
     check(tfo_qk_norm_rope_backward(
@@ -431,11 +437,12 @@ py::object lora(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, c
   const auto st = at::cuda::getCurrentCUDAStream(x.device().index()).stream();
   at::Tensor y = out.has_value() ? *out : fresh({tokens, n}, x.scalar_type(), x.device());
   const int dtype = dtype_code(x.scalar_type());
-  at::Tensor ws = workspace(tfo_lora_workspace_bytes(tokens, adapters), x.device(), st);
+  const at::Tensor ws = scratch(tfo_lora_workspace_bytes(tokens, adapters), x.device());
   check(tfo_lora(x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ids.data_ptr(), pos_code(ids.scalar_type()),
                  scaling.has_value() ? scaling->data_ptr<float>() : nullptr,
                  base.has_value() ? base->data_ptr() : nullptr, base.has_value() ? base->stride(0) : 0, y.data_ptr(),
-                 y.stride(0), tokens, adapters, rank, k, n, dtype, ws.data_ptr(), static_cast<size_t>(ws.numel()), st),
+                 y.stride(0), tokens, adapters, rank, k, n, dtype, out_or_null(ws),
+                 ws.defined() ? static_cast<size_t>(ws.numel()) : 0, st),
         "tfo_lora");
   return py::cast(y);
 }

@@ -342,6 +342,12 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return buf
 
 
+def scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
+    """Scratch of one call of several launches (None for none), not kept between calls: two threads may call on
+    one stream, and their launches may then alternate there."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def clear_workspaces() -> None:
     """Releases every cached scratch buffer (they return to torch's caching allocator)."""
     with _ws_lock:

@@ -89,11 +89,11 @@ def fused_lora(
     ids = adapter_ids.reshape(-1).contiguous()
     dtype = _lib.dtype_code(x.dtype, "x")
     with _lib.on_device(x):
-        ws = _lib.workspace(_lib.load().tfo_lora_workspace_bytes(tokens, adapters), x.device)
+        ws = _lib.scratch(_lib.load().tfo_lora_workspace_bytes(tokens, adapters), x.device)
         _lib.call("tfo_lora", x2.data_ptr(), x2.stride(0), lora_a.data_ptr(), lora_b.data_ptr(), ids.data_ptr(),
                   _IDS_CODE[ids.dtype], _lib.ptr(scaling), _lib.ptr(base2), 0 if base2 is None else base2.stride(0),
-                  out2.data_ptr(), out2.stride(0), tokens, adapters, rank, k, n, dtype, ws.data_ptr(), ws.numel(),
-                  _lib.stream_of(x))
+                  out2.data_ptr(), out2.stride(0), tokens, adapters, rank, k, n, dtype, _lib.ptr(ws),
+                  0 if ws is None else ws.numel(), _lib.stream_of(x))
     return out
 
 

@@ -74,7 +74,7 @@ class _FusedQKNormRoPE(torch.autograd.Function):
         with _lib.on_device(q):
             ws = None
             if dqw is not None or dkw is not None:
-                ws = _lib.workspace(_lib.load().tfo_qk_norm_rope_backward_workspace_bytes(q.shape[-1]), q.device)
+                ws = _lib.scratch(_lib.load().tfo_qk_norm_rope_backward_workspace_bytes(q.shape[-1]), q.device)
             _lib.call("tfo_qk_norm_rope_backward", gq.data_ptr(), _strides(gq), _lib.ptr(gk), _strides(gk), q.data_ptr(),
                       _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(qw), _lib.ptr(kw),
                       *_table_args(cos, sin, positions, q), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dqw), _lib.ptr(dkw),
