@@ -350,8 +350,8 @@ TFO_API int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_
  * x [tokens, k] (rows x_stride elements apart, innermost stride 1), a
  * [adapters, rank, k] and b [adapters, n, rank] contiguous, ids [tokens]
  * (TFO_POS_I32 or _I64), scaling [adapters] fp32 or NULL (ones), base and out
- * [tokens, n] with their row strides; base may be NULL (zeros) or out itself,
- * out must not overlap any other input. ids < 0: no adapter, out = base (left
+ * [tokens, n] with their row strides (out's at least n); base may be NULL
+ * (zeros) or out itself, out must not overlap any other input. ids < 0: no adapter, out = base (left
  * untouched when base == out). An id >= adapters reads nothing: its row becomes
  * NaN and the device error word gets bit 7. rank <= 256, adapters <= 16384.
  * fp32 sums; one rounding of the result. No counterpart in the reference. */

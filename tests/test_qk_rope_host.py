@@ -172,17 +172,30 @@ def test_lora_argument_checks(monkeypatch):
             check(*args)
 
 
+def test_the_factors_of_adapters_stay_fp32():
+    from triton_ops import FP8LoRALinear
+
+    m = FP8LoRALinear(16, 8, max_adapters=2, rank=4)
+    m.set_adapter(1, torch.ones(4, 16), torch.ones(8, 4), 1 / 3)
+    factors = m.scaling.clone()
+    for convert in (m.half, m.bfloat16, lambda: m.to("cpu", torch.float16)):
+        convert()
+        assert m.scaling.dtype == torch.float32 and torch.equal(m.scaling, factors)
+    assert m.lora_a.dtype == m.lora_b.dtype == torch.float16
+    assert m.state_dict()["scaling"].dtype == torch.float32
+
+
 def test_lora_entry_point_reports_bad_arguments():
     lib = _lib.load()
 
-    def lora(tokens=2, adapters=1, rank=4, k=8, n=8, dtype=2, ids_dtype=2, x=16, ws=None, bytes_=0):
-        return lib.tfo_lora(x, 8, 16, 16, 16, ids_dtype, None, None, 0, 16, 8, tokens, adapters, rank, k, n, dtype, ws,
+    def lora(tokens=2, adapters=1, rank=4, k=8, n=8, dtype=2, ids_dtype=2, x=16, ws=None, bytes_=0, base=None):
+        return lib.tfo_lora(x, 8, 16, 16, 16, ids_dtype, None, base, 0, 16, 8, tokens, adapters, rank, k, n, dtype, ws,
                             bytes_, None)
 
     assert lora(tokens=0) == _lib.OK and lora(n=0) == _lib.OK
     assert lora(dtype=3) == _lib.ERR_DTYPE and lora(ids_dtype=0) == _lib.ERR_DTYPE
     for bad in ({"rank": 257}, {"rank": 0}, {"k": 0}, {"adapters": 0}, {"adapters": 16385}, {"tokens": -1}, {"x": None},
-                {"tokens": 300}, {"tokens": 300, "ws": 8, "bytes_": 1 << 40}):
+                {"tokens": 300}, {"tokens": 300, "ws": 8, "bytes_": 1 << 40}, {"n": 9}, {"base": 16}):
         assert lora(**bad) == _lib.ERR_INVALID, bad
     assert lib.tfo_lora_workspace_bytes(300, 4) >= 300 * 4
     assert lib.tfo_lora_workspace_bytes(300, 0) == 0

@@ -38,6 +38,9 @@ int tfo_lora(const void* x, int64_t x_stride, const void* a, const void* b, cons
     return fail(TFO_ERR_INVALID, std::string(fn) + ": rank must be in 1..256 and k positive");
   if (tokens == 0 || n == 0) return TFO_OK;
   if (!x || !a || !b || !ids || !out) return fail(TFO_ERR_INVALID, std::string(fn) + ": NULL pointer");
+  if (tokens > 1 && out_stride < n) return fail(TFO_ERR_INVALID, std::string(fn) + ": rows of out overlap");
+  if (base == out && tokens > 1 && base_stride != out_stride)
+    return fail(TFO_ERR_INVALID, std::string(fn) + ": base and out share memory but not their rows");
   const size_t need = lora_workspace_bytes(tokens, adapters);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
     return fail(TFO_ERR_INVALID, std::string(fn) + ": workspace too small or not 16-byte aligned");

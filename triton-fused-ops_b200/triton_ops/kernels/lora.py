@@ -131,6 +131,13 @@ class FP8LoRALinear(FP8Linear):
         self.register_buffer("lora_b", torch.zeros(max_adapters, out_features, rank, dtype=adapter_dtype))
         self.register_buffer("scaling", torch.ones(max_adapters, dtype=torch.float32))
 
+    def _apply(self, fn, recurse=True):
+        scaling = self.scaling
+        super()._apply(fn, recurse)
+        if self.scaling.dtype != torch.float32:  # .half() and the like: the factors stay fp32
+            self.scaling = scaling.to(self.scaling.device)
+        return self
+
     @torch.no_grad()
     def set_adapter(self, index: int, a: torch.Tensor, b: torch.Tensor, scaling: float = 1.0) -> None:
         """Puts an adapter a [r, in_features], b [out_features, r], r <= rank, into slot `index`."""
