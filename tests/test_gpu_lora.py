@@ -88,6 +88,9 @@ CASES = [
     (9000, 20, 8, 64, 64, "bf16"),     # more rows than the sort holds at once
     (20, 16384, 1, 8, 8, "bf16"),      # the most adapters
     (300, 16384, 1, 8, 8, "bf16"),
+    (3000, 16384, 1, 8, 8, "f16"),
+    (2049, 5, 4, 16, 8, "f32"),        # a last row alone in its CTA's share of the sort
+    (70000, 20, 8, 16, 8, "bf16"),     # more rows than the sort's CTAs hold at once
     (5000, 3, 48, 640, 328, "bf16"),   # full tiles, a last one, columns that end inside a step
     (1500, 40, 128, 512, 264, "f16"),
     (600, 2, 64, 4096, 512, "bf16"),   # a cluster for each tile
