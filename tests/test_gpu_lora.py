@@ -88,6 +88,14 @@ CASES = [
     (9000, 20, 8, 64, 64, "bf16"),     # more rows than the sort holds at once
     (20, 16384, 1, 8, 8, "bf16"),      # the most adapters
     (300, 16384, 1, 8, 8, "bf16"),
+    (384, 40, 16, 128, 96, "bf16"),    # the most rows of the single launch, and one more
+    (385, 40, 16, 128, 96, "bf16"),
+    (384, 1, 8, 64, 40, "f32"),
+    (500, 3, 256, 512, 72, "f16"),
+    (500, 16384, 1, 8, 8, "bf16"),
+    (500, 1, 72, 1000, 64, "f16"),
+    (500, 2, 200, 128, 64, "f32"),
+    (500, 2, 200, 128, 64, "f16"),
     (3000, 16384, 1, 8, 8, "f16"),
     (2049, 5, 4, 16, 8, "f32"),        # a last row alone in its CTA's share of the sort
     (70000, 20, 8, 16, 8, "bf16"),     # more rows than the sort's CTAs hold at once
@@ -173,7 +181,7 @@ def test_large_low_rank_values_in_fp16(cuda):
     """v passes 65504 (fp16's largest) and falls below its smallest while the result stays in range."""
     from triton_ops import fused_lora
 
-    for t in (5, 300):
+    for t in (5, 300, 500):
         x, a, b, ids, _, base = make(t, 2, 16, 256, 64, "f16", seed=5, none=0)
         scaling = torch.tensor([1.0, 2.0**-20], device="cuda")
         x, a = x * 64, a * 1024  # v of order 2^16 and more
@@ -183,7 +191,7 @@ def test_large_low_rank_values_in_fp16(cuda):
         check(fused_lora(x, a, b, ids, scaling), x, a, b, ids, scaling, None)
 
 
-@pytest.mark.parametrize("t", [3, 300])
+@pytest.mark.parametrize("t", [3, 300, 500])
 @pytest.mark.parametrize("where", ["x", "a"])
 def test_infinity_beside_values_past_the_fp16_range(cuda, t, where):
     """Low-rank values 6e7 and 1e6 beside an infinite one, in fp16.

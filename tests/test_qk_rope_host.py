@@ -195,7 +195,7 @@ def test_lora_entry_point_reports_bad_arguments():
     assert lora(tokens=0) == _lib.OK and lora(n=0) == _lib.OK
     assert lora(dtype=3) == _lib.ERR_DTYPE and lora(ids_dtype=0) == _lib.ERR_DTYPE
     for bad in ({"rank": 257}, {"rank": 0}, {"k": 0}, {"adapters": 0}, {"adapters": 16385}, {"tokens": -1}, {"x": None},
-                {"tokens": 300}, {"tokens": 300, "ws": 8, "bytes_": 1 << 40}, {"n": 9}, {"base": 16}):
+                {"tokens": 400}, {"tokens": 400, "ws": 8, "bytes_": 1 << 40}, {"n": 9}, {"base": 16}):
         assert lora(**bad) == _lib.ERR_INVALID, bad
-    assert lib.tfo_lora_workspace_bytes(300, 4) >= 300 * 4
-    assert lib.tfo_lora_workspace_bytes(300, 0) == 0
+    assert lib.tfo_lora_workspace_bytes(400, 4) >= 400 * 4
+    assert lib.tfo_lora_workspace_bytes(400, 0) == 0

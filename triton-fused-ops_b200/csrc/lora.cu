@@ -10,7 +10,7 @@
 // both in one kernel, v never leaves the SMs.
 // Rows that use the same adapter are grouped into tiles, so that an adapter's
 // matrices are read once per tile and not once per row:
-//   up to 256 tokens, one launch (lora_small_kernel): every CTA finds its tile
+//   up to 384 tokens, one launch (lora_small_kernel): every CTA finds its tile
 //     of up to 16 rows from the ids; a cluster of CTAs shares a tile, each
 //     shrinks a part of K, sends its sums to the others' shared memory and
 //     expands a part of the columns;
@@ -45,7 +45,10 @@
 
 namespace tfo {
 
-constexpr int kSmallTokens = 256;  // at most: each CTA reads all ids (one per thread)
+// At most: each CTA reads all ids (two per thread). Measured over five sets of
+// adapters and sizes, this way / sorted: 300 tokens 10-15 / 14-21 us, 400
+// 11-19 / 15-22, 512 15-25 / 16-23.
+constexpr int kSmallTokens = 384;
 constexpr int kSmallRows = 16, kSmallWarps = 8, kMaxCluster = 8;
 constexpr int kLargeRows = 64, kLargeThreads = 256;
 
@@ -160,41 +163,64 @@ struct Tile {
   int group, count;  // count 0: nothing to do
 };
 
-// Tile `index` of at most 256 rows, by the whole CTA (256 threads); rows gets
-// its rows. A row leads a tile if 0, 16, 32, ... rows before it are of its
-// group; tiles are counted in the order of their leaders.
+// Tile `index` of at most kSmallTokens rows, by the whole CTA (256 threads of
+// kIds rows each); rows gets its rows. A row leads a tile if 0, 16, 32, ...
+// rows before it are of its group; tiles are counted in the order of their
+// leaders.
+constexpr int kIds = (kSmallTokens + 255) / 256;
 __device__ __forceinline__ Tile find_tile(const LoraArgs& a, int index, int* rows, int* groups, int* scratch) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int tokens = static_cast<int>(a.tokens);
-  const int group = t < tokens ? row_group(a, t) : -1;
-  groups[t] = group;
+  int group[kIds], rank[kIds], before[kIds];  // rank: rows of the group before this one
+  bool leads[kIds];
+#pragma unroll
+  for (int k = 0; k < kIds; ++k) {
+    const int i = k * 256 + t;
+    group[k] = i < tokens ? row_group(a, i) : -1;
+    if (k * 256 < tokens) groups[i] = group[k];
+  }
+  if (t == 0) scratch[8 * kIds] = -1;
   __syncthreads();
-  int rank = 0;  // rows of the group before this one
-  const int end = t < tokens ? t : 0;
+#pragma unroll
+  for (int k = 0; k < kIds; ++k) {
+    rank[k] = before[k] = 0;
+    leads[k] = false;
+    if (k * 256 >= tokens) continue;
+    const int end = k * 256 + t < tokens ? k * 256 + t : 0;
 #pragma unroll 8
-  for (int i = 0; i + 4 <= end; i += 4) {
-    const int4 g = *reinterpret_cast<const int4*>(groups + i);
-    rank += (g.x == group) + (g.y == group) + (g.z == group) + (g.w == group);
-  }
-  for (int i = end & ~3; i < end; ++i) rank += groups[i] == group;
-  const bool leads = group >= 0 && rank % kSmallRows == 0;
-  const uint32_t votes = __ballot_sync(0xffffffffu, leads);
-  if (lane == 0) scratch[warp] = __popc(votes);
-  if (t == 0) scratch[8] = -1;
-  __syncthreads();
-  int before = __popc(votes & ((1u << lane) - 1));
-  for (int w = 0; w < warp; ++w) before += scratch[w];
-  if (leads && before == index) {
-    scratch[8] = t;
-    scratch[9] = rank;
+    for (int i = 0; i + 4 <= end; i += 4) {
+      const int4 g = *reinterpret_cast<const int4*>(groups + i);
+      rank[k] += (g.x == group[k]) + (g.y == group[k]) + (g.z == group[k]) + (g.w == group[k]);
+    }
+    for (int i = end & ~3; i < end; ++i) rank[k] += groups[i] == group[k];
+    leads[k] = group[k] >= 0 && rank[k] % kSmallRows == 0;
+    const uint32_t votes = __ballot_sync(0xffffffffu, leads[k]);
+    if (lane == 0) scratch[k * 8 + warp] = __popc(votes);
+    before[k] = __popc(votes & ((1u << lane) - 1));
   }
   __syncthreads();
-  const int lead = scratch[8];
+#pragma unroll
+  for (int k = 0; k < kIds; ++k) {
+    if (k * 256 >= tokens) continue;
+    for (int w = 0; w < k * 8 + warp; ++w) before[k] += scratch[w];
+    if (leads[k] && before[k] == index) {
+      scratch[8 * kIds] = k * 256 + t;
+      scratch[8 * kIds + 1] = rank[k];
+    }
+  }
+  __syncthreads();
+  const int lead = scratch[8 * kIds];
   if (lead < 0) return Tile{0, 0};
-  const int want = groups[lead], place = rank - scratch[9];
-  const bool mine = group == want && place >= 0 && place < kSmallRows;
-  if (mine) rows[place] = t;
-  const int count = __syncthreads_count(mine);
+  const int want = groups[lead];
+  int count = 0;
+#pragma unroll
+  for (int k = 0; k < kIds; ++k) {
+    if (k * 256 >= tokens) continue;
+    const int place = rank[k] - scratch[8 * kIds + 1];
+    const bool mine = group[k] == want && place >= 0 && place < kSmallRows;
+    if (mine) rows[place] = k * 256 + t;
+    count += __syncthreads_count(mine);
+  }
   return Tile{want, count};
 }
 
@@ -629,8 +655,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) lora_small_kernel
   constexpr int M = kSmallRows, RB = 8 * NT;  // ranks of a pass
   constexpr int BATCH = NT == 8 ? 1 : 2;
   constexpr bool SCALED = std::is_same<T, __half>::value;
-  __shared__ int rows[M], scratch[10];
-  __shared__ __align__(16) int groups[kSmallTokens];
+  __shared__ int rows[M], scratch[8 * kIds + 2];
+  __shared__ __align__(16) int groups[kIds * 256];
   __shared__ float row_scale[M];
   __shared__ unsigned row_max[M];
   __shared__ uint64_t received;

@@ -2,7 +2,7 @@
 
 ``fused_lora`` adds ``scaling[i] * B[i] (A[i] x[t])`` of each row's own adapter
 ``i`` to the shared projection's output (``tfo_lora``, csrc/lora.cu: one launch
-for up to 256 rows, a sort and one launch for more), whatever the order of the
+for up to 384 rows, a sort and one launch for more), whatever the order of the
 requests. ``FP8LoRALinear`` is
 :class:`~triton_ops.kernels.fp8_gemm.FP8Linear` with such adapters.
 
