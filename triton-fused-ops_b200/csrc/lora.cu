@@ -41,6 +41,10 @@
 // the row's largest value, by which the row is scaled to stay in fp16's
 // range); fp32 operands are split into two tf32 values on both sides and the
 // three larger products are added. The result is rounded once.
+#include <map>
+#include <mutex>
+#include <tuple>
+
 #include "heads.cuh"
 
 namespace tfo {
@@ -1144,6 +1148,48 @@ cudaError_t launch_grid(void (*kernel)(KArgs...), dim3 grid, int block, int clus
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// Clusters of a kernel that are resident at once (the SMs of a cluster share a
+// processing cluster: fewer than their CTAs alone would allow).
+cudaError_t resident_clusters(const void* kernel, int block, int cluster, size_t smem, int* count) {
+  if (const cudaError_t e = ensure_smem_attr(kernel, smem + 4096); e != cudaSuccess) return e;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, size_t, int, int>, int> known;
+  std::lock_guard<std::mutex> lock(mu);
+  const auto [at, fresh] = known.try_emplace(std::make_tuple(kernel, smem, cluster, dev), 0);
+  if (fresh) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(cluster));
+    cfg.blockDim = dim3(static_cast<unsigned>(block));
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (const cudaError_t e = cudaOccupancyMaxActiveClusters(&at->second, kernel, &cfg); e != cudaSuccess) {
+      known.erase(at);
+      return e;
+    }
+  }
+  *count = at->second;
+  return cudaSuccess;
+}
+
+// Few clusters: an SM for each CTA, by asking for more than half of its memory
+// (two would share one while others idle: 64 tokens over 8 adapters of rank 64
+// 10.8 -> 9.0 us, 512 over 4 of rank 16 16.7 -> 14.2; 4096 x 4096).
+cudaError_t spread(const void* kernel, int block, int cluster, int64_t clusters, size_t* smem) {
+  constexpr size_t kAlone = 120 * 1024;
+  if (*smem >= kAlone || clusters * cluster > num_sms()) return cudaSuccess;
+  int resident = 0;
+  const cudaError_t e = resident_clusters(kernel, block, cluster, kAlone, &resident);
+  if (e == cudaSuccess && clusters <= resident) *smem = kAlone;
+  return e;
+}
+
 // Elements that rows of `length` starting at p (and `stride` apart) are aligned to: 16 bytes' worth, 8's, or 1.
 template <typename T>
 int row_width(const void* p, int64_t length, int64_t stride) {
@@ -1178,8 +1224,9 @@ cudaError_t launch_small(const LoraArgs& a, cudaStream_t st) {
     cluster *= 2;
   const size_t smem = kSmallRows * (sizeof(float) * v_rank * cluster + (sizeof(T) == 2 ? 2 : 1) * sizeof(T) * (v_rank + E));
   auto launch = [&](auto* kernel, int nt) {
-    const size_t red = sizeof(float) * kSmallWarps * kSmallRows * (8 * nt + 4);
-    return launch_grid(kernel, dim3(static_cast<unsigned>(tiles * cluster)), 256, cluster, smem + red, st, a, log2_of(cluster),
+    size_t bytes = smem + sizeof(float) * kSmallWarps * kSmallRows * (8 * nt + 4);
+    if (const cudaError_t e = spread(reinterpret_cast<const void*>(kernel), 256, cluster, tiles, &bytes); e != cudaSuccess) return e;
+    return launch_grid(kernel, dim3(static_cast<unsigned>(tiles * cluster)), 256, cluster, bytes, st, a, log2_of(cluster),
                        width, v_rank, error_word_ptr());
   };
   const bool vec = width.k == E && width.b == E && width.n;
@@ -1193,21 +1240,27 @@ cudaError_t launch_shape(const LoraArgs& a, const PlanBytes& p, const LoraPlan& 
   using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
   // As many CTAs a tile as are resident at once with the tiles to expect (more
   // of them only queue: 8192 tokens, 136 tiles, rank 32: 62 / 50 / 84 us for
-  // one, two, four), each with four steps of K at least.
+  // one, two, four), each with four steps of K or of the columns at least. A few
+  // queued ones cost less than half the CTAs (4096 tokens, 72 tiles for 70
+  // clusters of four: 40 us, with clusters of two 44).
   auto* kernel = lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>;
-  const void* fn = reinterpret_cast<const void*>(kernel);
   const int64_t groups = std::min(a.tokens, a.adapters + 1);
   const int64_t likely = std::max(groups, a.tokens / kLargeRows + groups / 2);
-  const int64_t steps = (a.k + S::KS - 1) / S::KS;
+  const int64_t steps = (std::max(a.k, a.n) + S::KS - 1) / S::KS;
   int cluster = 1;
   while (cluster < kMaxCluster && 8 * cluster <= steps && S::smem(2 * cluster) <= 216 * 1024) {
-    const size_t smem = S::smem(2 * cluster);
-    if (const cudaError_t e = ensure_smem_attr(fn, smem + 4096); e != cudaSuccess) return e;
-    if (likely * 2 * cluster > static_cast<int64_t>(num_sms()) * cached_occupancy(fn, kLargeThreads, smem)) break;
+    int resident = 0;
+    if (const cudaError_t e = resident_clusters(reinterpret_cast<const void*>(kernel), kLargeThreads, 2 * cluster, S::smem(2 * cluster), &resident);
+        e != cudaSuccess)
+      return e;
+    if (likely > resident + resident / 8) break;
     cluster *= 2;
   }
-  return launch_grid(lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>, dim3(static_cast<unsigned>(p.tiles * cluster)),
-                     kLargeThreads, cluster, S::smem(cluster), st, a, plan, log2_of(cluster), error_word_ptr());
+  size_t smem = S::smem(cluster);
+  if (const cudaError_t e = spread(reinterpret_cast<const void*>(kernel), kLargeThreads, cluster, likely, &smem); e != cudaSuccess)
+    return e;
+  return launch_grid(kernel, dim3(static_cast<unsigned>(p.tiles * cluster)), kLargeThreads, cluster, smem, st, a, plan,
+                     log2_of(cluster), error_word_ptr());
 }
 
 template <typename T>
@@ -1232,14 +1285,15 @@ cudaError_t launch_large(const LoraArgs& a, void* ws, cudaStream_t st) {
        : launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, false>(a, p, plan, st))
   // 256 bytes of a row a step: fewer barriers, one or two CTAs on an SM. 8192
   // tokens (136 tiles) 61 -> 50 us; 1024 tokens over 32 adapters (33 tiles, four
-  // CTAs each instead of two) 19 -> 24 us.
+  // CTAs each instead of two) 19 -> 24 us. Three stages of rank 32 let two CTAs
+  // on an SM in clusters of eight (512 tokens over 16 adapters 22.6 -> 17.4 us).
   const int64_t groups = std::min(a.tokens, a.adapters + 1);
   const bool wide = std::max(groups, a.tokens / kLargeRows + groups / 2) * 3 >= num_sms() * 2;
   if (a.rank <= 16 && wide) return TFO_LORA(16, 16, 256, 3);
   if (a.rank <= 32 && wide) return TFO_LORA(32, 32, 256, 3);
   if (a.rank <= 64 && wide) return TFO_LORA(64, 64, 256, 3);
   if (a.rank <= 16) return TFO_LORA(16, 16, 128, 4);
-  if (a.rank <= 32) return TFO_LORA(32, 32, 128, 4);
+  if (a.rank <= 32) return TFO_LORA(32, 32, 128, 3);
   if (a.rank <= 64) return TFO_LORA(64, 64, 128, 4);
   if (a.rank <= 128) return TFO_LORA(128, 128, 128, 3);
   return TFO_LORA(128, 256, 128, 2);
