@@ -1283,15 +1283,20 @@ cudaError_t launch_large(const LoraArgs& a, void* ws, cudaStream_t st) {
 #define TFO_LORA(RANKS, VR, STEP, STAGES)                                        \
   (vec ? launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, true>(a, p, plan, st) \
        : launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, false>(a, p, plan, st))
-  // 256 bytes of a row a step: fewer barriers, one or two CTAs on an SM. 8192
-  // tokens (136 tiles) 61 -> 50 us; 1024 tokens over 32 adapters (33 tiles, four
-  // CTAs each instead of two) 19 -> 24 us. Three stages of rank 32 let two CTAs
-  // on an SM in clusters of eight (512 tokens over 16 adapters 22.6 -> 17.4 us).
+  // 256 bytes of a row a step mean fewer barriers, but fewer CTAs on an SM. By
+  // the tiles to expect, for each SM (us with 256 / 128 bytes, 4096 x 4096 bf16):
+  //   rank 16: 0.17 20.1 / 20.1; 0.22 24 / 19; 0.27 27.6 / 31.8; 0.37 28.7 / 33.7;
+  //            0.54 43.5 / 36.0 (clusters of two instead of four); 0.9 50 / 61
+  //   rank 32: 0.21 33.2 / 29.4; 0.27 33.6 / 30.9; 0.45 35.0 / 34.1; 0.49 35.7 / 44.8;
+  //            0.54 45.6 / 49.6
+  //   rank 64: 0.17 28.1 / 28.1; 0.27 40.8 / 43.8; 0.45 41.8 / 44.9; 0.54 73.7 / 80.1
+  // Three stages of rank 32 let two CTAs on an SM in clusters of eight (512
+  // tokens over 16 adapters 22.6 -> 17.4 us).
   const int64_t groups = std::min(a.tokens, a.adapters + 1);
-  const bool wide = std::max(groups, a.tokens / kLargeRows + groups / 2) * 3 >= num_sms() * 2;
-  if (a.rank <= 16 && wide) return TFO_LORA(16, 16, 256, 3);
-  if (a.rank <= 32 && wide) return TFO_LORA(32, 32, 256, 3);
-  if (a.rank <= 64 && wide) return TFO_LORA(64, 64, 256, 3);
+  const double tiles = static_cast<double>(std::max(groups, a.tokens / kLargeRows + groups / 2)) / num_sms();
+  if (a.rank <= 16 && ((tiles >= 0.25 && tiles < 0.5) || tiles >= 0.67)) return TFO_LORA(16, 16, 256, 3);
+  if (a.rank > 16 && a.rank <= 32 && tiles >= 0.47) return TFO_LORA(32, 32, 256, 3);
+  if (a.rank > 32 && a.rank <= 64 && tiles >= 0.2) return TFO_LORA(64, 64, 256, 3);
   if (a.rank <= 16) return TFO_LORA(16, 16, 128, 4);
   if (a.rank <= 32) return TFO_LORA(32, 32, 128, 3);
   if (a.rank <= 64) return TFO_LORA(64, 64, 128, 4);
