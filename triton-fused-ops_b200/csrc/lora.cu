@@ -1235,37 +1235,78 @@ cudaError_t launch_small(const LoraArgs& a, cudaStream_t st) {
   return vec ? launch(lora_small_kernel<T, 8, true>, 8) : launch(lora_small_kernel<T, 8, false>, 8);
 }
 
-template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
-cudaError_t launch_shape(const LoraArgs& a, const PlanBytes& p, const LoraPlan& plan, cudaStream_t st) {
-  using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
-  // As many CTAs a tile as are resident at once with the tiles to expect (more
-  // of them only queue: 8192 tokens, 136 tiles, rank 32: 62 / 50 / 84 us for
-  // one, two, four), each with four steps of K or of the columns at least. A few
-  // queued ones cost less than half the CTAs (4096 tokens, 72 tiles for 70
-  // clusters of four: 40 us, with clusters of two 44).
-  auto* kernel = lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>;
-  const int64_t groups = std::min(a.tokens, a.adapters + 1);
-  const int64_t likely = std::max(groups, a.tokens / kLargeRows + groups / 2);
-  const int64_t steps = (std::max(a.k, a.n) + S::KS - 1) / S::KS;
+// The number of CTAs that share a tile, and the time to expect. The tiles run
+// in waves of as many clusters as are resident at once; a tile's time is 5 us
+// (first loads, the exchange) and its steps, shared by the cluster. Measured
+// for rows of K + N = 8192 bf16 values, alone on a tile: 72 us with 256 bytes a
+// step, 83 with 128. Less than a whole wave costs a whole one (4096 x 4096,
+// rank 16, 256 bytes: 8192 tokens 50 us, 12000 84, 16384 88), so that more
+// CTAs on an SM, or larger clusters, pay where they save a wave (12000 tokens
+// with 128 bytes a step 66).
+struct ShapeChoice {
   int cluster = 1;
-  while (cluster < kMaxCluster && 8 * cluster <= steps && S::smem(2 * cluster) <= 216 * 1024) {
+  double us = 0;
+};
+template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
+cudaError_t choose_cluster(const LoraArgs& a, int64_t tiles, ShapeChoice* best) {
+  using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
+  const void* kernel = reinterpret_cast<const void*>(lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>);
+  const int64_t steps = (std::max(a.k, a.n) + S::KS - 1) / S::KS;
+  const double alone = static_cast<double>(a.k + a.n) * sizeof(T) / 16384 * (STEP >= 256 ? 72 : 83);
+  for (int c = 1; c <= kMaxCluster && (c == 1 || 4 * c <= steps) && (c == 1 || S::smem(c) <= 216 * 1024); c *= 2) {
     int resident = 0;
-    if (const cudaError_t e = resident_clusters(reinterpret_cast<const void*>(kernel), kLargeThreads, 2 * cluster, S::smem(2 * cluster), &resident);
-        e != cudaSuccess)
-      return e;
-    if (likely > resident + resident / 8) break;
-    cluster *= 2;
+    if (const cudaError_t e = resident_clusters(kernel, kLargeThreads, c, S::smem(c), &resident); e != cudaSuccess) return e;
+    const int64_t waves = (tiles + std::max(resident, 1) - 1) / std::max(resident, 1);
+    const double us = static_cast<double>(waves) * (5 + alone / c);
+    if (c == 1 || us < best->us) *best = ShapeChoice{c, us};
   }
+  return cudaSuccess;
+}
+
+template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
+cudaError_t launch_shape(const LoraArgs& a, const PlanBytes& p, const LoraPlan& plan, int64_t tiles, int cluster, cudaStream_t st) {
+  using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
+  auto* kernel = lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>;
   size_t smem = S::smem(cluster);
-  if (const cudaError_t e = spread(reinterpret_cast<const void*>(kernel), kLargeThreads, cluster, likely, &smem); e != cudaSuccess)
+  if (const cudaError_t e = spread(reinterpret_cast<const void*>(kernel), kLargeThreads, cluster, tiles, &smem); e != cudaSuccess)
     return e;
   return launch_grid(kernel, dim3(static_cast<unsigned>(p.tiles * cluster)), kLargeThreads, cluster, smem, st, a, plan,
                      log2_of(cluster), error_word_ptr());
 }
 
+// Up to 64 ranks: 128 or 256 bytes of a row a step, whichever is expected to be faster.
+template <typename T, int RANKS, int STAGES, bool VEC>
+cudaError_t launch_best(const LoraArgs& a, const PlanBytes& p, const LoraPlan& plan, int64_t tiles, cudaStream_t st) {
+  constexpr int C = chunk_elems(sizeof(T)), VR = RANKS > C ? RANKS : C;
+  ShapeChoice narrow, wide;
+  if (const cudaError_t e = choose_cluster<T, RANKS, VR, 128, STAGES, VEC>(a, tiles, &narrow); e != cudaSuccess) return e;
+  if (const cudaError_t e = choose_cluster<T, RANKS, VR, 256, 3, VEC>(a, tiles, &wide); e != cudaSuccess) return e;
+  if (wide.us < narrow.us) return launch_shape<T, RANKS, VR, 256, 3, VEC>(a, p, plan, tiles, wide.cluster, st);
+  return launch_shape<T, RANKS, VR, 128, STAGES, VEC>(a, p, plan, tiles, narrow.cluster, st);
+}
+
+// More ranks: in passes of 128.
+template <typename T, int VR, int STAGES, bool VEC>
+cudaError_t launch_ranks(const LoraArgs& a, const PlanBytes& p, const LoraPlan& plan, int64_t tiles, cudaStream_t st) {
+  ShapeChoice choice;
+  if (const cudaError_t e = choose_cluster<T, 128, VR, 128, STAGES, VEC>(a, tiles, &choice); e != cudaSuccess) return e;
+  return launch_shape<T, 128, VR, 128, STAGES, VEC>(a, p, plan, tiles, choice.cluster, st);
+}
+
+template <typename T, bool VEC>
+cudaError_t launch_tiles(const LoraArgs& a, const PlanBytes& p, const LoraPlan& plan, cudaStream_t st) {
+  // the tiles to expect: each group's last one is half full on average
+  const int64_t groups = std::min(a.tokens, a.adapters + 1);
+  const int64_t tiles = std::max(groups, a.tokens / kLargeRows + groups / 2);
+  if (a.rank <= 16) return launch_best<T, 16, 4, VEC>(a, p, plan, tiles, st);
+  if (a.rank <= 32) return launch_best<T, 32, 3, VEC>(a, p, plan, tiles, st);  // three stages: two CTAs on an SM in clusters of eight
+  if (a.rank <= 64) return launch_best<T, 64, 4, VEC>(a, p, plan, tiles, st);
+  return a.rank <= 128 ? launch_ranks<T, 128, 3, VEC>(a, p, plan, tiles, st) : launch_ranks<T, 256, 2, VEC>(a, p, plan, tiles, st);
+}
+
 template <typename T>
 cudaError_t launch_large(const LoraArgs& a, void* ws, cudaStream_t st) {
-  constexpr int E = 16 / sizeof(T), C = chunk_elems(sizeof(T));
+  constexpr int E = 16 / sizeof(T);
   const PlanBytes p = plan_bytes(a.tokens, a.adapters);
   char* at = static_cast<char*>(ws);
   const LoraPlan plan{reinterpret_cast<int*>(at), reinterpret_cast<int4*>(at + p.perm),
@@ -1280,29 +1321,7 @@ cudaError_t launch_large(const LoraArgs& a, void* ws, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const bool vec = row_width<T>(a.x, a.k, a.x_stride) == E && row_width<T>(a.a, a.k, 0) == E &&
                    row_width<T>(a.b, a.rank, 0) == E && output_vectors<T>(a);
-#define TFO_LORA(RANKS, VR, STEP, STAGES)                                        \
-  (vec ? launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, true>(a, p, plan, st) \
-       : launch_shape<T, RANKS, (VR > C ? VR : C), STEP, STAGES, false>(a, p, plan, st))
-  // 256 bytes of a row a step mean fewer barriers, but fewer CTAs on an SM. By
-  // the tiles to expect, for each SM (us with 256 / 128 bytes, 4096 x 4096 bf16):
-  //   rank 16: 0.17 20.1 / 20.1; 0.22 24 / 19; 0.27 27.6 / 31.8; 0.37 28.7 / 33.7;
-  //            0.54 43.5 / 36.0 (clusters of two instead of four); 0.9 50 / 61
-  //   rank 32: 0.21 33.2 / 29.4; 0.27 33.6 / 30.9; 0.45 35.0 / 34.1; 0.49 35.7 / 44.8;
-  //            0.54 45.6 / 49.6
-  //   rank 64: 0.17 28.1 / 28.1; 0.27 40.8 / 43.8; 0.45 41.8 / 44.9; 0.54 73.7 / 80.1
-  // Three stages of rank 32 let two CTAs on an SM in clusters of eight (512
-  // tokens over 16 adapters 22.6 -> 17.4 us).
-  const int64_t groups = std::min(a.tokens, a.adapters + 1);
-  const double tiles = static_cast<double>(std::max(groups, a.tokens / kLargeRows + groups / 2)) / num_sms();
-  if (a.rank <= 16 && ((tiles >= 0.25 && tiles < 0.5) || tiles >= 0.67)) return TFO_LORA(16, 16, 256, 3);
-  if (a.rank > 16 && a.rank <= 32 && tiles >= 0.47) return TFO_LORA(32, 32, 256, 3);
-  if (a.rank > 32 && a.rank <= 64 && tiles >= 0.2) return TFO_LORA(64, 64, 256, 3);
-  if (a.rank <= 16) return TFO_LORA(16, 16, 128, 4);
-  if (a.rank <= 32) return TFO_LORA(32, 32, 128, 3);
-  if (a.rank <= 64) return TFO_LORA(64, 64, 128, 4);
-  if (a.rank <= 128) return TFO_LORA(128, 128, 128, 3);
-  return TFO_LORA(128, 256, 128, 2);
-#undef TFO_LORA
+  return vec ? launch_tiles<T, true>(a, p, plan, st) : launch_tiles<T, false>(a, p, plan, st);
 }
 
 template <typename T>
