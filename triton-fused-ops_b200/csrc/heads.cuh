@@ -339,6 +339,28 @@ struct LaneGroup {
     for (int i = 0; i < lanes; ++i) t += __shfl_sync(0xffffffffu, v, base + i);
     return t;
   }
+  // Two sums side by side: their shuffles overlap.
+  template <int O> __device__ static void xor_add(float& u, float& v) {
+    const float a = __shfl_xor_sync(0xffffffffu, u, O), b = __shfl_xor_sync(0xffffffffu, v, O);
+    u += a;
+    v += b;
+  }
+  __device__ void sum(float& u, float& v) const {
+    if (lanes == 8 || lanes == 16 || lanes == 4) {
+      if (lanes == 16) xor_add<8>(u, v);
+      if (lanes >= 8) xor_add<4>(u, v);
+      xor_add<2>(u, v);
+      xor_add<1>(u, v);
+    } else {
+      float s = 0.f, t = 0.f;
+      for (int i = 0; i < lanes; ++i) {
+        s += __shfl_sync(0xffffffffu, u, base + i);
+        t += __shfl_sync(0xffffffffu, v, base + i);
+      }
+      u = s;
+      v = t;
+    }
+  }
 };
 
 // CTAs [0, q_ctas) of a streaming launch take the queries, the rest the keys.

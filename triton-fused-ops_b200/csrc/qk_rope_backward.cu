@@ -111,8 +111,10 @@ __global__ void __launch_bounds__(kBwdThreads, 2) qk_norm_rope_backward_kernel(
         tb[j] = mul2(fb[j], ub[j]);
         dot = fma2(tb[j], wb[j], fma2(ta[j], wa[j], dot));
       }
-      const float r = rsqrtf(group.sum(ss.x + ss.y) * inv_d + a.eps);
-      const float k = group.sum(dot.x + dot.y) * inv_d * r * r * r;  // in this order: r^3 alone can overflow
+      float squares = ss.x + ss.y, products = dot.x + dot.y;
+      group.sum(squares, products);
+      const float r = rsqrtf(squares * inv_d + a.eps);
+      const float k = products * inv_d * r * r * r;  // in this order: r^3 alone can overflow
       if (i < mine) {
         const F2 r2 = f2(r, r), k2 = f2(-k, -k);
 #pragma unroll
