@@ -339,26 +339,28 @@ struct LaneGroup {
     for (int i = 0; i < lanes; ++i) t += __shfl_sync(0xffffffffu, v, base + i);
     return t;
   }
-  // Two sums side by side: their shuffles overlap.
-  template <int O> __device__ static void xor_add(float& u, float& v) {
-    const float a = __shfl_xor_sync(0xffffffffu, u, O), b = __shfl_xor_sync(0xffffffffu, v, O);
-    u += a;
-    v += b;
+  // Sums side by side: their shuffles overlap.
+  template <int O, int N> __device__ static void xor_add(float (&v)[N]) {
+    float o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = __shfl_xor_sync(0xffffffffu, v[i], O);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += o[i];
   }
-  __device__ void sum(float& u, float& v) const {
+  template <int N> __device__ void sum(float (&v)[N]) const {
     if (lanes == 8 || lanes == 16 || lanes == 4) {
-      if (lanes == 16) xor_add<8>(u, v);
-      if (lanes >= 8) xor_add<4>(u, v);
-      xor_add<2>(u, v);
-      xor_add<1>(u, v);
+      if (lanes == 16) xor_add<8>(v);
+      if (lanes >= 8) xor_add<4>(v);
+      xor_add<2>(v);
+      xor_add<1>(v);
     } else {
-      float s = 0.f, t = 0.f;
+      float t[N] = {};
       for (int i = 0; i < lanes; ++i) {
-        s += __shfl_sync(0xffffffffu, u, base + i);
-        t += __shfl_sync(0xffffffffu, v, base + i);
+#pragma unroll
+        for (int k = 0; k < N; ++k) t[k] += __shfl_sync(0xffffffffu, v[k], base + i);
       }
-      u = s;
-      v = t;
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = t[k];
     }
   }
 };

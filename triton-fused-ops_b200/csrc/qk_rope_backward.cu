@@ -14,8 +14,8 @@
 // atomics).
 //
 // Floor: HBM (x and dy read, dx written). Measured at 32768 tokens of 32 + 8
-// heads of 128 columns, bf16: 188 us with the weights' gradients, 82 % of the
-// measured copy rate; 8192 tokens 55 us (70 %). The two sums over a head's
+// heads of 128 columns, bf16: 183 us with the weights' gradients, 84 % of the
+// measured copy rate; 8192 tokens 53 us (73 %). The two sums over a head's
 // lanes and 128 registers a thread (16 warps an SM) bound it: the schedulers
 // issue in 49 % of the cycles and the rest is latency within a warp.
 #include "heads.cuh"
@@ -94,38 +94,58 @@ __global__ void __launch_bounds__(kBwdThreads, 2) qk_norm_rope_backward_kernel(
     }
     T* out = static_cast<T*>(side.out) + (static_cast<int64_t>(token) * heads + h0) * D + column;
     st.wait();
+    // Heads of full warps one at a time. Lane groups that are no power of two sum
+    // by a shuffle for each lane: there the sums of all heads go side by side and
+    // the heads are read again after them (12 + 3 heads of 80 columns, f16, 32768
+    // tokens 69.0 -> 62.6 us; heads of 128 no faster).
+    constexpr int AT_ONCE = FULL ? 1 : NH;
 #pragma unroll
-    for (int i = 0; i < NH; ++i) {
-      if (i >= most) break;
-      F2 ua[E / 2], ub[E / 2], fa[E / 2], fb[E / 2];
-      V::unpack(*st.slot(stage, 0, i, 0), ua);
-      V::unpack(*st.slot(stage, 0, i, 1), ub);
-      V::unpack(*st.slot(stage, 1, i, 0), fa);
-      V::unpack(*st.slot(stage, 1, i, 1), fb);
-      rot.apply(fa, fb, col);
-      F2 ss = f2(0.f, 0.f), dot = ss, ta[E / 2], tb[E / 2];
-#pragma unroll
-      for (int j = 0; j < E / 2; ++j) {
-        ss = fma2(ub[j], ub[j], fma2(ua[j], ua[j], ss));
-        ta[j] = mul2(fa[j], ua[j]);
-        tb[j] = mul2(fb[j], ub[j]);
-        dot = fma2(tb[j], wb[j], fma2(ta[j], wa[j], dot));
-      }
-      float squares = ss.x + ss.y, products = dot.x + dot.y;
-      group.sum(squares, products);
-      const float r = rsqrtf(squares * inv_d + a.eps);
-      const float k = products * inv_d * r * r * r;  // in this order: r^3 alone can overflow
-      if (i < mine) {
-        const F2 r2 = f2(r, r), k2 = f2(-k, -k);
+    for (int i0 = 0; i0 < NH; i0 += AT_ONCE) {
+      if (i0 >= most) break;
+      F2 ua[E / 2], ub[E / 2], fa[E / 2], fb[E / 2], ta[E / 2], tb[E / 2];
+      auto read = [&](int i) {  // a head, with its sums
+        V::unpack(*st.slot(stage, 0, i, 0), ua);
+        V::unpack(*st.slot(stage, 0, i, 1), ub);
+        V::unpack(*st.slot(stage, 1, i, 0), fa);
+        V::unpack(*st.slot(stage, 1, i, 1), fb);
+        rot.apply(fa, fb, col);
+        F2 ss = f2(0.f, 0.f), dot = ss;
 #pragma unroll
         for (int j = 0; j < E / 2; ++j) {
-          acc_a[j] = fma2(ta[j], r2, acc_a[j]);
-          acc_b[j] = fma2(tb[j], r2, acc_b[j]);
-          fa[j] = fma2(mul2(fa[j], wa[j]), r2, mul2(ua[j], k2));
-          fb[j] = fma2(mul2(fb[j], wb[j]), r2, mul2(ub[j], k2));
+          ss = fma2(ub[j], ub[j], fma2(ua[j], ua[j], ss));
+          ta[j] = mul2(fa[j], ua[j]);
+          tb[j] = mul2(fb[j], ub[j]);
+          dot = fma2(tb[j], wb[j], fma2(ta[j], wa[j], dot));
         }
-        if (FULL || st.has_a) V::store(out + i * D, fa);
-        if (FULL || st.has_b) V::store(out + i * D + st.vb_offset, fb);
+        return make_float2(ss.x + ss.y, dot.x + dot.y);
+      };
+      float sums[2 * AT_ONCE];  // of squares, and of b w x, of each head
+#pragma unroll
+      for (int n = 0; n < AT_ONCE; ++n) {
+        const float2 both = read(i0 + n);
+        sums[2 * n] = both.x;
+        sums[2 * n + 1] = both.y;
+      }
+      group.sum(sums);
+      if constexpr (AT_ONCE > 1) asm volatile("" ::: "memory");  // registers are not kept over the sums
+#pragma unroll
+      for (int n = 0; n < AT_ONCE; ++n) {
+        const int i = i0 + n;
+        if constexpr (AT_ONCE > 1) read(i);
+        const float r = rsqrtf(sums[2 * n] * inv_d + a.eps);
+        const float k = sums[2 * n + 1] * inv_d * r * r * r;  // in this order: r^3 alone can overflow
+        if (i < mine) {
+          const F2 r2 = f2(r, r), k2 = f2(-k, -k);
+#pragma unroll
+          for (int j = 0; j < E / 2; ++j) {
+            acc_a[j] = fma2(ta[j], r2, acc_a[j]);
+            acc_b[j] = fma2(tb[j], r2, acc_b[j]);
+            fa[j] = fma2(mul2(fa[j], wa[j]), r2, mul2(ua[j], k2));
+            fb[j] = fma2(mul2(fb[j], wb[j]), r2, mul2(ub[j], k2));
+          }
+          if (FULL || st.has_a) V::store(out + i * D, fa);
+          if (FULL || st.has_b) V::store(out + i * D + st.vb_offset, fb);
+        }
       }
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
