@@ -1256,6 +1256,7 @@ cudaError_t choose_cluster(const LoraArgs& a, int64_t tiles, ShapeChoice* best) 
   for (int c = 1; c <= kMaxCluster && (c == 1 || 4 * c <= steps) && (c == 1 || S::smem(c) <= 216 * 1024); c *= 2) {
     int resident = 0;
     if (const cudaError_t e = resident_clusters(kernel, kLargeThreads, c, S::smem(c), &resident); e != cudaSuccess) return e;
+    if (resident == 0 && c > 1) break;  // no room for such a cluster
     const int64_t waves = (tiles + std::max(resident, 1) - 1) / std::max(resident, 1);
     const double us = static_cast<double>(waves) * (5 + alone / c);
     if (c == 1 || us < best->us) *best = ShapeChoice{c, us};

@@ -14,8 +14,8 @@
 //
 // Measured: 8 x 8192 tokens of 32 + 8 heads of 128 columns, bf16, with the
 // norm: 215 us, 95 % of the measured copy rate (1.34 GB); 65536 tokens of
-// 16 + 16 heads of 64, fp32: 174 us (94 %); of 12 + 3 heads of 80, f16: 73 us
-// (66 %; five lanes a head, summed by five shuffles); of 8 + 1 heads of 256,
+// 16 + 16 heads of 64, fp32: 174 us (94 %); of 12 + 3 heads of 80, f16: 69 us
+// (70 %; five lanes a head, summed by five shuffles); of 8 + 1 heads of 256,
 // bf16: 126 us (73 %; a key head's table row costs as much as itself). One
 // token: 1.9 us, a launch.
 #include "heads.cuh"
@@ -25,19 +25,23 @@ namespace tfo {
 template <int E, bool PAIRS, bool NORM>
 using Rotation = std::conditional_t<NORM, WeightedRotation<E, PAIRS>, PlainRotation<E, PAIRS>>;
 
-// One head on a lane's two vectors, in place.
+// This lane's part of a head's sum of squares.
+template <int E>
+__device__ __forceinline__ float lane_squares(const F2 (&fa)[E / 2], const F2 (&fb)[E / 2]) {
+  F2 ss = mul2(fa[0], fa[0]);
+#pragma unroll
+  for (int j = 1; j < E / 2; ++j) ss = fma2(fa[j], fa[j], ss);
+#pragma unroll
+  for (int j = 0; j < E / 2; ++j) ss = fma2(fb[j], fb[j], ss);
+  return ss.x + ss.y;
+}
+
+// One head on a lane's two vectors, in place; `squares`: of the whole head.
 template <int E, bool PAIRS, bool NORM>
 __device__ __forceinline__ void norm_rotate(F2 (&fa)[E / 2], F2 (&fb)[E / 2], const Rotation<E, PAIRS, NORM>& rot, const LaneCols& col,
-                                            const LaneGroup& group, float inv_d, float eps) {
+                                            float squares, float inv_d, float eps) {
   float rstd = 1.f;
-  if constexpr (NORM) {
-    F2 ss = mul2(fa[0], fa[0]);
-#pragma unroll
-    for (int j = 1; j < E / 2; ++j) ss = fma2(fa[j], fa[j], ss);
-#pragma unroll
-    for (int j = 0; j < E / 2; ++j) ss = fma2(fb[j], fb[j], ss);
-    rstd = rsqrtf(group.sum(ss.x + ss.y) * inv_d + eps);
-  }
+  if constexpr (NORM) rstd = rsqrtf(squares * inv_d + eps);
   rot.apply(fa, fb, col);
   if constexpr (NORM) {
     const F2 r2 = f2(rstd, rstd);
@@ -106,7 +110,8 @@ __global__ void __launch_bounds__(256) qk_rope_kernel(const HeadArgs a, int lane
     F2 fa[E / 2], fb[E / 2];
     V::unpack(ra[i], fa);
     V::unpack(rb[i], fb);
-    norm_rotate<E, PAIRS, NORM>(fa, fb, rot, col, group, inv_d, a.eps);
+    const float squares = NORM ? group.sum(lane_squares<E>(fa, fb)) : 0.f;
+    norm_rotate<E, PAIRS, NORM>(fa, fb, rot, col, squares, inv_d, a.eps);
     if (i < heads) {
       if (col.va >= 0) V::store(out + i * D + col.va * E, fa);
       if (col.vb >= 0) V::store(out + i * D + col.vb * E, fb);
@@ -162,16 +167,36 @@ __global__ void __launch_bounds__(256, 2) qk_rope_stream_kernel(const HeadArgs a
     token_rotation<E, PAIRS, NORM>(rot, a, side, col, pos);
     T* out = static_cast<T*>(side.out) + (static_cast<int64_t>(token) * heads + h0) * D + column;
     st.wait();
+    // Lane groups that are no power of two sum by a shuffle for each lane: there
+    // the heads' sums go side by side and the heads are read again after them
+    // (12 + 3 heads of 80, f16, 65536 tokens 72.4 -> 68.8 us).
+    constexpr int AT_ONCE = FULL || !NORM ? 1 : NH;
 #pragma unroll
-    for (int i = 0; i < NH; ++i) {
-      if (i >= most) break;
+    for (int i0 = 0; i0 < NH; i0 += AT_ONCE) {
+      if (i0 >= most) break;
       F2 fa[E / 2], fb[E / 2];
-      V::unpack(*st.slot(stage, 0, i, 0), fa);
-      V::unpack(*st.slot(stage, 0, i, 1), fb);
-      norm_rotate<E, PAIRS, NORM>(fa, fb, rot, col, group, inv_d, a.eps);
-      if (i < mine) {
-        if (FULL || st.has_a) V::store(out + i * D, fa);
-        if (FULL || st.has_b) V::store(out + i * D + st.vb_offset, fb);
+      auto read = [&](int i) {
+        V::unpack(*st.slot(stage, 0, i, 0), fa);
+        V::unpack(*st.slot(stage, 0, i, 1), fb);
+      };
+      float squares[AT_ONCE] = {};
+#pragma unroll
+      for (int n = 0; n < AT_ONCE; ++n) {
+        read(i0 + n);
+        if constexpr (NORM) squares[n] = lane_squares<E>(fa, fb);
+      }
+      if constexpr (NORM && AT_ONCE == 1) squares[0] = group.sum(squares[0]);
+      if constexpr (NORM && AT_ONCE > 1) group.sum(squares);
+      if constexpr (AT_ONCE > 1) asm volatile("" ::: "memory");  // registers are not kept over the sums
+#pragma unroll
+      for (int n = 0; n < AT_ONCE; ++n) {
+        const int i = i0 + n;
+        if constexpr (AT_ONCE > 1) read(i);
+        norm_rotate<E, PAIRS, NORM>(fa, fb, rot, col, squares[n], inv_d, a.eps);
+        if (i < mine) {
+          if (FULL || st.has_a) V::store(out + i * D, fa);
+          if (FULL || st.has_b) V::store(out + i * D + st.vb_offset, fb);
+        }
       }
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;

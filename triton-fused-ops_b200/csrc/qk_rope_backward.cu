@@ -310,7 +310,7 @@ template <typename T, int E, bool PAIRS>
 cudaError_t launch_vec(const HeadArgs& a, SideSplit* split, float* partials, cudaStream_t st) {
   // 16-byte slots: 3 heads x 2 tensors x 2 stages = 96 KB a CTA, two CTAs an SM.
   // Measured, us at 8192 / 32768 tokens of 32 + 8 heads of 128 columns, bf16:
-  // 3 heads, 2 stages 55 / 188; 2 heads, 3 stages 59 / 215; 1 head, 5 stages
+  // 3 heads, 2 stages 53 / 183; 2 heads, 3 stages 59 / 215; 1 head, 5 stages
   // 71 / 255; 4 heads, 2 stages (one CTA of 416 threads) 65 / 232.
   constexpr int NH = 3, STAGES = 2;
   const int lanes = (a.head_dim / E + 1) / 2;
