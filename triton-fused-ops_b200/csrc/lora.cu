@@ -1057,38 +1057,43 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
     load(free);
     if (busy && (BLOCKS > 1 || (step & 1) == half)) {
       constexpr int MINE = BLOCKS > 1 ? BLOCKS / 2 : 1;
+      const uint8_t* es = ring + now + e_at;
+      float acc[MINE][4][4] = {};
+      Eight<T> e0[MINE], e1[MINE];
+      // all blocks' operands before the first store, which the compiler would not move them over
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
         const int blk = BLOCKS > 1 ? half * MINE + i : 0;
-        const uint8_t* es = ring + now + e_at;
         const uint8_t* bs = ring + now + b_at + blk * 32 * NCH * 64;
-        float acc[4][4] = {};
         auto bf = [&](int j, int c) {  // chunk c of an odd row may be swapped
           const int on = (NCH & 1) ? c * 64 : ((c ^ (g & 1)) - (g & 1)) * 64;
           return lds16(bs + j * 2 * NCH * 64 + on);
         };
         if constexpr (HELD) {
-          held.expand(acc, bf);
+          held.expand(acc[i], bf);
         } else {
 #pragma unroll 2
-          for (int c = 0; c < NCH; ++c) expand_chunk<T>(acc, hi0, lo0, stride, c, bf);
+          for (int c = 0; c < NCH; ++c) expand_chunk<T>(acc[i], hi0, lo0, stride, c, bf);
         }
+        if constexpr (VEC) {
+#pragma unroll
+          for (int k = 0; k < Eight<T>::W; ++k) {
+            const int w = (blk * 4 + q) * Eight<T>::W + k;  // 16-byte vector of the row; odd rows' chunks are swapped
+            const uint32_t off = ((w >> 2) ^ (g & 1)) * 64 + (w & 3) * 16;
+            e0[i].u[k] = lds16(es + off);
+            e1[i].u[k] = lds16(es + off + 8 * S::SB);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const int blk = BLOCKS > 1 ? half * MINE + i : 0;
         float f0[8], f1[8];
-        block_values(acc, f0s, f1s, f0, f1);
+        block_values(acc[i], f0s, f1s, f0, f1);
         const int left = cols - step * KS - blk * 32 - q * 8;
         if constexpr (VEC) {
-          if (left > 0) {
-            Eight<T> e0, e1;
-#pragma unroll
-            for (int k = 0; k < Eight<T>::W; ++k) {
-              const int w = (blk * 4 + q) * Eight<T>::W + k;  // 16-byte vector of the row; odd rows' chunks are swapped
-              const uint32_t off = ((w >> 2) ^ (g & 1)) * 64 + (w & 3) * 16;
-              e0.u[k] = lds16(es + off);
-              e1.u[k] = lds16(es + off + 8 * S::SB);
-            }
-            if (in0) store_sum<T>(out0 + blk * 32, e0, with_base, f0);
-            if (in1) store_sum<T>(out1 + blk * 32, e1, with_base, f1);
-          }
+          if (left > 0 && in0) store_sum<T>(out0 + blk * 32, e0[i], with_base, f0);
+          if (left > 0 && in1) store_sum<T>(out1 + blk * 32, e1[i], with_base, f1);
         } else {
           const T* base = static_cast<const T*>(a.base);
           const int64_t at = col0 + step * KS + blk * 32 + q * 8;
@@ -1286,12 +1291,19 @@ cudaError_t launch_best(const LoraArgs& a, const PlanBytes& p, const LoraPlan& p
   return launch_shape<T, RANKS, VR, 128, STAGES, VEC>(a, p, plan, tiles, narrow.cluster, st);
 }
 
-// More ranks: in passes of 128.
-template <typename T, int VR, int STAGES, bool VEC>
+// More ranks: in passes of 128. Two stages leave room for clusters of four with
+// 128 ranks, three for two.
+template <typename T, bool VEC>
 cudaError_t launch_ranks(const LoraArgs& a, const PlanBytes& p, const LoraPlan& plan, int64_t tiles, cudaStream_t st) {
-  ShapeChoice choice;
-  if (const cudaError_t e = choose_cluster<T, 128, VR, 128, STAGES, VEC>(a, tiles, &choice); e != cudaSuccess) return e;
-  return launch_shape<T, 128, VR, 128, STAGES, VEC>(a, p, plan, tiles, choice.cluster, st);
+  ShapeChoice three, two;
+  if (a.rank > 128) {
+    if (const cudaError_t e = choose_cluster<T, 128, 256, 128, 2, VEC>(a, tiles, &two); e != cudaSuccess) return e;
+    return launch_shape<T, 128, 256, 128, 2, VEC>(a, p, plan, tiles, two.cluster, st);
+  }
+  if (const cudaError_t e = choose_cluster<T, 128, 128, 128, 3, VEC>(a, tiles, &three); e != cudaSuccess) return e;
+  if (const cudaError_t e = choose_cluster<T, 128, 128, 128, 2, VEC>(a, tiles, &two); e != cudaSuccess) return e;
+  if (two.us < three.us) return launch_shape<T, 128, 128, 128, 2, VEC>(a, p, plan, tiles, two.cluster, st);
+  return launch_shape<T, 128, 128, 128, 3, VEC>(a, p, plan, tiles, three.cluster, st);
 }
 
 template <typename T, bool VEC>
@@ -1302,7 +1314,7 @@ cudaError_t launch_tiles(const LoraArgs& a, const PlanBytes& p, const LoraPlan& 
   if (a.rank <= 16) return launch_best<T, 16, 4, VEC>(a, p, plan, tiles, st);
   if (a.rank <= 32) return launch_best<T, 32, 3, VEC>(a, p, plan, tiles, st);  // three stages: two CTAs on an SM in clusters of eight
   if (a.rank <= 64) return launch_best<T, 64, 4, VEC>(a, p, plan, tiles, st);
-  return a.rank <= 128 ? launch_ranks<T, 128, 3, VEC>(a, p, plan, tiles, st) : launch_ranks<T, 256, 2, VEC>(a, p, plan, tiles, st);
+  return launch_ranks<T, VEC>(a, p, plan, tiles, st);
 }
 
 template <typename T>
