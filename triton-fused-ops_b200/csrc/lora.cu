@@ -1257,13 +1257,15 @@ cudaError_t choose_cluster(const LoraArgs& a, int64_t tiles, ShapeChoice* best) 
   using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
   const void* kernel = reinterpret_cast<const void*>(lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>);
   const int64_t steps = (std::max(a.k, a.n) + S::KS - 1) / S::KS;
-  const double alone = static_cast<double>(a.k + a.n) * sizeof(T) / 16384 * (STEP >= 256 ? 72 : 83);
-  for (int c = 1; c <= kMaxCluster && (c == 1 || 4 * c <= steps) && (c == 1 || S::smem(c) <= 216 * 1024); c *= 2) {
+  const double alone = static_cast<double>(a.k + a.n) * sizeof(T) / 16384 * (STEP >= 256 ? 72 : 83) * (VEC ? 1 : 3);
+  constexpr int kFewest = STEP >= 256 ? 4 : VEC ? 2 : 1;  // steps of a CTA
+  for (int c = 1; c <= kMaxCluster && (c == 1 || kFewest * c <= steps) && (c == 1 || S::smem(c) <= 216 * 1024); c *= 2) {
     int resident = 0;
     if (const cudaError_t e = resident_clusters(kernel, kLargeThreads, c, S::smem(c), &resident); e != cudaSuccess) return e;
     if (resident == 0 && c > 1) break;  // no room for such a cluster
     const int64_t waves = (tiles + std::max(resident, 1) - 1) / std::max(resident, 1);
-    const double us = static_cast<double>(waves) * (5 + alone / c);
+    const double sent = static_cast<double>(std::min<int64_t>(tiles, resident)) * c * c * kLargeRows * 4 * a.rank;  // bytes of a wave
+    const double us = static_cast<double>(waves) * (5 + 0.35 * (c - 1) + sent / 3e6 + alone / c);
     if (c == 1 || us < best->us) *best = ShapeChoice{c, us};
   }
   return cudaSuccess;
