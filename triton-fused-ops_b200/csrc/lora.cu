@@ -29,8 +29,8 @@
 // neighbouring ones.
 //
 // Measured (us; 4096 x 4096, bf16): one token of rank 16 4.8; 64 tokens over 32
-// adapters 7.2; 256: 12.1; 512: 15.4; 8192 tokens of 16 adapters of rank 32 51,
-// 63 % of the measured copy rate (rank 64 72, rank 128 136: the legacy tensor
+// adapters 7.2; 256: 12.1; 512: 15.4; 8192 tokens of 16 adapters of rank 32 49,
+// 66 % of the measured copy rate (rank 64 72, rank 128 136: the legacy tensor
 // path's 530 TFLOP/s bounds those). A form of the large kernel on tcgen05
 // (128-row tiles copied into swizzled shared memory, v and the outputs in
 // tensor memory) took 67 us at rank 32, 98 at 64 and 152 at 128: its steps'
