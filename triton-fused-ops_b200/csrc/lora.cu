@@ -36,11 +36,16 @@
 // tensor memory) took 67 us at rank 32, 98 at 64 and 152 at 128: its steps'
 // waits, proxy fences and barriers ran 750 cycles with one CTA on an SM.
 //
-// Rounding: products and sums are fp32. v enters the second product as the sum
-// of two values of x's type, hi + lo (16 bits of bf16, 22 of fp16 relative to
-// the row's largest value, by which the row is scaled to stay in fp16's
-// range); fp32 operands are split into two tf32 values on both sides and the
-// three larger products are added. The result is rounded once.
+// Rounding: products and sums are fp32. v enters the second product as a sum
+// of values of x's type. fp16: two, 23 bits (rows are scaled by a power of two to
+// use fp16's whole range). bf16 up to 384 tokens: three, all 24 bits; more
+// tokens: two, 16 bits, with which 1 to 2 of 1000 outputs are not the nearest
+// value to the 64-bit result (three: 2 of 10000; the error against 64 bits is
+// the output's own rounding either way). Few tokens wait for memory, and the
+// third product costs them 0.1 to 0.3 us (one token 4.6 -> 4.7, 256 9.0 -> 9.3); many
+// are bound by the products: 8192 tokens of rank 32 47 -> 51 us with three, rank
+// 128 135 -> 157. fp32 operands are split into two tf32 values on both sides
+// and the three larger products are added. The result is rounded once.
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -477,35 +482,55 @@ __device__ __forceinline__ void fill_rows(const LoraArgs& a, const Tile& tile, c
   }
 }
 
-// Stages the tile's v as operands in shared memory: hi and lo (16-bit types;
-// fp32 as it is), [M][stride] elements. sum(m, r) gives four neighbouring
-// values of row m, summed and scaled. fp16 rows are scaled by a power of two
-// to below 2 (row_scale takes it back; `sums`, [M][sums_stride], holds them meanwhile
-// and may be what sum(m, r) reads); rows past the tile and ranks past the end
-// are zero.
-template <typename T, int M, typename Sum>
-__device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int stride, T* hi, T* lo, float* sums,
+// The values of x's type that v is split into: v = the sum of them.
+template <typename T, bool FEW> constexpr int kSplits = sizeof(T) == 4 ? 1 : FEW && std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
+
+// The staged values of v, [M][stride] elements each, one after the other.
+template <typename T, int SPLITS, int M> struct Staged {
+  T* at;
+  int stride;
+  __device__ T* split(int i) const { return at + i * M * stride; }
+  __device__ Staged from(int elements) const { return Staged{at + elements, stride}; }
+};
+
+// Stages the tile's v as operands in shared memory. sum(m, r) gives four
+// neighbouring values of row m, summed and scaled. fp16 rows are scaled by a
+// power of two to below 2^15, so that values down to 2^-15 of a row's largest
+// keep all their bits (row_scale takes it back; `sums`, [M][sums_stride], holds
+// them meanwhile and may be what sum(m, r) reads); rows past the tile and ranks
+// past the end are zero.
+template <typename T, int SPLITS, int M, typename Sum>
+__device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, const Staged<T, SPLITS, M>& v, float* sums,
                                         int sums_stride, float* row_scale, unsigned* row_max, Sum sum) {
-  constexpr bool SPLIT = sizeof(T) == 2;
   constexpr bool SCALED = std::is_same<T, __half>::value;
   const int shift = 31 - __clz(vr / 4), quads = 1 << shift, threads = blockDim.x;  // vr is a power of two
   if constexpr (SCALED) {
     for (int m = threadIdx.x; m < M; m += threads) row_max[m] = 0;
     __syncthreads();
   }
+  // four values of row m, split
   auto put = [&](int m, int r, const float (&t)[4], float down) {
+    const int to = m * v.stride + r;
+    if constexpr (SPLITS == 1) {
+      *reinterpret_cast<float4*>(v.split(0) + to) = make_float4(t[0], t[1], t[2], t[3]);
+    } else {
+      alignas(8) T part[SPLITS][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x = SCALED ? t[j] * down : t[j];
-      const T h = Ty<T>::from_f(x);
-      hi[m * stride + r + j] = h;
-      if constexpr (SPLIT) {
-        const float hf = Ty<T>::to_f(h);
-        lo[m * stride + r + j] = Ty<T>::from_f(fabsf(hf) <= 3.402823466e38f ? x - hf : 0.f);  // infinities are all in hi
+      for (int j = 0; j < 4; ++j) {
+        float x = SCALED ? t[j] * down : t[j];
+#pragma unroll
+        for (int i = 0; i < SPLITS; ++i) {
+          part[i][j] = Ty<T>::from_f(x);
+          const float f = Ty<T>::to_f(part[i][j]);
+          x = fabsf(f) <= 3.402823466e38f ? x - f : 0.f;  // infinities are all in the first
+        }
       }
+#pragma unroll
+      for (int i = 0; i < SPLITS; ++i) *reinterpret_cast<uint2*>(v.split(i) + to) = *reinterpret_cast<const uint2*>(part[i]);
     }
   };
-#pragma unroll 2
+  // Not unrolled: most launches take one turn or two (64 tokens over 32 adapters 7.5 -> 7.3 us).
+#pragma unroll 1
   for (int i = threadIdx.x; i < M * quads; i += threads) {
     const int m = i >> shift, r = (i & (quads - 1)) * 4;
     float t[4] = {};
@@ -533,9 +558,10 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, int 
   if constexpr (SCALED) {
     for (int m = threadIdx.x; m < M; m += threads) {
       const float most = __uint_as_float(row_max[m]);
-      row_scale[m] = most > 0.f ? ldexpf(1.f, min(126, max(-126, ilogbf(most)))) : 1.f;
+      row_scale[m] = most > 0.f ? ldexpf(1.f, max(-126, ilogbf(most) - 14)) : 1.f;
     }
     __syncthreads();
+#pragma unroll 1
     for (int i = threadIdx.x; i < M * quads; i += threads) {
       const int m = i >> shift, r = (i & (quads - 1)) * 4;
       float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -565,37 +591,37 @@ template <int M> struct SumParts {
   }
 };
 
-// The product over chunk c of 16 staged rows (hi0 / lo0: this lane's place in
-// row g) with 32 rows of B given by bf(j, chunk): adds to acc.
-template <typename T, typename LoadB>
-__device__ __forceinline__ void expand_chunk(float (&acc)[4][4], const T* hi0, const T* lo0, int stride, int c, LoadB bf) {
+// The product over chunk c of 16 staged rows (v: this lane's place in row g)
+// with 32 rows of B given by bf(j, chunk): adds to acc, the smallest of the
+// split values first.
+template <typename T, int SPLITS, int M, typename LoadB>
+__device__ __forceinline__ void expand_chunk(float (&acc)[4][4], const Staged<T, SPLITS, M>& v, int c, LoadB bf) {
   constexpr int C = chunk_elems(sizeof(T));
   uint4 b[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) b[j] = bf(j, c);
-  const uint4 a0 = *reinterpret_cast<const uint4*>(hi0 + c * C);
-  const uint4 a1 = *reinterpret_cast<const uint4*>(hi0 + 8 * stride + c * C);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) Chunk<T>::mma(acc[j], a0, a1, b[j]);
-  if constexpr (sizeof(T) == 2) {
-    const uint4 l0 = *reinterpret_cast<const uint4*>(lo0 + c * C);
-    const uint4 l1 = *reinterpret_cast<const uint4*>(lo0 + 8 * stride + c * C);
+  for (int i = SPLITS - 1; i >= 0; --i) {
+    const uint4 a0 = *reinterpret_cast<const uint4*>(v.split(i) + c * C);
+    const uint4 a1 = *reinterpret_cast<const uint4*>(v.split(i) + 8 * v.stride + c * C);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) Chunk<T>::mma(acc[j], l0, l1, b[j]);
+    for (int j = 0; j < 4; ++j) Chunk<T>::mma(acc[j], a0, a1, b[j]);
   }
 }
 // The same with the rows' few chunks kept in registers.
-template <typename T, int NCH>
+template <typename T, int SPLITS, int NCH>
 struct StagedRows {
-  uint4 h0[NCH], h1[NCH], l0[NCH], l1[NCH];
-  __device__ void load(const T* hi0, const T* lo0, int stride) {
+  uint4 a0[SPLITS][NCH], a1[SPLITS][NCH];
+  template <int M>
+  __device__ void load(const Staged<T, SPLITS, M>& v) {
     constexpr int C = chunk_elems(sizeof(T));
 #pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-      h0[c] = *reinterpret_cast<const uint4*>(hi0 + c * C);
-      h1[c] = *reinterpret_cast<const uint4*>(hi0 + 8 * stride + c * C);
-      l0[c] = *reinterpret_cast<const uint4*>(lo0 + c * C);
-      l1[c] = *reinterpret_cast<const uint4*>(lo0 + 8 * stride + c * C);
+    for (int i = 0; i < SPLITS; ++i) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        a0[i][c] = *reinterpret_cast<const uint4*>(v.split(i) + c * C);
+        a1[i][c] = *reinterpret_cast<const uint4*>(v.split(i) + 8 * v.stride + c * C);
+      }
     }
   }
   template <typename LoadB>
@@ -605,8 +631,8 @@ struct StagedRows {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint4 b = bf(j, c);
-        Chunk<T>::mma(acc[j], h0[c], h1[c], b);
-        Chunk<T>::mma(acc[j], l0[c], l1[c], b);
+#pragma unroll
+        for (int i = SPLITS - 1; i >= 0; --i) Chunk<T>::mma(acc[j], a0[i][c], a1[i][c], b);
       }
     }
   }
@@ -693,9 +719,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) lora_small_kernel
   const int vr = static_cast<int>(v_rank), rank = static_cast<int>(a.rank);
   const int stride = vr + E, quads = (rank + 3) / 4;
   float* parts = reinterpret_cast<float*>(smem);  // [cluster][M][vr]: the CTAs' parts of v
-  T* hi = reinterpret_cast<T*>(smem + sizeof(float) * cluster * M * vr);
-  T* lo = hi + M * stride;
-  auto* red = reinterpret_cast<float(*)[M][RB + 4]>(lo + (sizeof(T) == 2 ? M * stride : 0));  // [kSmallWarps]
+  constexpr int SPLITS = kSplits<T, true>;
+  const Staged<T, SPLITS, M> v{reinterpret_cast<T*>(smem + sizeof(float) * cluster * M * vr), stride};
+  auto* red = reinterpret_cast<float(*)[M][RB + 4]>(v.split(SPLITS));  // [kSmallWarps]
   if (t == 0) mbar_arrive_expect_tx(&received, static_cast<uint32_t>(cluster * tile.count * quads * 16));
   const bool in0 = g < tile.count, in1 = g + 8 < tile.count;
   const int64_t t0 = rows[in0 ? g : 0], t1 = rows[in1 ? g + 8 : 0];
@@ -781,18 +807,17 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) lora_small_kernel
   const float scale = a.scaling != nullptr ? a.scaling[tile.group] : 1.f;
   const bool arrived = mbar_wait(&received, 0, err, ERR_WAIT_TIMEOUT_OTHER);
   if (__syncthreads_or(!arrived)) return;
-  stage_v<T, M>(tile, rank, vr, stride, hi, lo, parts, vr, row_scale, row_max, SumParts<M>{parts, cluster, vr, scale});
+  stage_v(tile, rank, vr, v, parts, vr, row_scale, row_max, SumParts<M>{parts, cluster, vr, scale});
   const float s0 = SCALED ? row_scale[g] : 1.f, s1 = SCALED ? row_scale[g + 8] : 1.f;
-  const T* hi0 = hi + g * stride + q * E;
-  const T* lo0 = lo + g * stride + q * E;
+  const Staged<T, SPLITS, M> mine = v.from(g * stride + q * E);
   T* out0 = static_cast<T*>(a.out) + t0 * a.out_stride + q * 8;
   T* out1 = static_cast<T*>(a.out) + t1 * a.out_stride + q * 8;
   for (int64_t n0 = first; n0 < col1; n0 += kStride) {
     const Block now = next;
     if (n0 + kStride < col1) load_block(next, n0 + kStride);
     float acc[4][4] = {};
-    expand_chunk<T>(acc, hi0, lo0, stride, 0, [&](int j, int) { return now.b[j]; });
-    for (int c = 1; c < vr / C; ++c) expand_chunk<T>(acc, hi0, lo0, stride, c, [&](int j, int k) { return b_chunk(n0, j, k); });
+    expand_chunk(acc, mine, 0, [&](int j, int) { return now.b[j]; });
+    for (int c = 1; c < vr / C; ++c) expand_chunk(acc, mine, c, [&](int j, int k) { return b_chunk(n0, j, k); });
     float f0[8], f1[8];
     block_values(acc, s0, s1, f0, f1);
     const int64_t left = col1 - n0 - q * 8;
@@ -827,7 +852,7 @@ struct LargeShape {
   static constexpr int kShrink = kRows + RANKS * SB, kExpand = kRows + KS * NCH * 64;
   static constexpr int kStage = kShrink > kExpand ? kShrink : kExpand;
   static constexpr int stride = VR + E;
-  static constexpr size_t kStaged = static_cast<size_t>(sizeof(T) == 2 ? 2 : 1) * sizeof(T) * M * stride;
+  static constexpr size_t kStaged = static_cast<size_t>(kSplits<T, false>) * sizeof(T) * M * stride;
   static_assert(kStaged >= sizeof(float) * M * (RANKS + 4), "the halves' sums fit where v is staged later");
   static constexpr int PR = VR > RANKS && RANKS < 128 ? RANKS : VR;  // ranks of a row of an exchanged part
   static size_t smem(int cluster) { return STAGES * kStage + kStaged + sizeof(float) * cluster * M * PR; }
@@ -867,9 +892,9 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
   }
   const int rank = static_cast<int>(a.rank), quads = (rank + 3) / 4;
   uint8_t* ring = smem;
-  T* hi = reinterpret_cast<T*>(smem + STAGES * S::kStage);
-  T* lo = hi + M * stride;
-  auto* halves = reinterpret_cast<float(*)[RANKS + 4]>(hi);  // until v is staged
+  constexpr int SPLITS = kSplits<T, false>;
+  const Staged<T, SPLITS, M> v{reinterpret_cast<T*>(smem + STAGES * S::kStage), stride};
+  auto* halves = reinterpret_cast<float(*)[RANKS + 4]>(v.at);  // until v is staged
   float* parts = reinterpret_cast<float*>(smem + STAGES * S::kStage + S::kStaged);  // [cluster][M][PR]
   if (t == 0) mbar_arrive_expect_tx(&received, static_cast<uint32_t>(cluster * tile.count * quads * 16));
   const int g = lane >> 2, q = lane & 3;
@@ -1035,17 +1060,16 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
     asm volatile("cp.async.wait_all;" ::: "memory");
     return;
   }
-  stage_v<T, M>(tile, rank, VR, stride, hi, lo, parts, S::PR, row_scale, row_max, SumParts<M>{parts, cluster, S::PR, scale});
+  stage_v(tile, rank, VR, v, parts, S::PR, row_scale, row_max, SumParts<M>{parts, cluster, S::PR, scale});
   const bool in0 = m0 + g < tile.count, in1 = m0 + g + 8 < tile.count;
   const float f0s = SCALED ? row_scale[m0 + g] : 1.f, f1s = SCALED ? row_scale[m0 + g + 8] : 1.f;
-  const T* hi0 = hi + (m0 + g) * stride + q * E;
-  const T* lo0 = lo + (m0 + g) * stride + q * E;
+  const Staged<T, SPLITS, M> mine = v.from((m0 + g) * stride + q * E);
   const int64_t t0 = rows[in0 ? m0 + g : 0], t1 = rows[in1 ? m0 + g + 8 : 0];
   T* out0 = static_cast<T*>(a.out) + t0 * a.out_stride + col0 + q * 8;
   T* out1 = static_cast<T*>(a.out) + t1 * a.out_stride + col0 + q * 8;
   constexpr bool HELD = NCH <= 2 && sizeof(T) == 2;
-  StagedRows<T, HELD ? NCH : 1> held;
-  if constexpr (HELD) held.load(hi0, lo0, stride);
+  StagedRows<T, SPLITS, HELD ? NCH : 1> held;
+  if constexpr (HELD) held.load(mine);
   constexpr int BLOCKS = KS / 32;  // of a step: the halves of the warps share them, or take turns
   const uint32_t b_at = S::kRows + tile_offset(block_column(g), NCH, 0, q);
   const uint32_t e_at = (m0 + g) * S::SB;
@@ -1073,7 +1097,7 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
           held.expand(acc[i], bf);
         } else {
 #pragma unroll 2
-          for (int c = 0; c < NCH; ++c) expand_chunk<T>(acc[i], hi0, lo0, stride, c, bf);
+          for (int c = 0; c < NCH; ++c) expand_chunk(acc[i], mine, c, bf);
         }
         if constexpr (VEC) {
 #pragma unroll
@@ -1227,7 +1251,7 @@ cudaError_t launch_small(const LoraArgs& a, cudaStream_t st) {
   int cluster = 1;
   while (cluster < kMaxCluster && cluster < want && 2 * cluster * tiles <= 4 * num_sms() && 2 * cluster * v_rank <= 512)
     cluster *= 2;
-  const size_t smem = kSmallRows * (sizeof(float) * v_rank * cluster + (sizeof(T) == 2 ? 2 : 1) * sizeof(T) * (v_rank + E));
+  const size_t smem = kSmallRows * (sizeof(float) * v_rank * cluster + kSplits<T, true> * sizeof(T) * (v_rank + E));
   auto launch = [&](auto* kernel, int nt) {
     size_t bytes = smem + sizeof(float) * kSmallWarps * kSmallRows * (8 * nt + 4);
     if (const cudaError_t e = spread(reinterpret_cast<const void*>(kernel), 256, cluster, tiles, &bytes); e != cudaSuccess) return e;
