@@ -1,8 +1,4 @@
-"""What fused_lora keeps of its fp32 low-rank values, on cases with exact answers.
-
-Every product, partial sum and result below is exact in fp32 and in the operands' type: the outputs have to be equal,
-not near.
-"""
+"""What fused_lora keeps of its fp32 sums and low-rank values, on cases made for it."""
 
 import pytest
 import torch
@@ -17,6 +13,7 @@ DT = {"f16": torch.float16, "bf16": torch.bfloat16}
 def test_low_rank_values_keep_their_bits(cuda, dtype, bits, t, rank):
     """Two low-rank values below 2^bits that differ by less than 128, one subtracted from the other.
 
+    Every product, partial sum and result is exact in fp32 and in the operands' type, so the outputs have to be equal.
     A holds a value in four parts of six bits, x the parts' weights. The two values are the first and the last of the
     rank, so that from rank 40 on they enter different tensor instructions."""
     from triton_ops import fused_lora
@@ -43,3 +40,27 @@ def test_low_rank_values_keep_their_bits(cuda, dtype, bits, t, rank):
     x, a, b = (v.to(DT[dtype]).cuda() for v in (x, a, b))
     got = fused_lora(x, a, b, ids.cuda(), torch.full((m,), scale, device="cuda"))
     assert torch.equal(got.double().cpu(), want)
+
+
+@pytest.mark.parametrize("rank", [8, 64, 128, 256])
+@pytest.mark.parametrize("t", [9, 500])
+def test_fp32_sums_are_rounded_not_cut(cuda, t, rank):
+    """Low-rank values of 4096 positive terms: errors that all have one sign would add up.
+
+    Bound relative to v, in units of 2^-24: the 16 terms of a chunk within one instruction chain, 6 steps of at most
+    two units: 12; the chunks of half of K one after the other, each addition off by at most one unit of what is there
+    by then, which grows evenly: K / 64; the halves, warps and CTAs: 12 more additions; operands of two tf32 values
+    with the smallest product left out: three times 2^-22, 12; the same for v times one: 4 (B is one at one place).
+    """
+    from triton_ops import fused_lora
+
+    k, n = 4096, 32
+    g = torch.Generator(device="cuda").manual_seed(rank)
+    x = 0.5 + torch.rand(t, k, device="cuda", generator=g)
+    a = 0.5 + torch.rand(1, rank, k, device="cuda", generator=g)
+    b = torch.zeros(1, n, rank, device="cuda")
+    at = torch.arange(n, device="cuda") * 7 % rank
+    b[0, torch.arange(n), at] = 1.0
+    got = fused_lora(x, a, b, torch.zeros(t, dtype=torch.int64, device="cuda"))
+    want = (x.double() @ a[0].double().t())[:, at]
+    assert ((got.double() - want).abs() <= (k / 64 + 40) * 2.0**-24 * want).all()
