@@ -389,9 +389,10 @@ py::object qk_norm_rope(const at::Tensor& q, const OptTensor& k, const OptTensor
                                          interleaved)));
 }
 
-// rope_tables of given positions: (cos, sin), or None outside the common case.
+// rope_tables of given positions: (cos, sin), or None outside the common case. turns: doubles in host memory.
 py::object rope_tables(const at::Tensor& positions, const at::Tensor& turns, double gain, int64_t out_code) {
   if (!positions.is_cuda() || !positions.is_contiguous() || pos_code(positions.scalar_type()) < 0) return py::none();
+  if (!turns.is_cpu() || turns.scalar_type() != at::kDouble || !turns.is_contiguous()) return py::none();
   const c10::cuda::CUDAGuard guard(positions.device());
   const int64_t half = turns.numel();
   std::vector<int64_t> shape(positions.sizes().begin(), positions.sizes().end());

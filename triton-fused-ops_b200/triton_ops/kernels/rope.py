@@ -130,10 +130,11 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[R
 
 @lru_cache(maxsize=64)
 def _turns(rotary_dim: int, base: float, scaling: Optional[RoPEScaling]):
-    """The frequencies as a host array of turns per position (what the kernel takes), and the gain."""
+    """The frequencies as host arrays of turns per position (what the kernel takes; torch's default device may be another
+    one), and the gain."""
     freq, gain = rope_frequencies(rotary_dim, base, scaling)
     values = [f / (2 * math.pi) for f in freq]
-    return (ctypes.c_double * len(values))(*values), torch.tensor(values, dtype=torch.float64), gain
+    return (ctypes.c_double * len(values))(*values), torch.tensor(values, dtype=torch.float64, device="cpu"), gain
 
 
 def rope_tables(
