@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 pytestmark = pytest.mark.gpu
 
@@ -31,3 +32,42 @@ def test_the_extension_takes_frequencies_from_the_host_alone(cuda):
     assert _lib.ext().rope_tables(at, turns, 1.0, _lib.F32) is not None
     for other in (turns.cuda(), turns.float(), torch.rand(8, dtype=torch.float64)[::2]):
         assert _lib.ext().rope_tables(at, other, 1.0, _lib.F32) is None
+
+
+@pytest.mark.parametrize("extension", [True, False])
+def test_forward_mode_is_refused(cuda, monkeypatch, extension):
+    """No output without its tangent, on either path."""
+    from triton_ops import _lib, fused_lora, fused_qk_norm_rope, fused_rope
+
+    if not extension:
+        monkeypatch.setattr(_lib, "ext", lambda: None)
+    q, k, t, w = (torch.ones(s, device="cuda") for s in ((2, 4, 3, 8), (2, 4, 1, 8), (4, 8), (8,)))
+    x, a, b, scaling, base = (torch.ones(s, device="cuda") for s in ((3, 8), (2, 4, 8), (2, 6, 4), (2,), (3, 6)))
+    ids = torch.zeros(3, dtype=torch.int64, device="cuda")
+    for op, args in (
+        (lambda q, k, c, s: fused_rope(q, k, c, s), (q, k, t, t)),
+        (lambda q, k, c, s, v, w: fused_qk_norm_rope(q, k, v, w, c, s), (q, k, t, t, w, w)),
+        (lambda x, a, b, s, y: fused_lora(x, a, b, ids, s, base=y), (x, a, b, scaling, base)),
+        (lambda y: fused_lora(x, a, b, ids, scaling, out=y), (base,)),
+    ):
+        op(*args)
+        with forward_ad.dual_level():
+            for i in range(len(args)):
+                dual = forward_ad.make_dual(args[i].clone(), torch.ones_like(args[i]))
+                with pytest.raises(ValueError, match="tangent"):
+                    op(*args[:i], dual, *args[i + 1:])
+            op(*args)
+
+
+@pytest.mark.parametrize("extension", [True, False])
+def test_forward_mode_over_a_backward_pass_is_refused(cuda, monkeypatch, extension):
+    from triton_ops import _lib, fused_qk_norm_rope, fused_rope
+
+    if not extension:
+        monkeypatch.setattr(_lib, "ext", lambda: None)
+    q, t = torch.ones(2, 4, 3, 8, device="cuda", requires_grad=True), torch.ones(4, 8, device="cuda")
+    for y in (fused_rope(q, None, t, t)[0], fused_qk_norm_rope(q, None, None, None, t, t)[0]):
+        g = torch.ones_like(y)
+        torch.autograd.grad(y, q, g, retain_graph=True)
+        with forward_ad.dual_level(), pytest.raises(ValueError, match="tangent"):
+            torch.autograd.grad(y, q, forward_ad.make_dual(g, g))

@@ -194,8 +194,12 @@ bool heads_ok(const at::Tensor& t) {
 
 bool weight_ok(const OptTensor& w, const at::Tensor& q) {
   return !w.has_value() || (w->device() == q.device() && is_float(w->scalar_type()) && w->dim() == 1 &&
-                            w->size(0) == q.size(-1) && w->is_contiguous());
+                            w->size(0) == q.size(-1) && w->is_contiguous() && !w->_fw_grad(0).defined());
 }
+
+// Forward mode: the Python wrappers refuse what carries a tangent.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
 
 // Everything the shared arguments of the head functions must satisfy here.
 bool heads_common(const at::Tensor& q, const OptTensor& k, const at::Tensor& cos, const at::Tensor& sin,
@@ -212,6 +216,7 @@ bool heads_common(const at::Tensor& q, const OptTensor& k, const at::Tensor& cos
       !is_float(cos.scalar_type()) || sin.scalar_type() != cos.scalar_type() || cos.sizes() != sin.sizes() ||
       cos.strides() != sin.strides() || cos.stride(1) != 1 || cos.requires_grad() || sin.requires_grad())
     return false;
+  if (has_tangent(q) || has_tangent(k) || has_tangent(cos) || has_tangent(sin)) return false;
   const int64_t dim = q.size(-1), rot = cos.size(1);
   if (dim < 2 || dim > 1024 || rot < 2 || rot % 2 != 0 || rot > dim || cos.size(0) == 0) return false;
   if (!positions.has_value()) return cos.size(0) >= q.size(-3);
@@ -290,6 +295,12 @@ variable_list outputs_of(const std::array<at::Tensor, 2>& out) {
   return out[1].defined() ? variable_list{out[0], out[1]} : variable_list{out[0]};
 }
 
+// Forward mode over a backward pass: a gradient's tangent would be lost.
+void refuse_tangents(const variable_list& grads) {
+  for (const at::Tensor& g : grads)
+    TORCH_CHECK_VALUE(!g.defined() || !has_tangent(g), "a gradient carries a forward-mode tangent: only reverse-mode gradients are there");
+}
+
 // The gradient of a rotation is the rotation by the opposite angle, itself differentiable.
 struct RopeNode : public torch::autograd::Function<RopeNode> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k, const at::Tensor& cos,
@@ -302,6 +313,7 @@ struct RopeNode : public torch::autograd::Function<RopeNode> {
     return outputs_of(rope_call(q, kt, cos, sin, pos, interleaved, inverse));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents(grads);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor dq = dense_heads(grads[0]);
     OptTensor dk, pos;
@@ -334,6 +346,7 @@ struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (at::GradMode::is_enabled())
       throw std::runtime_error("fused_qk_norm_rope is differentiable once: its gradients cannot be differentiated");
+    refuse_tangents(grads);
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3], &cos = saved[4], &sin = saved[5];
     const c10::cuda::CUDAGuard guard(q.device());
@@ -431,6 +444,8 @@ py::object lora(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, c
   }
   if (at::GradMode::is_enabled() && (x.requires_grad() || a.requires_grad() || b.requires_grad() ||
                                      wants_grad(scaling) || wants_grad(base) || wants_grad(out)))
+    return py::none();
+  if (has_tangent(x) || has_tangent(a) || has_tangent(b) || has_tangent(scaling) || has_tangent(base) || has_tangent(out))
     return py::none();
   // rows of one output may not share memory
   if (out.has_value() && tokens > 1 && out->stride(0) < n) return py::none();

@@ -64,7 +64,8 @@ def fused_lora(
 
     Returns:
         [..., out_features] in x's dtype. Sums are fp32, the result is rounded
-        once. Serving only: refuses tensors that ask for a gradient.
+        once. Serving only: refuses tensors that ask for a gradient or carry a
+        forward-mode tangent.
     """
     fast = _lib.ext()
     if fast is not None and x.dim() == 2:

@@ -30,7 +30,7 @@ from triton_ops.kernels.rope import (
     _table_args,
     rope_heads_reference,
 )
-from triton_ops.validation import validate_head_weight, validate_rope_heads
+from triton_ops.validation import refuse_tangents, validate_head_weight, validate_rope_heads
 
 fused_qk_norm_rope_kernel = NativeKernel(
     "fused_qk_norm_rope_kernel", "tfo_qk_norm_rope", "per-head RMSNorm + rotation of queries and keys in one pass"
@@ -67,6 +67,7 @@ class _FusedQKNormRoPE(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gq, gk=None):
         q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
+        refuse_tangents(gq, gk)
         gq, gk = _dense_heads(gq), _dense_heads(gk if k is not None else None)
         dq, dk = _empty_like_heads(q), _empty_like_heads(k)
         dqw = torch.empty_like(qw) if qw is not None and ctx.needs_input_grad[2] else None
@@ -106,7 +107,8 @@ def fused_qk_norm_rope(
 
     Returns:
         (q, k or None) normed and rotated, contiguous, in q's dtype.
-        Differentiable (once) in q, k and the weights.
+        Differentiable (once, in reverse mode) in q, k and the weights; a tensor
+        with a forward-mode tangent is refused.
     """
     fast = _lib.ext()
     if fast is not None:

@@ -23,7 +23,7 @@ import torch
 from triton_ops import _lib
 from triton_ops.exceptions import DeviceError, ShapeMismatchError, UnsupportedDtypeError
 from triton_ops.kernels._native import NativeKernel
-from triton_ops.validation import SUPPORTED_DTYPES_FLOAT, validate_rope_heads
+from triton_ops.validation import SUPPORTED_DTYPES_FLOAT, refuse_tangents, validate_rope_heads
 
 rope_tables_kernel = NativeKernel(
     "rope_tables_kernel", "tfo_rope_tables", "cos/sin rows of rotary positions, angles reduced exactly"
@@ -253,6 +253,7 @@ class _FusedRoPE(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk=None):
         cos, sin, positions = ctx.saved_tensors
+        refuse_tangents(dq, dk)
         dq, dk = _dense_heads(dq), _dense_heads(dk if ctx.with_k else None)
         out = _FusedRoPE.apply(dq, dk, cos, sin, positions, ctx.interleaved, not ctx.inverse)
         dq, dk = out if ctx.with_k else (out, None)
@@ -286,7 +287,8 @@ def fused_rope(
             with 2i + 1
 
     Returns:
-        (rotated q, rotated k or None), contiguous. Differentiable in q and k.
+        (rotated q, rotated k or None), contiguous. Differentiable in q and k, in
+        reverse mode (a tensor with a forward-mode tangent is refused).
     """
     fast = _lib.ext()
     if fast is not None:

@@ -256,6 +256,19 @@ def validate_fp8_quantize_inputs(tensor: torch.Tensor, scale: Optional[torch.Ten
         _check_cuda(scale, "scale")
 
 
+def _check_no_tangent(tensor: torch.Tensor, name: str) -> None:
+    """Forward mode: the ops of the query/key path have reverse-mode gradients alone, and a tangent would be lost."""
+    if torch.autograd.forward_ad.unpack_dual(tensor).tangent is not None:
+        raise ValueError(f"{name} carries a forward-mode tangent: only reverse-mode gradients are there")
+
+
+def refuse_tangents(*grads: Optional[torch.Tensor]) -> None:
+    """The same for the gradients that a backward pass is given."""
+    for g in grads:
+        if g is not None:
+            _check_no_tangent(g, "a gradient")
+
+
 def check_rope_table(ref: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Checks cos/sin ([rows, rotary_dim] or [1, rows, 1, rotary_dim]) and returns them as 2-D rows of stride 1."""
     for t, n in ((cos, "cos"), (sin, "sin")):
@@ -264,6 +277,7 @@ def check_rope_table(ref: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) ->
         _check_same_device(ref, t, n)
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{n} must not require a gradient: the rotary tables have none")
+        _check_no_tangent(t, n)
     if cos.dim() == 4 and cos.shape[0] == 1 and cos.shape[2] == 1:
         cos = cos[0, :, 0]
     elif cos.dim() != 2:
@@ -295,6 +309,7 @@ def _check_heads(t: torch.Tensor, name: str) -> None:
         )
     if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have contiguous heads (innermost stride 1), got strides {t.stride()}")
+    _check_no_tangent(t, name)
 
 
 def validate_rope_heads(
@@ -365,6 +380,7 @@ def validate_head_weight(q: torch.Tensor, weight: Optional[torch.Tensor], name: 
             expected=(q.shape[-1],), actual=weight.shape, tensor_name=name,
         )
     _check_contiguous(weight, name)
+    _check_no_tangent(weight, name)
 
 
 def validate_lora_inputs(
@@ -422,4 +438,7 @@ def validate_lora_inputs(
         _check_contiguous(scaling, "scaling")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, lora_a, lora_b, scaling, base, out)):
         raise ValueError("the adapters of many requests serve and have no gradient: call under torch.no_grad()")
+    for t, name in (*named, (scaling, "scaling")):
+        if t is not None:
+            _check_no_tangent(t, name)
     return x.numel() // k, adapters, rank, k, n
