@@ -1,4 +1,4 @@
-"""What fused_lora keeps of its fp32 sums and low-rank values, on cases made for it."""
+"""What fused_lora keeps of its fp32 sums and low-rank values, and what autograd hears of its writes."""
 
 import pytest
 import torch
@@ -64,3 +64,29 @@ def test_fp32_sums_are_rounded_not_cut(cuda, t, rank):
     got = fused_lora(x, a, b, torch.zeros(t, dtype=torch.int64, device="cuda"))
     want = (x.double() @ a[0].double().t())[:, at]
     assert ((got.double() - want).abs() <= (k / 64 + 40) * 2.0**-24 * want).all()
+
+
+@pytest.mark.parametrize("extension", [True, False])
+@pytest.mark.parametrize("t", [9, 500])
+def test_autograd_hears_of_a_write(cuda, monkeypatch, extension, t):
+    """`out` may be a tensor that another operation keeps for its backward pass: that pass has to refuse."""
+    from triton_ops import _lib, fused_lora
+
+    if not extension:
+        monkeypatch.setattr(_lib, "ext", lambda: None)
+    x, a, b = (torch.ones(s, device="cuda") for s in ((t, 16), (2, 4, 16), (2, 8, 4)))
+    ids = torch.zeros(t, dtype=torch.int64, device="cuda")
+    w = torch.ones(t, 8, device="cuda", requires_grad=True)
+    y = torch.ones(t, 8, device="cuda")
+    z = w * y
+    fused_lora(x, a, b, ids, base=y)  # writes a tensor of its own
+    torch.autograd.grad(z.sum(), w, retain_graph=True)
+    view = y[:, :]
+    fused_lora(x, a, b, ids, base=view, out=view)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(z.sum(), w)
+    with torch.inference_mode():
+        y = torch.ones(t, 8, device="cuda")
+        want = fused_lora(x, a, b, ids, base=y)
+        assert torch.equal(fused_lora(x, a, b, ids, base=y, out=y), want)
+    assert torch.equal(fused_lora(x, a, b, ids, out=y), want - 1)  # a tensor of inference mode keeps no version

@@ -452,6 +452,8 @@ py::object lora(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, c
   const c10::cuda::CUDAGuard guard(x.device());
   const auto st = at::cuda::getCurrentCUDAStream(x.device().index()).stream();
   at::Tensor y = out.has_value() ? *out : fresh({tokens, n}, x.scalar_type(), x.device());
+  // written through its pointer: autograd has to know, if it keeps out for a backward pass
+  if (out.has_value() && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
   const int dtype = dtype_code(x.scalar_type());
   const at::Tensor ws = scratch(tfo_lora_workspace_bytes(tokens, adapters), x.device());
   check(tfo_lora(x.data_ptr(), x.stride(0), a.data_ptr(), b.data_ptr(), ids.data_ptr(), pos_code(ids.scalar_type()),

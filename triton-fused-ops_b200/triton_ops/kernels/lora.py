@@ -76,6 +76,7 @@ def fused_lora(
         if got is not None:
             return got
     tokens, adapters, rank, k, n = validate_lora_inputs(x, lora_a, lora_b, adapter_ids, scaling, base, out)
+    given = out is not None
     if out is None:
         out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
     if out.numel() == 0:
@@ -86,6 +87,8 @@ def fused_lora(
         out2 = None
     if out2 is None or (n > 1 and out2.stride(1) != 1) or (tokens > 1 and out2.stride(0) < n):
         raise ValueError(f"out must be viewable as distinct rows of innermost stride 1, got strides {out.stride()}")
+    if given and not out.is_inference():  # written through its pointer: autograd has to know, if it keeps out
+        torch.autograd.graph.increment_version(out)
     x2, base2 = _rows(x, k), out2 if base is out else _rows(base, n)
     ids = adapter_ids.reshape(-1).contiguous()
     dtype = _lib.dtype_code(x.dtype, "x")
