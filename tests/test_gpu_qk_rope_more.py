@@ -71,3 +71,31 @@ def test_forward_mode_over_a_backward_pass_is_refused(cuda, monkeypatch, extensi
         torch.autograd.grad(y, q, g, retain_graph=True)
         with forward_ad.dual_level(), pytest.raises(ValueError, match="tangent"):
             torch.autograd.grad(y, q, forward_ad.make_dual(g, g))
+
+
+@pytest.mark.parametrize("extension", [True, False])
+@pytest.mark.parametrize("with_graph", [True, False], ids=["g has a graph", "g is plain"])
+def test_gradients_made_with_create_graph(cuda, monkeypatch, extension, with_graph):
+    """They are the gradients, another part of the graph may be differentiated, and they themselves raise: also where
+    the outputs' gradients ask for none, since they depend on q, k and the weights too."""
+    from triton_ops import _lib, fused_qk_norm_rope
+
+    if not extension:
+        monkeypatch.setattr(_lib, "ext", lambda: None)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, k, w = (torch.randn(s, device="cuda", generator=gen).requires_grad_() for s in ((1, 5, 3, 16), (1, 5, 1, 16), (16,)))
+    angle = torch.randn(5, 8, device="cuda", generator=gen)
+    cos, sin = angle.cos().repeat(1, 2), angle.sin().repeat(1, 2)
+    g = torch.randn(q.shape, device="cuda", generator=gen).requires_grad_(with_graph)
+    y, z = fused_qk_norm_rope(q, k, w, None, cos, sin)
+    plain = torch.autograd.grad([y, z], [q, k, w], [g, torch.ones_like(z)], retain_graph=True)
+    got = torch.autograd.grad([y, z], [q, k, w], [g, torch.ones_like(z)], create_graph=True)
+    assert all(torch.equal(a, b) and b.requires_grad for a, b in zip(plain, got))
+    other = torch.randn(7, device="cuda", generator=gen).requires_grad_()
+    (first,) = torch.autograd.grad(other.pow(3).sum() + y.sum() * 0, other, create_graph=True)
+    assert torch.equal(torch.autograd.grad(first.sum(), other)[0], 6 * other.detach())
+    for d in got:
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(d.square().sum() + q.sum(), q, retain_graph=True)
+        with pytest.raises(RuntimeError, match="once"):
+            (d.square().sum() + q.square().sum()).backward(retain_graph=True)

@@ -13,6 +13,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <array>
@@ -301,6 +303,15 @@ void refuse_tangents(const variable_list& grads) {
     TORCH_CHECK_VALUE(!g.defined() || !has_tangent(g), "a gradient carries a forward-mode tangent: only reverse-mode gradients are there");
 }
 
+// Puts a node that only raises between the gradients and what they depend on.
+void differentiable_once(const variable_list& gradients, const variable_list& sources) {
+  const auto node = std::make_shared<torch::autograd::Error>(
+      "fused_qk_norm_rope is differentiable once: its gradients cannot be differentiated",
+      torch::autograd::collect_next_edges(sources));
+  for (const at::Tensor& g : gradients)
+    if (g.defined()) torch::autograd::set_history(g, node);
+}
+
 // The gradient of a rotation is the rotation by the opposite angle, itself differentiable.
 struct RopeNode : public torch::autograd::Function<RopeNode> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k, const at::Tensor& cos,
@@ -344,10 +355,18 @@ struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
     return outputs_of(qk_norm_call(q, kt, qwt, kwt, cos, sin, pos, eps, interleaved));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    if (at::GradMode::is_enabled())
-      throw std::runtime_error("fused_qk_norm_rope is differentiable once: its gradients cannot be differentiated");
-    refuse_tangents(grads);
     const auto saved = ctx->get_saved_variables();
+    variable_list d = gradients(ctx, saved, grads);
+    if (at::GradMode::is_enabled()) {  // create_graph: differentiating one of the gradients is the error
+      variable_list sources(saved.begin(), saved.begin() + 4);
+      sources.insert(sources.end(), grads.begin(), grads.end());
+      differentiable_once(d, sources);
+    }
+    return d;
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& saved, const variable_list& grads) {
+    const at::AutoGradMode no_graph(false);
+    refuse_tangents(grads);
     const at::Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3], &cos = saved[4], &sin = saved[5];
     const c10::cuda::CUDAGuard guard(q.device());
     const auto st = at::cuda::getCurrentCUDAStream(q.device().index()).stream();

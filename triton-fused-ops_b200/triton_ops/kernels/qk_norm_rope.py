@@ -18,7 +18,6 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from triton_ops import _lib
 from triton_ops.kernels._native import NativeKernel
@@ -55,6 +54,18 @@ def _forward(q, k, qw, kw, cos, sin, positions, eps, interleaved):
     return q_out, k_out
 
 
+class _DifferentiableOnce(torch.autograd.Function):
+    """Gradients behind what they depend on, with an error where one of them is differentiated."""
+
+    @staticmethod
+    def forward(ctx, gradients, *sources):
+        return tuple(g.detach() for g in gradients)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("fused_qk_norm_rope is differentiable once: its gradients cannot be differentiated")
+
+
 class _FusedQKNormRoPE(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, cos, sin, positions, eps, interleaved):
@@ -64,25 +75,34 @@ class _FusedQKNormRoPE(torch.autograd.Function):
         return (q_out, k_out) if k is not None else q_out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk=None):
-        q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
-        refuse_tangents(gq, gk)
-        gq, gk = _dense_heads(gq), _dense_heads(gk if k is not None else None)
-        dq, dk = _empty_like_heads(q), _empty_like_heads(k)
-        dqw = torch.empty_like(qw) if qw is not None and ctx.needs_input_grad[2] else None
-        dkw = torch.empty_like(kw) if kw is not None and ctx.needs_input_grad[3] else None
-        with _lib.on_device(q):
-            ws = None
-            if dqw is not None or dkw is not None:
-                ws = _lib.scratch(_lib.load().tfo_qk_norm_rope_backward_workspace_bytes(q.shape[-1]), q.device)
-            _lib.call("tfo_qk_norm_rope_backward", gq.data_ptr(), _strides(gq), _lib.ptr(gk), _strides(gk), q.data_ptr(),
-                      _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(qw), _lib.ptr(kw),
-                      *_table_args(cos, sin, positions, q), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dqw), _lib.ptr(dkw),
-                      *_size_args(q, k, cos, ctx.interleaved), float(ctx.eps), _lib.dtype_code(q.dtype, "q"),
-                      _weight_code(qw, "q_weight"), _weight_code(kw, "k_weight"), _lib.dtype_code(cos.dtype, "cos"),
-                      _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q))
-        return dq, dk, dqw, dkw, None, None, None, None, None
+        with torch.no_grad():
+            d = _backward(ctx, gq, gk)
+        if torch.is_grad_enabled():  # create_graph
+            sealed = iter(_DifferentiableOnce.apply([t for t in d if t is not None], *ctx.saved_tensors[:4], gq, gk))
+            d = tuple(None if t is None else next(sealed) for t in d)
+        return (*d, None, None, None, None, None)
+
+
+def _backward(ctx, gq, gk):
+    """Gradients of q, k (or None) and the weights that want one."""
+    q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
+    refuse_tangents(gq, gk)
+    gq, gk = _dense_heads(gq), _dense_heads(gk if k is not None else None)
+    dq, dk = _empty_like_heads(q), _empty_like_heads(k)
+    dqw = torch.empty_like(qw) if qw is not None and ctx.needs_input_grad[2] else None
+    dkw = torch.empty_like(kw) if kw is not None and ctx.needs_input_grad[3] else None
+    with _lib.on_device(q):
+        ws = None
+        if dqw is not None or dkw is not None:
+            ws = _lib.scratch(_lib.load().tfo_qk_norm_rope_backward_workspace_bytes(q.shape[-1]), q.device)
+        _lib.call("tfo_qk_norm_rope_backward", gq.data_ptr(), _strides(gq), _lib.ptr(gk), _strides(gk), q.data_ptr(),
+                  _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(qw), _lib.ptr(kw),
+                  *_table_args(cos, sin, positions, q), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dqw), _lib.ptr(dkw),
+                  *_size_args(q, k, cos, ctx.interleaved), float(ctx.eps), _lib.dtype_code(q.dtype, "q"),
+                  _weight_code(qw, "q_weight"), _weight_code(kw, "k_weight"), _lib.dtype_code(cos.dtype, "cos"),
+                  _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(q))
+    return dq, dk, dqw, dkw
 
 
 def fused_qk_norm_rope(
@@ -107,7 +127,8 @@ def fused_qk_norm_rope(
 
     Returns:
         (q, k or None) normed and rotated, contiguous, in q's dtype.
-        Differentiable (once, in reverse mode) in q, k and the weights; a tensor
+        Differentiable (once, in reverse mode) in q, k and the weights: gradients
+        made with ``create_graph`` raise where they are differentiated. A tensor
         with a forward-mode tangent is refused.
     """
     fast = _lib.ext()
