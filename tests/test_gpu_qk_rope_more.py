@@ -1,5 +1,8 @@
 """rope_tables, fused_rope and fused_qk_norm_rope on the GPU: torch's default device, derivatives, small angles."""
 
+import math
+from fractions import Fraction
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -99,3 +102,37 @@ def test_gradients_made_with_create_graph(cuda, monkeypatch, extension, with_gra
             torch.autograd.grad(d.square().sum() + q.sum(), q, retain_graph=True)
         with pytest.raises(RuntimeError, match="once"):
             (d.square().sum() + q.square().sum()).backward(retain_graph=True)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("base, kind, factor", [(10000.0, None, 1.0), (5e5, "wavelength", 8.0), (1e7, "linear", 4.0), (1e6, "yarn", 16.0)])
+def test_small_sines_and_cosines_keep_their_bits(cuda, dtype, base, kind, factor):
+    """Tables relative to each value, not to the largest: slow pairs have angles of 1e-8 rad, and far positions pass
+    close by multiples of a quarter turn.
+
+    Relative bound in units of 2^-24: the remainder of the angle 1 (x cot x and x tan x are below 1 up to an eighth of
+    a turn), its series 2, the factor's own rounding 1 and its product 1: 5, taken as 8; then the type's half step.
+    Absolute: half a unit of 2^-64 turns at each position, and the fp16 subnormals' half step.
+    """
+    from triton_ops import RoPEScaling, rope_tables
+    from triton_ops.kernels.rope import rope_frequencies
+
+    dt, rot = getattr(torch, dtype), 128
+    at = [0, 1, 2, 3, 5, 100, 1023, 4097, 8191, 65537, 131071, 999983, 1000000, 2**31 - 1, -1, -77]
+    scaling = None if kind is None else RoPEScaling(kind, factor, 8192)
+    cos, sin = (t.cpu() for t in rope_tables(torch.tensor(at, device="cuda"), rot, base, scaling, dtype=dt))
+    freq, gain = rope_frequencies(rot, base, scaling)
+    want = torch.empty(2, len(at), rot // 2, dtype=torch.float64)
+    for j, f in enumerate(freq):
+        turns = Fraction(f / (2 * math.pi))
+        for i, p in enumerate(at):
+            quarters = turns * p * 4
+            near = round(quarters)
+            r = float(quarters - near) * (math.pi / 2)
+            c, s = ((math.cos(r), math.sin(r)), (-math.sin(r), math.cos(r)), (-math.cos(r), -math.sin(r)), (math.sin(r), -math.cos(r)))[near % 4]
+            want[0, i, j], want[1, i, j] = gain * c, gain * s
+    slack = gain * math.pi * 2.0**-64 * torch.tensor(at).abs().double()[:, None] + (2.0**-25 if dt == torch.float16 else 0.0)
+    for got, ref, name in ((cos, want[0], "cos"), (sin, want[1], "sin")):
+        assert torch.equal(got[:, : rot // 2], got[:, rot // 2 :])
+        over = (got[:, : rot // 2].double() - ref).abs() - ref.abs() * (8 * 2.0**-24 + torch.finfo(dt).eps / 2 * 1.01) - slack
+        assert over.max().item() <= 0, f"{name}: {over.max().item():.3e} over the bound"
