@@ -5,7 +5,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-DT = {"f16": torch.float16, "bf16": torch.bfloat16}
+DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 
 
 @pytest.mark.parametrize("rank", [2, 20, 40, 100, 256])
@@ -49,8 +49,9 @@ def test_fp32_sums_are_rounded_not_cut(cuda, t, rank):
 
     Bound relative to v, in units of 2^-24: the 16 terms of a chunk within one instruction chain, 6 steps of at most
     two units: 12; the chunks of half of K one after the other, each addition off by at most one unit of what is there
-    by then, which grows evenly: K / 64; the halves, warps and CTAs: 12 more additions; operands of two tf32 values
-    with the smallest product left out: three times 2^-22, 12; the same for v times one: 4 (B is one at one place).
+    by then, which grows evenly: K / 64; the halves, warps and CTAs: 12 more additions; each operand's lower tf32 value
+    2^-22, and the products of two of them left out, at most 2^-20 and 2^-22 on average over the terms: 12; the same for v
+    times one: 4 (B is one at one place).
     """
     from triton_ops import fused_lora
 
@@ -90,3 +91,78 @@ def test_autograd_hears_of_a_write(cuda, monkeypatch, extension, t):
         want = fused_lora(x, a, b, ids, base=y)
         assert torch.equal(fused_lora(x, a, b, ids, base=y, out=y), want)
     assert torch.equal(fused_lora(x, a, b, ids, out=y), want - 1)  # a tensor of inference mode keeps no version
+
+
+@pytest.mark.parametrize("rank", [1, 12, 32, 48, 128, 200])
+@pytest.mark.parametrize("t", [3, 40, 600])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_infinities_where_the_formula_has_them(cuda, dtype, t, rank):
+    """Infinities of x, A, B, the factors and base give infinities and NaN where the formula does, and nowhere else."""
+    from triton_ops import fused_lora
+
+    g = torch.Generator().manual_seed(100 * rank + t)
+    m, k, n, inf = 4, 24, 72, float("inf")
+    # quarters between 1 and 2, of both signs: exact in each type, no zero beside an infinity
+    x, a, b, base = ((1 + torch.randint(4, s, generator=g) / 4) * (1 - 2 * torch.randint(2, s, generator=g).float())
+                     for s in ((t, k), (m, rank, k), (m, n, rank), (t, n)))
+    scaling = torch.tensor([1.0, -0.5, 2.0, 1.5])
+    ids = torch.arange(t) % m
+    b[0, 5, 0], b[0, 6, rank - 1], b[1, 64, rank // 2] = inf, -inf, inf
+    if rank > 1:
+        b[0, 7, 0], b[0, 7, 1] = inf, -inf
+    a[2, rank // 2, 3] = -inf
+    b[2, 70, rank // 2] = inf
+    x[t - 1, 7] = inf
+    base[t // 2, 8], base[0, 9] = inf, float("nan")
+    for numbers in (x, a, b):  # where fp32 is split: values that a tf32 holds, and values that it does not
+        numbers.mul_(1.0 + (2.0**-20 if dtype == "f32" and t != 40 else 0.0))
+    ref = base.double() + torch.stack([(b[i].double() * (a[i].double() * x[r].double()).sum(-1)).sum(-1) * scaling[i]
+                                       for r, i in enumerate(ids.tolist())])
+    to = DT[dtype]
+    got = fused_lora(x.to(to).cuda(), a.to(to).cuda(), b.to(to).cuda(), ids.cuda(), scaling.cuda(),
+                     base=base.to(to).cuda()).double().cpu()
+    # Where fp32 operands are no tf32 values, a low-rank value whose terms cancel to zero is one only within its sum's
+    # rounding: times an infinity it is a NaN, or an infinity if the sum is not quite zero. Both are right.
+    if dtype == "f32" and t != 40:
+        for r, i in enumerate(ids.tolist()):
+            v = (a[i].double() * x[r].double()).sum(-1)
+            either = ((v == 0) & torch.isinf(b[i])).any(-1)
+            assert not torch.isfinite(got[r, either]).any()
+            got[r, either] = ref[r, either]
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    assert torch.equal(torch.isinf(got), torch.isinf(ref)) and torch.equal(got[torch.isinf(ref)], ref[torch.isinf(ref)])
+    fine = torch.isfinite(ref)
+    # |v| <= 1.75^2 k and |B|, |scaling| <= 2: magnitudes of at most 16 k rank; v of 16 bits: 2^-16 of them (its sum is
+    # exact); fp32: 2^-19 for both products; and the result's rounding
+    slack = rank * k * 16 * (2.0**-19 if dtype == "f32" else 2.0**-16)
+    assert ((got - ref).abs() <= ref.abs() * torch.finfo(to).eps / 2 * 1.01 + slack)[fine].all()
+
+
+def test_the_largest_fp32_values(cuda):
+    """Finite operands that round past the largest tf32."""
+    from triton_ops import fused_lora
+
+    big = torch.finfo(torch.float32).max
+    for t in (3, 500):
+        x, a, b = torch.full((t, 8), big, device="cuda"), torch.zeros(1, 1, 8, device="cuda"), torch.ones(1, 4, 1, device="cuda")
+        a[0, 0, 2] = 0.25
+        got = fused_lora(x, a, b, torch.zeros(t, dtype=torch.int64, device="cuda"))
+        assert ((got.double() - big / 4).abs() <= big / 4 * 2.0**-21).all()
+
+
+@pytest.mark.parametrize("t", [3, 500])
+def test_any_nan_is_a_nan(cuda, t):
+    """Also one whose bits past those of a tf32 are all that sets it apart from an infinity."""
+    from triton_ops import fused_lora
+
+    x, a, b = (torch.ones(s, device="cuda") for s in ((t, 8), (1, 4, 8), (1, 8, 4)))
+    ids = torch.zeros(t, dtype=torch.int64, device="cuda")
+    for bits in (0x7F800001, 0x7FC00000, 0x7FFFFFFF, -0x7FFFFF):  # the last: 0xff800001
+        for v, at, where in ((x, (1, 3), (slice(1, 2), slice(None))), (a, (0, 2, 5), (slice(None), slice(None))),
+                             (b, (0, 6, 1), (slice(None), slice(6, 7)))):
+            with_nan = v.clone()
+            with_nan.view(torch.int32)[at] = bits
+            got = fused_lora(*(with_nan if u is v else u for u in (x, a, b)), ids)
+            want = torch.zeros(t, 8, dtype=torch.bool, device="cuda")
+            want[where] = True
+            assert torch.equal(torch.isnan(got), want)

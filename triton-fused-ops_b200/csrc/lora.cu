@@ -37,17 +37,17 @@
 // waits, proxy fences and barriers ran 750 cycles with one CTA on an SM.
 //
 // Rounding: products and sums are fp32. v enters the second product as a sum
-// of values of x's type. fp16: two, 23 bits (rows are scaled by a power of two to
-// use fp16's whole range). bf16 up to 384 tokens: three, all 24 bits; more
-// tokens: two, 16 bits, with which 1 to 2 of 1000 outputs are not the nearest
-// value to the 64-bit result (three: 2 of 10000; the error against 64 bits is
-// the output's own rounding either way). Few tokens wait for memory, and the
-// third product costs them 0.1 to 0.3 us (one token 4.6 -> 4.7, 256 9.0 -> 9.3); many
-// are bound by the products: 8192 tokens of rank 32 47 -> 51 us with three, rank
-// 128 135 -> 157. fp32 operands are split into two tf32 values on both sides
-// and the three larger products are added, 16 terms at a time (Chunk<float>); the
-// sums of 16-bit types stay in the tensor instructions, whose cuts (1e-6) lie far
-// below the result's rounding. The result is rounded once.
+// of values of x's type, cut so that they have v's sign (stage_v). fp16: two, 22
+// bits (rows are scaled by a power of two to use fp16's whole range). bf16 up to
+// 384 tokens: three, all 24 bits; more tokens: two, 16 bits, with which 3 of 1000
+// outputs are not the nearest value to the 64-bit result (three: 1 of 10000; the
+// error against 64 bits is the output's own rounding either way). Few tokens wait
+// for memory, and the third product costs them 0.1 to 0.4 us (one token 4.6 ->
+// 4.8, 256 9.0 -> 9.4); many are bound by the products: 8192 tokens of rank 32 47
+// -> 51 us with three, rank 128 135 -> 157. fp32 operands are split into two tf32
+// values on both sides and the three larger products are added, 16 terms at a time
+// (Chunk<float>); the sums of 16-bit types stay in the tensor instructions, whose
+// cuts (1e-6) lie far below the result's rounding. The result is rounded once.
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -93,12 +93,19 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// x = hi + lo in two tf32 values (an infinity or NaN is all in hi).
+// x = hi + lo in two tf32 values of one sign, both infinite if x is, and neither
+// of them zero unless x is (or below 2^-62): an infinity of the other operand then
+// has the same sign in every product, where 0 * infinity or infinities of both
+// signs would be a NaN. 2^-64 of x in place of a zero lo lies below what a tensor
+// instruction keeps beside hi's product, so exact sums stay exact. hi is cut, not
+// rounded (lo's sign), and the product of both lo, left out, is 2^-23 of the
+// whole on average: results are 2.2e-7 to 3.2e-7 off 64 bits, 1.4e-7 to 2.0e-7
+// with a rounded hi.
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(__uint_as_float(x)));
-  const float h = __uint_as_float(hi);
-  const float rest = fabsf(h) <= 3.402823466e38f ? __uint_as_float(x) - h : 0.f;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+  hi = x & 0xffffe000u;  // cut
+  const float f = __uint_as_float(x);
+  const float rest = fmaxf(fabsf(f - __uint_as_float(hi)), fabsf(f * 0x1p-64f));  // infinity - infinity gives way
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(copysignf(rest, f)));
 }
 
 // d += the product over one 64-byte chunk: a0 / a1 are rows g and g + 8 of the
@@ -120,8 +127,8 @@ template <> struct Chunk<float> {
   // A chunk's sum starts at zero and is added to d by a rounded addition: the
   // tensor instructions cut their sum instead of rounding it, which over a long K
   // is a drift. Error of 1000 tokens of rank 256, K = 1024, against 64 bits 3.8e-6
-  // without these additions, 2.0e-7 with them; 8192 tokens of 4096 x 4096, rank
-  // 32 164 -> 163 us, rank 64 289 -> 324.
+  // without these additions, 3.2e-7 with them; 8192 tokens of 4096 x 4096, rank
+  // 16 161 -> 110 us, 32 164 -> 155, 64 289 -> 314 (with the present split).
   __device__ static void mma(float (&d)[4], const uint4& a0, const uint4& a1, const uint4& b) {
     float t[4] = {};
     half(t, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
@@ -503,12 +510,19 @@ template <typename T, int SPLITS, int M> struct Staged {
   __device__ Staged from(int elements) const { return Staged{at + elements, stride}; }
 };
 
-// Stages the tile's v as operands in shared memory. sum(m, r) gives four
-// neighbouring values of row m, summed and scaled. fp16 rows are scaled by a
-// power of two to below 2^15, so that values down to 2^-15 of a row's largest
-// keep all their bits (row_scale takes it back; `sums`, [M][sums_stride], holds
-// them meanwhile and may be what sum(m, r) reads); rows past the tile and ranks
-// past the end are zero.
+// x cut, not rounded, to T's bits.
+template <typename T> __device__ __forceinline__ float cut(float x);
+template <> __device__ __forceinline__ float cut<__half>(float x) { return __half2float(__float2half_rz(x)); }
+template <> __device__ __forceinline__ float cut<__nv_bfloat16>(float x) { return __bfloat162float(__float2bfloat16_rz(x)); }
+
+// Stages the tile's v as operands in shared memory, split into values of one
+// sign, of which none is zero unless v is (a zero one becomes 2^-24 of the scaled
+// row, or 2^-64 of v) and all are infinite if v is: beside an infinity of B their
+// products have one sign, as the whole v's. sum(m, r) gives four neighbouring
+// values of row m, summed and scaled. fp16 rows are scaled by a power of two to
+// below 2^15, so that values down to 2^-15 of a row's largest keep all their bits
+// (row_scale takes it back; `sums`, [M][sums_stride], holds them meanwhile and may
+// be what sum(m, r) reads); rows past the tile and ranks past the end are zero.
 template <typename T, int SPLITS, int M, typename Sum>
 __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, const Staged<T, SPLITS, M>& v, float* sums,
                                         int sums_stride, float* row_scale, unsigned* row_max, Sum sum) {
@@ -530,9 +544,10 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, cons
         float x = SCALED ? t[j] * down : t[j];
 #pragma unroll
         for (int i = 0; i < SPLITS; ++i) {
-          part[i][j] = Ty<T>::from_f(x);
-          const float f = Ty<T>::to_f(part[i][j]);
-          x = fabsf(f) <= 3.402823466e38f ? x - f : 0.f;  // infinities are all in the first
+          float f = i + 1 < SPLITS ? cut<T>(x) : Ty<T>::to_f(Ty<T>::from_f(x));
+          if (fabsf(f) <= 3.402823466e38f) x -= f;  // an infinity is all of them
+          if (f == 0.f && t[j] != 0.f) f = SCALED ? copysignf(0x1p-24f, t[j]) : 0x1p-64f * t[j];
+          part[i][j] = Ty<T>::from_f(f);
         }
       }
 #pragma unroll
