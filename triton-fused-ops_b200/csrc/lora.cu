@@ -1323,6 +1323,7 @@ cudaError_t choose_cluster(const LoraArgs& a, int64_t tiles, ShapeChoice* best) 
 template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
 cudaError_t launch_shape(const LoraArgs& a, const PlanBytes& p, const LoraPlan& plan, int64_t tiles, int cluster, cudaStream_t st) {
   using S = LargeShape<T, RANKS, VR, STEP, STAGES, VEC>;
+  if (a.rank > S::PR || a.rank > VR) return cudaErrorInvalidValue;  // the exchanged parts' rows would be written past their ends
   auto* kernel = lora_large_kernel<T, RANKS, VR, STEP, STAGES, VEC>;
   size_t smem = S::smem(cluster);
   if (const cudaError_t e = spread(reinterpret_cast<const void*>(kernel), kLargeThreads, cluster, tiles, &smem); e != cudaSuccess)
