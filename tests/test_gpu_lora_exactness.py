@@ -8,8 +8,8 @@ pytestmark = pytest.mark.gpu
 DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 
 
-@pytest.mark.parametrize("rank", [2, 20, 40, 100, 256])
-@pytest.mark.parametrize("dtype, bits, t", [("bf16", 24, 3), ("bf16", 24, 300), ("bf16", 16, 500), ("f16", 22, 3), ("f16", 22, 500)])
+@pytest.mark.parametrize("rank", [2, 13, 16, 20, 40, 100, 256])
+@pytest.mark.parametrize("dtype, bits, t", [("bf16", 24, 3), ("bf16", 24, 300), ("bf16", 24, 500), ("f16", 22, 3), ("f16", 22, 500)])
 def test_low_rank_values_keep_their_bits(cuda, dtype, bits, t, rank):
     """Two low-rank values below 2^bits that differ by less than 128, one subtracted from the other.
 

@@ -28,26 +28,27 @@
 // four instructions are dealt out so that a thread ends up with eight
 // neighbouring ones.
 //
-// Measured (us; 4096 x 4096, bf16): one token of rank 16 4.8; 64 tokens over 32
-// adapters 7.2; 256: 12.1; 512: 15.4; 8192 tokens of 16 adapters of rank 32 49,
-// 66 % of the measured copy rate (rank 64 72, rank 128 136: the legacy tensor
-// path's 530 TFLOP/s bounds those). A form of the large kernel on tcgen05
-// (128-row tiles copied into swizzled shared memory, v and the outputs in
+// Measured (us; 4096 x 4096, bf16): one token of rank 16 4.3; 64 tokens over 32
+// adapters 6.6, 256 over 16 8.5; 1024 over 16 17.9; 512 of rank 32 over 16 20.5;
+// 8192 tokens of 16 adapters of rank 16 47, of rank 32 51, 63 % of the measured
+// copy rate (rank 64 84, rank 128 171: the legacy tensor path's 530 TFLOP/s bounds
+// those). fp32: 8192 tokens of rank 16 106, 32 156, 64 312, bound by splitting the
+// operands and by three products. A form of the large kernel on tcgen05 (128-row
+// tiles copied into swizzled shared memory, v as two values and the outputs in
 // tensor memory) took 67 us at rank 32, 98 at 64 and 152 at 128: its steps'
 // waits, proxy fences and barriers ran 750 cycles with one CTA on an SM.
 //
-// Rounding: products and sums are fp32. v enters the second product as a sum
-// of values of x's type, cut so that they have v's sign (stage_v). fp16: two, 22
-// bits (rows are scaled by a power of two to use fp16's whole range). bf16 up to
-// 384 tokens: three, all 24 bits; more tokens: two, 16 bits, with which 3 of 1000
-// outputs are not the nearest value to the 64-bit result (three: 1 of 10000; the
-// error against 64 bits is the output's own rounding either way). Few tokens wait
-// for memory, and the third product costs them 0.1 to 0.4 us (one token 4.6 ->
-// 4.8, 256 9.0 -> 9.4); many are bound by the products: 8192 tokens of rank 32 47
-// -> 51 us with three, rank 128 135 -> 157. fp32 operands are split into two tf32
+// Rounding: products and sums are fp32. v enters the second product as a sum of
+// values of x's type, cut so that they have v's sign (stage_v): three of bf16, all
+// 24 bits; two of fp16, 22 bits (rows are scaled by a power of two to use fp16's
+// whole range). With two of bf16, 16 bits, 2 to 3 of 1000 outputs were not the
+// nearest value to the 64-bit result, with three 1 to 14 of 10000. The third
+// product costs where the products bound (8192 tokens of rank 32 47 -> 50 us, 64
+// 72 -> 83, 128 135 -> 160); up to 16 ranks half of a chunk's instructions had
+// multiplied zeros, and without them three are faster than two were (8192 tokens
+// 48.7 -> 46.8, one token 4.6 -> 4.3). fp32 operands are split into two tf32
 // values on both sides and the three larger products are added, 16 terms at a time
-// (Chunk<float>); the sums of 16-bit types stay in the tensor instructions, whose
-// cuts (1e-6) lie far below the result's rounding. The result is rounded once.
+// (Chunk<float>). The result is rounded once.
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -116,11 +117,19 @@ template <> struct Chunk<__half> {
     mma_f16(d, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
     mma_f16(d, a0.z, a1.z, a0.w, a1.w, b.z, b.w);
   }
+  // over half of one, 32 bytes: thread q has the q-th 8
+  __device__ static void mma(float (&d)[4], const uint2& a0, const uint2& a1, const uint2& b) {
+    mma_f16(d, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
+  }
 };
 template <> struct Chunk<__nv_bfloat16> {
   __device__ static void mma(float (&d)[4], const uint4& a0, const uint4& a1, const uint4& b) {
     mma_bf16(d, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
     mma_bf16(d, a0.z, a1.z, a0.w, a1.w, b.z, b.w);
+  }
+  // over half of one, 32 bytes: thread q has the q-th 8
+  __device__ static void mma(float (&d)[4], const uint2& a0, const uint2& a1, const uint2& b) {
+    mma_bf16(d, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
   }
 };
 template <> struct Chunk<float> {
@@ -128,7 +137,7 @@ template <> struct Chunk<float> {
   // tensor instructions cut their sum instead of rounding it, which over a long K
   // is a drift. Error of 1000 tokens of rank 256, K = 1024, against 64 bits 3.8e-6
   // without these additions, 3.2e-7 with them; 8192 tokens of 4096 x 4096, rank
-  // 16 161 -> 110 us, 32 164 -> 155, 64 289 -> 314 (with the present split).
+  // 16 161 -> 106 us, 32 164 -> 156, 64 289 -> 312 (with the present split).
   __device__ static void mma(float (&d)[4], const uint4& a0, const uint4& a1, const uint4& b) {
     float t[4] = {};
     half(t, a0.x, a1.x, a0.y, a1.y, b.x, b.y);
@@ -168,6 +177,18 @@ __device__ __forceinline__ uint4 load_chunk(const T* row, int64_t i, int64_t lim
 #pragma unroll
   for (int j = 0; j < E; ++j) t[j] = i + j < limit ? row[i + j] : Ty<T>::from_f(0.f);
   return *reinterpret_cast<const uint4*>(t);
+}
+
+// 8 bytes at row + i, likewise.
+template <typename T>
+__device__ __forceinline__ uint2 load_half(const T* row, int64_t i, int64_t limit, int width) {
+  constexpr int E = 8 / sizeof(T);
+  if (row == nullptr || i >= limit) return make_uint2(0, 0);
+  if (width >= E) return *reinterpret_cast<const uint2*>(row + i);
+  alignas(8) T t[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) t[j] = i + j < limit ? row[i + j] : Ty<T>::from_f(0.f);
+  return *reinterpret_cast<const uint2*>(t);
 }
 
 // ---- tiles of rows with the same adapter ------------------------------------------
@@ -500,14 +521,14 @@ __device__ __forceinline__ void fill_rows(const LoraArgs& a, const Tile& tile, c
 }
 
 // The values of x's type that v is split into: v = the sum of them.
-template <typename T, bool FEW> constexpr int kSplits = sizeof(T) == 4 ? 1 : FEW && std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
+template <typename T> constexpr int kSplits = sizeof(T) == 4 ? 1 : std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
 
-// The staged values of v, [M][stride] elements each, one after the other.
-template <typename T, int SPLITS, int M> struct Staged {
-  T* at;
+// The staged values of v, [M][stride] elements each; a third one lies elsewhere.
+template <typename T, int M> struct Staged {
+  T *at, *third;
   int stride;
-  __device__ T* split(int i) const { return at + i * M * stride; }
-  __device__ Staged from(int elements) const { return Staged{at + elements, stride}; }
+  __device__ T* split(int i) const { return i == 2 ? third : at + i * M * stride; }
+  __device__ Staged from(int elements) const { return Staged{at + elements, third + elements, stride}; }
 };
 
 // x cut, not rounded, to T's bits.
@@ -523,9 +544,16 @@ template <> __device__ __forceinline__ float cut<__nv_bfloat16>(float x) { retur
 // below 2^15, so that values down to 2^-15 of a row's largest keep all their bits
 // (row_scale takes it back; `sums`, [M][sums_stride], holds them meanwhile and may
 // be what sum(m, r) reads); rows past the tile and ranks past the end are zero.
-template <typename T, int SPLITS, int M, typename Sum>
-__device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, const Staged<T, SPLITS, M>& v, float* sums,
+// OVER_VR: if not 0, vr, and the third of the split values lies over what sum(m, r)
+// reads: it is held until all of that has been read (256 threads).
+template <typename T, int OVER_VR, int M, typename Sum>
+__device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, const Staged<T, M>& v, float* sums,
                                         int sums_stride, float* row_scale, unsigned* row_max, Sum sum) {
+  constexpr int SPLITS = kSplits<T>;
+  constexpr bool OVER = OVER_VR > 0 && SPLITS == 3;
+  constexpr int TURNS = OVER ? M * OVER_VR / 4 / 256 : 1;
+  static_assert(!OVER || M * OVER_VR / 4 % 256 == 0, "whole turns of the threads");
+  uint2 held[TURNS];
   constexpr bool SCALED = std::is_same<T, __half>::value;
   const int shift = 31 - __clz(vr / 4), quads = 1 << shift, threads = blockDim.x;  // vr is a power of two
   if constexpr (SCALED) {
@@ -533,7 +561,7 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, cons
     __syncthreads();
   }
   // four values of row m, split
-  auto put = [&](int m, int r, const float (&t)[4], float down) {
+  auto put = [&](int m, int r, const float (&t)[4], float down, uint2& third) {
     const int to = m * v.stride + r;
     if constexpr (SPLITS == 1) {
       *reinterpret_cast<float4*>(v.split(0) + to) = make_float4(t[0], t[1], t[2], t[3]);
@@ -551,12 +579,14 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, cons
         }
       }
 #pragma unroll
-      for (int i = 0; i < SPLITS; ++i) *reinterpret_cast<uint2*>(v.split(i) + to) = *reinterpret_cast<const uint2*>(part[i]);
+      for (int i = 0; i < SPLITS; ++i) {
+        const uint2 u = *reinterpret_cast<const uint2*>(part[i]);
+        if (OVER && i == 2) third = u;
+        else *reinterpret_cast<uint2*>(v.split(i) + to) = u;
+      }
     }
   };
-  // Not unrolled: most launches take one turn or two (64 tokens over 32 adapters 7.5 -> 7.3 us).
-#pragma unroll 1
-  for (int i = threadIdx.x; i < M * quads; i += threads) {
+  auto take = [&](int i, uint2& third) {
     const int m = i >> shift, r = (i & (quads - 1)) * 4;
     float t[4] = {};
     if (m < tile.count && r < rank) {
@@ -576,10 +606,26 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, cons
       }
       if (most != 0.f) atomicMax(row_max + m, __float_as_uint(most));  // ordered like the floats
     } else {
-      put(m, r, t, 1.f);
+      put(m, r, t, 1.f, third);
     }
+  };
+  if constexpr (OVER) {
+#pragma unroll
+    for (int n = 0; n < TURNS; ++n) take(n * 256 + static_cast<int>(threadIdx.x), held[n]);
+  } else {
+    // Not unrolled: most launches take one turn or two (64 tokens over 32 adapters 7.5 -> 7.3 us).
+#pragma unroll 1
+    for (int i = threadIdx.x; i < M * quads; i += threads) take(i, held[0]);
   }
   __syncthreads();
+  if constexpr (OVER) {
+#pragma unroll
+    for (int n = 0; n < TURNS; ++n) {
+      const int i = n * 256 + static_cast<int>(threadIdx.x);
+      *reinterpret_cast<uint2*>(v.third + (i >> shift) * v.stride + (i & (quads - 1)) * 4) = held[n];
+    }
+    __syncthreads();
+  }
   if constexpr (SCALED) {
     for (int m = threadIdx.x; m < M; m += threads) {
       const float most = __uint_as_float(row_max[m]);
@@ -592,7 +638,7 @@ __device__ __forceinline__ void stage_v(const Tile& tile, int rank, int vr, cons
       float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < sums_stride) u = *reinterpret_cast<const float4*>(sums + m * sums_stride + r);
       const float t[4] = {u.x, u.y, u.z, u.w};
-      put(m, r, t, 1.f / row_scale[m]);
+      put(m, r, t, 1.f / row_scale[m], held[0]);
     }
     __syncthreads();
   }
@@ -619,33 +665,41 @@ template <int M> struct SumParts {
 // The product over chunk c of 16 staged rows (v: this lane's place in row g)
 // with 32 rows of B given by bf(j, chunk): adds to acc, the smallest of the
 // split values first.
-template <typename T, int SPLITS, int M, typename LoadB>
-__device__ __forceinline__ void expand_chunk(float (&acc)[4][4], const Staged<T, SPLITS, M>& v, int c, LoadB bf) {
+template <typename T, int M, typename LoadB>
+__device__ __forceinline__ void expand_chunk(float (&acc)[4][4], const Staged<T, M>& v, int c, LoadB bf) {
   constexpr int C = chunk_elems(sizeof(T));
   uint4 b[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) b[j] = bf(j, c);
 #pragma unroll
-  for (int i = SPLITS - 1; i >= 0; --i) {
+  for (int i = kSplits<T> - 1; i >= 0; --i) {
     const uint4 a0 = *reinterpret_cast<const uint4*>(v.split(i) + c * C);
     const uint4 a1 = *reinterpret_cast<const uint4*>(v.split(i) + 8 * v.stride + c * C);
 #pragma unroll
     for (int j = 0; j < 4; ++j) Chunk<T>::mma(acc[j], a0, a1, b[j]);
   }
 }
-// The same with the rows' few chunks kept in registers.
-template <typename T, int SPLITS, int NCH>
+// What a thread holds of a row in the expand step: the q-th 16 bytes of a chunk
+// or, where ranks end with its first half (HALF: 16-bit types, up to 16 ranks), the
+// q-th 8 of that half, for which one instruction does instead of two.
+template <bool HALF> using Operand = std::conditional_t<HALF, uint2, uint4>;
+
+// expand_chunk's product with the rows' few chunks kept in registers.
+template <typename T, int NCH, bool HALF>
 struct StagedRows {
-  uint4 a0[SPLITS][NCH], a1[SPLITS][NCH];
+  static constexpr int SPLITS = kSplits<T>;
+  using Vec = Operand<HALF>;
+  static_assert(!HALF || NCH == 1, "half of the only chunk");
+  Vec a0[SPLITS][NCH], a1[SPLITS][NCH];
   template <int M>
-  __device__ void load(const Staged<T, SPLITS, M>& v) {
+  __device__ void load(const Staged<T, M>& v) {
     constexpr int C = chunk_elems(sizeof(T));
 #pragma unroll
     for (int i = 0; i < SPLITS; ++i) {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        a0[i][c] = *reinterpret_cast<const uint4*>(v.split(i) + c * C);
-        a1[i][c] = *reinterpret_cast<const uint4*>(v.split(i) + 8 * v.stride + c * C);
+        a0[i][c] = *reinterpret_cast<const Vec*>(v.split(i) + c * C);
+        a1[i][c] = *reinterpret_cast<const Vec*>(v.split(i) + 8 * v.stride + c * C);
       }
     }
   }
@@ -655,7 +709,7 @@ struct StagedRows {
     for (int c = 0; c < NCH; ++c) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 b = bf(j, c);
+        const Vec b = bf(j, c);
 #pragma unroll
         for (int i = SPLITS - 1; i >= 0; --i) Chunk<T>::mma(acc[j], a0[i][c], a1[i][c], b);
       }
@@ -699,7 +753,7 @@ struct SmallWidths {  // elements that rows are aligned to: of x and A, of B; wh
 // base values before the exchange, and each next block's before the one at hand
 // is computed. Its instructions are fetched once, too, so the kernel is kept
 // short: four chunks or two blocks in flight were 0.2 and 0.3 us slower. One
-// token, 4096 x 4096, rank 16, bf16: 4.8 us, of which the launch is 1.5 (two
+// token, 4096 x 4096, rank 16, bf16: 4.3 us, of which the launch is 1.5 (two
 // launches with v in global memory took 6.3).
 template <typename T, int NT, bool VEC>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) lora_small_kernel(const LoraArgs a, int log_cluster, SmallWidths given, int64_t v_rank,
@@ -744,9 +798,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) lora_small_kernel
   const int vr = static_cast<int>(v_rank), rank = static_cast<int>(a.rank);
   const int stride = vr + E, quads = (rank + 3) / 4;
   float* parts = reinterpret_cast<float*>(smem);  // [cluster][M][vr]: the CTAs' parts of v
-  constexpr int SPLITS = kSplits<T, true>;
-  const Staged<T, SPLITS, M> v{reinterpret_cast<T*>(smem + sizeof(float) * cluster * M * vr), stride};
-  auto* red = reinterpret_cast<float(*)[M][RB + 4]>(v.split(SPLITS));  // [kSmallWarps]
+  T* const staged = reinterpret_cast<T*>(smem + sizeof(float) * cluster * M * vr);
+  const Staged<T, M> v{staged, staged + 2 * M * stride, stride};
+  auto* red = reinterpret_cast<float(*)[M][RB + 4]>(staged + kSplits<T> * M * stride);  // [kSmallWarps]
   if (t == 0) mbar_arrive_expect_tx(&received, static_cast<uint32_t>(cluster * tile.count * quads * 16));
   const bool in0 = g < tile.count, in1 = g + 8 < tile.count;
   const int64_t t0 = rows[in0 ? g : 0], t1 = rows[in1 ? g + 8 : 0];
@@ -809,12 +863,15 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) lora_small_kernel
   const T* b = static_cast<const T*>(a.b) + static_cast<int64_t>(tile.group) * a.n * rank;
   const T* base0 = a.base != nullptr ? static_cast<const T*>(a.base) + t0 * a.base_stride + q * 8 : nullptr;
   const T* base1 = a.base != nullptr ? static_cast<const T*>(a.base) + t1 * a.base_stride + q * 8 : nullptr;
+  constexpr bool HALF = NT == 2 && sizeof(T) == 2;
   auto b_chunk = [&](int64_t n0, int j, int c) {
     const int64_t col = n0 + block_column(g) + 2 * j;
-    return load_chunk<T>(col < col1 ? b + col * rank : nullptr, c * C + q * E, rank, width.b);
+    const T* row = col < col1 ? b + col * rank : nullptr;
+    if constexpr (HALF) return load_half<T>(row, q * (E / 2), rank, width.b);
+    else return load_chunk<T>(row, c * C + q * E, rank, width.b);
   };
   struct Block {
-    uint4 b[4];
+    Operand<HALF> b[4];
     Eight<T> e0, e1;
   };
   auto load_block = [&](Block& k, int64_t n0) {
@@ -832,17 +889,23 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) lora_small_kernel
   const float scale = a.scaling != nullptr ? a.scaling[tile.group] : 1.f;
   const bool arrived = mbar_wait(&received, 0, err, ERR_WAIT_TIMEOUT_OTHER);
   if (__syncthreads_or(!arrived)) return;
-  stage_v(tile, rank, vr, v, parts, vr, row_scale, row_max, SumParts<M>{parts, cluster, vr, scale});
+  stage_v<T, 0>(tile, rank, vr, v, parts, vr, row_scale, row_max, SumParts<M>{parts, cluster, vr, scale});
   const float s0 = SCALED ? row_scale[g] : 1.f, s1 = SCALED ? row_scale[g + 8] : 1.f;
-  const Staged<T, SPLITS, M> mine = v.from(g * stride + q * E);
+  const Staged<T, M> mine = v.from(g * stride + q * (HALF ? E / 2 : E));
+  StagedRows<T, 1, HALF> held;
+  if constexpr (HALF) held.load(mine);
   T* out0 = static_cast<T*>(a.out) + t0 * a.out_stride + q * 8;
   T* out1 = static_cast<T*>(a.out) + t1 * a.out_stride + q * 8;
   for (int64_t n0 = first; n0 < col1; n0 += kStride) {
     const Block now = next;
     if (n0 + kStride < col1) load_block(next, n0 + kStride);
     float acc[4][4] = {};
-    expand_chunk(acc, mine, 0, [&](int j, int) { return now.b[j]; });
-    for (int c = 1; c < vr / C; ++c) expand_chunk(acc, mine, c, [&](int j, int k) { return b_chunk(n0, j, k); });
+    if constexpr (HALF) {
+      held.expand(acc, [&](int j, int) { return now.b[j]; });
+    } else {
+      expand_chunk(acc, mine, 0, [&](int j, int) { return now.b[j]; });
+      for (int c = 1; c < vr / C; ++c) expand_chunk(acc, mine, c, [&](int j, int k) { return b_chunk(n0, j, k); });
+    }
     float f0[8], f1[8];
     block_values(acc, s0, s1, f0, f1);
     const int64_t left = col1 - n0 - q * 8;
@@ -877,10 +940,13 @@ struct LargeShape {
   static constexpr int kShrink = kRows + RANKS * SB, kExpand = kRows + KS * NCH * 64;
   static constexpr int kStage = kShrink > kExpand ? kShrink : kExpand;
   static constexpr int stride = VR + E;
-  static constexpr size_t kStaged = static_cast<size_t>(kSplits<T, false>) * sizeof(T) * M * stride;
+  // v's split values, a third one over the exchanged parts (they are summed by then)
+  static constexpr size_t kSplit = sizeof(T) * M * stride, kStaged = (kSplits<T> == 1 ? 1 : 2) * kSplit;
   static_assert(kStaged >= sizeof(float) * M * (RANKS + 4), "the halves' sums fit where v is staged later");
   static constexpr int PR = VR > RANKS && RANKS < 128 ? RANKS : VR;  // ranks of a row of an exchanged part
-  static size_t smem(int cluster) { return STAGES * kStage + kStaged + sizeof(float) * cluster * M * PR; }
+  static size_t smem(int cluster) {
+    return STAGES * kStage + kStaged + std::max(kSplits<T> == 3 ? kSplit : 0, sizeof(float) * cluster * M * PR);
+  }
 };
 
 template <typename T, int RANKS, int VR, int STEP, int STAGES, bool VEC>
@@ -917,10 +983,9 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
   }
   const int rank = static_cast<int>(a.rank), quads = (rank + 3) / 4;
   uint8_t* ring = smem;
-  constexpr int SPLITS = kSplits<T, false>;
-  const Staged<T, SPLITS, M> v{reinterpret_cast<T*>(smem + STAGES * S::kStage), stride};
-  auto* halves = reinterpret_cast<float(*)[RANKS + 4]>(v.at);  // until v is staged
   float* parts = reinterpret_cast<float*>(smem + STAGES * S::kStage + S::kStaged);  // [cluster][M][PR]
+  const Staged<T, M> v{reinterpret_cast<T*>(smem + STAGES * S::kStage), reinterpret_cast<T*>(parts), stride};
+  auto* halves = reinterpret_cast<float(*)[RANKS + 4]>(v.at);  // until v is staged
   if (t == 0) mbar_arrive_expect_tx(&received, static_cast<uint32_t>(cluster * tile.count * quads * 16));
   const int g = lane >> 2, q = lane & 3;
   const int m0 = (warp & 3) * 16, half = warp >> 2;
@@ -1085,18 +1150,19 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
     asm volatile("cp.async.wait_all;" ::: "memory");
     return;
   }
-  stage_v(tile, rank, VR, v, parts, S::PR, row_scale, row_max, SumParts<M>{parts, cluster, S::PR, scale});
+  stage_v<T, VR>(tile, rank, VR, v, parts, S::PR, row_scale, row_max, SumParts<M>{parts, cluster, S::PR, scale});
   const bool in0 = m0 + g < tile.count, in1 = m0 + g + 8 < tile.count;
   const float f0s = SCALED ? row_scale[m0 + g] : 1.f, f1s = SCALED ? row_scale[m0 + g + 8] : 1.f;
-  const Staged<T, SPLITS, M> mine = v.from((m0 + g) * stride + q * E);
+  constexpr bool HALF = RANKS == 16 && sizeof(T) == 2;
+  const Staged<T, M> mine = v.from((m0 + g) * stride + q * (HALF ? E / 2 : E));
   const int64_t t0 = rows[in0 ? m0 + g : 0], t1 = rows[in1 ? m0 + g + 8 : 0];
   T* out0 = static_cast<T*>(a.out) + t0 * a.out_stride + col0 + q * 8;
   T* out1 = static_cast<T*>(a.out) + t1 * a.out_stride + col0 + q * 8;
   constexpr bool HELD = NCH <= 2 && sizeof(T) == 2;
-  StagedRows<T, SPLITS, HELD ? NCH : 1> held;
+  StagedRows<T, HELD ? NCH : 1, HALF> held;
   if constexpr (HELD) held.load(mine);
   constexpr int BLOCKS = KS / 32;  // of a step: the halves of the warps share them, or take turns
-  const uint32_t b_at = S::kRows + tile_offset(block_column(g), NCH, 0, q);
+  const uint32_t b_at = S::kRows + (HALF ? tile_offset(block_column(g), NCH, 0, 0) + q * 8 : tile_offset(block_column(g), NCH, 0, q));
   const uint32_t e_at = (m0 + g) * S::SB;
   uint32_t now = 0, free = (STAGES - 1) * S::kStage;
   const int steps = s1i - s0i;
@@ -1116,7 +1182,7 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
         const uint8_t* bs = ring + now + b_at + blk * 32 * NCH * 64;
         auto bf = [&](int j, int c) {  // chunk c of an odd row may be swapped
           const int on = (NCH & 1) ? c * 64 : ((c ^ (g & 1)) - (g & 1)) * 64;
-          return lds16(bs + j * 2 * NCH * 64 + on);
+          return *reinterpret_cast<const Operand<HALF>*>(bs + j * 2 * NCH * 64 + on);
         };
         if constexpr (HELD) {
           held.expand(acc[i], bf);
@@ -1270,13 +1336,13 @@ cudaError_t launch_small(const LoraArgs& a, cudaStream_t st) {
   // at most so many tiles, most of them there when the adapters are mixed
   const int64_t tiles = std::min(a.tokens, a.tokens / kSmallRows + a.adapters + 2);
   // enough CTAs that a warp has about two chunks of K and two blocks of
-  // columns, about one wave of them, and 16 KB of exchanged sums at most
+  // columns, about one wave of them, and 32 KB of exchanged sums at most
   const int64_t chunks = (a.k + chunk_elems(sizeof(T)) - 1) / chunk_elems(sizeof(T));
   const int64_t want = std::max(chunks / (2 * kSmallWarps), a.n / (2 * 32 * kSmallWarps));
   int cluster = 1;
   while (cluster < kMaxCluster && cluster < want && 2 * cluster * tiles <= 4 * num_sms() && 2 * cluster * v_rank <= 512)
     cluster *= 2;
-  const size_t smem = kSmallRows * (sizeof(float) * v_rank * cluster + kSplits<T, true> * sizeof(T) * (v_rank + E));
+  const size_t smem = kSmallRows * (sizeof(float) * v_rank * cluster + kSplits<T> * sizeof(T) * (v_rank + E));
   auto launch = [&](auto* kernel, int nt) {
     size_t bytes = smem + sizeof(float) * kSmallWarps * kSmallRows * (8 * nt + 4);
     if (const cudaError_t e = spread(reinterpret_cast<const void*>(kernel), 256, cluster, tiles, &bytes); e != cudaSuccess) return e;
