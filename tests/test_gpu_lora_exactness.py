@@ -67,6 +67,38 @@ def test_fp32_sums_are_rounded_not_cut(cuda, t, rank):
     assert ((got.double() - want).abs() <= (k / 64 + 40) * 2.0**-24 * want).all()
 
 
+@pytest.mark.parametrize("rank", [2, 30, 60, 120])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_long_sums_have_no_drift(cuda, dtype, rank):
+    """The mean error of sums of 4096 positive terms in 16-bit types, in units of 2^-24 of the sum.
+
+    Each row's sum S (products of 16 bits, 27 bits in all) is subtracted from itself: x holds its first 24 bits in three
+    further columns, which the last rank adds up exactly. Rounded additions and rounded split values are off by as
+    much either way; what is left of the mean is cut inside a step, at most eight instructions of at most two units of
+    the step's own sum: 16, and 2 for the mean of the rest over 8192 rows. Sums kept in the instructions lose half an
+    ulp, on average, of what is there at each of 128 (or with two CTAs a tile 64): 48 units (24)."""
+    from triton_ops import fused_lora
+
+    t, k, n = 8192, 4096, 16
+    g = torch.Generator(device="cuda").manual_seed(rank)
+    x = torch.zeros(t, k + 32, device="cuda")
+    x[:, :k] = 1 + torch.randint(128, (t, k), device="cuda", generator=g) / 128
+    a = torch.zeros(1, rank, k + 32, device="cuda")
+    a[0, 0, :k] = 1 + torch.randint(128, (k,), device="cuda", generator=g) / 128
+    a[0, rank - 1, k:] = 1.0
+    total = x.double() @ a[0, 0].double()
+    step = 2.0 ** (torch.floor(torch.log2(total)) - 23)
+    whole = torch.round(total / step).long()
+    for i, shift in enumerate((16, 8, 0)):  # eight bits each: values of both types
+        x[:, k + i] = ((whole >> shift) % 256 * 2**shift).double().mul(step).float()
+    b = torch.zeros(1, n, rank, device="cuda")
+    b[0, :, 0], b[0, :, rank - 1] = 1.0, -1.0
+    dt = DT[dtype]
+    got = fused_lora(x.to(dt), a.to(dt), b.to(dt), torch.zeros(t, dtype=torch.int64, device="cuda"))
+    want = total - whole.double() * step
+    assert abs(((got.double() - want[:, None]) / total[:, None]).mean().item()) <= 18 * 2.0**-24
+
+
 @pytest.mark.parametrize("extension", [True, False])
 @pytest.mark.parametrize("t", [9, 500])
 def test_autograd_hears_of_a_write(cuda, monkeypatch, extension, t):

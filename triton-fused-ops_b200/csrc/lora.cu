@@ -38,17 +38,18 @@
 // tensor memory) took 67 us at rank 32, 98 at 64 and 152 at 128: its steps'
 // waits, proxy fences and barriers ran 750 cycles with one CTA on an SM.
 //
-// Rounding: products and sums are fp32. v enters the second product as a sum of
-// values of x's type, cut so that they have v's sign (stage_v): three of bf16, all
-// 24 bits; two of fp16, 22 bits (rows are scaled by a power of two to use fp16's
-// whole range). With two of bf16, 16 bits, 2 to 3 of 1000 outputs were not the
-// nearest value to the 64-bit result, with three 1 to 14 of 10000. The third
-// product costs where the products bound (8192 tokens of rank 32 47 -> 50 us, 64
-// 72 -> 83, 128 135 -> 160); up to 16 ranks half of a chunk's instructions had
-// multiplied zeros, and without them three are faster than two were (8192 tokens
-// 48.7 -> 46.8, one token 4.6 -> 4.3). fp32 operands are split into two tf32
-// values on both sides and the three larger products are added, 16 terms at a time
-// (Chunk<float>). The result is rounded once.
+// Rounding: products and sums are fp32 (long sums by rounded additions, see the
+// shrink step and Chunk<float>: a tensor instruction cuts what it adds to). v enters
+// the second product as a sum of values of x's type, cut so that they have v's
+// sign (stage_v): three of bf16, all 24 bits; two of fp16, 22 bits (rows are scaled
+// by a power of two to use fp16's whole range). With two of bf16, 16 bits, 2 of 1000
+// outputs were not the nearest value to the 64-bit result, with three and rounded
+// sums 1 to 3 of 10000, like an fp32 matrix product's. The third product costs
+// where the products bound (8192 tokens of rank 32 47 -> 50 us, 64 72 -> 83, 128
+// 135 -> 160); up to 16 ranks half of a chunk's instructions had multiplied zeros,
+// and without them three are faster than two were (8192 tokens 48.7 -> 47.2, one
+// token 4.6 -> 4.3). fp32 operands are split into two tf32 values on both sides
+// and the three larger products are added. The result is rounded once.
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -1052,6 +1053,11 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
     };
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) load(i * S::kStage);
+    // A tensor instruction cuts what it adds to: over 4096 columns 3e-6 of the sum (8192 tokens of rank 64 in fp16:
+    // 1 of 100 outputs off by a step, 1 of 700 without it; the time of rank 32 is the same, of 128 160 -> 171 us). So a
+    // step's sums start at zero and are added by rounded additions, GROUP at a time where that was faster (an instruction
+    // waits for the one before it on the same sum; rank 64 88 -> 84 us, 128 in fp32 168 -> 158, in bf16 171 -> 174).
+    constexpr int GROUP = NT == 8 || (NT == 16 && sizeof(T) == 4) ? 4 : 1;
     float acc[NT][4] = {};
     uint32_t now = 0, free = (STAGES - 1) * S::kStage;  // the stage at hand, and the one before it
     for (int step = k0; step < k1; ++step) {
@@ -1061,14 +1067,45 @@ __global__ void __launch_bounds__(kLargeThreads) lora_large_kernel(const LoraArg
       if (busy) {
         const uint8_t* xs = ring + now + x_at;
         const uint8_t* as = ring + now + a_at;
+        // the next chunk: 64 bytes on, or where the swap of odd rows puts it
+        int on[kHalfChunks];
+        uint4 a0[kHalfChunks], a1[kHalfChunks];
 #pragma unroll
         for (int h = 0; h < kHalfChunks; ++h) {
-          // the next chunk: 64 bytes on, or where the swap of odd rows puts it
-          const int on = h == 0 ? 0 : static_cast<int>(tile_offset(g, kChunks, half * kHalfChunks + h, q)) -
-                                          static_cast<int>(tile_offset(g, kChunks, half * kHalfChunks, q));
-          const uint4 a0 = lds16(xs + on), a1 = lds16(xs + on + 8 * S::SB);
+          on[h] = h == 0 ? 0 : static_cast<int>(tile_offset(g, kChunks, half * kHalfChunks + h, q)) -
+                                   static_cast<int>(tile_offset(g, kChunks, half * kHalfChunks, q));
+          a0[h] = lds16(xs + on[h]);
+          a1[h] = lds16(xs + on[h] + 8 * S::SB);
+        }
 #pragma unroll
-          for (int j = 0; j < NT; ++j) Chunk<T>::mma(acc[j], a0, a1, lds16(as + on + j * 8 * S::SB));
+        for (int j0 = 0; j0 < NT; j0 += GROUP) {
+          float t[GROUP][4] = {};
+#pragma unroll
+          for (int h = 0; h < kHalfChunks; ++h) {
+            uint4 b[GROUP];
+#pragma unroll
+            for (int j = 0; j < GROUP; ++j) b[j] = lds16(as + on[h] + (j0 + j) * 8 * S::SB);
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+              for (int j = 0; j < GROUP; ++j)
+                Chunk<T>::mma(t[j], make_uint2(a0[h].x, a0[h].y), make_uint2(a1[h].x, a1[h].y), make_uint2(b[j].x, b[j].y));
+#pragma unroll
+              for (int j = 0; j < GROUP; ++j)
+                Chunk<T>::mma(t[j], make_uint2(a0[h].z, a0[h].w), make_uint2(a1[h].z, a1[h].w), make_uint2(b[j].z, b[j].w));
+            } else {
+#pragma unroll
+              for (int j = 0; j < GROUP; ++j) Chunk<T>::mma(t[j], a0[h], a1[h], b[j]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < GROUP; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              const F2 sum = add2(f2(acc[j0 + j][i], acc[j0 + j][i + 1]), f2(t[j][i], t[j][i + 1]));
+              acc[j0 + j][i] = sum.x;
+              acc[j0 + j][i + 1] = sum.y;
+            }
+          }
         }
       }
       free = now;
