@@ -330,7 +330,8 @@ struct LaneGroup {
     p = spare ? 0 : lane - base;
   }
   template <int O> __device__ static float xor_add(float v) { return v + __shfl_xor_sync(0xffffffffu, v, O); }
-  // Sum over the group's lanes, the same bits in each of them.
+  // Sum over the group's lanes, the same bits in each of them: a tree for 4, 8 and
+  // 16 lanes, else (1 to 32, the widest heads) a shuffle for each.
   __device__ float sum(float v) const {
     if (lanes == 8) return xor_add<1>(xor_add<2>(xor_add<4>(v)));
     if (lanes == 16) return xor_add<1>(xor_add<2>(xor_add<4>(xor_add<8>(v))));

@@ -16,8 +16,8 @@
 // norm: 215 us, 95 % of the measured copy rate (1.34 GB); 65536 tokens of
 // 16 + 16 heads of 64, fp32: 174 us (94 %); of 12 + 3 heads of 80, f16: 69 us
 // (70 %; five lanes a head, summed by five shuffles); of 8 + 1 heads of 256,
-// bf16: 126 us (73 %; a key head's table row costs as much as itself). One
-// token: 1.9 us, a launch.
+// bf16: 126 us (73 %; a unit of the keys holds one head where it has room for four,
+// and both sides read a token's table row). One token: 1.9 us, a launch.
 #include "heads.cuh"
 
 namespace tfo {
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(256, 2) qk_rope_stream_kernel(const HeadArgs a
     token_rotation<E, PAIRS, NORM>(rot, a, side, col, pos);
     T* out = static_cast<T*>(side.out) + (static_cast<int64_t>(token) * heads + h0) * D + column;
     st.wait();
-    // Lane groups that are no power of two sum by a shuffle for each lane: there
+    // Lane groups that do not fill the warp mostly sum by a shuffle for each lane: there
     // the heads' sums go side by side and the heads are read again after them
     // (12 + 3 heads of 80, f16, 65536 tokens 72.4 -> 68.8 us).
     constexpr int AT_ONCE = FULL || !NORM ? 1 : NH;

@@ -15,9 +15,11 @@
 //
 // Floor: HBM (x and dy read, dx written). Measured at 32768 tokens of 32 + 8
 // heads of 128 columns, bf16: 183 us with the weights' gradients, 84 % of the
-// measured copy rate; 8192 tokens 53 us (73 %). The two sums over a head's
-// lanes and 128 registers a thread (16 warps an SM) bound it: the schedulers
-// issue in 49 % of the cycles and the rest is latency within a warp.
+// measured copy rate; 8192 tokens 53 us (73 %). What bounds it is latency within
+// a warp, of which an SM holds 16 (128 registers a thread): the schedulers issue in
+// 50 % of the cycles, and waits for loads are the longest stall. A unit's copies are
+// issued after the arithmetic of the one before, so that with two stages none is in
+// flight meanwhile: a copy's whole latency shows in every unit.
 #include "heads.cuh"
 
 namespace tfo {
@@ -94,8 +96,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) qk_norm_rope_backward_kernel(
     }
     T* out = static_cast<T*>(side.out) + (static_cast<int64_t>(token) * heads + h0) * D + column;
     st.wait();
-    // Heads of full warps one at a time. Lane groups that are no power of two sum
-    // by a shuffle for each lane: there the sums of all heads go side by side and
+    // Heads of full warps one at a time. In the others lane groups mostly sum by a
+    // shuffle for each lane (LaneGroup::sum): there the sums of all heads go side by side and
     // the heads are read again after them (12 + 3 heads of 80 columns, f16, 32768
     // tokens 69.0 -> 62.6 us; heads of 128 no faster).
     constexpr int AT_ONCE = FULL ? 1 : NH;
