@@ -361,6 +361,73 @@ TFO_API int tfo_lora(const void* x, int64_t x_stride, const void* a, const void*
                      int64_t tokens, int64_t adapters, int64_t rank, int64_t k, int64_t n, int dtype, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The residual stream between the blocks: a block's branch added to it with
+ * the norms before and after, and dropout. No counterpart in the reference.
+ * ------------------------------------------------------------------------- */
+
+/* Which elements a dropout drops. Element i of a call (in the order of a
+ * contiguous tensor) is dropped when word i % 4 of the Philox4x32-10 block of
+ * counter (i / 4, offset) under the key `seed` is below p 2^32 (rounded to an
+ * integer); what is kept is multiplied by 1 / (1 - p). */
+typedef struct tfo_dropout_params {
+  double p;             /* in [0, 1] */
+  const int64_t* seed;  /* on the device, or NULL: seed_value */
+  uint64_t seed_value;
+  uint64_t offset;
+} tfo_dropout_params;
+
+/* out[i] = x[i] / (1 - p) where kept and 0 elsewhere, + residual[i] unless it
+ * is NULL; n contiguous elements, fp32 with one rounding. residual and out
+ * have out_dtype: x_dtype; or F32 for a 16-bit x with a residual; or a 16-bit
+ * type for an F32 x without one (the gradient of the former). The gradient of
+ * x is the same call on out's gradient, without a residual. */
+TFO_API int tfo_dropout(const void* x, const void* residual, void* out, int64_t n, const tfo_dropout_params* dropout,
+                        int x_dtype, int out_dtype, void* stream);
+
+/* A parameter of `hidden` columns: one row for all (seq_stride 0), or one for
+ * each sequence, seq_stride elements apart. data NULL: ones (a shift: zeros). */
+typedef struct tfo_row_param {
+  const void* data;
+  int64_t seq_stride;
+  int dtype;
+  void* grad; /* backward only: where its gradient goes, contiguous rows in `dtype`, or NULL */
+} tfo_row_param;
+
+/* For each row of `hidden` columns (params: branch_weight, gate, weight, shift):
+ *   u = x * branch_weight / sqrt(mean(x^2) + eps), or with branch_norm == 0 x (and no branch_weight)
+ *   h = residual + scale * gate * dropout(u)
+ *   y = h * weight / sqrt(mean(h^2) + eps) + shift
+ * in fp32 with one rounding of h (residual_dtype) and one of y (x_dtype); y is
+ * made of the h before its rounding. y NULL: only h (weight and shift unread).
+ * x and residual have rows x_stride / residual_stride elements apart (innermost
+ * stride 1), h and y are contiguous. rows_per_seq divides rows. residual_dtype:
+ * x_dtype or F32. dropout NULL: none; element i of row r counts as r * hidden + i.
+ * rstd: [rows, 2] fp32 for the backward pass, or NULL. */
+TFO_API int tfo_residual_rmsnorm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                                 const tfo_row_param* params, void* h, void* y, float* rstd, int64_t rows,
+                                 int64_t rows_per_seq, int64_t hidden, int branch_norm, double scale, double eps,
+                                 const tfo_dropout_params* dropout, int x_dtype, int residual_dtype, void* stream);
+
+/* Gradients of tfo_residual_rmsnorm, given its inputs, rstd and the gradients
+ * dh (residual_dtype) and dy (x_dtype) of its outputs (either may be NULL:
+ * zeros). dx and dresidual are contiguous (NULL: not wanted), the parameters'
+ * go to their `grad`. Sums over rows are fp32 within runs of at most 2048 rows
+ * and fp64 over those, in a fixed order (no atomics). No rows: nothing is
+ * written. The workspace (16-byte aligned) is needed for the parameters'
+ * gradients and not shared by calls that may alternate on a stream; its size
+ * depends on the same arguments. */
+TFO_API size_t tfo_residual_rmsnorm_backward_workspace_bytes(
+    const void* dh, int64_t dh_stride, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+    const void* residual, int64_t residual_stride, const tfo_row_param* params, const void* dx, const void* dresidual,
+    int64_t rows, int64_t rows_per_seq, int64_t hidden, int x_dtype, int residual_dtype);
+TFO_API int tfo_residual_rmsnorm_backward(const void* dh, int64_t dh_stride, const void* dy, int64_t dy_stride,
+                                          const void* x, int64_t x_stride, const void* residual,
+                                          int64_t residual_stride, const tfo_row_param* params, const float* rstd,
+                                          void* dx, void* dresidual, int64_t rows, int64_t rows_per_seq, int64_t hidden,
+                                          int branch_norm, double scale, const tfo_dropout_params* dropout, int x_dtype,
+                                          int residual_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -290,4 +290,50 @@ struct LoraArgs {
 };
 size_t lora_workspace_bytes(int64_t tokens, int64_t adapters);
 cudaError_t lora_launch(const LoraArgs& a, void* ws, cudaStream_t st);
+
+// Dropout (philox.cuh, dropout.cu).
+struct DropoutArgs {
+  const int64_t* seed_ptr;  // on the device, or NULL: `seed`
+  uint64_t seed, offset;
+  uint32_t threshold;  // an element is dropped when its random word is below it
+  bool none, all;      // p 2^32 rounds to 0, or to 2^32: no words are made
+  float scale;         // 1 / (1 - p)
+};
+// out = dropout of x [+ residual, in out's type]; types: one for all, a 16-bit x with an
+// fp32 residual, or without a residual an fp32 x with a 16-bit out.
+cudaError_t dropout_launch(const void* x, int x_dtype, const void* residual, void* out, int out_dtype, int64_t n,
+                           const DropoutArgs& d, cudaStream_t st);
+
+// A block's branch added to the residual stream, with the norm before the next
+// block (residual_norm.cu), and the gradients (residual_norm_backward.cu).
+struct RowParam {
+  const void* p;       // [hidden], or a row for each sequence; NULL: ones (a shift: zeros)
+  int dtype;
+  int64_t seq_stride;  // elements between the sequences' rows (0: one for all)
+  void* grad;          // backward: a row for each of p's, contiguous, or NULL
+};
+struct ResidualArgs {
+  const void* x;
+  const void* res;
+  int64_t x_stride, res_stride;  // elements between rows
+  void* h;
+  void* y;      // NULL: no norm
+  float* rstd;  // [rows][2]: of the branch, of the sum; forward: may be NULL
+  RowParam branch_weight, gate, weight, shift;
+  int64_t rows, rows_per_seq;
+  int hidden;
+  bool branch_norm, dropped;
+  float scale, eps;
+  DropoutArgs drop;
+  int x_dtype, res_dtype;
+  // backward
+  const void* dy;  // NULL: zeros (no norm)
+  const void* dh;  // NULL: zeros
+  int64_t dy_stride, dh_stride;
+  void* dx;    // x_dtype, or NULL
+  void* dres;  // res_dtype, or NULL
+};
+cudaError_t residual_norm_launch(const ResidualArgs& a, cudaStream_t st);
+size_t residual_norm_backward_workspace_bytes(const ResidualArgs& a);
+cudaError_t residual_norm_backward_launch(const ResidualArgs& a, void* ws, cudaStream_t st);
 }  // namespace tfo

@@ -1,0 +1,65 @@
+// Counter-based random words for dropout: Philox4x32 with ten rounds (Salmon,
+// Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011).
+//
+// Element i of a call is dropped when word i % 4 of the block of counter
+// (i / 4, offset), under the key `seed`, is below p 2^32: what is kept depends
+// on the element's index alone, not on the launch, so that the backward pass
+// makes the same mask again and nothing is stored.
+#pragma once
+
+#include "capi_internal.h"
+#include "common.cuh"
+
+namespace tfo {
+
+struct DropKey {
+  uint32_t k0, k1;      // the seed
+  uint32_t off0, off1;  // the call's offset
+  uint32_t threshold;
+  __device__ explicit DropKey(const DropoutArgs& d) : threshold(d.threshold) {
+    const uint64_t seed = d.seed_ptr != nullptr ? static_cast<uint64_t>(*d.seed_ptr) : d.seed;
+    k0 = static_cast<uint32_t>(seed);
+    k1 = static_cast<uint32_t>(seed >> 32);
+    off0 = static_cast<uint32_t>(d.offset);
+    off1 = static_cast<uint32_t>(d.offset >> 32);
+  }
+  __device__ uint4 block(uint64_t counter) const {
+    uint32_t a = static_cast<uint32_t>(counter), b = static_cast<uint32_t>(counter >> 32), c = off0, d = off1;
+    uint32_t x = k0, y = k1;
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+      const uint64_t p = static_cast<uint64_t>(0xD2511F53u) * a, q = static_cast<uint64_t>(0xCD9E8D57u) * c;
+      a = static_cast<uint32_t>(q >> 32) ^ b ^ x;
+      b = static_cast<uint32_t>(q);
+      c = static_cast<uint32_t>(p >> 32) ^ d ^ y;
+      d = static_cast<uint32_t>(p);
+      x += 0x9E3779B9u;
+      y += 0xBB67AE85u;
+    }
+    return make_uint4(a, b, c, d);
+  }
+  // Bit j: element first + j is kept. `first` is a multiple of 4 if N is.
+  template <int N> __device__ uint32_t kept(uint64_t first) const {
+    uint32_t bits = 0;
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) {
+        const uint4 w = block(first / 4 + i);
+        bits |= (w.x >= threshold ? 1u : 0u) << (4 * i) | (w.y >= threshold ? 2u : 0u) << (4 * i) |
+                (w.z >= threshold ? 4u : 0u) << (4 * i) | (w.w >= threshold ? 8u : 0u) << (4 * i);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const uint64_t i = first + j;
+        const uint4 w = block(i / 4);
+        const uint32_t at = static_cast<uint32_t>(i) & 3u;
+        const uint32_t v = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
+        bits |= (v >= threshold ? 1u : 0u) << j;
+      }
+    }
+    return bits;
+  }
+};
+
+}  // namespace tfo

@@ -1,0 +1,460 @@
+// Gradients of the residual stream with its norms (residual_norm.cu). With
+// c = scale * gate * w1 / (1 - p), k the kept elements, r1 and r2 the saved
+// 1 / sqrt(mean + eps), x' = x r1, u = k c x', h = residual + u, h' = h r2 and
+// g = dy w2:
+//
+//   dH        = dh + r2 (g - h' mean(g h'))
+//   dresidual = dH
+//   dx        = r1 (k c dH - x' mean(u dH)),  or k c dH where the branch is not normed
+//   dw2       = sum over rows of dy h',   dshift = sum of dy
+//   A         = sum over rows of k dH x' / (1 - p):
+//   dgate     = scale w1 A,   dw1 = scale gate A   (summed over sequences where one is not)
+//
+// The second mean needs dH, which needs the first; written out,
+//   sum(u dH) = sum(u dh) + r2 (sum(u g) - mean(g h') sum(u h')),
+// so that one pass over a row and one exchange between its threads give both.
+// h is made again from x and residual: nothing but r1 and r2 is stored.
+//
+// Threads keep fp32 sums of A, dy h' and dy for their columns over the rows of
+// an item (a run of rows of one sequence, a fixed split) and write them out as
+// partial rows; a second kernel adds these in order, in fp64, with the other
+// parameter's factor. No atomics: the results do not depend on scheduling.
+//
+// Floor: HBM (x, residual, dy and dh read, dx and dresidual written).
+#include "residual.cuh"
+
+namespace tfo {
+
+// Sums over rows that the parameters' gradients are made of.
+enum RowSum : int { SUM_BRANCH = 0, SUM_WEIGHT = 1, SUM_SHIFT = 2, SUMS = 3 };
+
+// The split of the rows into items: `chunks` runs for each of `seqs` sequences (one of all rows where no parameter is
+// a sequence's own).
+struct RowItems {
+  int64_t seqs, seq_rows, chunks;
+  __host__ __device__ int64_t count() const { return seqs * chunks; }
+  __device__ int64_t first_row(int64_t item) const {
+    const int64_t b = item / chunks, c = item - b * chunks;
+    return b * seq_rows + c * seq_rows / chunks;
+  }
+};
+
+struct BackwardPlan {
+  RowPlan rows;
+  RowItems items;
+  float* partials[SUMS];  // [items][hidden], or NULL: not wanted
+};
+
+template <typename TX, typename TR, int E, int V, int STAGES>
+__global__ void __launch_bounds__(kRowThreads, 1)
+    residual_norm_backward_kernel(const __grid_constant__ ResidualArgs a, const __grid_constant__ BackwardPlan plan) {
+  using Cols = RowCols<E, V>;
+  constexpr int P = Cols::P;
+  constexpr bool KEEP_PARAMS = Cols::N <= 8;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ __align__(16) float red[2][kMaxRowWarps][4 * kMaxRowWarps];
+  griddep_launch_dependents();
+  const int threads = plan.rows.threads, warps = threads / 32;
+  const int group = (threadIdx.x >> 5) / warps, warp = (threadIdx.x >> 5) - group * warps;
+  const int t = threadIdx.x - group * threads;
+  for (int i = threadIdx.x; i < 8 * kMaxRowWarps * kMaxRowWarps; i += blockDim.x) (&red[0][0][0])[i] = 0.f;
+  __syncthreads();
+  griddep_wait();
+  const int64_t groups = static_cast<int64_t>(gridDim.x) * plan.rows.groups;
+  const int64_t me = static_cast<int64_t>(blockIdx.x) * plan.rows.groups + group;
+  const RowItems items = plan.items;
+  int64_t item = me * items.count() / groups;
+  const int64_t last = (me + 1) * items.count() / groups;
+  if (item >= last) return;
+  const int64_t r0 = items.first_row(item), r1 = items.first_row(last);
+  const Cols cols(t, threads, a.hidden);
+  RowStream<TX, TR, E, V, 2, 2, STAGES> rows;
+  rows.base[0] = a.x;
+  rows.stride[0] = a.x_stride;
+  rows.base[1] = a.dy;
+  rows.stride[1] = a.dy_stride;
+  rows.base[2] = a.dy != nullptr ? a.res : nullptr;  // h serves the norm alone
+  rows.stride[2] = a.res_stride;
+  rows.base[3] = a.dh;
+  rows.stride[3] = a.dh_stride;
+  rows.start(cols, reinterpret_cast<uint4*>(smem), r0, r1);
+  const DropKey key(a.drop);
+  const float inv_h = 1.f / static_cast<float>(a.hidden);
+  const int bar = 1 + group;
+  int turn = 0;  // of the parts of a sum
+  const float2* rstd = reinterpret_cast<const float2*>(a.rstd);
+  float2 next_r = rstd[r0];  // loaded a row ahead
+  F2 c[P], w[P], sums[SUMS][P];
+  auto params = [&](int64_t seq) {
+    F2 g[P];
+    cols.param(a.branch_weight, seq, 1.f, c);
+    cols.param(a.gate, seq, 1.f, g);
+    const float s = a.dropped ? a.scale * a.drop.scale : a.scale;
+#pragma unroll
+    for (int j = 0; j < P; ++j) c[j] = mul2(mul2(c[j], g[j]), f2(s, s));
+    cols.param(a.weight, seq, 1.f, w);
+  };
+  auto clear = [&] {
+#pragma unroll
+    for (int i = 0; i < SUMS; ++i) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) sums[i][j] = f2(0.f, 0.f);
+    }
+  };
+  int64_t seq = r0 / a.rows_per_seq, seq_end = (seq + 1) * a.rows_per_seq;
+  const bool by_seq = (a.branch_weight.seq_stride | a.gate.seq_stride | a.weight.seq_stride) != 0;
+  if (KEEP_PARAMS) params(seq);
+  clear();
+  int64_t item_end = items.first_row(item + 1);
+  for (int64_t r = r0; r < r1; ++r) {
+    if (r == seq_end) {
+      ++seq;
+      seq_end += a.rows_per_seq;
+      if (KEEP_PARAMS && by_seq) params(seq);
+    }
+    const uint32_t bits = a.dropped ? cols.kept(a.drop, key, r) : ~0u;
+    const float2 rs = next_r;
+    if (r + 1 < r1) next_r = rstd[r + 1];
+    rows.advance(cols);
+    if constexpr (!KEEP_PARAMS) params(seq);
+    F2 x[P], q[P], hat[P];  // x', dH and what it is made of, h'
+    rows.template get<0>(x);
+    rows.template get<3>(q);
+#pragma unroll
+    for (int j = 0; j < P; ++j) x[j] = mul2(x[j], f2(rs.x, rs.x));
+    float s[4] = {0.f, 0.f, 0.f, 0.f};  // of g h', u dh, u g, u h'
+    {
+      F2 u[P], s0 = f2(0.f, 0.f), s1 = s0, s2 = s0, s3 = s0;
+#pragma unroll
+      for (int j = 0; j < P; ++j) u[j] = mul2(x[j], c[j]);
+      if (a.dropped) Cols::drop(bits, u);
+      if (a.branch_norm) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) s1 = fma2(u[j], q[j], s1);
+      }
+      if (a.dy != nullptr) {
+        F2 dy[P];
+        rows.template get<1>(dy);
+        rows.template get<2>(hat);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          hat[j] = mul2(add2(hat[j], u[j]), f2(rs.y, rs.y));
+          sums[SUM_WEIGHT][j] = fma2(dy[j], hat[j], sums[SUM_WEIGHT][j]);
+          sums[SUM_SHIFT][j] = add2(dy[j], sums[SUM_SHIFT][j]);
+          const F2 g = mul2(dy[j], w[j]);
+          s0 = fma2(g, hat[j], s0);
+          s2 = fma2(u[j], g, s2);
+          s3 = fma2(u[j], hat[j], s3);
+          q[j] = fma2(g, f2(rs.y, rs.y), q[j]);
+        }
+      }
+      s[0] = s0.x + s0.y;
+      s[1] = s1.x + s1.y;
+      s[2] = s2.x + s2.y;
+      s[3] = s3.x + s3.y;
+    }
+    if (a.branch_norm) {
+      row_sum(s, red[turn ^= 1][group], warps, warp, bar);
+    } else if (a.dy != nullptr) {
+      float one[1] = {s[0]};
+      row_sum(one, red[turn ^= 1][group], warps, warp, bar);
+      s[0] = one[0];
+    }
+    const float mean = s[0] * inv_h;
+    if (a.dy != nullptr) {
+      const float m = -mean * rs.y;
+#pragma unroll
+      for (int j = 0; j < P; ++j) q[j] = fma2(hat[j], f2(m, m), q[j]);
+    }
+    if (a.dres != nullptr) cols.store(static_cast<TR*>(a.dres) + r * a.hidden, q);
+    if (a.dropped) Cols::drop(bits, q);
+    const float m1 = a.branch_norm ? -(s[1] + rs.y * (s[2] - mean * s[3])) * inv_h : 0.f;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      sums[SUM_BRANCH][j] = fma2(q[j], x[j], sums[SUM_BRANCH][j]);
+      q[j] = mul2(q[j], c[j]);
+    }
+    if (a.dx != nullptr) {
+      if (a.branch_norm) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) q[j] = mul2(fma2(x[j], f2(m1, m1), q[j]), f2(rs.x, rs.x));
+      }
+      cols.store(static_cast<TX*>(a.dx) + r * a.hidden, q);
+    }
+    if (r + 1 == item_end) {
+#pragma unroll
+      for (int i = 0; i < SUMS; ++i)
+        if (plan.partials[i] != nullptr) cols.store(plan.partials[i] + item * a.hidden, sums[i]);
+      clear();
+      ++item;
+      item_end = item < last ? items.first_row(item + 1) : 0;
+    }
+  }
+}
+
+// Rows of any width: a CTA for each, which reads it again for the results (from L1 and L2); a CTA's items' sums are
+// added up in the partial rows themselves, each column by one thread.
+template <typename TX, typename TR>
+__global__ void __launch_bounds__(kRowThreads)
+    residual_norm_backward_any_kernel(const __grid_constant__ ResidualArgs a, const __grid_constant__ BackwardPlan plan) {
+  __shared__ __align__(16) float red[2][4 * kMaxRowWarps];
+  griddep_launch_dependents();
+  griddep_wait();
+  const DropKey key(a.drop);
+  const float s_branch = a.dropped ? a.scale * a.drop.scale : a.scale;
+  const float inv_h = 1.f / static_cast<float>(a.hidden);
+  const RowItems items = plan.items;
+  int turn = 0;
+  for (int64_t item = blockIdx.x; item < items.count(); item += gridDim.x) {
+    const int64_t r0 = items.first_row(item), r1 = items.first_row(item + 1);
+    for (int64_t r = r0; r < r1; ++r) {
+      const int64_t seq = r / a.rows_per_seq;
+      const TX* x = static_cast<const TX*>(a.x) + r * a.x_stride;
+      const TX* dy = static_cast<const TX*>(a.dy) + r * a.dy_stride;
+      const TR* res = static_cast<const TR*>(a.res) + r * a.res_stride;
+      const TR* dh = static_cast<const TR*>(a.dh) + r * a.dh_stride;
+      const float2 rs = reinterpret_cast<const float2*>(a.rstd)[r];
+      auto param = [&](const RowParam& p, int i, float otherwise) {
+        return p.p != nullptr ? load_as_float(p.p, seq * p.seq_stride + i, p.dtype) : otherwise;
+      };
+      struct At {
+        float x, c, hat, g, dy, dh;
+        bool keep;
+      };
+      auto at = [&](int i) {
+        At v;
+        v.x = Ty<TX>::to_f(x[i]) * rs.x;
+        v.c = param(a.branch_weight, i, 1.f) * param(a.gate, i, 1.f) * s_branch;
+        v.keep = !a.dropped || (!a.drop.all && key.kept<1>(static_cast<uint64_t>(r * a.hidden + i)));
+        v.dh = a.dh != nullptr ? Ty<TR>::to_f(dh[i]) : 0.f;
+        v.dy = v.g = v.hat = 0.f;
+        if (a.dy != nullptr) {
+          v.dy = Ty<TX>::to_f(dy[i]);
+          v.g = v.dy * param(a.weight, i, 1.f);
+          v.hat = (Ty<TR>::to_f(res[i]) + (v.keep ? v.x * v.c : 0.f)) * rs.y;
+        }
+        return v;
+      };
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = threadIdx.x; i < a.hidden; i += kRowThreads) {
+        const At v = at(i);
+        const float u = v.keep ? v.x * v.c : 0.f;
+        s[0] = fmaf(v.g, v.hat, s[0]);
+        s[1] = fmaf(u, v.dh, s[1]);
+        s[2] = fmaf(u, v.g, s[2]);
+        s[3] = fmaf(u, v.hat, s[3]);
+      }
+      row_sum(s, red[turn ^= 1], kMaxRowWarps, threadIdx.x >> 5, 1);
+      const float mean = s[0] * inv_h;
+      const float m1 = a.branch_norm ? (s[1] + rs.y * (s[2] - mean * s[3])) * inv_h : 0.f;
+      for (int i = threadIdx.x; i < a.hidden; i += kRowThreads) {
+        const At v = at(i);
+        const float d = v.dh + rs.y * (v.g - v.hat * mean);
+        const float e = v.keep ? d : 0.f;
+        if (a.dres != nullptr) static_cast<TR*>(a.dres)[r * a.hidden + i] = Ty<TR>::from_f(d);
+        if (a.dx != nullptr) {
+          const float b = e * v.c;
+          static_cast<TX*>(a.dx)[r * a.hidden + i] = Ty<TX>::from_f(a.branch_norm ? rs.x * (b - v.x * m1) : b);
+        }
+        const float add[SUMS] = {e * v.x, v.dy * v.hat, v.dy};
+#pragma unroll
+        for (int p = 0; p < SUMS; ++p) {
+          if (plan.partials[p] == nullptr) continue;
+          float* o = plan.partials[p] + item * a.hidden + i;
+          *o = r == r0 ? add[p] : *o + add[p];
+        }
+      }
+    }
+  }
+}
+
+// One parameter's gradient: out[o, i] = factor * sum over the output's items of other[sequence, i] * partials[item, i].
+struct ParamSum {
+  const float* partials;
+  RowParam out;    // `grad` with dtype; one row for all or (seq_stride not 0) one for each sequence
+  RowParam other;  // the parameter that multiplies it, by sequence (p NULL: none)
+  float factor;
+};
+struct ParamSums {
+  ParamSum of[4];
+  int n;
+  RowItems items;
+  int64_t seqs;
+  int hidden;
+};
+
+// 32 columns of one output per CTA; `blockDim.y` threads a column take every so manyth item.
+__global__ void residual_param_grad_kernel(const __grid_constant__ ParamSums s) {
+  __shared__ double red[32][33];
+  griddep_launch_dependents();
+  griddep_wait();
+  const ParamSum& p = s.of[blockIdx.y];
+  const int64_t col_blocks = (s.hidden + 31) / 32;
+  const int64_t outs = p.out.seq_stride != 0 ? s.seqs : 1;
+  for (int64_t job = blockIdx.x; job < outs * col_blocks; job += gridDim.x) {
+    const int64_t o = job / col_blocks;
+    const int i = static_cast<int>(job - o * col_blocks) * 32 + threadIdx.x;
+    const int64_t i0 = p.out.seq_stride != 0 ? o * s.items.chunks : 0;
+    const int64_t i1 = p.out.seq_stride != 0 ? i0 + s.items.chunks : s.items.count();
+    double t = 0.0;
+    if (i < s.hidden) {
+      for (int64_t m = i0 + threadIdx.y; m < i1; m += blockDim.y) {
+        double v = p.partials[m * s.hidden + i];
+        if (p.other.p != nullptr)
+          v *= load_as_float(p.other.p, (m / s.items.chunks) * p.other.seq_stride + i, p.other.dtype);
+        t += v;
+      }
+    }
+    red[threadIdx.y][threadIdx.x] = t;
+    __syncthreads();
+    if (threadIdx.y == 0 && i < s.hidden) {
+      for (int y = 1; y < static_cast<int>(blockDim.y); ++y) t += red[y][threadIdx.x];
+      const float v = static_cast<float>(t * p.factor);
+      const int64_t at = o * s.hidden + i;
+      if (p.out.dtype == F32) static_cast<float*>(p.out.grad)[at] = v;
+      else if (p.out.dtype == F16) static_cast<__half*>(p.out.grad)[at] = __float2half_rn(v);
+      else static_cast<__nv_bfloat16*>(p.out.grad)[at] = __float2bfloat16_rn(v);
+    }
+    __syncthreads();
+  }
+}
+
+namespace {
+constexpr int64_t kItemRows = 2048;  // most rows that a thread adds up in fp32
+
+bool wants(const ResidualArgs& a, int sum) {
+  if (sum == SUM_BRANCH) return a.gate.grad != nullptr || a.branch_weight.grad != nullptr;
+  return sum == SUM_WEIGHT ? a.weight.grad != nullptr : a.shift.grad != nullptr;
+}
+
+struct Shape {
+  int e, v, threads;  // v 0: any
+};
+Shape shape_of(const ResidualArgs& a) {
+  const int full = 16 / row_elem_bytes(a.x_dtype);
+  if (row_chunk(a, true) == full) {
+    for (int v = 1; v * full <= 16; v *= 2)
+      if (const int t = row_threads(a.hidden, full, v)) return {full, v, t};
+  } else {
+    for (int v = 4; v <= 8; v *= 2)
+      if (const int t = row_threads(a.hidden, 1, v)) return {1, v, t};
+  }
+  return {1, 0, kRowThreads};
+}
+
+// The split: items for every group of a full grid, and short enough for fp32 sums.
+RowItems items_of(const ResidualArgs& a, int threads) {
+  bool by_seq = false;
+  for (const RowParam* p : {&a.branch_weight, &a.gate, &a.weight, &a.shift}) by_seq = by_seq || (p->seq_stride != 0);
+  RowItems it;
+  it.seqs = by_seq ? a.rows / a.rows_per_seq : 1;
+  it.seq_rows = by_seq ? a.rows_per_seq : a.rows;
+  const int64_t groups = static_cast<int64_t>(num_sms()) * (kRowThreads / threads);
+  it.chunks = std::max({groups / it.seqs, (it.seq_rows + kItemRows - 1) / kItemRows, int64_t{1}});
+  it.chunks = std::min(it.chunks, it.seq_rows);
+  return it;
+}
+
+template <typename TX, typename TR, int E, int V, int STAGES>
+cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t st) {
+  auto* kernel = residual_norm_backward_kernel<TX, TR, E, V, STAGES>;
+  using Stream = RowStream<TX, TR, E, V, 2, 2, STAGES>;
+  const int threads = plan.rows.threads;
+  const int64_t count = plan.items.count();
+  plan.rows.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, count / num_sms())));
+  const int block = plan.rows.groups * threads;
+  const size_t smem = Stream::smem_bytes(block);
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  // the limit of the largest block: also below it the static part comes on top
+  if (const cudaError_t e = ensure_smem_attr(fn, Stream::smem_bytes(kRowThreads)); e != cudaSuccess) return e;
+  const int64_t all = static_cast<int64_t>(num_sms()) * std::max(1, cached_occupancy(fn, block, smem));
+  const int64_t grid = std::min<int64_t>(all, (count + plan.rows.groups - 1) / plan.rows.groups);
+  note_launch();
+  return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a, plan);
+}
+
+template <typename TX, typename TR>
+cudaError_t launch_types(const ResidualArgs& a, BackwardPlan& plan, const Shape& sh, cudaStream_t st) {
+  constexpr int E = 16 / sizeof(TX);
+  if (sh.e == E) {
+    if (sh.v == 1) return launch_rows<TX, TR, E, 1, 4>(a, plan, st);
+    if (sh.v == 2) return launch_rows<TX, TR, E, 2, 2>(a, plan, st);
+    if constexpr (E == 4) {
+      if (sh.v == 4) return launch_rows<TX, TR, E, 4, 1>(a, plan, st);
+    }
+  } else {
+    if (sh.v == 4) return launch_rows<TX, TR, 1, 4, 1>(a, plan, st);
+    if (sh.v == 8) return launch_rows<TX, TR, 1, 8, 1>(a, plan, st);
+  }
+  note_launch();
+  return launch_dependent(residual_norm_backward_any_kernel<TX, TR>,
+                          static_cast<int>(std::min<int64_t>(plan.items.count(), num_sms() * 4ll)), kRowThreads, st, a, plan);
+}
+}  // namespace
+
+size_t residual_norm_backward_workspace_bytes(const ResidualArgs& a) {
+  int64_t wanted = 0;
+  for (int i = 0; i < SUMS; ++i) wanted += wants(a, i);
+  if (wanted == 0) return 0;
+  const int64_t row = (static_cast<int64_t>(a.hidden) * 4 + 15) / 16 * 16;
+  return static_cast<size_t>(wanted * items_of(a, shape_of(a).threads).count() * row);
+}
+
+cudaError_t residual_norm_backward_launch(const ResidualArgs& a, void* ws, cudaStream_t st) {
+  const Shape sh = shape_of(a);
+  BackwardPlan plan{};
+  plan.rows.threads = sh.threads;
+  plan.items = items_of(a, sh.threads);
+  float* at = static_cast<float*>(ws);
+  const int64_t count = plan.items.count();
+  bool any = false;
+  for (int i = 0; i < SUMS; ++i) {
+    if (!wants(a, i)) continue;
+    plan.partials[i] = at;
+    at += count * ((a.hidden + 3) / 4 * 4);
+    any = true;
+  }
+  cudaError_t e;
+  if (a.x_dtype == F16)
+    e = a.res_dtype == F32 ? launch_types<__half, float>(a, plan, sh, st) : launch_types<__half, __half>(a, plan, sh, st);
+  else if (a.x_dtype == BF16)
+    e = a.res_dtype == F32 ? launch_types<__nv_bfloat16, float>(a, plan, sh, st)
+                           : launch_types<__nv_bfloat16, __nv_bfloat16>(a, plan, sh, st);
+  else
+    e = launch_types<float, float>(a, plan, sh, st);
+  if (e != cudaSuccess || !any) return e;
+  ParamSums s{};
+  s.items = plan.items;
+  s.seqs = a.rows / a.rows_per_seq;
+  s.hidden = a.hidden;
+  const float f = a.dropped ? a.scale * a.drop.scale : a.scale;
+  const RowParam none{};
+  auto add = [&](int sum, const RowParam& p, const RowParam& other, float factor) {
+    if (p.grad != nullptr) s.of[s.n++] = ParamSum{plan.partials[sum], p, other, factor};
+  };
+  add(SUM_BRANCH, a.gate, a.branch_weight, f);
+  add(SUM_BRANCH, a.branch_weight, a.gate, f);
+  add(SUM_WEIGHT, a.weight, none, 1.f);
+  add(SUM_SHIFT, a.shift, none, 1.f);
+  int64_t outs = 1, most = 1;  // outputs, and items of one
+  for (int i = 0; i < s.n; ++i) {
+    const bool own = s.of[i].out.seq_stride != 0;
+    outs = std::max(outs, own ? s.seqs : 1);
+    most = std::max(most, own ? plan.items.chunks : count);
+  }
+  int lanes = 1;
+  while (lanes < 32 && lanes < most) lanes *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(outs * ((a.hidden + 31) / 32), num_sms() * 64ll)), s.n);
+  cfg.blockDim = dim3(32, lanes);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  note_launch();
+  return cudaLaunchKernelEx(&cfg, residual_param_grad_kernel, s);
+}
+
+}  // namespace tfo

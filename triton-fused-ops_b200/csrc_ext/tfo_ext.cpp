@@ -304,9 +304,9 @@ void refuse_tangents(const variable_list& grads) {
 }
 
 // Puts a node that only raises between the gradients and what they depend on.
-void differentiable_once(const variable_list& gradients, const variable_list& sources) {
+void differentiable_once(const char* op, const variable_list& gradients, const variable_list& sources) {
   const auto node = std::make_shared<torch::autograd::Error>(
-      "fused_qk_norm_rope is differentiable once: its gradients cannot be differentiated",
+      std::string(op) + " is differentiable once: its gradients cannot be differentiated",
       torch::autograd::collect_next_edges(sources));
   for (const at::Tensor& g : gradients)
     if (g.defined()) torch::autograd::set_history(g, node);
@@ -360,7 +360,7 @@ struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
     if (at::GradMode::is_enabled()) {  // create_graph: differentiating one of the gradients is the error
       variable_list sources(saved.begin(), saved.begin() + 4);
       sources.insert(sources.end(), grads.begin(), grads.end());
-      differentiable_once(d, sources);
+      differentiable_once("fused_qk_norm_rope", d, sources);
     }
     return d;
   }
@@ -484,6 +484,244 @@ py::object lora(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, c
   return py::cast(y);
 }
 
+// ---------------------------------------------------------------------------
+// The residual stream: dropout, and a block's branch added to it with the norms
+// before and after.
+// ---------------------------------------------------------------------------
+struct Dropout {  // a call's tfo_dropout_params, and what its backward pass keeps of them
+  double p = 0.0;
+  at::Tensor seed;  // undefined: value
+  uint64_t value = 0, offset = 0;
+  tfo_dropout_params params() const {
+    return {p, seed.defined() ? seed.data_ptr<int64_t>() : nullptr, value, offset};
+  }
+  void save(AutogradContext* ctx) const {
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["value"] = static_cast<int64_t>(value);
+    ctx->saved_data["offset"] = static_cast<int64_t>(offset);
+  }
+  static Dropout saved(AutogradContext* ctx, const at::Tensor& seed) {
+    return {ctx->saved_data["p"].toDouble(), seed, static_cast<uint64_t>(ctx->saved_data["value"].toInt()),
+            static_cast<uint64_t>(ctx->saved_data["offset"].toInt())};
+  }
+  static bool ok(const at::Tensor& x, double p, const OptTensor& seed, bool seeded) {
+    if (!(p >= 0.0 && p <= 1.0) || (p > 0.0 && !seeded)) return false;
+    return !seed.has_value() || (seed->device() == x.device() && seed->scalar_type() == at::kLong && seed->numel() == 1);
+  }
+};
+
+bool residual_ok(const at::Tensor& x, const at::Tensor& r) {
+  return r.device() == x.device() && (r.scalar_type() == x.scalar_type() || r.scalar_type() == at::kFloat) &&
+         r.sizes() == x.sizes() && !has_tangent(r);
+}
+
+at::Tensor drop_call(const at::Tensor& x, const at::Tensor& residual, const Dropout& d, at::ScalarType type) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor out = fresh(x.sizes(), type, x.device());
+  const tfo_dropout_params params = d.params();
+  check(tfo_dropout(x.data_ptr(), ptr_or_null(residual), out.data_ptr(), x.numel(), &params, dtype_code(x.scalar_type()),
+                    dtype_code(type), at::cuda::getCurrentCUDAStream(x.device().index()).stream()),
+        "tfo_dropout");
+  return out;
+}
+
+// The gradient of a dropout is the dropout of the gradient, itself differentiable.
+struct DropoutNode : public torch::autograd::Function<DropoutNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& residual, const Dropout& d,
+                            at::ScalarType type) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor res = residual.value_or(at::Tensor());
+    ctx->save_for_backward({d.seed});
+    d.save(ctx);
+    ctx->saved_data["type"] = static_cast<int64_t>(x.scalar_type());
+    ctx->saved_data["dx"] = x.requires_grad();
+    ctx->saved_data["dres"] = res.defined() && res.requires_grad();
+    ctx->set_materialize_grads(false);
+    return drop_call(x.contiguous(), res.defined() ? res.contiguous() : res, d, type);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const at::Tensor& g = grads[0];
+    if (!g.defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    refuse_tangents(grads);
+    const Dropout d = Dropout::saved(ctx, ctx->get_saved_variables()[0]);
+    const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+    at::Tensor dx;
+    if (ctx->saved_data["dx"].toBool()) {
+      // the 16-bit gradient of an fp32 one's gradient (a second differentiation) goes through fp32
+      const at::Tensor from = g.scalar_type() == type || g.scalar_type() == at::kFloat ? g : g.to(type);
+      dx = at::GradMode::is_enabled() ? DropoutNode::apply(from, OptTensor(), d, type)
+                                      : drop_call(from.contiguous(), at::Tensor(), d, type);
+    }
+    return {dx, ctx->saved_data["dres"].toBool() ? g : at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// fused_dropout: the result, or None outside the common case.
+py::object dropout(const at::Tensor& x, const OptTensor& residual, double p, const OptTensor& seed, uint64_t value,
+                   bool seeded, uint64_t offset) {
+  if (!x.is_cuda() || !is_float(x.scalar_type()) || has_tangent(x) || !Dropout::ok(x, p, seed, seeded) ||
+      (residual.has_value() && !residual_ok(x, *residual)))
+    return py::none();
+  const Dropout d{p, seed.value_or(at::Tensor()), value, offset};
+  const auto type = residual.has_value() ? residual->scalar_type() : x.scalar_type();
+  if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(residual)))
+    return py::cast(DropoutNode::apply(x, residual, d, type));
+  return py::cast(drop_call(x.contiguous(), residual.has_value() ? residual->contiguous() : at::Tensor(), d, type));
+}
+
+// Whether t [..., hidden] is rows of innermost stride 1 a fixed step apart.
+bool flat_rows(const at::Tensor& t, int64_t* stride) {
+  const int64_t hidden = t.size(-1);
+  if (hidden > 1 && t.stride(-1) != 1) return false;
+  int64_t step = -1, next = 0;
+  for (int64_t i = t.dim() - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (step < 0) step = t.stride(i);
+    else if (t.stride(i) != next) return false;
+    next = t.stride(i) * t.size(i);
+  }
+  *stride = step < 0 ? hidden : step;
+  return true;
+}
+at::Tensor as_rows(const at::Tensor& t, int64_t* stride) {
+  if (!t.defined() || flat_rows(t, stride)) return t;
+  *stride = t.size(-1);
+  return t.contiguous();
+}
+
+// [hidden], or a row for each sequence [batch, (1, ...) hidden] that shares no memory with another.
+bool row_param_ok(const OptTensor& p, const at::Tensor& x) {
+  if (!p.has_value()) return true;
+  const at::Tensor& t = *p;
+  const int64_t hidden = x.size(-1), n = t.dim();
+  if (t.device() != x.device() || !is_float(t.scalar_type()) || n < 1 || t.size(-1) != hidden || has_tangent(t) ||
+      (hidden > 1 && t.stride(-1) != 1))
+    return false;
+  if (n == 1) return true;
+  if (n > x.dim() || t.size(0) != x.size(0) || (t.size(0) > 1 && t.stride(0) <= 0)) return false;
+  for (int64_t i = 1; i < n - 1; ++i)
+    if (t.size(i) != 1) return false;
+  return true;
+}
+tfo_row_param row_param(const at::Tensor& t, const at::Tensor& grad) {
+  if (!t.defined()) return {nullptr, 0, TFO_DTYPE_F32, nullptr};
+  const int64_t own = t.dim() == 1 ? 0 : t.size(0) > 1 ? t.stride(0) : t.size(-1);
+  return {t.data_ptr(), own, dtype_code(t.scalar_type()), out_or_null(grad)};
+}
+
+struct ResidualCall {  // the arguments that both directions share
+  bool branch_norm, norm;
+  double scale, eps;
+  Dropout drop;
+};
+int64_t rows_of(const at::Tensor& x) { return x.numel() / x.size(-1); }
+int64_t rows_per_seq(const at::Tensor& x) { return x.dim() > 1 ? rows_of(x) / x.size(0) : 1; }
+
+// {h, y or undefined, rstd or undefined}
+std::array<at::Tensor, 3> residual_call(const at::Tensor& x, const at::Tensor& residual,
+                                        const std::array<at::Tensor, 4>& p, const ResidualCall& c, bool keep) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  int64_t xs = 0, rs = 0;
+  const at::Tensor x2 = as_rows(x, &xs), r2 = as_rows(residual, &rs);
+  std::array<at::Tensor, 3> out;
+  out[0] = fresh(x.sizes(), residual.scalar_type(), x.device());
+  if (c.norm) out[1] = fresh(x.sizes(), x.scalar_type(), x.device());
+  if (keep) out[2] = fresh({rows_of(x), 2}, at::kFloat, x.device());
+  const tfo_row_param params[4] = {row_param(p[0], {}), row_param(p[1], {}), row_param(p[2], {}), row_param(p[3], {})};
+  const tfo_dropout_params d = c.drop.params();
+  check(tfo_residual_rmsnorm(x2.data_ptr(), xs, r2.data_ptr(), rs, params, out[0].data_ptr(), out_or_null(out[1]),
+                             keep ? out[2].data_ptr<float>() : nullptr, rows_of(x), rows_per_seq(x), x.size(-1),
+                             c.branch_norm, c.scale, c.eps, c.drop.p > 0 ? &d : nullptr, dtype_code(x.scalar_type()),
+                             dtype_code(residual.scalar_type()),
+                             at::cuda::getCurrentCUDAStream(x.device().index()).stream()),
+        "tfo_residual_rmsnorm");
+  return out;
+}
+
+struct ResidualNode : public torch::autograd::Function<ResidualNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& residual, const OptTensor& bw,
+                               const OptTensor& gate, const OptTensor& w, const OptTensor& shift, const ResidualCall& c) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const std::array<at::Tensor, 4> p{bw.value_or(at::Tensor()), gate.value_or(at::Tensor()), w.value_or(at::Tensor()),
+                                      shift.value_or(at::Tensor())};
+    const auto out = residual_call(x, residual, p, c, true);
+    ctx->save_for_backward({x, residual, p[0], p[1], p[2], p[3], out[2], c.drop.seed});
+    std::vector<bool> wanted{x.requires_grad(), residual.requires_grad()};
+    for (const at::Tensor& t : p) wanted.push_back(t.defined() && t.requires_grad());
+    ctx->saved_data["wanted"] = c10::List<bool>(std::initializer_list<bool>{wanted[0], wanted[1], wanted[2], wanted[3],
+                                                                            wanted[4], wanted[5]});
+    ctx->saved_data["branch_norm"] = c.branch_norm;
+    ctx->saved_data["scale"] = c.scale;
+    c.drop.save(ctx);
+    ctx->set_materialize_grads(false);
+    return c.norm ? variable_list{out[0], out[1]} : variable_list{out[0]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    variable_list d = gradients(ctx, saved, grads);
+    if (at::GradMode::is_enabled()) {  // create_graph: differentiating one of the gradients is the error
+      variable_list sources(saved.begin(), saved.begin() + 6);
+      sources.insert(sources.end(), grads.begin(), grads.end());
+      differentiable_once("fused_residual_rmsnorm", d, sources);
+    }
+    return d;
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& saved, const variable_list& grads) {
+    const at::AutoGradMode no_graph(false);
+    refuse_tangents(grads);
+    const at::Tensor &x = saved[0], &residual = saved[1];
+    const c10::List<bool> wanted = ctx->saved_data["wanted"].toBoolList();
+    const at::Tensor dh = grads[0], dy = grads.size() > 1 ? grads[1] : at::Tensor();
+    variable_list d(7);
+    if (!dh.defined() && !dy.defined()) return d;
+    const c10::cuda::CUDAGuard guard(x.device());
+    for (size_t i = 0; i < 6; ++i)
+      if (wanted[i]) d[i] = fresh(saved[i].sizes(), saved[i].scalar_type(), x.device());
+    int64_t xs = 0, rs = 0, hs = 0, ys = 0;
+    const at::Tensor x2 = as_rows(x, &xs), r2 = as_rows(residual, &rs), dh2 = as_rows(dh, &hs), dy2 = as_rows(dy, &ys);
+    const tfo_row_param params[4] = {row_param(saved[2], d[2]), row_param(saved[3], d[3]), row_param(saved[4], d[4]),
+                                     row_param(saved[5], d[5])};
+    const int xt = dtype_code(x.scalar_type()), rt = dtype_code(residual.scalar_type());
+    const int64_t rows = rows_of(x), per = rows_per_seq(x), hidden = x.size(-1);
+    const at::Tensor ws = scratch(
+        tfo_residual_rmsnorm_backward_workspace_bytes(ptr_or_null(dh2), hs, ptr_or_null(dy2), ys, x2.data_ptr(), xs,
+                                                      r2.data_ptr(), rs, params, out_or_null(d[0]), out_or_null(d[1]), rows,
+                                                      per, hidden, xt, rt),
+        x.device());
+    const Dropout drop = Dropout::saved(ctx, saved[7]);
+    const tfo_dropout_params dp = drop.params();
+    check(tfo_residual_rmsnorm_backward(ptr_or_null(dh2), hs, ptr_or_null(dy2), ys, x2.data_ptr(), xs, r2.data_ptr(), rs,
+                                        params, saved[6].data_ptr<float>(), out_or_null(d[0]), out_or_null(d[1]), rows, per,
+                                        hidden, ctx->saved_data["branch_norm"].toBool(), ctx->saved_data["scale"].toDouble(),
+                                        drop.p > 0 ? &dp : nullptr, xt, rt, out_or_null(ws),
+                                        ws.defined() ? static_cast<size_t>(ws.numel()) : 0,
+                                        at::cuda::getCurrentCUDAStream(x.device().index()).stream()),
+          "tfo_residual_rmsnorm_backward");
+    return d;
+  }
+};
+
+// fused_residual_rmsnorm: (h, y or None), or None outside the common case.
+py::object residual_rmsnorm(const at::Tensor& x, const at::Tensor& residual, const OptTensor& bw, const OptTensor& gate,
+                            const OptTensor& w, const OptTensor& shift, bool branch_norm, bool norm, double scale,
+                            double eps, double p, const OptTensor& seed, uint64_t value, bool seeded, uint64_t offset) {
+  if (!x.is_cuda() || !is_float(x.scalar_type()) || x.dim() < 1 || x.numel() == 0 || has_tangent(x) ||
+      x.size(-1) > (1 << 24) || rows_of(x) >= (1ll << 31) || !residual_ok(x, residual) ||
+      !Dropout::ok(x, p, seed, seeded) || (bw.has_value() && !branch_norm) ||
+      (!norm && (w.has_value() || shift.has_value())))
+    return py::none();
+  for (const OptTensor* t : {&bw, &gate, &w, &shift})
+    if (!row_param_ok(*t, x)) return py::none();
+  const ResidualCall c{branch_norm, norm, scale, eps, Dropout{p, seed.value_or(at::Tensor()), value, offset}};
+  if (at::GradMode::is_enabled() && (x.requires_grad() || residual.requires_grad() || wants_grad(bw) || wants_grad(gate) ||
+                                     wants_grad(w) || wants_grad(shift)))
+    return pair_of(ResidualNode::apply(x, residual, bw, gate, w, shift, c));
+  const at::Tensor none;
+  const auto out = residual_call(x, residual, {bw.value_or(none), gate.value_or(none), w.value_or(none),
+                                               shift.value_or(none)}, c, false);
+  return pair_of(norm ? variable_list{out[0], out[1]} : variable_list{out[0]});
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tfo_ext, m) {
@@ -494,5 +732,7 @@ PYBIND11_MODULE(_tfo_ext, m) {
   m.def("qk_norm_rope", &qk_norm_rope, "fused_qk_norm_rope, or None");
   m.def("rope_tables", &rope_tables, "rope_tables of given positions, or None");
   m.def("lora", &lora, "fused_lora on 2-D operands, or None");
+  m.def("dropout", &dropout, "fused_dropout, or None");
+  m.def("residual_rmsnorm", &residual_rmsnorm, "fused_residual_rmsnorm, or None");
   m.def("clear_workspaces", &clear_workspaces, "releases the cached scratch buffers");
 }

@@ -7,6 +7,8 @@ Ops (each one launches hand-written sm_100a CUDA kernels through the C ABI in
 * ``fused_gated_mlp`` / ``FusedGatedMLP``
 * ``rope_tables`` / ``RoPEScaling``, ``fused_rope``
 * ``fused_qk_norm_rope`` / ``FusedQKNormRoPE``
+* ``fused_residual_rmsnorm`` / ``FusedResidualRMSNorm``
+* ``fused_dropout`` / ``FusedDropout``
 * ``fp8_gemm`` / ``FP8Linear``
 * ``fused_lora`` / ``FP8LoRALinear``
 * ``quantize_fp8`` / ``dequantize_fp8``
@@ -40,11 +42,13 @@ from triton_ops.exceptions import (
     TuningFailedError,
     UnsupportedDtypeError,
 )
+from triton_ops.kernels.dropout import FusedDropout, fused_dropout
 from triton_ops.kernels.fp8_gemm import FP8Linear, fp8_gemm
 from triton_ops.kernels.fp8_quantize import dequantize_fp8, quantize_fp8, quantize_fp8_per_token
 from triton_ops.kernels.gated_mlp import FusedGatedMLP, fused_gated_mlp, fused_gated_mlp_quantize
 from triton_ops.kernels.lora import FP8LoRALinear, fused_lora
 from triton_ops.kernels.qk_norm_rope import FusedQKNormRoPE, fused_qk_norm_rope
+from triton_ops.kernels.residual import FusedResidualRMSNorm, fused_residual_rmsnorm
 from triton_ops.kernels.rmsnorm_rope import FusedRMSNormRoPE, fused_rmsnorm_rope, fused_rmsnorm_rope_quantize
 from triton_ops.kernels.rope import RoPEScaling, fused_rope, rope_tables
 from triton_ops.models import (
@@ -66,6 +70,10 @@ __all__ = [
     "fused_rope",
     "fused_qk_norm_rope",
     "FusedQKNormRoPE",
+    "fused_residual_rmsnorm",
+    "FusedResidualRMSNorm",
+    "fused_dropout",
+    "FusedDropout",
     "fused_gated_mlp",
     "fused_gated_mlp_quantize",
     "FusedGatedMLP",

@@ -59,6 +59,21 @@ _c_strides = ctypes.POINTER(ctypes.c_int64)
 _HEADS_TABLE = [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_int, _c_i64, _c_i64]
 _HEADS_SIZES = [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int]
 
+class DropoutParams(ctypes.Structure):
+    """tfo_dropout_params."""
+
+    _fields_ = [("p", ctypes.c_double), ("seed", _c_vp), ("seed_value", ctypes.c_uint64), ("offset", ctypes.c_uint64)]
+
+
+class RowParam(ctypes.Structure):
+    """tfo_row_param."""
+
+    _fields_ = [("data", _c_vp), ("seq_stride", _c_i64), ("dtype", _c_int), ("grad", _c_vp)]
+
+
+_c_dropout = ctypes.POINTER(DropoutParams)
+_c_row_params = ctypes.POINTER(RowParam)
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "tfo_version": (ctypes.c_char_p, []),
@@ -141,6 +156,22 @@ _SIGNATURES = {
         _c_int,
         [_c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64,
          _c_i64, _c_i64, _c_int, _c_vp, _c_size, _c_vp],
+    ),
+    "tfo_dropout": (_c_int, [_c_vp, _c_vp, _c_vp, _c_i64, _c_dropout, _c_int, _c_int, _c_vp]),
+    "tfo_residual_rmsnorm": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_i64, _c_row_params, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_int,
+         ctypes.c_double, ctypes.c_double, _c_dropout, _c_int, _c_int, _c_vp],
+    ),
+    "tfo_residual_rmsnorm_backward_workspace_bytes": (
+        _c_size,
+        [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_row_params, _c_vp, _c_vp, _c_i64, _c_i64,
+         _c_i64, _c_int, _c_int],
+    ),
+    "tfo_residual_rmsnorm_backward": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_row_params, _c_vp, _c_vp, _c_vp, _c_i64,
+         _c_i64, _c_i64, _c_int, ctypes.c_double, _c_dropout, _c_int, _c_int, _c_vp, _c_size, _c_vp],
     ),
     "tfo_gated_mlp_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_int, _c_int]),
     "tfo_gated_mlp": (

@@ -1,5 +1,6 @@
 """Op implementations (same module layout and names as the reference's triton_ops.kernels)."""
 
+from triton_ops.kernels.dropout import FusedDropout, fused_dropout, fused_dropout_kernel
 from triton_ops.kernels.fp8_gemm import FP8Linear, fp8_gemm, fp8_gemm_kernel
 from triton_ops.kernels.fp8_quantize import (
     dequantize_fp8,
@@ -14,6 +15,12 @@ from triton_ops.kernels.qk_norm_rope import (
     fused_qk_norm_rope,
     fused_qk_norm_rope_backward_kernel,
     fused_qk_norm_rope_kernel,
+)
+from triton_ops.kernels.residual import (
+    FusedResidualRMSNorm,
+    fused_residual_rmsnorm,
+    fused_residual_rmsnorm_backward_kernel,
+    fused_residual_rmsnorm_kernel,
 )
 from triton_ops.kernels.rmsnorm_rope import (
     FusedRMSNormRoPE,
@@ -45,6 +52,13 @@ __all__ = [
     "FusedQKNormRoPE",
     "fused_qk_norm_rope_kernel",
     "fused_qk_norm_rope_backward_kernel",
+    "fused_residual_rmsnorm",
+    "FusedResidualRMSNorm",
+    "fused_residual_rmsnorm_kernel",
+    "fused_residual_rmsnorm_backward_kernel",
+    "fused_dropout",
+    "FusedDropout",
+    "fused_dropout_kernel",
     "fused_gated_mlp",
     "FusedGatedMLP",
     "fused_gated_mlp_kernel",

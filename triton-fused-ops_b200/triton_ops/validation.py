@@ -442,3 +442,76 @@ def validate_lora_inputs(
         if t is not None:
             _check_no_tangent(t, name)
     return x.numel() // k, adapters, rank, k, n
+
+
+def validate_dropout(x: torch.Tensor, p: float, seed, offset: int, residual: Optional[torch.Tensor]) -> None:
+    """Checks a dropout's inputs: x of any shape, a residual of its shape and type (or fp32), probability and seed."""
+    _check_cuda(x, "x")
+    _check_dtype(x, "x", SUPPORTED_DTYPES_FLOAT)
+    _check_no_tangent(x, "x")
+    if residual is not None:
+        check_residual(x, residual)
+    check_dropout_key(x, p, seed, offset)
+
+
+def check_residual(x: torch.Tensor, residual: torch.Tensor) -> None:
+    """Checks the residual stream beside x: its shape, and its type or fp32."""
+    _check_cuda(residual, "residual")
+    _check_dtype(residual, "residual", [x.dtype, torch.float32])
+    _check_same_device(x, residual, "residual")
+    if residual.shape != x.shape:
+        raise ShapeMismatchError(f"residual shape {tuple(residual.shape)} doesn't match x {tuple(x.shape)}",
+                                 expected=x.shape, actual=residual.shape, tensor_name="residual")
+    _check_no_tangent(residual, "residual")
+
+
+def check_dropout_key(x: torch.Tensor, p: float, seed, offset: int) -> None:
+    """Checks a dropout's probability, seed (an int, or one int64 beside x) and offset."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"the dropout probability must be in 0..1, got {p}")
+    if not 0 <= offset < 2**64:
+        raise ValueError(f"the dropout offset must be in 0..2^64 - 1, got {offset}")
+    if seed is None:
+        if p > 0:
+            raise ValueError("dropout needs a seed")
+    elif isinstance(seed, torch.Tensor):
+        _check_cuda(seed, "seed")
+        _check_dtype(seed, "seed", [torch.int64])
+        _check_same_device(x, seed, "seed")
+        if seed.numel() != 1:
+            raise ShapeMismatchError(f"seed must hold one number, got {tuple(seed.shape)}", actual=seed.shape,
+                                     tensor_name="seed")
+    elif isinstance(seed, bool) or not isinstance(seed, int):
+        raise TypeError(f"seed must be an int or an int64 tensor, got {type(seed).__name__}")
+
+
+def validate_residual_inputs(x: torch.Tensor, residual: torch.Tensor, params: dict, branch_norm: bool, norm: bool, p: float,
+                             seed, offset: int) -> None:
+    """Checks the residual stream's inputs; `params` maps names to [hidden] or [batch, hidden] tensors or None."""
+    _check_cuda(x, "x")
+    _check_dtype(x, "x", SUPPORTED_DTYPES_FLOAT)
+    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] > 2**24:
+        raise ShapeMismatchError(f"x must be [..., hidden] with hidden in 1..2^24, got {tuple(x.shape)}", actual=x.shape,
+                                 tensor_name="x")
+    if x.numel() // x.shape[-1] >= 2**31:
+        raise ShapeMismatchError(f"x must have fewer than 2^31 rows, got {tuple(x.shape)}", actual=x.shape, tensor_name="x")
+    _check_no_tangent(x, "x")
+    check_residual(x, residual)
+    hidden = x.shape[-1]
+    for name, t in params.items():
+        if t is None:
+            continue
+        _check_cuda(t, name)
+        _check_dtype(t, name, SUPPORTED_DTYPES_FLOAT)
+        _check_same_device(x, t, name)
+        own = 2 <= t.dim() <= x.dim() and t.shape[0] == x.shape[0] and all(n == 1 for n in t.shape[1:-1])
+        if not (t.dim() == 1 or own) or t.shape[-1] != hidden:
+            raise ShapeMismatchError(
+                f"{name} must be [{hidden}], or [{x.shape[0]}, {hidden}] (a row for each sequence, with or without "
+                f"dimensions of 1 between), got {tuple(t.shape)}", expected=(hidden,), actual=t.shape, tensor_name=name)
+        _check_no_tangent(t, name)
+    if params["branch_weight"] is not None and not branch_norm:
+        raise ValueError("branch_weight needs branch_norm=True")
+    if not norm and (params["weight"] is not None or params["shift"] is not None):
+        raise ValueError("weight and shift need norm=True")
+    check_dropout_key(x, p, seed, offset)
