@@ -345,6 +345,46 @@ TFO_API int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_
                                       double eps, int dtype, int q_w_dtype, int k_w_dtype, int table_dtype,
                                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* Several positions for each token (time, height, width of a picture's or a
+ * clip's patches): pair i of columns turns by the position on axis
+ * axis_of_pair[i]. Positions are then integers at [axis * pos_stride + ...] with
+ * the strides of the plain call (of tfo_rope_tables: [axis * pos_stride + row]).
+ * The *_axes calls are the plain ones where axes is NULL. A bad position gives
+ * NaN in its axis' pairs. */
+typedef struct tfo_axes {
+  int axes;                    /* 2..4 */
+  int64_t pos_stride;          /* elements between the axes' positions */
+  const uint8_t* axis_of_pair; /* host memory, one for each pair of columns */
+} tfo_axes;
+
+TFO_API int tfo_rope_tables_axes(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half,
+                                 double gain, void* cos, void* sin, int out_dtype, const tfo_axes* axes,
+                                 void* stream);
+TFO_API int tfo_rope_axes(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          const void* cos, const void* sin, int64_t table_stride, int64_t table_rows,
+                          const void* positions, int pos_dtype, int64_t pos_stride_batch, int64_t pos_stride_seq,
+                          void* q_out, void* k_out, int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads,
+                          int64_t head_dim, int64_t rotary_dim, int interleaved, int inverse, int dtype,
+                          int table_dtype, const tfo_axes* axes, void* stream);
+TFO_API int tfo_qk_norm_rope_axes(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                  const void* q_weight, const void* k_weight, const void* cos, const void* sin,
+                                  int64_t table_stride, int64_t table_rows, const void* positions, int pos_dtype,
+                                  int64_t pos_stride_batch, int64_t pos_stride_seq, void* q_out, void* k_out,
+                                  int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t head_dim,
+                                  int64_t rotary_dim, int interleaved, double eps, int dtype, int q_w_dtype,
+                                  int k_w_dtype, int table_dtype, const tfo_axes* axes, void* stream);
+TFO_API int tfo_qk_norm_rope_backward_axes(const void* dq_out, const int64_t* dq_out_strides, const void* dk_out,
+                                           const int64_t* dk_out_strides, const void* q, const int64_t* q_strides,
+                                           const void* k, const int64_t* k_strides, const void* q_weight,
+                                           const void* k_weight, const void* cos, const void* sin,
+                                           int64_t table_stride, int64_t table_rows, const void* positions,
+                                           int pos_dtype, int64_t pos_stride_batch, int64_t pos_stride_seq, void* dq,
+                                           void* dk, void* dq_weight, void* dk_weight, int64_t batch, int64_t seq,
+                                           int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim,
+                                           int interleaved, double eps, int dtype, int q_w_dtype, int k_w_dtype,
+                                           int table_dtype, void* workspace, size_t workspace_bytes,
+                                           const tfo_axes* axes, void* stream);
+
 /* Low-rank adapters of many requests beside a shared projection:
  *   out[t, :] = base[t, :] + scaling[i] * b[i] . (a[i] . x[t, :]),  i = ids[t]
  * x [tokens, k] (rows x_stride elements apart, innermost stride 1), a

@@ -228,12 +228,17 @@ struct RopeTablesArgs {
   void* cos;
   void* sin;
   int out_dtype;
+  // several positions for each row: pair i takes that of axis axis_of[i] (host, `half` values), or NULL
+  const uint8_t* axis_of;
+  int64_t pos_stride_axis;
 };
 cudaError_t rope_tables_launch(const RopeTablesArgs& a, cudaStream_t st);
 
 // Rotation of query and key heads, alone or after an RMSNorm of each head
 // (qk_rope.cu), and the gradients (qk_rope_backward.cu; the rotation's own
 // gradient is the rotation with `inverse`).
+constexpr int kMaxAxes = 4;
+constexpr int kMaxAxisPairs = 512;
 struct HeadTables {
   const void* cos;
   const void* sin;
@@ -243,6 +248,10 @@ struct HeadTables {
   const void* positions;  // per token, or NULL: the token's index in its sequence
   int pos_dtype;
   int64_t pos_stride_batch, pos_stride_seq;
+  // several positions for each token (time, height, width): pair i turns by that of axis axis_of(i)
+  int axes;  // 0 or 1: one position
+  int64_t pos_stride_axis;
+  uint32_t axis_bits[kMaxAxisPairs / 16];  // two bits a pair
 };
 struct HeadSide {  // the queries or the keys
   const void* x;   // [batch, seq, heads, head_dim]
@@ -266,8 +275,10 @@ struct HeadArgs {
   int dtype;
 };
 cudaError_t qk_rope_launch(const HeadArgs& a, cudaStream_t st);
+cudaError_t qk_rope_axes_launch(const HeadArgs& a, cudaStream_t st);  // qk_rope_axes.cu: a.t.axes > 1
 size_t qk_norm_rope_backward_workspace_bytes(int head_dim);
 cudaError_t qk_norm_rope_backward_launch(const HeadArgs& a, void* ws, cudaStream_t st);
+cudaError_t qk_norm_rope_backward_axes_launch(const HeadArgs& a, void* ws, cudaStream_t st);  // qk_rope_backward_axes.cu
 // Elements per vector with which the vector kernels can take these heads (0: they cannot).
 int head_vector_elems(const HeadArgs& a, bool backward);
 

@@ -54,14 +54,35 @@ int set_heads(HeadArgs* a, const std::string& fn, const void* q, const int64_t* 
     return fail(TFO_ERR_INVALID, fn + ": NULL pointer");
   set_side(&a->q, q, q_strides, q_out, q_heads);
   set_side(&a->k, k, k_strides, k_out, k_heads);
-  a->t = HeadTables{cos,       sin,       table_stride,     table_rows,    table_dtype,
-                    positions, pos_dtype, pos_stride_batch, pos_stride_seq};
+  a->t = HeadTables{cos,       sin,       table_stride,     table_rows,     table_dtype,
+                    positions, pos_dtype, pos_stride_batch, pos_stride_seq, 0, 0, {}};
   a->batch = batch;
   a->seq = seq;
   a->head_dim = static_cast<int>(head_dim);
   a->rotary_dim = static_cast<int>(rotary_dim);
   a->pairs = interleaved != 0;
   a->dtype = dtype;
+  return TFO_OK;
+}
+
+// The axes of `pairs` pairs of columns; two bits each where `bits` is given.
+int check_axes(const std::string& fn, const tfo_axes& axes, int64_t pairs, int pos_dtype, uint32_t* bits) {
+  if (axes.axes < 2 || axes.axes > kMaxAxes) return fail(TFO_ERR_INVALID, fn + ": need 2 to 4 axes");
+  if (!axes.axis_of_pair) return fail(TFO_ERR_INVALID, fn + ": NULL pointer");
+  if (pos_dtype == TFO_POS_NONE) return fail(TFO_ERR_INVALID, fn + ": several axes need positions");
+  for (int64_t i = 0; i < pairs; ++i) {
+    if (axes.axis_of_pair[i] >= axes.axes) return fail(TFO_ERR_INVALID, fn + ": a pair's axis is past the last");
+    if (bits) bits[i / 16] |= static_cast<uint32_t>(axes.axis_of_pair[i]) << (2 * (i % 16));
+  }
+  return TFO_OK;
+}
+
+int set_axes(HeadArgs* a, const std::string& fn, const tfo_axes* axes) {
+  if (axes == nullptr) return TFO_OK;
+  const int st = check_axes(fn, *axes, a->rotary_dim / 2, a->t.pos_dtype, a->t.axis_bits);
+  if (st != TFO_OK) return st;
+  a->t.axes = axes->axes;
+  a->t.pos_stride_axis = axes->pos_stride;
   return TFO_OK;
 }
 
@@ -72,9 +93,9 @@ using namespace tfo;
 
 extern "C" {
 
-int tfo_rope_tables(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half, double gain,
-                    void* cos, void* sin, int out_dtype, void* stream) {
-  const char* fn = "tfo_rope_tables";
+int tfo_rope_tables_axes(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half,
+                         double gain, void* cos, void* sin, int out_dtype, const tfo_axes* axes, void* stream) {
+  const char* fn = axes != nullptr ? "tfo_rope_tables_axes" : "tfo_rope_tables";
   if (!is_float_dtype(out_dtype)) return fail(TFO_ERR_DTYPE, std::string(fn) + ": tables must be f16, bf16 or f32");
   if (pos_dtype < TFO_POS_NONE || pos_dtype > TFO_POS_I64)
     return fail(TFO_ERR_DTYPE, std::string(fn) + ": positions must be int32 or int64");
@@ -86,8 +107,36 @@ int tfo_rope_tables(const void* positions, int pos_dtype, int64_t n, const doubl
   for (int64_t i = 0; i < half; ++i) {
     if (!(turns[i] - turns[i] == 0.0)) return fail(TFO_ERR_INVALID, std::string(fn) + ": turns must be finite");
   }
-  const RopeTablesArgs a{positions, pos_dtype, n, turns, static_cast<int>(half), gain, cos, sin, out_dtype};
+  RopeTablesArgs a{positions, pos_dtype, n, turns, static_cast<int>(half), gain, cos, sin, out_dtype, nullptr, 0};
+  if (axes != nullptr) {
+    if (const int axes_st = check_axes(fn, *axes, half, pos_dtype, nullptr); axes_st != TFO_OK) return axes_st;
+    a.axis_of = axes->axis_of_pair;
+    a.pos_stride_axis = axes->pos_stride;
+  }
   const cudaError_t e = rope_tables_launch(a, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? TFO_OK : cuda_fail(e, fn);
+}
+
+int tfo_rope_tables(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half, double gain,
+                    void* cos, void* sin, int out_dtype, void* stream) {
+  return tfo_rope_tables_axes(positions, pos_dtype, n, turns, half, gain, cos, sin, out_dtype, nullptr, stream);
+}
+
+int tfo_rope_axes(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* cos,
+                  const void* sin, int64_t table_stride, int64_t table_rows, const void* positions, int pos_dtype,
+                  int64_t pos_stride_batch, int64_t pos_stride_seq, void* q_out, void* k_out, int64_t batch,
+                  int64_t seq, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim, int interleaved,
+                  int inverse, int dtype, int table_dtype, const tfo_axes* axes, void* stream) {
+  const char* fn = axes != nullptr ? "tfo_rope_axes" : "tfo_rope";
+  HeadArgs a{};
+  bool empty = false;
+  const int st = set_heads(&a, fn, q, q_strides, k, k_strides, cos, sin, table_stride, table_rows, positions, pos_dtype,
+                           pos_stride_batch, pos_stride_seq, q_out, k_out, batch, seq, q_heads, k_heads, head_dim,
+                           rotary_dim, interleaved, dtype, table_dtype, &empty);
+  if (st != TFO_OK || empty) return st;
+  if (const int axes_st = set_axes(&a, fn, axes); axes_st != TFO_OK) return axes_st;
+  a.inverse = inverse != 0;
+  const cudaError_t e = qk_rope_launch(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? TFO_OK : cuda_fail(e, fn);
 }
 
@@ -96,25 +145,19 @@ int tfo_rope(const void* q, const int64_t* q_strides, const void* k, const int64
              int64_t pos_stride_batch, int64_t pos_stride_seq, void* q_out, void* k_out, int64_t batch, int64_t seq,
              int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim, int interleaved, int inverse,
              int dtype, int table_dtype, void* stream) {
-  const char* fn = "tfo_rope";
-  HeadArgs a{};
-  bool empty = false;
-  const int st = set_heads(&a, fn, q, q_strides, k, k_strides, cos, sin, table_stride, table_rows, positions, pos_dtype,
-                           pos_stride_batch, pos_stride_seq, q_out, k_out, batch, seq, q_heads, k_heads, head_dim,
-                           rotary_dim, interleaved, dtype, table_dtype, &empty);
-  if (st != TFO_OK || empty) return st;
-  a.inverse = inverse != 0;
-  const cudaError_t e = qk_rope_launch(a, static_cast<cudaStream_t>(stream));
-  return e == cudaSuccess ? TFO_OK : cuda_fail(e, fn);
+  return tfo_rope_axes(q, q_strides, k, k_strides, cos, sin, table_stride, table_rows, positions, pos_dtype,
+                       pos_stride_batch, pos_stride_seq, q_out, k_out, batch, seq, q_heads, k_heads, head_dim,
+                       rotary_dim, interleaved, inverse, dtype, table_dtype, nullptr, stream);
 }
 
-int tfo_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                     const void* q_weight, const void* k_weight, const void* cos, const void* sin, int64_t table_stride,
-                     int64_t table_rows, const void* positions, int pos_dtype, int64_t pos_stride_batch,
-                     int64_t pos_stride_seq, void* q_out, void* k_out, int64_t batch, int64_t seq, int64_t q_heads,
-                     int64_t k_heads, int64_t head_dim, int64_t rotary_dim, int interleaved, double eps, int dtype,
-                     int q_w_dtype, int k_w_dtype, int table_dtype, void* stream) {
-  const char* fn = "tfo_qk_norm_rope";
+int tfo_qk_norm_rope_axes(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                          const void* q_weight, const void* k_weight, const void* cos, const void* sin,
+                          int64_t table_stride, int64_t table_rows, const void* positions, int pos_dtype,
+                          int64_t pos_stride_batch, int64_t pos_stride_seq, void* q_out, void* k_out, int64_t batch,
+                          int64_t seq, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t rotary_dim,
+                          int interleaved, double eps, int dtype, int q_w_dtype, int k_w_dtype, int table_dtype,
+                          const tfo_axes* axes, void* stream) {
+  const char* fn = axes != nullptr ? "tfo_qk_norm_rope_axes" : "tfo_qk_norm_rope";
   if ((q_weight && !is_float_dtype(q_w_dtype)) || (k_weight && !is_float_dtype(k_w_dtype)))
     return fail(TFO_ERR_DTYPE, std::string(fn) + ": weights must be f16, bf16 or f32");
   HeadArgs a{};
@@ -123,6 +166,7 @@ int tfo_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, con
                            pos_stride_batch, pos_stride_seq, q_out, k_out, batch, seq, q_heads, k_heads, head_dim,
                            rotary_dim, interleaved, dtype, table_dtype, &empty);
   if (st != TFO_OK || empty) return st;
+  if (const int axes_st = set_axes(&a, fn, axes); axes_st != TFO_OK) return axes_st;
   a.norm = true;
   a.eps = static_cast<float>(eps);
   a.q.weight = q_weight;
@@ -133,21 +177,34 @@ int tfo_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, con
   return e == cudaSuccess ? TFO_OK : cuda_fail(e, fn);
 }
 
+int tfo_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                     const void* q_weight, const void* k_weight, const void* cos, const void* sin, int64_t table_stride,
+                     int64_t table_rows, const void* positions, int pos_dtype, int64_t pos_stride_batch,
+                     int64_t pos_stride_seq, void* q_out, void* k_out, int64_t batch, int64_t seq, int64_t q_heads,
+                     int64_t k_heads, int64_t head_dim, int64_t rotary_dim, int interleaved, double eps, int dtype,
+                     int q_w_dtype, int k_w_dtype, int table_dtype, void* stream) {
+  return tfo_qk_norm_rope_axes(q, q_strides, k, k_strides, q_weight, k_weight, cos, sin, table_stride, table_rows,
+                               positions, pos_dtype, pos_stride_batch, pos_stride_seq, q_out, k_out, batch, seq,
+                               q_heads, k_heads, head_dim, rotary_dim, interleaved, eps, dtype, q_w_dtype, k_w_dtype,
+                               table_dtype, nullptr, stream);
+}
+
 size_t tfo_qk_norm_rope_backward_workspace_bytes(int64_t head_dim) {
   if (head_dim <= 0 || head_dim > kMaxHeadDim) return 0;
   return qk_norm_rope_backward_workspace_bytes(static_cast<int>(head_dim));
 }
 
-int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides, const void* dk_out,
-                              const int64_t* dk_out_strides, const void* q, const int64_t* q_strides, const void* k,
-                              const int64_t* k_strides, const void* q_weight, const void* k_weight, const void* cos,
-                              const void* sin, int64_t table_stride, int64_t table_rows, const void* positions,
-                              int pos_dtype, int64_t pos_stride_batch, int64_t pos_stride_seq, void* dq, void* dk,
-                              void* dq_weight, void* dk_weight, int64_t batch, int64_t seq, int64_t q_heads,
-                              int64_t k_heads, int64_t head_dim, int64_t rotary_dim, int interleaved, double eps,
-                              int dtype, int q_w_dtype, int k_w_dtype, int table_dtype, void* workspace,
-                              size_t workspace_bytes, void* stream) {
-  const char* fn = "tfo_qk_norm_rope_backward";
+int tfo_qk_norm_rope_backward_axes(const void* dq_out, const int64_t* dq_out_strides, const void* dk_out,
+                                   const int64_t* dk_out_strides, const void* q, const int64_t* q_strides,
+                                   const void* k, const int64_t* k_strides, const void* q_weight, const void* k_weight,
+                                   const void* cos, const void* sin, int64_t table_stride, int64_t table_rows,
+                                   const void* positions, int pos_dtype, int64_t pos_stride_batch,
+                                   int64_t pos_stride_seq, void* dq, void* dk, void* dq_weight, void* dk_weight,
+                                   int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t head_dim,
+                                   int64_t rotary_dim, int interleaved, double eps, int dtype, int q_w_dtype,
+                                   int k_w_dtype, int table_dtype, void* workspace, size_t workspace_bytes,
+                                   const tfo_axes* axes, void* stream) {
+  const char* fn = axes != nullptr ? "tfo_qk_norm_rope_backward_axes" : "tfo_qk_norm_rope_backward";
   if ((q_weight && !is_float_dtype(q_w_dtype)) || (k_weight && !is_float_dtype(k_w_dtype)))
     return fail(TFO_ERR_DTYPE, std::string(fn) + ": weights must be f16, bf16 or f32");
   if ((dq_weight && !q_weight) || (dk_weight && !k_weight))
@@ -170,6 +227,7 @@ int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides,
   if (e == cudaSuccess && (empty || k_heads == 0)) e = zero(dk_weight, k_w_dtype);
   if (e != cudaSuccess) return cuda_fail(e, fn);
   if (empty) return TFO_OK;
+  if (const int axes_st = set_axes(&a, fn, axes); axes_st != TFO_OK) return axes_st;
   if ((q_heads > 0 && (!dq_out || !dq_out_strides)) || (k_heads > 0 && (!dk_out || !dk_out_strides)))
     return fail(TFO_ERR_INVALID, std::string(fn) + ": NULL pointer");
   if ((dq_weight || dk_weight) && (!workspace || workspace_bytes < tfo_qk_norm_rope_backward_workspace_bytes(head_dim) ||
@@ -191,6 +249,22 @@ int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides,
   grads(&a.k, k_weight, k_w_dtype, dk_out, dk_out_strides, dk_weight);
   e = qk_norm_rope_backward_launch(a, workspace, st);
   return e == cudaSuccess ? TFO_OK : cuda_fail(e, fn);
+}
+
+int tfo_qk_norm_rope_backward(const void* dq_out, const int64_t* dq_out_strides, const void* dk_out,
+                              const int64_t* dk_out_strides, const void* q, const int64_t* q_strides, const void* k,
+                              const int64_t* k_strides, const void* q_weight, const void* k_weight, const void* cos,
+                              const void* sin, int64_t table_stride, int64_t table_rows, const void* positions,
+                              int pos_dtype, int64_t pos_stride_batch, int64_t pos_stride_seq, void* dq, void* dk,
+                              void* dq_weight, void* dk_weight, int64_t batch, int64_t seq, int64_t q_heads,
+                              int64_t k_heads, int64_t head_dim, int64_t rotary_dim, int interleaved, double eps,
+                              int dtype, int q_w_dtype, int k_w_dtype, int table_dtype, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  return tfo_qk_norm_rope_backward_axes(dq_out, dq_out_strides, dk_out, dk_out_strides, q, q_strides, k, k_strides,
+                                        q_weight, k_weight, cos, sin, table_stride, table_rows, positions, pos_dtype,
+                                        pos_stride_batch, pos_stride_seq, dq, dk, dq_weight, dk_weight, batch, seq,
+                                        q_heads, k_heads, head_dim, rotary_dim, interleaved, eps, dtype, q_w_dtype,
+                                        k_w_dtype, table_dtype, workspace, workspace_bytes, nullptr, stream);
 }
 
 }  // extern "C"

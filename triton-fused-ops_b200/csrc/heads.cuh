@@ -160,6 +160,89 @@ __device__ __forceinline__ int64_t token_position(const HeadTables& t, int64_t b
   return pos;
 }
 
+// The axes of a lane's pairs (in lane_table's order), two bits each.
+struct LaneAxes {
+  uint32_t bits;
+  bool one_a, one_b;  // all pairs of the lane (pair layout: of va, of vb) have the same axis
+  __device__ static uint32_t of(const HeadTables& t, int pair) { return t.axis_bits[pair / 16] >> (2 * (pair % 16)) & 3u; }
+  template <int E, bool PAIRS> __device__ static LaneAxes make(const HeadTables& t, const LaneCols& col) {
+    LaneAxes l{0, true, true};
+#pragma unroll
+    for (int v = 0; v < (PAIRS ? 2 : 1); ++v) {
+      if (v == 0 ? !col.rot_a : !col.rot_b) continue;
+      constexpr int H = PAIRS ? E / 2 : E;
+      const int first = (v == 0 ? col.va : col.vb) * H;
+      bool one = true;
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        const uint32_t axis = of(t, first + j);
+        l.bits |= axis << (2 * (v * H + j));
+        one = one && axis == of(t, first);
+      }
+      (v == 0 ? l.one_a : l.one_b) = one;
+    }
+    return l;
+  }
+};
+
+// A token's position on one axis, as token_position's.
+__device__ __forceinline__ int64_t axis_position(const HeadTables& t, int64_t b, int64_t s, uint32_t axis, uint32_t* err) {
+  const int64_t at = axis * t.pos_stride_axis + b * t.pos_stride_batch + s * t.pos_stride_seq;
+  int64_t pos = t.pos_dtype == POS_I64 ? reinterpret_cast<const int64_t*>(t.positions)[at]
+                                       : reinterpret_cast<const int32_t*>(t.positions)[at];
+  if (pos < 0 || pos >= t.rows) {
+    set_error(err, ERR_BAD_POSITION);
+    pos = -1;
+  }
+  return pos;
+}
+
+// lane_table for a token with a position on each axis. Pairs of an axis whose position is bad become NaN.
+template <int E, bool PAIRS>
+__device__ __forceinline__ void lane_table_axes(const HeadTables& t, int64_t b, int64_t s, const LaneCols& col,
+                                                const LaneAxes& ax, bool inverse, uint32_t* err, float (&c)[E], float (&sn)[E]) {
+  constexpr int H = PAIRS ? E / 2 : E;
+#pragma unroll
+  for (int v = 0; v < (PAIRS ? 2 : 1); ++v) {
+    if (v == 0 ? !col.rot_a : !col.rot_b) continue;
+    const int first = (v == 0 ? col.va : col.vb) * H;
+    if (v == 0 ? ax.one_a : ax.one_b) {
+      const int64_t pos = axis_position(t, b, s, ax.bits >> (2 * v * H) & 3u, err);
+      float x[H], y[H];
+      if (pos < 0) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) x[j] = y[j] = __int_as_float(0x7fffffff);
+      } else {
+        load_floats<H>(t.cos, pos * t.row_stride + first, t.dtype, x);
+        load_floats<H>(t.sin, pos * t.row_stride + first, t.dtype, y);
+      }
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        c[v * H + j] = x[j];
+        sn[v * H + j] = y[j];
+      }
+    } else {
+      int64_t row[kMaxAxes];  // a bad one is negative
+#pragma unroll
+      for (int i = 0; i < kMaxAxes; ++i) {
+        const int64_t pos = i < t.axes ? axis_position(t, b, s, i, err) : -1;
+        row[i] = pos < 0 ? -1 : pos * t.row_stride;
+      }
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        const uint32_t axis = ax.bits >> (2 * (v * H + j)) & 3u;
+        const int64_t at = axis == 0 ? row[0] : axis == 1 ? row[1] : axis == 2 ? row[2] : row[3];
+        c[v * H + j] = at < 0 ? __int_as_float(0x7fffffff) : load_as_float(t.cos, at + first + j, t.dtype);
+        sn[v * H + j] = at < 0 ? __int_as_float(0x7fffffff) : load_as_float(t.sin, at + first + j, t.dtype);
+      }
+    }
+  }
+  if (inverse) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) sn[j] = -sn[j];
+  }
+}
+
 // cos and signed sin of a lane's pairs: of its E pairs (half layout), or of
 // va's E/2 pairs and then vb's (pair layout). Entries of pairs that are not
 // rotated stay unset and are not used.
@@ -196,6 +279,19 @@ __device__ __forceinline__ void lane_table(const HeadTables& t, int64_t pos, con
     for (int j = 0; j < E; ++j) s[j] = -s[j];
   }
 }
+
+// Where a token's table columns come from, for the kernels of one position (lane_table) and of several.
+template <int E, bool PAIRS, bool AXES> struct TokenTable {
+  LaneAxes ax;
+  __device__ TokenTable(const HeadTables& t, const LaneCols& col) {
+    if constexpr (AXES) ax = LaneAxes::make<E, PAIRS>(t, col);
+  }
+  __device__ void load(const HeadTables& t, int64_t b, int64_t s, const LaneCols& col, bool inverse, bool report, uint32_t* err,
+                       float (&c)[E], float (&sn)[E]) const {
+    if constexpr (AXES) lane_table_axes<E, PAIRS>(t, b, s, col, ax, inverse, err, c, sn);
+    else lane_table<E, PAIRS>(t, token_position(t, b, s, err, report), col, inverse, c, sn);
+  }
+};
 
 // A lane's rotation with weights: (u, v) -> (u wu c - v wv s, u wu s + v wv c)
 // as one product and one multiply-add per output on packed pairs of columns,

@@ -33,6 +33,11 @@ struct TurnsParam {
   uint64_t v[kMaxRopeHalf];  // 2^-64 turns per position
 };
 
+struct AxesParam {
+  uint8_t of[kMaxRopeHalf];  // the axis of each pair
+  int64_t stride;            // between the axes' positions
+};
+
 __device__ __forceinline__ int64_t table_position(const void* positions, int pos_dtype, int64_t i) {
   if (pos_dtype == POS_I64) return reinterpret_cast<const int64_t*>(positions)[i];
   if (pos_dtype == POS_I32) return reinterpret_cast<const int32_t*>(positions)[i];
@@ -64,10 +69,12 @@ __device__ __forceinline__ void sincos_turns(uint64_t a, float* sine, float* cos
   *cosine = __uint_as_float(__float_as_uint(odd ? s : c) ^ (((quarter + 1) & 2) << 30));
 }
 
-template <typename T, int V>
+// AXES: a row has a position on each of several axes, and a pair takes that of its own.
+template <typename T, int V, bool AXES>
 __global__ void __launch_bounds__(256) rope_tables_kernel(const void* __restrict__ positions, int pos_dtype, int64_t n,
                                                           int half, float gain, T* __restrict__ cosp,
-                                                          T* __restrict__ sinp, const __grid_constant__ TurnsParam turns) {
+                                                          T* __restrict__ sinp, const __grid_constant__ TurnsParam turns,
+                                                          const __grid_constant__ AxesParam axes) {
   griddep_launch_dependents();
   // thread -> (slice of V pairs, position), positions strided over the grid
   const int slices = half / V;
@@ -77,20 +84,29 @@ __global__ void __launch_bounds__(256) rope_tables_kernel(const void* __restrict
   uint64_t t[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) t[j] = turns.v[slice * V + j];
+  int64_t from[AXES ? V : 1];
+#pragma unroll
+  for (int j = 0; j < (AXES ? V : 1); ++j) from[j] = AXES ? axes.of[slice * V + j] * axes.stride : 0;
   griddep_wait();
   if (first >= per_block) return;
   const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
   int64_t p = static_cast<int64_t>(blockIdx.x) * per_block + first;
   if (p >= n) return;
-  int64_t next = table_position(positions, pos_dtype, p);  // loaded one step ahead
+  int64_t next[AXES ? V : 1];  // loaded one step ahead
+#pragma unroll
+  for (int j = 0; j < (AXES ? V : 1); ++j) next[j] = table_position(positions, pos_dtype, from[j] + p);
   for (; p < n; p += step) {
-    const uint64_t pos = static_cast<uint64_t>(next);  // a negative one modulo 2^64
-    if (p + step < n) next = table_position(positions, pos_dtype, p + step);
+    uint64_t pos[AXES ? V : 1];
+#pragma unroll
+    for (int j = 0; j < (AXES ? V : 1); ++j) {
+      pos[j] = static_cast<uint64_t>(next[j]);  // a negative one modulo 2^64
+      if (p + step < n) next[j] = table_position(positions, pos_dtype, from[j] + p + step);
+    }
     alignas(16) T c[V], s[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float sv, cv;
-      sincos_turns(pos * t[j], &sv, &cv);
+      sincos_turns(pos[AXES ? j : 0] * t[j], &sv, &cv);
       c[j] = Ty<T>::from_f(cv * gain);
       s[j] = Ty<T>::from_f(sv * gain);
     }
@@ -107,7 +123,7 @@ __global__ void __launch_bounds__(256) rope_tables_kernel(const void* __restrict
   }
 }
 
-template <typename T>
+template <typename T, bool AXES>
 static cudaError_t launch_tables(const RopeTablesArgs& a, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   TurnsParam turns;
@@ -115,6 +131,9 @@ static cudaError_t launch_tables(const RopeTablesArgs& a, cudaStream_t st) {
     const double t = i < a.half ? a.turns[i] - std::floor(a.turns[i]) : 0.0;  // in [0, 1)
     turns.v[i] = t < 1.0 ? static_cast<uint64_t>(std::nearbyint(std::ldexp(t, 64))) : 0;
   }
+  AxesParam axes;
+  if constexpr (AXES) std::copy(a.axis_of, a.axis_of + a.half, axes.of);
+  axes.stride = a.pos_stride_axis;
   const bool vec = a.half % V == 0 && reinterpret_cast<uintptr_t>(a.cos) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(a.sin) % 16 == 0;
   const int slices = vec ? a.half / V : a.half;
@@ -125,16 +144,21 @@ static cudaError_t launch_tables(const RopeTablesArgs& a, cudaStream_t st) {
   auto* s = static_cast<T*>(a.sin);
   const float gain = static_cast<float>(a.gain);
   note_launch();
-  return vec ? launch_dependent(rope_tables_kernel<T, V>, static_cast<int>(blocks), 256, st, a.positions, a.pos_dtype,
-                                a.n, a.half, gain, c, s, turns)
-             : launch_dependent(rope_tables_kernel<T, 1>, static_cast<int>(blocks), 256, st, a.positions, a.pos_dtype,
-                                a.n, a.half, gain, c, s, turns);
+  return vec ? launch_dependent(rope_tables_kernel<T, V, AXES>, static_cast<int>(blocks), 256, st, a.positions, a.pos_dtype,
+                                a.n, a.half, gain, c, s, turns, axes)
+             : launch_dependent(rope_tables_kernel<T, 1, AXES>, static_cast<int>(blocks), 256, st, a.positions, a.pos_dtype,
+                                a.n, a.half, gain, c, s, turns, axes);
+}
+
+template <typename T>
+static cudaError_t launch_type(const RopeTablesArgs& a, cudaStream_t st) {
+  return a.axis_of != nullptr ? launch_tables<T, true>(a, st) : launch_tables<T, false>(a, st);
 }
 
 cudaError_t rope_tables_launch(const RopeTablesArgs& a, cudaStream_t st) {
-  if (a.out_dtype == F16) return launch_tables<__half>(a, st);
-  if (a.out_dtype == BF16) return launch_tables<__nv_bfloat16>(a, st);
-  return launch_tables<float>(a, st);
+  if (a.out_dtype == F16) return launch_type<__half>(a, st);
+  if (a.out_dtype == BF16) return launch_type<__nv_bfloat16>(a, st);
+  return launch_type<float>(a, st);
 }
 
 }  // namespace tfo

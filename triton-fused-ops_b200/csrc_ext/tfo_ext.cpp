@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <array>
 #include <mutex>
 #include <stdexcept>
@@ -199,13 +200,23 @@ bool weight_ok(const OptTensor& w, const at::Tensor& q) {
                             w->size(0) == q.size(-1) && w->is_contiguous() && !w->_fw_grad(0).defined());
 }
 
+// The axis of each of `pairs` pairs, in host memory.
+bool pair_axes_ok(const at::Tensor& t, int64_t pairs) {
+  return t.is_cpu() && t.scalar_type() == at::kByte && t.is_contiguous() && t.numel() == pairs;
+}
+int axis_count(const at::Tensor& t) {
+  const uint8_t* p = t.data_ptr<uint8_t>();
+  return 1 + *std::max_element(p, p + t.numel());
+}
+
 // Forward mode: the Python wrappers refuse what carries a tangent.
 bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
 bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
 
 // Everything the shared arguments of the head functions must satisfy here.
+// axes: the axis of each pair (host bytes) where a token has several positions.
 bool heads_common(const at::Tensor& q, const OptTensor& k, const at::Tensor& cos, const at::Tensor& sin,
-                  const OptTensor& positions) {
+                  const OptTensor& positions, const OptTensor& axes) {
   if (!heads_ok(q)) return false;
   if (k.has_value()) {
     if (!heads_ok(*k) || k->device() != q.device() || k->scalar_type() != q.scalar_type() || k->dim() != q.dim() ||
@@ -221,24 +232,29 @@ bool heads_common(const at::Tensor& q, const OptTensor& k, const at::Tensor& cos
   if (has_tangent(q) || has_tangent(k) || has_tangent(cos) || has_tangent(sin)) return false;
   const int64_t dim = q.size(-1), rot = cos.size(1);
   if (dim < 2 || dim > 1024 || rot < 2 || rot % 2 != 0 || rot > dim || cos.size(0) == 0) return false;
-  if (!positions.has_value()) return cos.size(0) >= q.size(-3);
-  if (positions->device() != q.device() || pos_code(positions->scalar_type()) < 0 || positions->dim() != q.dim() - 2)
+  if (!positions.has_value()) return !axes.has_value() && cos.size(0) >= q.size(-3);
+  const int64_t more = axes.has_value() ? 1 : 0;  // a dimension of the axes before the tokens'
+  if (positions->device() != q.device() || pos_code(positions->scalar_type()) < 0 ||
+      positions->dim() != q.dim() - 2 + more)
     return false;
   for (int64_t i = 0; i < q.dim() - 2; ++i)
-    if (positions->size(i) != q.size(i)) return false;
-  return true;
+    if (positions->size(i + more) != q.size(i)) return false;
+  return !more || (pair_axes_ok(*axes, rot / 2) && positions->size(0) == axis_count(*axes));
 }
 
 struct HeadsCall {  // the C ABI's shared arguments
   const at::Tensor* positions;
   int pos_dtype = TFO_POS_NONE;
   int64_t pos_sb = 0, pos_ss = 0, batch, seq, q_heads, k_heads, dim, rot;
-  HeadsCall(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos, const at::Tensor& pos) : positions(&pos) {
+  tfo_axes axes_of{};
+  HeadsCall(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos, const at::Tensor& pos, const at::Tensor& axes)
+      : positions(&pos) {
     if (pos.defined()) {
       pos_dtype = pos_code(pos.scalar_type());
-      pos_sb = q.dim() == 4 ? pos.stride(0) : 0;
+      pos_sb = q.dim() == 4 ? pos.stride(-2) : 0;
       pos_ss = pos.stride(-1);
     }
+    if (axes.defined()) axes_of = {axis_count(axes), pos.stride(0), axes.data_ptr<uint8_t>()};
     batch = q.dim() == 4 ? q.size(0) : 1;
     seq = q.size(-3);
     q_heads = q.size(-2);
@@ -247,6 +263,7 @@ struct HeadsCall {  // the C ABI's shared arguments
     rot = cos.size(1);
   }
   const void* pos_ptr() const { return positions->defined() ? positions->data_ptr() : nullptr; }
+  const tfo_axes* axes() const { return axes_of.axis_of_pair != nullptr ? &axes_of : nullptr; }
 };
 
 const void* ptr_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -260,15 +277,16 @@ at::Tensor dense_heads(const at::Tensor& t) {
 int weight_code(const at::Tensor& w) { return w.defined() ? dtype_code(w.scalar_type()) : TFO_DTYPE_F32; }
 
 std::array<at::Tensor, 2> rope_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos,
-                                    const at::Tensor& sin, const at::Tensor& positions, bool interleaved, bool inverse) {
+                                    const at::Tensor& sin, const at::Tensor& positions, bool interleaved, bool inverse,
+                                    const at::Tensor& axes) {
   const c10::cuda::CUDAGuard guard(q.device());
-  const HeadsCall h(q, k, cos, positions);
+  const HeadsCall h(q, k, cos, positions, axes);
   std::array<at::Tensor, 2> out{empty_heads(q), empty_heads(k)};
   const Strides3 qs = strides_of(q), ks = k.defined() ? strides_of(k) : Strides3{};
-  check(tfo_rope(q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(), cos.data_ptr(), sin.data_ptr(), cos.stride(0),
+  check(tfo_rope_axes(q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(), cos.data_ptr(), sin.data_ptr(), cos.stride(0),
                  cos.size(0), h.pos_ptr(), h.pos_dtype, h.pos_sb, h.pos_ss, out[0].data_ptr(), out_or_null(out[1]),
                  h.batch, h.seq, h.q_heads, h.k_heads, h.dim, h.rot, interleaved, inverse,
-                 dtype_code(q.scalar_type()), dtype_code(cos.scalar_type()),
+                 dtype_code(q.scalar_type()), dtype_code(cos.scalar_type()), h.axes(),
                  at::cuda::getCurrentCUDAStream(q.device().index()).stream()),
         "tfo_rope");
   return out;
@@ -276,16 +294,17 @@ std::array<at::Tensor, 2> rope_call(const at::Tensor& q, const at::Tensor& k, co
 
 std::array<at::Tensor, 2> qk_norm_call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& qw,
                                        const at::Tensor& kw, const at::Tensor& cos, const at::Tensor& sin,
-                                       const at::Tensor& positions, double eps, bool interleaved) {
+                                       const at::Tensor& positions, double eps, bool interleaved,
+                                       const at::Tensor& axes) {
   const c10::cuda::CUDAGuard guard(q.device());
-  const HeadsCall h(q, k, cos, positions);
+  const HeadsCall h(q, k, cos, positions, axes);
   std::array<at::Tensor, 2> out{empty_heads(q), empty_heads(k)};
   const Strides3 qs = strides_of(q), ks = k.defined() ? strides_of(k) : Strides3{};
-  check(tfo_qk_norm_rope(q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(), ptr_or_null(qw), ptr_or_null(kw),
+  check(tfo_qk_norm_rope_axes(q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(), ptr_or_null(qw), ptr_or_null(kw),
                          cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.size(0), h.pos_ptr(), h.pos_dtype, h.pos_sb,
                          h.pos_ss, out[0].data_ptr(), out_or_null(out[1]), h.batch, h.seq, h.q_heads, h.k_heads, h.dim,
                          h.rot, interleaved, eps, dtype_code(q.scalar_type()), weight_code(qw), weight_code(kw),
-                         dtype_code(cos.scalar_type()), at::cuda::getCurrentCUDAStream(q.device().index()).stream()),
+                         dtype_code(cos.scalar_type()), h.axes(), at::cuda::getCurrentCUDAStream(q.device().index()).stream()),
         "tfo_qk_norm_rope");
   return out;
 }
@@ -312,16 +331,23 @@ void differentiable_once(const char* op, const variable_list& gradients, const v
     if (g.defined()) torch::autograd::set_history(g, node);
 }
 
+at::Tensor saved_axes(AutogradContext* ctx) {
+  const auto at = ctx->saved_data.find("axes");
+  return at == ctx->saved_data.end() ? at::Tensor() : at->second.toTensor();
+}
+
 // The gradient of a rotation is the rotation by the opposite angle, itself differentiable.
 struct RopeNode : public torch::autograd::Function<RopeNode> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k, const at::Tensor& cos,
-                               const at::Tensor& sin, const OptTensor& positions, bool interleaved, bool inverse) {
+                               const at::Tensor& sin, const OptTensor& positions, bool interleaved, bool inverse,
+                               const OptTensor& axes) {
     at::AutoDispatchBelowADInplaceOrView below;
     const at::Tensor pos = positions.value_or(at::Tensor()), kt = k.value_or(at::Tensor());
+    if (axes.has_value()) ctx->saved_data["axes"] = *axes;
     ctx->save_for_backward({cos, sin, pos});
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["inverse"] = inverse;
-    return outputs_of(rope_call(q, kt, cos, sin, pos, interleaved, inverse));
+    return outputs_of(rope_call(q, kt, cos, sin, pos, interleaved, inverse, axes.value_or(at::Tensor())));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_tangents(grads);
@@ -331,20 +357,23 @@ struct RopeNode : public torch::autograd::Function<RopeNode> {
     if (grads.size() > 1) dk = dense_heads(grads[1]);
     if (saved[2].defined()) pos = saved[2];
     const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
+    const at::Tensor axes = saved_axes(ctx);
     const variable_list d =
         at::GradMode::is_enabled()
-            ? RopeNode::apply(dq, dk, saved[0], saved[1], pos, interleaved, inverse)
-            : outputs_of(rope_call(dq, dk.value_or(at::Tensor()), saved[0], saved[1], saved[2], interleaved, inverse));
+            ? RopeNode::apply(dq, dk, saved[0], saved[1], pos, interleaved, inverse,
+                              axes.defined() ? OptTensor(axes) : OptTensor())
+            : outputs_of(rope_call(dq, dk.value_or(at::Tensor()), saved[0], saved[1], saved[2], interleaved, inverse, axes));
     return {d[0], d.size() > 1 ? d[1] : at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
-            at::Tensor()};
+            at::Tensor(), at::Tensor()};
   }
 };
 
 struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k, const OptTensor& qw,
                                const OptTensor& kw, const at::Tensor& cos, const at::Tensor& sin,
-                               const OptTensor& positions, double eps, bool interleaved) {
+                               const OptTensor& positions, double eps, bool interleaved, const OptTensor& axes) {
     at::AutoDispatchBelowADInplaceOrView below;
+    if (axes.has_value()) ctx->saved_data["axes"] = *axes;
     const at::Tensor kt = k.value_or(at::Tensor()), qwt = qw.value_or(at::Tensor()), kwt = kw.value_or(at::Tensor()),
                      pos = positions.value_or(at::Tensor());
     ctx->save_for_backward({q, kt, qwt, kwt, cos, sin, pos});
@@ -352,7 +381,7 @@ struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["dqw"] = qwt.defined() && qwt.requires_grad();
     ctx->saved_data["dkw"] = kwt.defined() && kwt.requires_grad();
-    return outputs_of(qk_norm_call(q, kt, qwt, kwt, cos, sin, pos, eps, interleaved));
+    return outputs_of(qk_norm_call(q, kt, qwt, kwt, cos, sin, pos, eps, interleaved, axes.value_or(at::Tensor())));
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
@@ -370,7 +399,7 @@ struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
     const at::Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3], &cos = saved[4], &sin = saved[5];
     const c10::cuda::CUDAGuard guard(q.device());
     const auto st = at::cuda::getCurrentCUDAStream(q.device().index()).stream();
-    const HeadsCall h(q, k, cos, saved[6]);
+    const HeadsCall h(q, k, cos, saved[6], saved_axes(ctx));
     const at::Tensor gq = dense_heads(grads[0]), gk = k.defined() ? dense_heads(grads[1]) : at::Tensor();
     const at::Tensor dq = empty_heads(q), dk = empty_heads(k);
     at::Tensor dqw, dkw, ws;
@@ -379,15 +408,15 @@ struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
     if (dqw.defined() || dkw.defined()) ws = scratch(tfo_qk_norm_rope_backward_workspace_bytes(h.dim), q.device());
     const Strides3 qs = strides_of(q), gqs = strides_of(gq), ks = k.defined() ? strides_of(k) : Strides3{},
                    gks = k.defined() ? strides_of(gk) : Strides3{};
-    check(tfo_qk_norm_rope_backward(
+    check(tfo_qk_norm_rope_backward_axes(
               gq.data_ptr(), gqs.data(), ptr_or_null(gk), gks.data(), q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(),
               ptr_or_null(qw), ptr_or_null(kw), cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.size(0), h.pos_ptr(),
               h.pos_dtype, h.pos_sb, h.pos_ss, dq.data_ptr(), out_or_null(dk), out_or_null(dqw), out_or_null(dkw),
               h.batch, h.seq, h.q_heads, h.k_heads, h.dim, h.rot, ctx->saved_data["interleaved"].toBool(),
               ctx->saved_data["eps"].toDouble(), dtype_code(q.scalar_type()), weight_code(qw), weight_code(kw),
-              dtype_code(cos.scalar_type()), out_or_null(ws), ws.defined() ? static_cast<size_t>(ws.numel()) : 0, st),
+              dtype_code(cos.scalar_type()), out_or_null(ws), ws.defined() ? static_cast<size_t>(ws.numel()) : 0, h.axes(), st),
           "tfo_qk_norm_rope_backward");
-    return {dq, dk, dqw, dkw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    return {dq, dk, dqw, dkw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
@@ -400,42 +429,48 @@ py::object pair_of(const variable_list& out) {
 
 // fused_rope: (q, k or None) rotated, or None outside the common case.
 py::object rope(const at::Tensor& q, const OptTensor& k, const at::Tensor& cos, const at::Tensor& sin,
-                const OptTensor& positions, bool interleaved) {
-  if (!heads_common(q, k, cos, sin, positions)) return py::none();
+                const OptTensor& positions, bool interleaved, const OptTensor& axes) {
+  if (!heads_common(q, k, cos, sin, positions, axes)) return py::none();
   if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k)))
-    return pair_of(RopeNode::apply(q, k, cos, sin, positions, interleaved, false));
+    return pair_of(RopeNode::apply(q, k, cos, sin, positions, interleaved, false, axes));
   return pair_of(outputs_of(rope_call(q, k.value_or(at::Tensor()), cos, sin, positions.value_or(at::Tensor()),
-                                      interleaved, false)));
+                                      interleaved, false, axes.value_or(at::Tensor()))));
 }
 
 // fused_qk_norm_rope: (q, k or None) normed and rotated, or None outside the common case.
 py::object qk_norm_rope(const at::Tensor& q, const OptTensor& k, const OptTensor& qw, const OptTensor& kw,
                         const at::Tensor& cos, const at::Tensor& sin, const OptTensor& positions, double eps,
-                        bool interleaved) {
-  if (!heads_common(q, k, cos, sin, positions) || !weight_ok(qw, q) || (k.has_value() ? !weight_ok(kw, q) : kw.has_value()))
+                        bool interleaved, const OptTensor& axes) {
+  if (!heads_common(q, k, cos, sin, positions, axes) || !weight_ok(qw, q) || (k.has_value() ? !weight_ok(kw, q) : kw.has_value()))
     return py::none();
   if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k) || wants_grad(qw) || wants_grad(kw)))
-    return pair_of(QKNormRopeNode::apply(q, k, qw, kw, cos, sin, positions, eps, interleaved));
+    return pair_of(QKNormRopeNode::apply(q, k, qw, kw, cos, sin, positions, eps, interleaved, axes));
   return pair_of(outputs_of(qk_norm_call(q, k.value_or(at::Tensor()), qw.value_or(at::Tensor()),
                                          kw.value_or(at::Tensor()), cos, sin, positions.value_or(at::Tensor()), eps,
-                                         interleaved)));
+                                         interleaved, axes.value_or(at::Tensor()))));
 }
 
 // rope_tables of given positions: (cos, sin), or None outside the common case. turns: doubles in host memory.
-py::object rope_tables(const at::Tensor& positions, const at::Tensor& turns, double gain, int64_t out_code) {
+// With axes, positions is [axes, ...] and pair i takes that of axis axes[i].
+py::object rope_tables(const at::Tensor& positions, const at::Tensor& turns, double gain, int64_t out_code,
+                       const OptTensor& axes) {
   if (!positions.is_cuda() || !positions.is_contiguous() || pos_code(positions.scalar_type()) < 0) return py::none();
   if (!turns.is_cpu() || turns.scalar_type() != at::kDouble || !turns.is_contiguous()) return py::none();
   const c10::cuda::CUDAGuard guard(positions.device());
   const int64_t half = turns.numel();
-  std::vector<int64_t> shape(positions.sizes().begin(), positions.sizes().end());
+  if (axes.has_value() && (positions.dim() < 1 || !pair_axes_ok(*axes, half) || positions.size(0) != axis_count(*axes)))
+    return py::none();
+  std::vector<int64_t> shape(positions.sizes().begin() + (axes.has_value() ? 1 : 0), positions.sizes().end());
+  const int64_t rows = axes.has_value() ? positions.numel() / positions.size(0) : positions.numel();
+  const tfo_axes of = axes.has_value() ? tfo_axes{axis_count(*axes), rows, axes->data_ptr<uint8_t>()} : tfo_axes{};
   shape.push_back(2 * half);
   const auto type = out_code == TFO_DTYPE_F16 ? at::kHalf : out_code == TFO_DTYPE_BF16 ? at::kBFloat16 : at::kFloat;
   at::Tensor cos = fresh(shape, type, positions.device());
   at::Tensor sin = fresh(shape, type, positions.device());
-  check(tfo_rope_tables(positions.data_ptr(), pos_code(positions.scalar_type()), positions.numel(),
-                        turns.data_ptr<double>(), half, gain, cos.data_ptr(), sin.data_ptr(),
-                        static_cast<int>(out_code),
-                        at::cuda::getCurrentCUDAStream(positions.device().index()).stream()),
+  check(tfo_rope_tables_axes(positions.data_ptr(), pos_code(positions.scalar_type()), rows,
+                             turns.data_ptr<double>(), half, gain, cos.data_ptr(), sin.data_ptr(),
+                             static_cast<int>(out_code), axes.has_value() ? &of : nullptr,
+                             at::cuda::getCurrentCUDAStream(positions.device().index()).stream()),
         "tfo_rope_tables");
   return py::make_tuple(cos, sin);
 }
@@ -728,9 +763,13 @@ PYBIND11_MODULE(_tfo_ext, m) {
   m.doc() = "PyTorch entry points over the tfo_b200 C ABI for launch-latency-bound calls";
   m.def("quantize_dynamic", &quantize_dynamic, "dynamic-scale quantize (codes, scale) or None");
   m.def("linear_prepared", &linear_prepared, "FP8Linear forward with a prepared weight, or None");
-  m.def("rope", &rope, "fused_rope, or None");
-  m.def("qk_norm_rope", &qk_norm_rope, "fused_qk_norm_rope, or None");
-  m.def("rope_tables", &rope_tables, "rope_tables of given positions, or None");
+  m.def("rope", &rope, "fused_rope, or None", py::arg("q"), py::arg("k"), py::arg("cos"), py::arg("sin"),
+        py::arg("positions"), py::arg("interleaved"), py::arg("axes") = py::none());
+  m.def("qk_norm_rope", &qk_norm_rope, "fused_qk_norm_rope, or None", py::arg("q"), py::arg("k"), py::arg("q_weight"),
+        py::arg("k_weight"), py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("eps"), py::arg("interleaved"),
+        py::arg("axes") = py::none());
+  m.def("rope_tables", &rope_tables, "rope_tables of given positions, or None", py::arg("positions"), py::arg("turns"),
+        py::arg("gain"), py::arg("out_code"), py::arg("axes") = py::none());
   m.def("lora", &lora, "fused_lora on 2-D operands, or None");
   m.def("dropout", &dropout, "fused_dropout, or None");
   m.def("residual_rmsnorm", &residual_rmsnorm, "fused_residual_rmsnorm, or None");

@@ -5,7 +5,7 @@ Ops (each one launches hand-written sm_100a CUDA kernels through the C ABI in
 
 * ``fused_rmsnorm_rope`` / ``FusedRMSNormRoPE``
 * ``fused_gated_mlp`` / ``FusedGatedMLP``
-* ``rope_tables`` / ``RoPEScaling``, ``fused_rope``
+* ``rope_tables`` / ``RoPEScaling`` / ``RoPEAxes``, ``fused_rope``
 * ``fused_qk_norm_rope`` / ``FusedQKNormRoPE``
 * ``fused_residual_rmsnorm`` / ``FusedResidualRMSNorm``
 * ``fused_dropout`` / ``FusedDropout``
@@ -50,7 +50,7 @@ from triton_ops.kernels.lora import FP8LoRALinear, fused_lora
 from triton_ops.kernels.qk_norm_rope import FusedQKNormRoPE, fused_qk_norm_rope
 from triton_ops.kernels.residual import FusedResidualRMSNorm, fused_residual_rmsnorm
 from triton_ops.kernels.rmsnorm_rope import FusedRMSNormRoPE, fused_rmsnorm_rope, fused_rmsnorm_rope_quantize
-from triton_ops.kernels.rope import RoPEScaling, fused_rope, rope_tables
+from triton_ops.kernels.rope import RoPEAxes, RoPEScaling, fused_rope, rope_tables
 from triton_ops.models import (
     FP8Format,
     FP8GEMMInput,
@@ -67,6 +67,7 @@ __all__ = [
     "FusedRMSNormRoPE",
     "rope_tables",
     "RoPEScaling",
+    "RoPEAxes",
     "fused_rope",
     "fused_qk_norm_rope",
     "FusedQKNormRoPE",

@@ -71,6 +71,13 @@ class RowParam(ctypes.Structure):
     _fields_ = [("data", _c_vp), ("seq_stride", _c_i64), ("dtype", _c_int), ("grad", _c_vp)]
 
 
+class Axes(ctypes.Structure):
+    """tfo_axes."""
+
+    _fields_ = [("axes", _c_int), ("pos_stride", _c_i64), ("axis_of_pair", _c_vp)]
+
+
+_c_axes = ctypes.POINTER(Axes)
 _c_dropout = ctypes.POINTER(DropoutParams)
 _c_row_params = ctypes.POINTER(RowParam)
 
@@ -179,6 +186,11 @@ _SIGNATURES = {
         [_c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_vp, _c_size, _c_vp],
     ),
 }
+
+# the calls with positions of several axes take one more argument, before the stream
+for _name in ("tfo_rope_tables", "tfo_rope", "tfo_qk_norm_rope", "tfo_qk_norm_rope_backward"):
+    _res, _args = _SIGNATURES[_name]
+    _SIGNATURES[_name + "_axes"] = (_res, [*_args[:-1], _c_axes, _args[-1]])
 
 _lib = None
 _lock = threading.Lock()

@@ -30,6 +30,7 @@ from triton_ops.kernels.rmsnorm_rope import (
     rope_kernel,
 )
 from triton_ops.kernels.rope import (
+    RoPEAxes,
     RoPEScaling,
     fused_rope,
     fused_rope_kernel,
@@ -45,6 +46,7 @@ __all__ = [
     "fused_rmsnorm_rope_kernel",
     "rope_tables",
     "RoPEScaling",
+    "RoPEAxes",
     "fused_rope",
     "rope_tables_kernel",
     "fused_rope_kernel",

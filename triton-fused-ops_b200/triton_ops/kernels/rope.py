@@ -91,9 +91,73 @@ class RoPEScaling(_Scaling):
         return cls(*values)
 
 
+class _Axes(NamedTuple):
+    sections: Tuple[int, ...]
+    order: str
+    spectrum: str
+
+
+class RoPEAxes(_Axes):
+    """Which pairs of columns turn by which of a token's positions (time, height and width, say).
+
+    Args:
+        sections: pairs of columns of each axis, 2 to 4 axes; their sum is
+            rotary_dim / 2
+        order: "blocks": the first section's pairs come first, then the second's;
+            "cycle": the axes take turns, and one whose pairs are used up is passed
+            over
+        spectrum: "shared": pair i has the frequency that it has with one
+            position; "own": an axis has the frequencies of a rotary_dim of twice
+            its section, in its pairs' order (and the scaling of one)
+    """
+
+    __slots__ = ()
+
+    def __new__(cls, sections, order: str = "blocks", spectrum: str = "shared"):
+        sections = tuple(int(n) for n in sections)
+        if not 2 <= len(sections) <= 4 or min(sections) < 1:
+            raise ValueError(f"need 2 to 4 sections of at least one pair, got {sections}")
+        if order not in ("blocks", "cycle"):
+            raise ValueError(f"order must be 'blocks' or 'cycle', got '{order}'")
+        if spectrum not in ("shared", "own"):
+            raise ValueError(f"spectrum must be 'shared' or 'own', got '{spectrum}'")
+        return _Axes.__new__(cls, sections, order, spectrum)
+
+    @classmethod
+    def _make(cls, values):
+        """Checked too, so that ``_replace`` is."""
+        return cls(*values)
+
+    def axis_of_pairs(self) -> Tuple[int, ...]:
+        """The axis of each pair of columns."""
+        turns = [(k if self.order == "cycle" else 0, axis) for axis, n in enumerate(self.sections) for k in range(n)]
+        return tuple(axis for _, axis in sorted(turns))
+
+
 @lru_cache(maxsize=64)
-def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[RoPEScaling] = None) -> Tuple[tuple, float]:
+def _pair_axes(axes: RoPEAxes) -> torch.Tensor:
+    """The axis of each pair in host memory, as the library reads it."""
+    return torch.tensor(axes.axis_of_pairs(), dtype=torch.uint8, device="cpu")
+
+
+def _check_axes(axes: RoPEAxes, rotary_dim: int) -> None:
+    if not isinstance(axes, RoPEAxes):
+        raise TypeError(f"axes must be RoPEAxes, got {type(axes).__name__}")
+    if 2 * sum(axes.sections) != rotary_dim:
+        raise ShapeMismatchError(f"the sections {axes.sections} make {2 * sum(axes.sections)} columns, the tables have {rotary_dim}",
+                                 tensor_name="cos")
+
+
+@lru_cache(maxsize=64)
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[RoPEScaling] = None,
+                     axes: Optional[RoPEAxes] = None) -> Tuple[tuple, float]:
     """(angle per position of each pair, factor on cos and sin), in double precision on the host."""
+    if axes is not None:
+        _check_axes(axes, rotary_dim)
+        if axes.spectrum == "own":
+            own = [rope_frequencies(2 * n, base, scaling) for n in axes.sections]
+            left = [iter(freq) for freq, _ in own]
+            return tuple(next(left[a]) for a in axes.axis_of_pairs()), own[0][1]
     if rotary_dim < 2 or rotary_dim % 2 != 0 or rotary_dim > 512:
         raise ShapeMismatchError(f"rotary_dim must be even and in 2..512, got {rotary_dim}")
     if not (base > 1 and math.isfinite(base)):
@@ -129,10 +193,10 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[R
 
 
 @lru_cache(maxsize=64)
-def _turns(rotary_dim: int, base: float, scaling: Optional[RoPEScaling]):
+def _turns(rotary_dim: int, base: float, scaling: Optional[RoPEScaling], axes: Optional[RoPEAxes] = None):
     """The frequencies as host arrays of turns per position (what the kernel takes; torch's default device may be another
     one), and the gain."""
-    freq, gain = rope_frequencies(rotary_dim, base, scaling)
+    freq, gain = rope_frequencies(rotary_dim, base, scaling, axes)
     values = [f / (2 * math.pi) for f in freq]
     return (ctypes.c_double * len(values))(*values), torch.tensor(values, dtype=torch.float64, device="cpu"), gain
 
@@ -143,6 +207,7 @@ def rope_tables(
     base: float = 10000.0,
     scaling: Optional[RoPEScaling] = None,
     *,
+    axes: Optional[RoPEAxes] = None,
     dtype: torch.dtype = torch.float32,
     device: Optional[torch.device] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -155,23 +220,33 @@ def rope_tables(
         rotary_dim: columns that are rotated (even, at most 512)
         base: of the frequencies ``base^(-2i / rotary_dim)``
         scaling: :class:`RoPEScaling` for a longer context, or None
+        axes: :class:`RoPEAxes` for positions of several axes, or None. A count then
+            makes the table from which :func:`fused_rope` takes each pair's row;
+            a tensor [axes, ...] of positions makes whole rows, each pair at the
+            position of its axis (used like those of one position)
         dtype: float16, bfloat16 or float32
         device: where the rows are made if `positions` is a count (default: the
             current CUDA device)
 
     Returns:
-        (cos, sin), each [n, rotary_dim] or [*positions.shape, rotary_dim]; the
-        two halves of a row are equal.
+        (cos, sin), each [n, rotary_dim] or [*positions.shape, rotary_dim] (with
+        axes without the first dimension); the two halves of a row are equal.
     """
     if dtype not in SUPPORTED_DTYPES_FLOAT:
         raise UnsupportedDtypeError(f"tables must be float16, bfloat16 or float32, got {dtype}", dtype=dtype,
                                     supported_dtypes=list(SUPPORTED_DTYPES_FLOAT))
-    turns, turns_t, gain = _turns(int(rotary_dim), float(base), scaling)
+    turns, turns_t, gain = _turns(int(rotary_dim), float(base), scaling, axes)
+    pair_axes = None
     if isinstance(positions, torch.Tensor):
+        if axes is not None:
+            if positions.dim() < 1 or positions.shape[0] != len(axes.sections):
+                raise ShapeMismatchError(f"positions must be [{len(axes.sections)}, ...], got {tuple(positions.shape)}",
+                                         actual=positions.shape, tensor_name="positions")
+            pair_axes = _pair_axes(axes)
         fast = _lib.ext()
         if fast is not None:
             try:
-                out = fast.rope_tables(positions, turns_t, gain, _lib.dtype_code(dtype))
+                out = fast.rope_tables(positions, turns_t, gain, _lib.dtype_code(dtype), pair_axes)
             except RuntimeError as exc:
                 _lib.raise_ext_error(exc)
             if out is not None:
@@ -183,7 +258,7 @@ def rope_tables(
             raise UnsupportedDtypeError(f"positions must be int32 or int64, got {positions.dtype}",
                                         dtype=positions.dtype, supported_dtypes=list(_POS_CODE), tensor_name="positions")
         positions = positions.contiguous()
-        shape, dev, at, code = (*positions.shape, rotary_dim), positions.device, positions.data_ptr(), _POS_CODE[positions.dtype]
+        shape, dev, at, code = (*positions.shape[axes is not None:], rotary_dim), positions.device, positions.data_ptr(), _POS_CODE[positions.dtype]
     else:
         if positions < 0:
             raise ShapeMismatchError(f"the number of positions must not be negative, got {positions}")
@@ -195,8 +270,9 @@ def rope_tables(
     cos = torch.empty(shape, dtype=dtype, device=dev)
     sin = torch.empty(shape, dtype=dtype, device=dev)
     with _lib.on_device(cos):
-        _lib.call("tfo_rope_tables", at, code, cos.numel() // rotary_dim, turns, rotary_dim // 2, gain, cos.data_ptr(),
-                  sin.data_ptr(), _lib.dtype_code(dtype), _lib.stream_of(cos))
+        rows = cos.numel() // rotary_dim
+        _lib.call("tfo_rope_tables_axes", at, code, rows, turns, rotary_dim // 2, gain, cos.data_ptr(), sin.data_ptr(),
+                  _lib.dtype_code(dtype), _axes_arg(pair_axes, rows), _lib.stream_of(cos))
     return cos, sin
 
 
@@ -208,11 +284,22 @@ def _strides(t: Optional[torch.Tensor]):
     return (ctypes.c_int64 * 3)(*(s[:3] if t.dim() == 4 else (0, s[0], s[1])))
 
 
+def _axes_arg(pair_axes: Optional[torch.Tensor], pos_stride: int):
+    """The C ABI's axes: NULL for one position."""
+    if pair_axes is None:
+        return None
+    return ctypes.byref(_lib.Axes(int(pair_axes.max()) + 1, pos_stride, pair_axes.data_ptr()))
+
+
+def _heads_axes(pair_axes, positions):
+    return _axes_arg(pair_axes, 0 if pair_axes is None else positions.stride(0))
+
+
 def _table_args(cos, sin, positions, q):
     if positions is None:
         pos = (None, _lib.POS_NONE, 0, 0)
     else:
-        s = positions.stride()
+        s = positions.stride()[positions.dim() - q.dim() + 2:]  # of the axes' positions: of one
         pos = (positions.data_ptr(), _POS_CODE[positions.dtype], *(s if q.dim() == 4 else (0, s[0])))
     return (cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], *pos)
 
@@ -226,13 +313,14 @@ def _empty_like_heads(t):
     return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _rotate(q, k, cos, sin, positions, interleaved, inverse):
+def _rotate(q, k, cos, sin, positions, interleaved, inverse, pair_axes=None):
     """Launches tfo_rope on checked arguments."""
     q_out, k_out = _empty_like_heads(q), _empty_like_heads(k)
     with _lib.on_device(q):
-        _lib.call("tfo_rope", q.data_ptr(), _strides(q), _lib.ptr(k), _strides(k), *_table_args(cos, sin, positions, q),
+        _lib.call("tfo_rope_axes", q.data_ptr(), _strides(q), _lib.ptr(k), _strides(k), *_table_args(cos, sin, positions, q),
                   q_out.data_ptr(), _lib.ptr(k_out), *_size_args(q, k, cos, interleaved), int(inverse),
-                  _lib.dtype_code(q.dtype, "q"), _lib.dtype_code(cos.dtype, "cos"), _lib.stream_of(q))
+                  _lib.dtype_code(q.dtype, "q"), _lib.dtype_code(cos.dtype, "cos"), _heads_axes(pair_axes, positions),
+                  _lib.stream_of(q))
     return q_out, k_out
 
 
@@ -244,10 +332,10 @@ class _FusedRoPE(torch.autograd.Function):
     """fused_rope where a gradient is wanted: the gradient is the rotation by the opposite angle."""
 
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse):
+    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse, pair_axes=None):
         ctx.save_for_backward(cos, sin, positions)
-        ctx.interleaved, ctx.inverse, ctx.with_k = interleaved, inverse, k is not None
-        q_out, k_out = _rotate(q, k, cos, sin, positions, interleaved, inverse)
+        ctx.interleaved, ctx.inverse, ctx.with_k, ctx.pair_axes = interleaved, inverse, k is not None, pair_axes
+        q_out, k_out = _rotate(q, k, cos, sin, positions, interleaved, inverse, pair_axes)
         return (q_out, k_out) if k is not None else q_out
 
     @staticmethod
@@ -255,9 +343,19 @@ class _FusedRoPE(torch.autograd.Function):
         cos, sin, positions = ctx.saved_tensors
         refuse_tangents(dq, dk)
         dq, dk = _dense_heads(dq), _dense_heads(dk if ctx.with_k else None)
-        out = _FusedRoPE.apply(dq, dk, cos, sin, positions, ctx.interleaved, not ctx.inverse)
+        out = _FusedRoPE.apply(dq, dk, cos, sin, positions, ctx.interleaved, not ctx.inverse, ctx.pair_axes)
         dq, dk = out if ctx.with_k else (out, None)
-        return dq, dk, None, None, None, None, None
+        return dq, dk, None, None, None, None, None, None
+
+
+def heads_pair_axes(axes: Optional[RoPEAxes], cos: torch.Tensor, positions: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """The axis of each pair for the rotation of heads, checked against the tables; None for one position."""
+    if axes is None:
+        return None
+    _check_axes(axes, cos.shape[-1] if cos.dim() else 0)
+    if positions is None:
+        raise ValueError("axes needs positions")
+    return _pair_axes(axes)
 
 
 def fused_rope(
@@ -268,6 +366,7 @@ def fused_rope(
     positions: Optional[torch.Tensor] = None,
     *,
     interleaved: bool = False,
+    axes: Optional[RoPEAxes] = None,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Rotates query and key heads by their tokens' table rows, in one launch.
 
@@ -285,24 +384,29 @@ def fused_rope(
             columns and sets ``_lib.ERR_BAD_POSITION`` in the device error word
         interleaved: False pairs column i with i + rotary_dim / 2, True pairs 2i
             with 2i + 1
+        axes: :class:`RoPEAxes` where a token has several positions, or None.
+            positions (needed then) is [axes, batch, seq_len] (or [axes, tokens]),
+            and pair i turns by the table row at the position of its axis; a bad
+            position gives NaN in its axis' columns
 
     Returns:
         (rotated q, rotated k or None), contiguous. Differentiable in q and k, in
         reverse mode (a tensor with a forward-mode tangent is refused).
     """
+    pair_axes = heads_pair_axes(axes, cos, positions)
     fast = _lib.ext()
     if fast is not None:
         try:
-            out = fast.rope(q, k, cos, sin, positions, interleaved)
+            out = fast.rope(q, k, cos, sin, positions, interleaved, pair_axes)
         except RuntimeError as exc:
             _lib.raise_ext_error(exc)
         if out is not None:
             return out
-    cos, sin, positions = validate_rope_heads(q, k, cos, sin, positions)
+    cos, sin, positions = validate_rope_heads(q, k, cos, sin, positions, axes and len(axes.sections))
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        out = _FusedRoPE.apply(q, k, cos, sin, positions, interleaved, False)
+        out = _FusedRoPE.apply(q, k, cos, sin, positions, interleaved, False, pair_axes)
         return out if k is not None else (out, None)
-    return _rotate(q, k, cos, sin, positions, interleaved, False)
+    return _rotate(q, k, cos, sin, positions, interleaved, False, pair_axes)
 
 
 def rope_heads_reference(
@@ -311,12 +415,17 @@ def rope_heads_reference(
     sin: torch.Tensor,
     positions: Optional[torch.Tensor] = None,
     interleaved: bool = False,
+    axes: Optional[RoPEAxes] = None,
 ) -> torch.Tensor:
     """PyTorch restatement of the rotation of one tensor, in x's precision (at least fp32)."""
     rot = cos.shape[-1]
     wide = x if x.dtype == torch.float64 else x.float()
     at = torch.arange(x.shape[-3], device=x.device) if positions is None else positions.long()
-    c, s = (t[at][..., None, : rot // 2].to(wide.dtype) for t in (cos, sin))
+    if axes is None:
+        c, s = (t[at][..., None, : rot // 2].to(wide.dtype) for t in (cos, sin))
+    else:
+        c, s = (torch.stack([t[at[a], i] for i, a in enumerate(axes.axis_of_pairs())], -1)[..., None, :].to(wide.dtype)
+                for t in (cos, sin))
     u, v = (wide[..., 0:rot:2], wide[..., 1:rot:2]) if interleaved else (wide[..., : rot // 2], wide[..., rot // 2:rot])
     y = (u * c - v * s, u * s + v * c)
     y = torch.stack(y, dim=-1).flatten(-2) if interleaved else torch.cat(y, dim=-1)

@@ -318,11 +318,13 @@ def validate_rope_heads(
     cos: torch.Tensor,
     sin: torch.Tensor,
     positions: Optional[torch.Tensor],
+    axes: Optional[int] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
     """Checks query/key heads with their rotary tables and positions.
 
     Returns (cos, sin, positions) with 2-D tables of stride 1 and positions
-    (int32 or int64, or None) expanded to q's token dimensions.
+    (int32 or int64, or None) expanded to q's token dimensions (after one for the
+    axes where a token has `axes` positions).
     """
     _check_heads(q, "q")
     if k is not None:
@@ -355,12 +357,20 @@ def validate_rope_heads(
     _check_cuda(positions, "positions")
     _check_dtype(positions, "positions", [torch.int32, torch.int64])
     _check_same_device(q, positions, "positions")
+    tokens = tuple(q.shape[:-2]) if axes is None else (axes, *q.shape[:-2])
+    if axes is not None and (positions.dim() < 1 or positions.shape[0] != axes):
+        raise ShapeMismatchError(
+            f"positions of {axes} axes must be {tokens}, got {tuple(positions.shape)}", expected=tokens,
+            actual=positions.shape, tensor_name="positions",
+        )
     try:
-        positions = positions.expand(q.shape[:-2])
+        if axes is not None:  # dimensions that are left out lie behind the axes
+            positions = positions.view(axes, *(1,) * (len(tokens) - positions.dim()), *positions.shape[1:])
+        positions = positions.expand(tokens)
     except RuntimeError:
         raise ShapeMismatchError(
-            f"positions shape {tuple(positions.shape)} doesn't fit the tokens {tuple(q.shape[:-2])}",
-            expected=tuple(q.shape[:-2]), actual=positions.shape, tensor_name="positions",
+            f"positions shape {tuple(positions.shape)} doesn't fit the tokens {tokens}",
+            expected=tokens, actual=positions.shape, tensor_name="positions",
         ) from None
     if cos.shape[0] == 0 and positions.numel():
         raise ShapeMismatchError("the tables have no rows", actual=cos.shape, tensor_name="cos")
