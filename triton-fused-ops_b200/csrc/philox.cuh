@@ -38,24 +38,28 @@ struct DropKey {
     }
     return make_uint4(a, b, c, d);
   }
+  // bits * 2 + (whether an element with this word is kept); the threshold is not 0.
+  __device__ uint32_t push(uint32_t bits, uint32_t word) const {
+    // the carry of word - threshold, shifted in
+    asm("{\n\t.reg .u32 t;\n\tadd.cc.u32 t, %1, %2;\n\taddc.u32 %0, %0, %0;\n\t}" : "+r"(bits) : "r"(word), "r"(0u - threshold));
+    return bits;
+  }
   // Bit j: element first + j is kept. `first` is a multiple of 4 if N is.
   template <int N> __device__ uint32_t kept(uint64_t first) const {
     uint32_t bits = 0;
     if constexpr (N % 4 == 0) {
 #pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
+      for (int i = N / 4 - 1; i >= 0; --i) {
         const uint4 w = block(first / 4 + i);
-        bits |= (w.x >= threshold ? 1u : 0u) << (4 * i) | (w.y >= threshold ? 2u : 0u) << (4 * i) |
-                (w.z >= threshold ? 4u : 0u) << (4 * i) | (w.w >= threshold ? 8u : 0u) << (4 * i);
+        bits = push(push(push(push(bits, w.w), w.z), w.y), w.x);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
+      for (int j = N - 1; j >= 0; --j) {
         const uint64_t i = first + j;
         const uint4 w = block(i / 4);
         const uint32_t at = static_cast<uint32_t>(i) & 3u;
-        const uint32_t v = at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w;
-        bits |= (v >= threshold ? 1u : 0u) << j;
+        bits = push(bits, at == 0 ? w.x : at == 1 ? w.y : at == 2 ? w.z : w.w);
       }
     }
     return bits;

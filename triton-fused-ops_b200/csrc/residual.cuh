@@ -2,8 +2,8 @@
 // residual_norm_backward.cu): how a row is spread over threads, the stream of
 // rows through shared memory, sums over a row, and the parameters' columns.
 //
-// A row of `hidden` columns is chunks of E columns (16 bytes of x, or one
-// column where rows are not whole aligned 16-byte vectors). T threads (whole
+// A row of `hidden` columns is chunks of E columns (16 bytes of the wider of x
+// and the stream, or one column where rows are not whole aligned vectors). T threads (whole
 // warps) take a row, thread t its chunks t, t + T, ... (V of them): a group.
 // A CTA holds several groups when rows are short, each with rows of its own
 // and a named barrier for its sums.
@@ -27,67 +27,68 @@ struct RowPlan {
 // Sums over a group's threads, the same bits in each. `red`: this group's
 // kMaxRowWarps * N floats, the parts of warps that are not there zero; two
 // sums in a row must use different ones.
-template <int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float* red, int warps, int warp, int barrier) {
+//
+// One value: a tree of shuffles, the warps' parts through shared memory, a tree
+// again over as many lanes. Four values: each step of the tree also halves how
+// many of them a lane carries, so that all four take 6 shuffles instead of 20
+// and end in 8 lanes each (as after a reading of the parts), then one shuffle a value.
+__device__ __forceinline__ float lanes_sum(float v, int from) {  // over the lanes that differ in bits below `from` * 2
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    float w[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) w[j] = __shfl_xor_sync(0xffffffffu, v[j], o);
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] += w[j];
-  }
+  for (int o = 16; o > 0; o >>= 1)
+    if (o <= from) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ void row_sum(float (&v)[1], float* red, int warps, int warp, int barrier) {
+  v[0] = lanes_sum(v[0], 16);
   if (warps == 1) return;
-  if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) red[j * kMaxRowWarps + warp] = v[j];
-  }
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) red[warp] = v[0];
   asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    float4 s = *reinterpret_cast<const float4*>(red + j * kMaxRowWarps);
-#pragma unroll
-    for (int i = 4; i < kMaxRowWarps; i += 4) {
-      const float4 p = *reinterpret_cast<const float4*>(red + j * kMaxRowWarps + i);
-      s.x += p.x, s.y += p.y, s.z += p.z, s.w += p.w;
-    }
-    v[j] = (s.x + s.y) + (s.z + s.w);
+  if (warps > 8) v[0] = lanes_sum(red[lane & 15], 8);
+  else if (warps > 4) v[0] = lanes_sum(red[lane & 7], 4);
+  else v[0] = lanes_sum(red[lane & 3], 2);
+}
+__device__ __forceinline__ void row_sum(float (&v)[4], float* red, int warps, int warp, int barrier) {
+  const int lane = threadIdx.x & 31;
+  const bool up = lane & 16, right = lane & 8;
+  float a = up ? v[2] : v[0], b = up ? v[3] : v[1];
+  a += __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16);
+  b += __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16);
+  float mine = right ? b : a;
+  mine += __shfl_xor_sync(0xffffffffu, right ? a : b, 8);
+  mine = lanes_sum(mine, 4);  // of value lane / 8
+  if (warps > 1) {
+    if ((lane & 7) == 0) red[(lane >> 3) * kMaxRowWarps + warp] = mine;
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(warps * 32) : "memory");
+    const float2 p = *reinterpret_cast<const float2*>(red + (lane >> 3) * kMaxRowWarps + (lane & 7) * 2);
+    mine = lanes_sum(p.x + p.y, 4);
   }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = __shfl_sync(0xffffffffu, mine, 8 * j);
 }
 
 // ---- chunks -----------------------------------------------------------------
-// E columns of T as pairs of floats at `f`, from and to memory (E == 1: half a pair).
+// E columns of T as pairs of floats at `f`, from and to memory in vectors of 16 or 8 bytes.
 template <typename T, int E> struct Chunk {
-  static constexpr int kVecs = E * static_cast<int>(sizeof(T)) / 16;  // 16-byte vectors
-  static_assert(E % (16 / static_cast<int>(sizeof(T))) == 0, "whole vectors");
-  __device__ static void unpack(const uint4 (&r)[kVecs], F2* f) {
+  static constexpr int kBytes = E * static_cast<int>(sizeof(T));
+  static constexpr int kVecBytes = kBytes < 16 ? 8 : 16;
+  static constexpr int kVecs = kBytes / kVecBytes;
+  static_assert(kVecs * kVecBytes == kBytes, "whole vectors");
+  static constexpr int kVecCols = E / kVecs;
+  using Vec = HeadVec<T, kVecCols>;
+  __device__ static void unpack(const typename Vec::Raw& r, F2* f) {
+    F2 t[kVecCols / 2];
+    Vec::unpack(r, t);
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) {
-      const uint32_t w[4] = {r[v].x, r[v].y, r[v].z, r[v].w};
-      if constexpr (sizeof(T) == 4) {
-        f[2 * v] = f2(__uint_as_float(w[0]), __uint_as_float(w[1]));
-        f[2 * v + 1] = f2(__uint_as_float(w[2]), __uint_as_float(w[3]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 p = Pair16<T>::unpack(w[i]);
-          f[4 * v + i] = f2(p.x, p.y);
-        }
-      }
-    }
+    for (int i = 0; i < kVecCols / 2; ++i) f[i] = t[i];
   }
   __device__ static void store(T* p, const F2* f) {
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-      uint4 r;
-      if constexpr (sizeof(T) == 4) {
-        r = make_uint4(__float_as_uint(f[2 * v].x), __float_as_uint(f[2 * v].y), __float_as_uint(f[2 * v + 1].x),
-                       __float_as_uint(f[2 * v + 1].y));
-      } else {
-        r = make_uint4(Pair16<T>::pack(f[4 * v].x, f[4 * v].y), Pair16<T>::pack(f[4 * v + 1].x, f[4 * v + 1].y),
-                       Pair16<T>::pack(f[4 * v + 2].x, f[4 * v + 2].y), Pair16<T>::pack(f[4 * v + 3].x, f[4 * v + 3].y));
-      }
-      reinterpret_cast<uint4*>(p)[v] = r;
+      F2 t[kVecCols / 2];
+#pragma unroll
+      for (int i = 0; i < kVecCols / 2; ++i) t[i] = f[v * kVecCols / 2 + i];
+      Vec::store(p + v * kVecCols, t);
     }
   }
 };
@@ -129,8 +130,7 @@ template <int E, int V> struct RowCols {
     if (d.all) return 0u;
     uint32_t bits = 0;
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (has(k)) bits |= key.kept<E>(static_cast<uint64_t>(r * hidden + col(k))) << (k * E);
+    for (int k = 0; k < V; ++k) bits |= key.kept<E>(static_cast<uint64_t>(r * hidden + col(k))) << (k * E);
     return bits;
   }
   __device__ static void drop(uint32_t bits, F2 (&f)[P]) {
@@ -150,37 +150,39 @@ template <int E, int V> struct RowCols {
 template <typename TX, typename TR, int E, int V, int NX, int NR, int STAGES>
 struct RowStream {
   static constexpr int kTensors = NX + NR;
-  static constexpr int kVecsX = E == 1 ? 0 : Chunk<TX, E == 1 ? 16 : E>::kVecs;
-  static constexpr int kVecsR = E == 1 ? 0 : Chunk<TR, E == 1 ? 16 : E>::kVecs;
-  static constexpr int kVecsRow = V * (NX * kVecsX + NR * kVecsR);  // of a thread and row
-  static constexpr size_t smem_bytes(int threads) { return static_cast<size_t>(STAGES) * kVecsRow * threads * 16; }
+  using ChunkX = Chunk<TX, E == 1 ? 16 : E>;
+  using ChunkR = Chunk<TR, E == 1 ? 16 : E>;
+  static constexpr int kBytesX = V * ChunkX::kBytes, kBytesR = V * ChunkR::kBytes;  // of a thread and row
+  static constexpr int kRowBytes = E == 1 ? 0 : NX * kBytesX + NR * kBytesR;
+  static constexpr size_t smem_bytes(int threads) { return static_cast<size_t>(STAGES) * kRowBytes * threads; }
 
   const void* base[kTensors];  // NULL: zeros
   int64_t stride[kTensors];    // elements between rows
-  uint4* ring;                 // this thread's first slot
-  int slots;                   // threads of the CTA: distance of a thread's slots
+  uint32_t ring;               // shared memory
+  uint32_t stage_bytes;
   int64_t next, end;
   int load_stage, stage;
   float ahead[E == 1 ? kTensors * V : 1], now[E == 1 ? kTensors * V : 1];
 
-  __device__ uint4* slot(int st, int v) const { return ring + (st * kVecsRow + v) * slots; }
-  static __device__ constexpr int first_vec(int i) { return i < NX ? i * V * kVecsX : NX * V * kVecsX + (i - NX) * V * kVecsR; }
+  // Vector v of tensor i in a stage: the CTA's threads side by side.
+  template <int VEC_BYTES> __device__ uint32_t slot(int st, int i, int v) const {
+    const int before = (i < NX ? i * kBytesX : NX * kBytesX + (i - NX) * kBytesR) + v * VEC_BYTES;
+    return ring + st * stage_bytes + before * blockDim.x + threadIdx.x * VEC_BYTES;
+  }
 
-  __device__ void start(const RowCols<E, V>& cols, uint4* smem, int64_t r0, int64_t r1) {
+  __device__ void start(const RowCols<E, V>& cols, void* smem, int64_t r0, int64_t r1) {
     next = r0;
     end = r1;
     load_stage = 0;
     stage = STAGES - 1;
     if constexpr (E > 1) {
-      ring = smem + threadIdx.x;
-      slots = blockDim.x;
+      ring = smem_u32(smem);
+      stage_bytes = kRowBytes * blockDim.x;
       // what no copy ever fills stays zero
-      bool full = cols.has(V - 1);
 #pragma unroll
-      for (int i = 0; i < kTensors; ++i) full = full && base[i] != nullptr;
-      if (!full) {
-#pragma unroll 1
-        for (int i = 0; i < STAGES * kVecsRow; ++i) ring[i * slots] = make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < kTensors; ++i) {
+        if (i < NX) clear<ChunkX>(cols, i);
+        else clear<ChunkR>(cols, i);
       }
 #pragma unroll 1
       for (int i = 0; i < STAGES - 1; ++i) load(cols);
@@ -201,15 +203,18 @@ struct RowStream {
     }
   }
   template <int I> __device__ void get(F2 (&f)[RowCols<E, V>::P]) const {
-    using T = std::conditional_t<(I < NX), TX, TR>;
     if constexpr (E > 1) {
-      constexpr int n = Chunk<T, E>::kVecs;
+      using C = std::conditional_t<(I < NX), ChunkX, ChunkR>;
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        uint4 r[n];
-#pragma unroll
-        for (int v = 0; v < n; ++v) r[v] = *slot(stage, first_vec(I) + k * n + v);
-        Chunk<T, E>::unpack(r, f + k * E / 2);
+      for (int v = 0; v < V * C::kVecs; ++v) {
+        typename C::Vec::Raw r;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+        const uint32_t at = slot<C::kVecBytes>(stage, I, v);
+        if constexpr (C::kVecBytes == 16)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+        else
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+        C::unpack(r, f + v * C::kVecCols / 2);
       }
     } else {
 #pragma unroll
@@ -229,8 +234,8 @@ struct RowStream {
           }
           continue;
         }
-        if (i < NX) copy<TX, kVecsX>(cols, i);
-        else copy<TR, kVecsR>(cols, i);
+        if (i < NX) copy<TX, ChunkX>(cols, i);
+        else copy<TR, ChunkR>(cols, i);
       }
     }
     ++next;
@@ -239,7 +244,7 @@ struct RowStream {
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
   }
-  template <typename T, int VECS> __device__ void copy(const RowCols<E, V>& cols, int i) {
+  template <typename T, class C> __device__ void copy(const RowCols<E, V>& cols, int i) {
     const T* row = static_cast<const T*>(base[i]) + next * stride[i];
 #pragma unroll
     for (int k = 0; k < V; ++k) {
@@ -247,32 +252,59 @@ struct RowStream {
         ahead[i * V + k] = cols.has(k) ? Ty<T>::to_f(row[cols.col(k)]) : 0.f;
       } else if (cols.has(k)) {
 #pragma unroll
-        for (int v = 0; v < VECS; ++v)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                           smem_u32(slot(load_stage, first_vec(i) + k * VECS + v))),
-                       "l"(reinterpret_cast<const uint4*>(row + cols.col(k)) + v)
-                       : "memory");
+        for (int v = 0; v < C::kVecs; ++v) {
+          const uint32_t to = slot<C::kVecBytes>(load_stage, i, k * C::kVecs + v);
+          const T* from = row + cols.col(k) + v * C::kVecCols;
+          if constexpr (C::kVecBytes == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+          else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+        }
       }
+    }
+  }
+  template <class C> __device__ void clear(const RowCols<E, V>& cols, int i) {
+    if (cols.has(V - 1) && base[i] != nullptr) return;
+#pragma unroll 1
+    for (int v = 0; v < V * C::kVecs * STAGES; ++v) {
+      const uint32_t at = slot<C::kVecBytes>(v / (V * C::kVecs), i, v % (V * C::kVecs));
+      if constexpr (C::kVecBytes == 16)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+      else
+        asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(at), "r"(0u) : "memory");
     }
   }
 };
 
+// Rows ahead in shared memory: as many as a full CTA has room for, four at most.
+template <typename TX, typename TR> constexpr int row_stages(int cols, int nx, int nr) {
+  const int row = cols * (nx * static_cast<int>(sizeof(TX)) + nr * static_cast<int>(sizeof(TR))) * kRowThreads;
+  const int n = 208 * 1024 / row;
+  return n < 1 ? 1 : n > 4 ? 4 : n;
+}
+
 // ---- host: which rows are whole aligned vectors ------------------------------
 inline int row_elem_bytes(int dtype) { return dtype == F32 ? 4 : 2; }
-inline bool row_aligned(const void* p, int64_t stride, int64_t rows, int dtype) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (rows <= 1 || stride * row_elem_bytes(dtype) % 16 == 0);
-}
-// Columns of a chunk with which the vector kernels can take these rows: 16 bytes of x, or 1.
+// Columns of a vector chunk: 16 bytes of the wider type.
+template <typename TX, typename TR> constexpr int kRowChunk = 16 / (sizeof(TX) > sizeof(TR) ? sizeof(TX) : sizeof(TR));
+// Columns of a chunk with which the kernels can take these rows: kRowChunk, or 1.
 inline int row_chunk(const ResidualArgs& a, bool backward) {
-  const int e = 16 / row_elem_bytes(a.x_dtype);
+  const int e = 16 / std::max(row_elem_bytes(a.x_dtype), row_elem_bytes(a.res_dtype));
   bool ok = a.hidden % e == 0;
-  const int64_t h = a.hidden;
-  ok = ok && row_aligned(a.x, a.x_stride, a.rows, a.x_dtype) && row_aligned(a.res, a.res_stride, a.rows, a.res_dtype);
+  auto aligned = [&](const void* p, int64_t stride, int dtype) {
+    const int bytes = e * row_elem_bytes(dtype);
+    ok = ok && reinterpret_cast<uintptr_t>(p) % bytes == 0 && (a.rows <= 1 || stride * row_elem_bytes(dtype) % bytes == 0);
+  };
+  aligned(a.x, a.x_stride, a.x_dtype);
+  aligned(a.res, a.res_stride, a.res_dtype);
   if (backward) {
-    ok = ok && row_aligned(a.dy, a.dy_stride, a.rows, a.x_dtype) && row_aligned(a.dh, a.dh_stride, a.rows, a.res_dtype);
-    ok = ok && row_aligned(a.dx, h, a.rows, a.x_dtype) && row_aligned(a.dres, h, a.rows, a.res_dtype);
+    aligned(a.dy, a.dy_stride, a.x_dtype);
+    aligned(a.dh, a.dh_stride, a.res_dtype);
+    aligned(a.dx, a.hidden, a.x_dtype);
+    aligned(a.dres, a.hidden, a.res_dtype);
   } else {
-    ok = ok && row_aligned(a.h, h, a.rows, a.res_dtype) && row_aligned(a.y, h, a.rows, a.x_dtype);
+    aligned(a.h, a.hidden, a.res_dtype);
+    aligned(a.y, a.hidden, a.x_dtype);
   }
   for (const RowParam* p : {&a.branch_weight, &a.gate, &a.weight, &a.shift})
     ok = ok && (p->p == nullptr || (reinterpret_cast<uintptr_t>(p->p) % 16 == 0 &&

@@ -31,16 +31,16 @@ __device__ __forceinline__ void branch_coefficient(const ResidualArgs& a, const 
 }
 
 // Parameters stay in registers up to this many columns a thread; above it they are read again for every row.
-constexpr int kParamCols = 8;
+constexpr int kParamCols = 16;
 
 template <typename TX, typename TR, int E, int V, int STAGES>
-__global__ void __launch_bounds__(kRowThreads, E * V <= 8 ? 2 : 1)
+__global__ void __launch_bounds__(kRowThreads, 1)
     residual_norm_kernel(const __grid_constant__ ResidualArgs a, RowPlan plan) {
   using Cols = RowCols<E, V>;
   constexpr int P = Cols::P;
   constexpr bool KEEP_PARAMS = Cols::N <= kParamCols;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ __align__(16) float red[2][kMaxRowWarps][kMaxRowWarps];
+  __shared__ float red[2][kMaxRowWarps][kMaxRowWarps];
   griddep_launch_dependents();
   const int warps = plan.threads / 32;
   const int group = (threadIdx.x >> 5) / warps, warp = (threadIdx.x >> 5) - group * warps;
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kRowThreads, E * V <= 8 ? 2 : 1)
   rows.stride[0] = a.x_stride;
   rows.base[1] = a.res;
   rows.stride[1] = a.res_stride;
-  rows.start(cols, reinterpret_cast<uint4*>(smem), r0, r1);
+  rows.start(cols, smem, r0, r1);
   const DropKey key(a.drop);
   const float inv_h = 1.f / static_cast<float>(a.hidden);
   const int bar = 1 + group;
@@ -178,14 +178,15 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_any_kernel(const __
 }
 
 namespace {
-template <typename TX, typename TR, int E, int V, int STAGES>
+template <typename TX, typename TR, int E, int V>
 cudaError_t launch_rows(const ResidualArgs& a, int threads, cudaStream_t st) {
+  constexpr int STAGES = row_stages<TX, TR>(E * V, 1, 1);
   auto* kernel = residual_norm_kernel<TX, TR, E, V, STAGES>;
   using Stream = RowStream<TX, TR, E, V, 1, 1, STAGES>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   // as many groups a CTA as still leave every SM a row
-  const int groups = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>(std::min(kRowThreads, 32 * kMaxRowWarps) / threads, a.rows / num_sms())));
+  const int groups =
+      static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, a.rows / num_sms())));
   const int block = groups * threads;
   const size_t smem = Stream::smem_bytes(block);
   // the limit of the largest block: also below it the static part comes on top
@@ -198,14 +199,17 @@ cudaError_t launch_rows(const ResidualArgs& a, int threads, cudaStream_t st) {
 
 template <typename TX, typename TR>
 cudaError_t launch_types(const ResidualArgs& a, cudaStream_t st) {
-  constexpr int E = 16 / sizeof(TX);
+  constexpr int E = kRowChunk<TX, TR>;
   if (row_chunk(a, false) == E) {
-    if (const int t = row_threads(a.hidden, E, 1)) return launch_rows<TX, TR, E, 1, 4>(a, t, st);
-    if (const int t = row_threads(a.hidden, E, 2)) return launch_rows<TX, TR, E, 2, 3>(a, t, st);
-    if (const int t = row_threads(a.hidden, E, 4)) return launch_rows<TX, TR, E, 4, 2>(a, t, st);
+    // A warp a row as far as 16 columns a thread carry it, then 16 columns a thread.
+    constexpr int FULL = 16 / E;
+    if (a.hidden <= 32 * E) return launch_rows<TX, TR, E, 1>(a, 32, st);
+    if (FULL > 2 && a.hidden <= 64 * E) return launch_rows<TX, TR, E, 2>(a, 32, st);
+    if (const int t = row_threads(a.hidden, E, FULL)) return launch_rows<TX, TR, E, FULL>(a, t, st);
+    if (const int t = row_threads(a.hidden, E, 2 * FULL)) return launch_rows<TX, TR, E, 2 * FULL>(a, t, st);
   } else {
-    if (const int t = row_threads(a.hidden, 1, 4)) return launch_rows<TX, TR, 1, 4, 1>(a, t, st);
-    if (const int t = row_threads(a.hidden, 1, 8)) return launch_rows<TX, TR, 1, 8, 1>(a, t, st);
+    if (const int t = row_threads(a.hidden, 1, 4)) return launch_rows<TX, TR, 1, 4>(a, t, st);
+    if (const int t = row_threads(a.hidden, 1, 8)) return launch_rows<TX, TR, 1, 8>(a, t, st);
   }
   note_launch();
   return launch_dependent(residual_norm_any_kernel<TX, TR>, static_cast<int>(std::min<int64_t>(a.rows, num_sms() * 4ll)),

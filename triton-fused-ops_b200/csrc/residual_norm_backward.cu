@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   rows.stride[2] = a.res_stride;
   rows.base[3] = a.dh;
   rows.stride[3] = a.dh_stride;
-  rows.start(cols, reinterpret_cast<uint4*>(smem), r0, r1);
+  rows.start(cols, smem, r0, r1);
   const DropKey key(a.drop);
   const float inv_h = 1.f / static_cast<float>(a.hidden);
   const int bar = 1 + group;
@@ -331,10 +331,10 @@ struct Shape {
   int e, v, threads;  // v 0: any
 };
 Shape shape_of(const ResidualArgs& a) {
-  const int full = 16 / row_elem_bytes(a.x_dtype);
-  if (row_chunk(a, true) == full) {
-    for (int v = 1; v * full <= 16; v *= 2)
-      if (const int t = row_threads(a.hidden, full, v)) return {full, v, t};
+  const int e = row_chunk(a, true);
+  if (e > 1) {
+    for (int v = 8 / e; v * e <= 16; v *= 2)
+      if (const int t = row_threads(a.hidden, e, v)) return {e, v, t};
   } else {
     for (int v = 4; v <= 8; v *= 2)
       if (const int t = row_threads(a.hidden, 1, v)) return {1, v, t};
@@ -355,8 +355,9 @@ RowItems items_of(const ResidualArgs& a, int threads) {
   return it;
 }
 
-template <typename TX, typename TR, int E, int V, int STAGES>
+template <typename TX, typename TR, int E, int V>
 cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t st) {
+  constexpr int STAGES = row_stages<TX, TR>(E * V, 2, 2);
   auto* kernel = residual_norm_backward_kernel<TX, TR, E, V, STAGES>;
   using Stream = RowStream<TX, TR, E, V, 2, 2, STAGES>;
   const int threads = plan.rows.threads;
@@ -375,16 +376,14 @@ cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t 
 
 template <typename TX, typename TR>
 cudaError_t launch_types(const ResidualArgs& a, BackwardPlan& plan, const Shape& sh, cudaStream_t st) {
-  constexpr int E = 16 / sizeof(TX);
+  constexpr int E = kRowChunk<TX, TR>;
   if (sh.e == E) {
-    if (sh.v == 1) return launch_rows<TX, TR, E, 1, 4>(a, plan, st);
-    if (sh.v == 2) return launch_rows<TX, TR, E, 2, 2>(a, plan, st);
-    if constexpr (E == 4) {
-      if (sh.v == 4) return launch_rows<TX, TR, E, 4, 1>(a, plan, st);
-    }
+    constexpr int HALF = 8 / E;  // chunks of 8 columns
+    if (sh.v == HALF) return launch_rows<TX, TR, E, HALF>(a, plan, st);
+    if (sh.v == 2 * HALF) return launch_rows<TX, TR, E, 2 * HALF>(a, plan, st);
   } else {
-    if (sh.v == 4) return launch_rows<TX, TR, 1, 4, 1>(a, plan, st);
-    if (sh.v == 8) return launch_rows<TX, TR, 1, 8, 1>(a, plan, st);
+    if (sh.v == 4) return launch_rows<TX, TR, 1, 4>(a, plan, st);
+    if (sh.v == 8) return launch_rows<TX, TR, 1, 8>(a, plan, st);
   }
   note_launch();
   return launch_dependent(residual_norm_backward_any_kernel<TX, TR>,
