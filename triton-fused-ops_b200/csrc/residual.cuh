@@ -19,8 +19,10 @@ constexpr int kMaxRowWarps = 16;   // of a group
 
 // How a launch spreads the rows.
 struct RowPlan {
-  int threads;  // T
-  int groups;   // of a CTA
+  int threads;      // T
+  int groups;       // of a CTA
+  int64_t step[4];  // bytes between the rows of the streamed tensors
+  int present;      // a bit for each of them that is there (the others are zeros)
 };
 
 // ---- sums over a row --------------------------------------------------------
@@ -95,49 +97,63 @@ template <typename T, int E> struct Chunk {
 
 __device__ __forceinline__ float& lane_of(F2* f, int i) { return i & 1 ? f[i >> 1].y : f[i >> 1].x; }
 
-// Which columns this thread takes.
+// Which columns this thread takes, in blocks of up to 8 of them (whole chunks).
 template <int E, int V> struct RowCols {
-  static constexpr int N = E * V;        // columns
-  static constexpr int P = (N + 1) / 2;  // pairs of them
-  static_assert(E > 1 || V % 2 == 0, "whole pairs");
+  static constexpr int N = E * V;         // columns
+  static constexpr int B = N < 8 ? N : 8;  // of a block
+  static constexpr int BLOCKS = N / B;
+  static constexpr int BP = B / 2;  // pairs of a block
+  static_assert(B % 2 == 0 && B % E == 0 && N % B == 0, "whole pairs and chunks");
   int first, step, hidden;
   __device__ RowCols(int t, int threads, int h) : first(t * E), step(threads * E), hidden(h) {}
   __device__ int col(int k) const { return first + k * step; }
   __device__ bool has(int k) const { return col(k) < hidden; }
 
-  // p's columns of a sequence (otherwise: of a parameter that is not there, and past the row).
-  __device__ void param(const RowParam& p, int64_t seq, float otherwise, F2 (&f)[P]) const {
+  // Block b of p's columns of a sequence (otherwise: of a parameter that is not there, and past the row).
+  __device__ void param(const RowParam& p, int64_t seq, float otherwise, int b, F2 (&f)[BP]) const {
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
+    for (int k = 0; k < B / E; ++k) {
       float v[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) v[j] = otherwise;
-      if (p.p != nullptr && has(k)) load_floats<E>(p.p, seq * p.seq_stride + col(k), p.dtype, v);
+      const int at = b * (B / E) + k;
+      if (p.p != nullptr && has(at)) load_floats<E>(p.p, seq * p.seq_stride + col(at), p.dtype, v);
 #pragma unroll
       for (int j = 0; j < E; ++j) lane_of(f, k * E + j) = v[j];
     }
   }
-  template <typename T> __device__ void store(T* row, F2 (&f)[P]) const {
+  // scale * gate * w1 (* 1 / (1 - p)): what a normed branch is multiplied by.
+  __device__ void branch_coefficient(const ResidualArgs& a, int64_t seq, int b, F2 (&c)[BP]) const {
+    F2 g[BP];
+    param(a.branch_weight, seq, 1.f, b, c);
+    param(a.gate, seq, 1.f, b, g);
+    const float s = a.dropped ? a.scale * a.drop.scale : a.scale;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      if (!has(k)) continue;
-      if constexpr (E == 1) row[col(k)] = Ty<T>::from_f(lane_of(f, k));
-      else Chunk<T, E>::store(row + col(k), f + k * E / 2);
+    for (int j = 0; j < BP; ++j) c[j] = mul2(mul2(c[j], g[j]), f2(s, s));
+  }
+  // Block b to this thread's first column of a row.
+  template <typename T> __device__ void store(T* mine, int b, F2 (&f)[BP]) const {
+#pragma unroll
+    for (int k = 0; k < B / E; ++k) {
+      const int at = b * (B / E) + k;
+      if (!has(at)) continue;
+      if constexpr (E == 1) mine[at * step] = Ty<T>::from_f(lane_of(f, k));
+      else Chunk<T, E>::store(mine + at * step, f + k * E / 2);
     }
   }
-  // Which of this thread's columns of row r are kept.
-  __device__ uint32_t kept(const DropoutArgs& d, const DropKey& key, int64_t r) const {
+  // Which of this thread's columns are kept in the row whose first element has this index.
+  __device__ uint32_t kept(const DropoutArgs& d, const DropKey& key, uint64_t row) const {
     if (d.all) return 0u;
     uint32_t bits = 0;
 #pragma unroll
-    for (int k = 0; k < V; ++k) bits |= key.kept<E>(static_cast<uint64_t>(r * hidden + col(k))) << (k * E);
+    for (int k = 0; k < V; ++k) bits |= key.kept<E>(row + static_cast<uint32_t>(col(k))) << (k * E);
     return bits;
   }
-  __device__ static void drop(uint32_t bits, F2 (&f)[P]) {
+  __device__ static void drop(uint32_t bits, int b, F2 (&f)[BP]) {
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-      if (!(bits >> (2 * j) & 1)) f[j].x = 0.f;
-      if (!(bits >> (2 * j + 1) & 1)) f[j].y = 0.f;
+    for (int j = 0; j < BP; ++j) {
+      if (!(bits >> (b * B + 2 * j) & 1)) f[j].x = 0.f;
+      if (!(bits >> (b * B + 2 * j + 1) & 1)) f[j].y = 0.f;
     }
   }
 };
@@ -154,80 +170,88 @@ struct RowStream {
   using ChunkR = Chunk<TR, E == 1 ? 16 : E>;
   static constexpr int kBytesX = V * ChunkX::kBytes, kBytesR = V * ChunkR::kBytes;  // of a thread and row
   static constexpr int kRowBytes = E == 1 ? 0 : NX * kBytesX + NR * kBytesR;
-  static constexpr size_t smem_bytes(int threads) { return static_cast<size_t>(STAGES) * kRowBytes * threads; }
+  // Slots lie as for a full CTA, so that all but the stage of an address is known when this is compiled.
+  static constexpr uint32_t kStageBytes = kRowBytes * kRowThreads;
+  static constexpr size_t kSmemBytes = static_cast<size_t>(STAGES) * kStageBytes;
 
-  const void* base[kTensors];  // NULL: zeros
-  int64_t stride[kTensors];    // elements between rows
-  uint32_t ring;               // shared memory
-  uint32_t stage_bytes;
-  int64_t next, end;
-  int load_stage, stage;
+  const char* at[kTensors];  // this thread's first column of the next row to load
+  int left;                  // rows to load
+  uint32_t ring, write, read;  // shared memory: all stages, and the stages to fill and to read
   float ahead[E == 1 ? kTensors * V : 1], now[E == 1 ? kTensors * V : 1];
 
   // Vector v of tensor i in a stage: the CTA's threads side by side.
-  template <int VEC_BYTES> __device__ uint32_t slot(int st, int i, int v) const {
-    const int before = (i < NX ? i * kBytesX : NX * kBytesX + (i - NX) * kBytesR) + v * VEC_BYTES;
-    return ring + st * stage_bytes + before * blockDim.x + threadIdx.x * VEC_BYTES;
+  static __device__ constexpr uint32_t offset(int i, int v, int vec_bytes) {
+    return ((i < NX ? i * kBytesX : NX * kBytesX + (i - NX) * kBytesR) + v * vec_bytes) * kRowThreads;
   }
 
-  __device__ void start(const RowCols<E, V>& cols, void* smem, int64_t r0, int64_t r1) {
-    next = r0;
-    end = r1;
-    load_stage = 0;
-    stage = STAGES - 1;
+  template <typename T> __device__ void set(int i, const void* base, int64_t row, int64_t step, const RowCols<E, V>& cols) {
+    at[i] = static_cast<const char*>(base) + row * step + cols.first * static_cast<int>(sizeof(T));
+  }
+  // After set() of each tensor: `rows` rows from there.
+  __device__ void start(const RowCols<E, V>& cols, const RowPlan& plan, void* smem, int rows) {
+    left = rows;
     if constexpr (E > 1) {
-      ring = smem_u32(smem);
-      stage_bytes = kRowBytes * blockDim.x;
+      ring = write = smem_u32(smem);
+      read = ring + (STAGES - 1) * kStageBytes;
       // what no copy ever fills stays zero
 #pragma unroll
       for (int i = 0; i < kTensors; ++i) {
-        if (i < NX) clear<ChunkX>(cols, i);
-        else clear<ChunkR>(cols, i);
+        if (cols.has(V - 1) && (plan.present >> i & 1)) continue;
+        if (i < NX) clear<ChunkX>(i);
+        else clear<ChunkR>(i);
       }
 #pragma unroll 1
-      for (int i = 0; i < STAGES - 1; ++i) load(cols);
+      for (int i = 0; i < STAGES - 1; ++i) load(cols, plan);
     } else {
-      load(cols);
+      load(cols, plan);
     }
   }
   // The next row: its values are there for get(), and the loads of a later one are under way.
-  __device__ void advance(const RowCols<E, V>& cols) {
+  __device__ void advance(const RowCols<E, V>& cols, const RowPlan& plan) {
     if constexpr (E > 1) {
-      load(cols);
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      load(cols, plan);
+      read = next_stage(read);
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     } else {
 #pragma unroll
       for (int i = 0; i < kTensors * V; ++i) now[i] = ahead[i];
-      load(cols);
+      load(cols, plan);
     }
   }
-  template <int I> __device__ void get(F2 (&f)[RowCols<E, V>::P]) const {
+  // Block b of tensor I.
+  template <int I> __device__ void get(int b, F2 (&f)[RowCols<E, V>::BP]) const {
+    constexpr int CHUNKS = RowCols<E, V>::B / E;
     if constexpr (E > 1) {
       using C = std::conditional_t<(I < NX), ChunkX, ChunkR>;
+      const uint32_t mine = read + threadIdx.x * C::kVecBytes;
 #pragma unroll
-      for (int v = 0; v < V * C::kVecs; ++v) {
+      for (int v = 0; v < CHUNKS * C::kVecs; ++v) {
         typename C::Vec::Raw r;
         uint32_t* w = reinterpret_cast<uint32_t*>(&r);
-        const uint32_t at = slot<C::kVecBytes>(stage, I, v);
+        const uint32_t from = mine + offset(I, b * CHUNKS * C::kVecs + v, C::kVecBytes);
         if constexpr (C::kVecBytes == 16)
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(from));
         else
-          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from));
         C::unpack(r, f + v * C::kVecCols / 2);
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < V; ++k) lane_of(f, k) = now[I * V + k];
+      for (int k = 0; k < CHUNKS; ++k) lane_of(f, k) = now[I * V + b * CHUNKS + k];
     }
   }
 
  private:
-  __device__ void load(const RowCols<E, V>& cols) {
-    if (next < end) {
+  __device__ uint32_t next_stage(uint32_t st) const {
+    return st == ring + (STAGES - 1) * kStageBytes ? ring : st + kStageBytes;
+  }
+  __device__ void load(const RowCols<E, V>& cols, const RowPlan& plan) {
+    if (left > 0) {
 #pragma unroll
       for (int i = 0; i < kTensors; ++i) {
-        if (base[i] == nullptr) {
+        if (!(plan.present >> i & 1)) {
           if constexpr (E == 1) {
 #pragma unroll
             for (int k = 0; k < V; ++k) ahead[i * V + k] = 0.f;
@@ -236,42 +260,48 @@ struct RowStream {
         }
         if (i < NX) copy<TX, ChunkX>(cols, i);
         else copy<TR, ChunkR>(cols, i);
+        at[i] += plan.step[i];
       }
     }
-    ++next;
+    --left;
     if constexpr (E > 1) {
-      load_stage = load_stage + 1 == STAGES ? 0 : load_stage + 1;
+      write = next_stage(write);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
   }
   template <typename T, class C> __device__ void copy(const RowCols<E, V>& cols, int i) {
-    const T* row = static_cast<const T*>(base[i]) + next * stride[i];
+    const T* from = reinterpret_cast<const T*>(at[i]);
+    const uint32_t to = write + threadIdx.x * C::kVecBytes;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       if constexpr (E == 1) {
-        ahead[i * V + k] = cols.has(k) ? Ty<T>::to_f(row[cols.col(k)]) : 0.f;
+        ahead[i * V + k] = cols.has(k) ? Ty<T>::to_f(from[k * cols.step]) : 0.f;
       } else if (cols.has(k)) {
 #pragma unroll
         for (int v = 0; v < C::kVecs; ++v) {
-          const uint32_t to = slot<C::kVecBytes>(load_stage, i, k * C::kVecs + v);
-          const T* from = row + cols.col(k) + v * C::kVecCols;
           if constexpr (C::kVecBytes == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + offset(i, k * C::kVecs + v, 16)),
+                         "l"(from + k * cols.step + v * C::kVecCols)
+                         : "memory");
           else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to + offset(i, k * C::kVecs + v, 8)),
+                         "l"(from + k * cols.step + v * C::kVecCols)
+                         : "memory");
         }
       }
     }
   }
-  template <class C> __device__ void clear(const RowCols<E, V>& cols, int i) {
-    if (cols.has(V - 1) && base[i] != nullptr) return;
+  template <class C> __device__ void clear(int i) const {
 #pragma unroll 1
-    for (int v = 0; v < V * C::kVecs * STAGES; ++v) {
-      const uint32_t at = slot<C::kVecBytes>(v / (V * C::kVecs), i, v % (V * C::kVecs));
-      if constexpr (C::kVecBytes == 16)
-        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
-      else
-        asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(at), "r"(0u) : "memory");
+    for (int st = 0; st < STAGES; ++st) {
+      const uint32_t mine = ring + st * kStageBytes + threadIdx.x * C::kVecBytes;
+#pragma unroll
+      for (int v = 0; v < V * C::kVecs; ++v) {
+        if constexpr (C::kVecBytes == 16)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(mine + offset(i, v, 16)), "r"(0u) : "memory");
+        else
+          asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(mine + offset(i, v, 8)), "r"(0u) : "memory");
+      }
     }
   }
 };

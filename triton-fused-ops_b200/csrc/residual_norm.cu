@@ -17,27 +17,14 @@
 
 namespace tfo {
 
-// scale * gate * w1 (* 1 / (1 - p)) of a sequence: what a normed branch is multiplied by.
-template <int E, int V>
-__device__ __forceinline__ void branch_coefficient(const ResidualArgs& a, const RowCols<E, V>& cols, int64_t seq,
-                                                   F2 (&c)[RowCols<E, V>::P]) {
-  constexpr int P = RowCols<E, V>::P;
-  F2 g[P];
-  cols.param(a.branch_weight, seq, 1.f, c);
-  cols.param(a.gate, seq, 1.f, g);
-  const float s = a.dropped ? a.scale * a.drop.scale : a.scale;
-#pragma unroll
-  for (int j = 0; j < P; ++j) c[j] = mul2(mul2(c[j], g[j]), f2(s, s));
-}
-
 // Parameters stay in registers up to this many columns a thread; above it they are read again for every row.
 constexpr int kParamCols = 16;
 
 template <typename TX, typename TR, int E, int V, int STAGES>
 __global__ void __launch_bounds__(kRowThreads, 1)
-    residual_norm_kernel(const __grid_constant__ ResidualArgs a, RowPlan plan) {
+    residual_norm_kernel(const __grid_constant__ ResidualArgs a, const __grid_constant__ RowPlan plan) {
   using Cols = RowCols<E, V>;
-  constexpr int P = Cols::P;
+  constexpr int NB = Cols::BLOCKS, BP = Cols::BP;
   constexpr bool KEEP_PARAMS = Cols::N <= kParamCols;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red[2][kMaxRowWarps][kMaxRowWarps];
@@ -50,79 +37,102 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   griddep_wait();
   const int64_t groups = static_cast<int64_t>(gridDim.x) * plan.groups;
   const int64_t me = static_cast<int64_t>(blockIdx.x) * plan.groups + group;
-  const int64_t r0 = me * a.rows / groups, r1 = (me + 1) * a.rows / groups;
-  if (r0 >= r1) return;
+  const int64_t r0 = me * a.rows / groups;
+  int left = static_cast<int>((me + 1) * a.rows / groups - r0);
+  if (left == 0) return;
   const Cols cols(t, plan.threads, a.hidden);
   RowStream<TX, TR, E, V, 1, 1, STAGES> rows;
-  rows.base[0] = a.x;
-  rows.stride[0] = a.x_stride;
-  rows.base[1] = a.res;
-  rows.stride[1] = a.res_stride;
-  rows.start(cols, smem, r0, r1);
+  rows.template set<TX>(0, a.x, r0, plan.step[0], cols);
+  rows.template set<TR>(1, a.res, r0, plan.step[1], cols);
+  rows.start(cols, plan, smem, left);
   const DropKey key(a.drop);
   const float inv_h = 1.f / static_cast<float>(a.hidden);
   const int bar = 1 + group;
   int turn = 0;  // of the parts of a sum
-  int64_t seq = r0 / a.rows_per_seq, seq_end = (seq + 1) * a.rows_per_seq;
+  int64_t seq = r0 / a.rows_per_seq;
+  int seq_left = static_cast<int>((seq + 1) * a.rows_per_seq - r0);
   const bool by_seq = (a.branch_weight.seq_stride | a.gate.seq_stride | a.weight.seq_stride) != 0;
-  F2 c[P], w[P];
-  if constexpr (KEEP_PARAMS) {
-    branch_coefficient(a, cols, seq, c);
-    cols.param(a.weight, seq, 1.f, w);
-  }
-  for (int64_t r = r0; r < r1; ++r) {
-    if (r == seq_end) {
-      ++seq;
-      seq_end += a.rows_per_seq;
-      if (KEEP_PARAMS && by_seq) {
-        branch_coefficient(a, cols, seq, c);
-        cols.param(a.weight, seq, 1.f, w);
-      }
+  uint64_t element = static_cast<uint64_t>(r0) * a.hidden;  // the row's first
+  TR* h_out = static_cast<TR*>(a.h) + element + cols.first;
+  TX* y_out = static_cast<TX*>(a.y) + element + cols.first;
+  float* rstd = a.rstd + 2 * r0;
+  F2 c[KEEP_PARAMS ? NB : 1][BP], w[KEEP_PARAMS ? NB : 1][BP];
+  auto params = [&] {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      cols.branch_coefficient(a, seq, b, c[b]);
+      cols.param(a.weight, seq, 1.f, b, w[b]);
     }
-    const uint32_t bits = a.dropped ? cols.kept(a.drop, key, r) : ~0u;
-    rows.advance(cols);
-    F2 h[P];
+  };
+  if constexpr (KEEP_PARAMS) params();
+  for (;;) {
+    const uint32_t bits = a.dropped ? cols.kept(a.drop, key, element) : ~0u;
+    rows.advance(cols, plan);
+    F2 h[NB][BP];
     float r_branch = 1.f;
-    {
-      F2 x[P], res[P];
-      rows.template get<0>(x);
-      rows.template get<1>(res);
-      if (a.branch_norm) {
-        F2 s2 = f2(0.f, 0.f);
-#pragma unroll
-        for (int j = 0; j < P; ++j) s2 = fma2(x[j], x[j], s2);
-        float s[1] = {s2.x + s2.y};
-        row_sum(s, red[turn ^= 1][group], warps, warp, bar);
-        r_branch = rsqrtf(s[0] * inv_h + a.eps);
-      }
-      if constexpr (!KEEP_PARAMS) branch_coefficient(a, cols, seq, c);
-#pragma unroll
-      for (int j = 0; j < P; ++j) x[j] = mul2(mul2(x[j], f2(r_branch, r_branch)), c[j]);
-      if (a.dropped) Cols::drop(bits, x);
-#pragma unroll
-      for (int j = 0; j < P; ++j) h[j] = add2(res[j], x[j]);
-    }
-    cols.store(static_cast<TR*>(a.h) + r * a.hidden, h);
-    float r_sum = 1.f;
-    if (a.y != nullptr) {
+    if (a.branch_norm) {
       F2 s2 = f2(0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < P; ++j) s2 = fma2(h[j], h[j], s2);
+      for (int b = 0; b < NB; ++b) {
+        rows.template get<0>(b, h[b]);
+#pragma unroll
+        for (int j = 0; j < BP; ++j) s2 = fma2(h[b][j], h[b][j], s2);
+      }
+      float s[1] = {s2.x + s2.y};
+      row_sum(s, red[turn ^= 1][group], warps, warp, bar);
+      r_branch = rsqrtf(s[0] * inv_h + a.eps);
+    }
+    F2 s2 = f2(0.f, 0.f);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      F2 res[BP];
+      if (!a.branch_norm) rows.template get<0>(b, h[b]);
+      rows.template get<1>(b, res);
+      F2(&cb)[BP] = c[KEEP_PARAMS ? b : 0];
+      if constexpr (!KEEP_PARAMS) cols.branch_coefficient(a, seq, b, cb);
+#pragma unroll
+      for (int j = 0; j < BP; ++j) h[b][j] = mul2(mul2(h[b][j], f2(r_branch, r_branch)), cb[j]);
+      if (a.dropped) Cols::drop(bits, b, h[b]);
+#pragma unroll
+      for (int j = 0; j < BP; ++j) {
+        h[b][j] = add2(res[j], h[b][j]);
+        s2 = fma2(h[b][j], h[b][j], s2);
+      }
+      cols.store(h_out, b, h[b]);
+    }
+    h_out += a.hidden;
+    float r_sum = 1.f;
+    if (a.y != nullptr) {
       float s[1] = {s2.x + s2.y};
       row_sum(s, red[turn ^= 1][group], warps, warp, bar);
       r_sum = rsqrtf(s[0] * inv_h + a.eps);
-      if constexpr (!KEEP_PARAMS) cols.param(a.weight, seq, 1.f, w);
 #pragma unroll
-      for (int j = 0; j < P; ++j) h[j] = mul2(mul2(h[j], f2(r_sum, r_sum)), w[j]);
-      if (a.shift.p != nullptr) {
-        F2 b[P];
-        cols.param(a.shift, seq, 0.f, b);
+      for (int b = 0; b < NB; ++b) {
+        F2(&wb)[BP] = w[KEEP_PARAMS ? b : 0];
+        if constexpr (!KEEP_PARAMS) cols.param(a.weight, seq, 1.f, b, wb);
 #pragma unroll
-        for (int j = 0; j < P; ++j) h[j] = add2(h[j], b[j]);
+        for (int j = 0; j < BP; ++j) h[b][j] = mul2(mul2(h[b][j], f2(r_sum, r_sum)), wb[j]);
+        if (a.shift.p != nullptr) {
+          F2 sh[BP];
+          cols.param(a.shift, seq, 0.f, b, sh);
+#pragma unroll
+          for (int j = 0; j < BP; ++j) h[b][j] = add2(h[b][j], sh[j]);
+        }
+        cols.store(y_out, b, h[b]);
       }
-      cols.store(static_cast<TX*>(a.y) + r * a.hidden, h);
+      y_out += a.hidden;
     }
-    if (a.rstd != nullptr && t == 0) *reinterpret_cast<float2*>(a.rstd + 2 * r) = make_float2(r_branch, r_sum);
+    if (a.rstd != nullptr) {
+      if (t == 0) *reinterpret_cast<float2*>(rstd) = make_float2(r_branch, r_sum);
+      rstd += 2;
+    }
+    if (--left == 0) return;
+    element += a.hidden;
+    if (--seq_left == 0) {
+      ++seq;
+      seq_left = static_cast<int>(a.rows_per_seq);
+      if (KEEP_PARAMS && by_seq) params();
+    }
   }
 }
 
@@ -188,13 +198,15 @@ cudaError_t launch_rows(const ResidualArgs& a, int threads, cudaStream_t st) {
   const int groups =
       static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, a.rows / num_sms())));
   const int block = groups * threads;
-  const size_t smem = Stream::smem_bytes(block);
-  // the limit of the largest block: also below it the static part comes on top
-  if (const cudaError_t e = ensure_smem_attr(fn, Stream::smem_bytes(kRowThreads)); e != cudaSuccess) return e;
+  const size_t smem = Stream::kSmemBytes;
+  // at least a little over 48 KB: the sums' static part comes on top
+  if (const cudaError_t e = ensure_smem_attr(fn, std::max<size_t>(smem, 49 * 1024)); e != cudaSuccess) return e;
   const int64_t all = static_cast<int64_t>(num_sms()) * std::max(1, cached_occupancy(fn, block, smem));
   const int64_t grid = std::min<int64_t>(all, (a.rows + groups - 1) / groups);
   note_launch();
-  return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a, RowPlan{threads, groups});
+  return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a,
+                          RowPlan{threads, groups, {a.x_stride * static_cast<int64_t>(sizeof(TX)),
+                                                    a.res_stride * static_cast<int64_t>(sizeof(TR))}, 3});
 }
 
 template <typename TX, typename TR>

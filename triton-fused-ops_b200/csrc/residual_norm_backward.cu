@@ -39,6 +39,46 @@ struct RowItems {
   }
 };
 
+// What a thread keeps from row to row, in blocks of its columns: the sums over
+// rows, c and w2. With 16 columns these are 80 values, which live in tensor
+// memory: a block of 8 is read or written by one instruction, and the registers
+// are free for the row. Warp w of the CTA uses the lanes of its sub-partition
+// (w % 4) and columns of its own. With 8 columns or less they are registers.
+enum Kept : int { KEPT_C = SUMS, KEPT_W = SUMS + 1, KEPT = SUMS + 2 };
+template <class Cols, bool TENSOR> struct RowKept {
+  F2 v[KEPT][Cols::BLOCKS][Cols::BP];
+  __device__ explicit RowKept(uint32_t) {}
+  __device__ void settle() {}
+  __device__ void read(int i, int b, F2 (&out)[Cols::BP]) const {
+#pragma unroll
+    for (int j = 0; j < Cols::BP; ++j) out[j] = v[i][b][j];
+  }
+  __device__ void wait() {}
+  __device__ void arrived(F2 (&)[Cols::BP]) const {}
+  __device__ void write(int i, int b, const F2 (&in)[Cols::BP]) {
+#pragma unroll
+    for (int j = 0; j < Cols::BP; ++j) v[i][b][j] = in[j];
+  }
+};
+template <class Cols> struct RowKept<Cols, true> {
+  static_assert(Cols::N == 16 && Cols::B == 8, "two blocks of 8 columns");
+  static constexpr uint32_t kColumns = 512;  // of the CTA: KEPT * 16 for each of a sub-partition's four warps, a power of two
+  uint32_t mine;
+  __device__ explicit RowKept(uint32_t base) {
+    const uint32_t w = threadIdx.x >> 5;
+    mine = base + ((w & 3u) << 21) + (w >> 2) * (KEPT * 16);  // lane 32 * (w % 4) in the upper half
+  }
+  // Between a write and a read of the same values.
+  __device__ void settle() { tmem_st_wait(); }
+  // Asks for a block; it is there after wait() and arrived() of it.
+  __device__ void read(int i, int b, F2 (&out)[4]) const {
+    tmem_ld8(mine + 16 * i + 8 * b, *reinterpret_cast<uint32_t(*)[8]>(&out));
+  }
+  __device__ void wait() { tmem_ld_wait(); }
+  __device__ void arrived(F2 (&out)[4]) const { tmem_ld_fence(*reinterpret_cast<uint32_t(*)[8]>(&out)); }
+  __device__ void write(int i, int b, const F2 (&in)[4]) { tmem_st8(mine + 16 * i + 8 * b, *reinterpret_cast<const uint32_t(*)[8]>(&in)); }
+};
+
 struct BackwardPlan {
   RowPlan rows;
   RowItems items;
@@ -49,10 +89,22 @@ template <typename TX, typename TR, int E, int V, int STAGES>
 __global__ void __launch_bounds__(kRowThreads, 1)
     residual_norm_backward_kernel(const __grid_constant__ ResidualArgs a, const __grid_constant__ BackwardPlan plan) {
   using Cols = RowCols<E, V>;
-  constexpr int P = Cols::P;
-  constexpr bool KEEP_PARAMS = Cols::N <= 8;
+  constexpr int NB = Cols::BLOCKS, BP = Cols::BP;
+  constexpr bool TENSOR = Cols::N == 16;
+  using KeptRows = RowKept<Cols, TENSOR>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ __align__(16) float red[2][kMaxRowWarps][4 * kMaxRowWarps];
+  __shared__ uint32_t tensor_base;
+  if constexpr (TENSOR) {
+    if (threadIdx.x < 32) {
+      tmem_alloc(&tensor_base, KeptRows::kColumns);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  }
+  // only now: a dependent kernel that takes tensor memory and then waits for this one must not come first
   griddep_launch_dependents();
   const int threads = plan.rows.threads, warps = threads / 32;
   const int group = (threadIdx.x >> 5) / warps, warp = (threadIdx.x >> 5) - group * warps;
@@ -65,130 +117,187 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   const RowItems items = plan.items;
   int64_t item = me * items.count() / groups;
   const int64_t last = (me + 1) * items.count() / groups;
-  if (item >= last) return;
-  const int64_t r0 = items.first_row(item), r1 = items.first_row(last);
-  const Cols cols(t, threads, a.hidden);
-  RowStream<TX, TR, E, V, 2, 2, STAGES> rows;
-  rows.base[0] = a.x;
-  rows.stride[0] = a.x_stride;
-  rows.base[1] = a.dy;
-  rows.stride[1] = a.dy_stride;
-  rows.base[2] = a.dy != nullptr ? a.res : nullptr;  // h serves the norm alone
-  rows.stride[2] = a.res_stride;
-  rows.base[3] = a.dh;
-  rows.stride[3] = a.dh_stride;
-  rows.start(cols, smem, r0, r1);
-  const DropKey key(a.drop);
-  const float inv_h = 1.f / static_cast<float>(a.hidden);
-  const int bar = 1 + group;
-  int turn = 0;  // of the parts of a sum
-  const float2* rstd = reinterpret_cast<const float2*>(a.rstd);
-  float2 next_r = rstd[r0];  // loaded a row ahead
-  F2 c[P], w[P], sums[SUMS][P];
-  auto params = [&](int64_t seq) {
-    F2 g[P];
-    cols.param(a.branch_weight, seq, 1.f, c);
-    cols.param(a.gate, seq, 1.f, g);
-    const float s = a.dropped ? a.scale * a.drop.scale : a.scale;
+  if (item < last) {
+    const int64_t r0 = items.first_row(item);
+    int left = static_cast<int>(items.first_row(last) - r0);
+    const Cols cols(t, threads, a.hidden);
+    RowStream<TX, TR, E, V, 2, 2, STAGES> rows;
+    rows.template set<TX>(0, a.x, r0, plan.rows.step[0], cols);
+    rows.template set<TX>(1, a.dy, r0, plan.rows.step[1], cols);
+    rows.template set<TR>(2, a.res, r0, plan.rows.step[2], cols);
+    rows.template set<TR>(3, a.dh, r0, plan.rows.step[3], cols);
+    rows.start(cols, plan.rows, smem, left);
+    const DropKey key(a.drop);
+    const float inv_h = 1.f / static_cast<float>(a.hidden);
+    const int bar = 1 + group;
+    int turn = 0;  // of the parts of a sum
+    const float2* rstd = reinterpret_cast<const float2*>(a.rstd) + r0;
+    float2 next_r = *rstd;  // loaded a row ahead
+    KeptRows kept(TENSOR ? tensor_base : 0u);
+    int64_t seq = r0 / a.rows_per_seq;
+    int seq_left = static_cast<int>((seq + 1) * a.rows_per_seq - r0);
+    const bool by_seq = (a.branch_weight.seq_stride | a.gate.seq_stride | a.weight.seq_stride) != 0;
+    auto params = [&] {
 #pragma unroll
-    for (int j = 0; j < P; ++j) c[j] = mul2(mul2(c[j], g[j]), f2(s, s));
-    cols.param(a.weight, seq, 1.f, w);
-  };
-  auto clear = [&] {
-#pragma unroll
-    for (int i = 0; i < SUMS; ++i) {
-#pragma unroll
-      for (int j = 0; j < P; ++j) sums[i][j] = f2(0.f, 0.f);
-    }
-  };
-  int64_t seq = r0 / a.rows_per_seq, seq_end = (seq + 1) * a.rows_per_seq;
-  const bool by_seq = (a.branch_weight.seq_stride | a.gate.seq_stride | a.weight.seq_stride) != 0;
-  if (KEEP_PARAMS) params(seq);
-  clear();
-  int64_t item_end = items.first_row(item + 1);
-  for (int64_t r = r0; r < r1; ++r) {
-    if (r == seq_end) {
-      ++seq;
-      seq_end += a.rows_per_seq;
-      if (KEEP_PARAMS && by_seq) params(seq);
-    }
-    const uint32_t bits = a.dropped ? cols.kept(a.drop, key, r) : ~0u;
-    const float2 rs = next_r;
-    if (r + 1 < r1) next_r = rstd[r + 1];
-    rows.advance(cols);
-    if constexpr (!KEEP_PARAMS) params(seq);
-    F2 x[P], q[P], hat[P];  // x', dH and what it is made of, h'
-    rows.template get<0>(x);
-    rows.template get<3>(q);
-#pragma unroll
-    for (int j = 0; j < P; ++j) x[j] = mul2(x[j], f2(rs.x, rs.x));
-    float s[4] = {0.f, 0.f, 0.f, 0.f};  // of g h', u dh, u g, u h'
-    {
-      F2 u[P], s0 = f2(0.f, 0.f), s1 = s0, s2 = s0, s3 = s0;
-#pragma unroll
-      for (int j = 0; j < P; ++j) u[j] = mul2(x[j], c[j]);
-      if (a.dropped) Cols::drop(bits, u);
-      if (a.branch_norm) {
-#pragma unroll
-        for (int j = 0; j < P; ++j) s1 = fma2(u[j], q[j], s1);
+      for (int b = 0; b < NB; ++b) {
+        F2 f[BP];
+        cols.branch_coefficient(a, seq, b, f);
+        __syncwarp();
+        kept.write(KEPT_C, b, f);
+        cols.param(a.weight, seq, 1.f, b, f);
+        __syncwarp();
+        kept.write(KEPT_W, b, f);
       }
-      if (a.dy != nullptr) {
-        F2 dy[P];
-        rows.template get<1>(dy);
-        rows.template get<2>(hat);
+    };
+    auto clear = [&] {
+      F2 zero[BP];
 #pragma unroll
-        for (int j = 0; j < P; ++j) {
-          hat[j] = mul2(add2(hat[j], u[j]), f2(rs.y, rs.y));
-          sums[SUM_WEIGHT][j] = fma2(dy[j], hat[j], sums[SUM_WEIGHT][j]);
-          sums[SUM_SHIFT][j] = add2(dy[j], sums[SUM_SHIFT][j]);
-          const F2 g = mul2(dy[j], w[j]);
-          s0 = fma2(g, hat[j], s0);
-          s2 = fma2(u[j], g, s2);
-          s3 = fma2(u[j], hat[j], s3);
-          q[j] = fma2(g, f2(rs.y, rs.y), q[j]);
+      for (int j = 0; j < BP; ++j) zero[j] = f2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < SUMS; ++i) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) kept.write(i, b, zero);
+      }
+    };
+    uint64_t element = static_cast<uint64_t>(r0) * a.hidden;  // the row's first
+    TX* dx = static_cast<TX*>(a.dx) + element + cols.first;
+    TR* dres = static_cast<TR*>(a.dres) + element + cols.first;
+    const bool sum_branch = plan.partials[SUM_BRANCH] != nullptr, sum_weight = plan.partials[SUM_WEIGHT] != nullptr,
+               sum_shift = plan.partials[SUM_SHIFT] != nullptr, normed = a.dy != nullptr;
+    params();
+    clear();
+    int item_left = static_cast<int>(items.first_row(item + 1) - r0);
+    for (;;) {
+      const uint32_t bits = a.dropped ? cols.kept(a.drop, key, element) : ~0u;
+      const float2 rs = next_r;
+      if (left > 1) next_r = *++rstd;
+      rows.advance(cols, plan.rows);
+      kept.settle();
+      F2 x[NB][BP], q[NB][BP], hat[NB][BP];  // x', dH and what it is made of, h'
+      F2 s0 = f2(0.f, 0.f), s1 = s0, s2 = s0, s3 = s0;  // of g h', u dh, u g, u h'
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        F2 u[BP], c[BP];
+        kept.read(KEPT_C, b, c);
+        rows.template get<0>(b, x[b]);
+        rows.template get<3>(b, q[b]);
+        kept.wait();
+        kept.arrived(c);
+#pragma unroll
+        for (int j = 0; j < BP; ++j) {
+          x[b][j] = mul2(x[b][j], f2(rs.x, rs.x));
+          u[j] = mul2(x[b][j], c[j]);
+        }
+        if (a.dropped) Cols::drop(bits, b, u);
+#pragma unroll
+        for (int j = 0; j < BP; ++j) s1 = fma2(u[j], q[b][j], s1);
+        if (normed) {
+          F2 dy[BP], w[BP], sum[BP];
+          kept.read(KEPT_W, b, w);
+          kept.read(SUM_WEIGHT, b, sum);
+          rows.template get<1>(b, dy);
+          rows.template get<2>(b, hat[b]);
+          kept.wait();
+          kept.arrived(w);
+          kept.arrived(sum);
+#pragma unroll
+          for (int j = 0; j < BP; ++j) {
+            hat[b][j] = mul2(add2(hat[b][j], u[j]), f2(rs.y, rs.y));
+            sum[j] = fma2(dy[j], hat[b][j], sum[j]);
+            const F2 g = mul2(dy[j], w[j]);
+            s0 = fma2(g, hat[b][j], s0);
+            s2 = fma2(u[j], g, s2);
+            s3 = fma2(u[j], hat[b][j], s3);
+            q[b][j] = fma2(g, f2(rs.y, rs.y), q[b][j]);
+          }
+          if (sum_weight) kept.write(SUM_WEIGHT, b, sum);
+          if (sum_shift) {
+            kept.read(SUM_SHIFT, b, sum);
+            kept.wait();
+            kept.arrived(sum);
+#pragma unroll
+            for (int j = 0; j < BP; ++j) sum[j] = add2(dy[j], sum[j]);
+            kept.write(SUM_SHIFT, b, sum);
+          }
         }
       }
-      s[0] = s0.x + s0.y;
-      s[1] = s1.x + s1.y;
-      s[2] = s2.x + s2.y;
-      s[3] = s3.x + s3.y;
-    }
-    if (a.branch_norm) {
-      row_sum(s, red[turn ^= 1][group], warps, warp, bar);
-    } else if (a.dy != nullptr) {
-      float one[1] = {s[0]};
-      row_sum(one, red[turn ^= 1][group], warps, warp, bar);
-      s[0] = one[0];
-    }
-    const float mean = s[0] * inv_h;
-    if (a.dy != nullptr) {
-      const float m = -mean * rs.y;
-#pragma unroll
-      for (int j = 0; j < P; ++j) q[j] = fma2(hat[j], f2(m, m), q[j]);
-    }
-    if (a.dres != nullptr) cols.store(static_cast<TR*>(a.dres) + r * a.hidden, q);
-    if (a.dropped) Cols::drop(bits, q);
-    const float m1 = a.branch_norm ? -(s[1] + rs.y * (s[2] - mean * s[3])) * inv_h : 0.f;
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      sums[SUM_BRANCH][j] = fma2(q[j], x[j], sums[SUM_BRANCH][j]);
-      q[j] = mul2(q[j], c[j]);
-    }
-    if (a.dx != nullptr) {
+      float s[4] = {s0.x + s0.y, s1.x + s1.y, s2.x + s2.y, s3.x + s3.y};
       if (a.branch_norm) {
-#pragma unroll
-        for (int j = 0; j < P; ++j) q[j] = mul2(fma2(x[j], f2(m1, m1), q[j]), f2(rs.x, rs.x));
+        row_sum(s, red[turn ^= 1][group], warps, warp, bar);
+      } else if (normed) {
+        float one[1] = {s[0]};
+        row_sum(one, red[turn ^= 1][group], warps, warp, bar);
+        s[0] = one[0];
       }
-      cols.store(static_cast<TX*>(a.dx) + r * a.hidden, q);
-    }
-    if (r + 1 == item_end) {
+      const float mean = s[0] * inv_h, m = -mean * rs.y;
+      const float m1 = a.branch_norm ? -(s[1] + rs.y * (s[2] - mean * s[3])) * inv_h : 0.f;
 #pragma unroll
-      for (int i = 0; i < SUMS; ++i)
-        if (plan.partials[i] != nullptr) cols.store(plan.partials[i] + item * a.hidden, sums[i]);
-      clear();
-      ++item;
-      item_end = item < last ? items.first_row(item + 1) : 0;
+      for (int b = 0; b < NB; ++b) {
+        F2 c[BP], sum[BP];
+        kept.read(KEPT_C, b, c);
+        kept.read(SUM_BRANCH, b, sum);
+        if (normed) {
+#pragma unroll
+          for (int j = 0; j < BP; ++j) q[b][j] = fma2(hat[b][j], f2(m, m), q[b][j]);
+        }
+        kept.wait();
+        kept.arrived(c);
+        kept.arrived(sum);
+        if (a.dres != nullptr) cols.store(dres, b, q[b]);
+        if (a.dropped) Cols::drop(bits, b, q[b]);
+        if (sum_branch) {
+#pragma unroll
+          for (int j = 0; j < BP; ++j) sum[j] = fma2(q[b][j], x[b][j], sum[j]);
+          __syncwarp();
+          kept.write(SUM_BRANCH, b, sum);
+        }
+        if (a.dx != nullptr) {
+#pragma unroll
+          for (int j = 0; j < BP; ++j) q[b][j] = mul2(q[b][j], c[j]);
+          if (a.branch_norm) {
+#pragma unroll
+            for (int j = 0; j < BP; ++j) q[b][j] = mul2(fma2(x[b][j], f2(m1, m1), q[b][j]), f2(rs.x, rs.x));
+          }
+          cols.store(dx, b, q[b]);
+        }
+        __syncwarp();
+      }
+      dx += a.hidden;
+      dres += a.hidden;
+      if (--item_left == 0) {
+        kept.settle();
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) {
+          if (plan.partials[i] == nullptr) continue;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            F2 v[BP];
+            kept.read(i, b, v);
+            kept.wait();
+            kept.arrived(v);
+            cols.store(plan.partials[i] + item * a.hidden + cols.first, b, v);
+            __syncwarp();
+          }
+        }
+        clear();
+        ++item;
+        if (item < last) item_left = static_cast<int>(items.first_row(item + 1) - items.first_row(item));
+      }
+      if (--left == 0) break;
+      element += a.hidden;
+      if (--seq_left == 0) {
+        ++seq;
+        seq_left = static_cast<int>(a.rows_per_seq);
+        if (by_seq) params();
+      }
     }
+  }
+  if constexpr (TENSOR) {
+    tmem_st_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (threadIdx.x < 32) tmem_dealloc(tensor_base, KeptRows::kColumns);
   }
 }
 
@@ -333,8 +442,9 @@ struct Shape {
 Shape shape_of(const ResidualArgs& a) {
   const int e = row_chunk(a, true);
   if (e > 1) {
-    for (int v = 8 / e; v * e <= 16; v *= 2)
-      if (const int t = row_threads(a.hidden, e, v)) return {e, v, t};
+    // a warp a row as far as 8 columns a thread carry it, then 16 columns a thread
+    if (a.hidden <= 256) return {e, 8 / e, 32};
+    if (const int t = row_threads(a.hidden, e, 16 / e)) return {e, 16 / e, t};
   } else {
     for (int v = 4; v <= 8; v *= 2)
       if (const int t = row_threads(a.hidden, 1, v)) return {1, v, t};
@@ -361,13 +471,16 @@ cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t 
   auto* kernel = residual_norm_backward_kernel<TX, TR, E, V, STAGES>;
   using Stream = RowStream<TX, TR, E, V, 2, 2, STAGES>;
   const int threads = plan.rows.threads;
-  const int64_t count = plan.items.count();
+  const int64_t count = plan.items.count(), x = sizeof(TX), r = sizeof(TR);
+  const int64_t step[4] = {a.x_stride * x, a.dy_stride * x, a.res_stride * r, a.dh_stride * r};
+  std::copy(step, step + 4, plan.rows.step);
+  plan.rows.present = 1 | (a.dy != nullptr ? 2 | 4 : 0) | (a.dh != nullptr ? 8 : 0);  // h serves the norm alone
   plan.rows.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, count / num_sms())));
   const int block = plan.rows.groups * threads;
-  const size_t smem = Stream::smem_bytes(block);
+  const size_t smem = Stream::kSmemBytes;
   const void* fn = reinterpret_cast<const void*>(kernel);
-  // the limit of the largest block: also below it the static part comes on top
-  if (const cudaError_t e = ensure_smem_attr(fn, Stream::smem_bytes(kRowThreads)); e != cudaSuccess) return e;
+  // at least a little over 48 KB: the sums' static part comes on top
+  if (const cudaError_t e = ensure_smem_attr(fn, std::max<size_t>(smem, 49 * 1024)); e != cudaSuccess) return e;
   const int64_t all = static_cast<int64_t>(num_sms()) * std::max(1, cached_occupancy(fn, block, smem));
   const int64_t grid = std::min<int64_t>(all, (count + plan.rows.groups - 1) / plan.rows.groups);
   note_launch();
