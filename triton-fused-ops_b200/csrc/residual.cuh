@@ -17,12 +17,22 @@ namespace tfo {
 constexpr int kRowThreads = 512;   // most threads of a CTA
 constexpr int kMaxRowWarps = 16;   // of a group
 
+// `count` things over `parts` of them as evenly as can be, the first ones one more (no division on the device).
+struct Split {
+  uint32_t each, more;
+  static Split make(int64_t count, int64_t parts) {
+    return Split{static_cast<uint32_t>(count / parts), static_cast<uint32_t>(count % parts)};
+  }
+  __device__ uint32_t first(uint32_t part) const { return part * each + min(part, more); }
+};
+
 // How a launch spreads the rows.
 struct RowPlan {
   int threads;      // T
   int groups;       // of a CTA
   int64_t step[4];  // bytes between the rows of the streamed tensors
   int present;      // a bit for each of them that is there (the others are zeros)
+  Split share;      // rows (backward: items) of the launch's groups
 };
 
 // ---- sums over a row --------------------------------------------------------

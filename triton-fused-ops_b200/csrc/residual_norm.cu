@@ -35,10 +35,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   for (int i = threadIdx.x; i < 2 * kMaxRowWarps * kMaxRowWarps; i += blockDim.x) (&red[0][0][0])[i] = 0.f;
   __syncthreads();
   griddep_wait();
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * plan.groups;
-  const int64_t me = static_cast<int64_t>(blockIdx.x) * plan.groups + group;
-  const int64_t r0 = me * a.rows / groups;
-  int left = static_cast<int>((me + 1) * a.rows / groups - r0);
+  const uint32_t me = blockIdx.x * plan.groups + group;
+  const int64_t r0 = plan.share.first(me);
+  int left = static_cast<int>(plan.share.first(me + 1) - r0);
   if (left == 0) return;
   const Cols cols(t, plan.threads, a.hidden);
   RowStream<TX, TR, E, V, 1, 1, STAGES> rows;
@@ -49,7 +48,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   const float inv_h = 1.f / static_cast<float>(a.hidden);
   const int bar = 1 + group;
   int turn = 0;  // of the parts of a sum
-  int64_t seq = r0 / a.rows_per_seq;
+  int64_t seq = static_cast<uint32_t>(r0) / static_cast<uint32_t>(a.rows_per_seq);
   int seq_left = static_cast<int>((seq + 1) * a.rows_per_seq - r0);
   const bool by_seq = (a.branch_weight.seq_stride | a.gate.seq_stride | a.weight.seq_stride) != 0;
   uint64_t element = static_cast<uint64_t>(r0) * a.hidden;  // the row's first
@@ -206,7 +205,8 @@ cudaError_t launch_rows(const ResidualArgs& a, int threads, cudaStream_t st) {
   note_launch();
   return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a,
                           RowPlan{threads, groups, {a.x_stride * static_cast<int64_t>(sizeof(TX)),
-                                                    a.res_stride * static_cast<int64_t>(sizeof(TR))}, 3});
+                                                    a.res_stride * static_cast<int64_t>(sizeof(TR))}, 3,
+                                  Split::make(a.rows, grid * groups)});
 }
 
 template <typename TX, typename TR>

@@ -32,10 +32,11 @@ enum RowSum : int { SUM_BRANCH = 0, SUM_WEIGHT = 1, SUM_SHIFT = 2, SUMS = 3 };
 // a sequence's own).
 struct RowItems {
   int64_t seqs, seq_rows, chunks;
+  Split runs;  // a sequence's rows over its items
   __host__ __device__ int64_t count() const { return seqs * chunks; }
-  __device__ int64_t first_row(int64_t item) const {
-    const int64_t b = item / chunks, c = item - b * chunks;
-    return b * seq_rows + c * seq_rows / chunks;
+  __device__ int64_t first_row(uint32_t item) const {
+    const uint32_t b = item / static_cast<uint32_t>(chunks), c = item - b * static_cast<uint32_t>(chunks);
+    return b * seq_rows + runs.first(c);
   }
 };
 
@@ -82,7 +83,9 @@ template <class Cols> struct RowKept<Cols, true> {
 struct BackwardPlan {
   RowPlan rows;
   RowItems items;
-  float* partials[SUMS];  // [items][hidden], or NULL: not wanted
+  bool joined;            // a group has one item at most, and a CTA joins its groups' sums into one partial row
+  int64_t parts;          // partial rows: items, or CTAs
+  float* partials[SUMS];  // [parts][hidden], or NULL: not wanted
 };
 
 template <typename TX, typename TR, int E, int V, int STAGES>
@@ -112,15 +115,38 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   for (int i = threadIdx.x; i < 8 * kMaxRowWarps * kMaxRowWarps; i += blockDim.x) (&red[0][0][0])[i] = 0.f;
   __syncthreads();
   griddep_wait();
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * plan.rows.groups;
-  const int64_t me = static_cast<int64_t>(blockIdx.x) * plan.rows.groups + group;
+  const uint32_t me = blockIdx.x * plan.rows.groups + group;
   const RowItems items = plan.items;
-  int64_t item = me * items.count() / groups;
-  const int64_t last = (me + 1) * items.count() / groups;
+  uint32_t item = plan.rows.share.first(me);
+  const uint32_t last = plan.rows.share.first(me + 1);
+  const Cols cols(t, threads, a.hidden);
+  KeptRows kept(TENSOR ? tensor_base : 0u);
+  auto clear = [&] {
+    F2 zero[BP];
+#pragma unroll
+    for (int j = 0; j < BP; ++j) zero[j] = f2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < SUMS; ++i) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) kept.write(i, b, zero);
+    }
+  };
+  // This thread's columns of the sums to a partial row.
+  auto give = [&](int i, float* row) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      F2 v[BP];
+      kept.read(i, b, v);
+      kept.wait();
+      kept.arrived(v);
+      cols.store(row + cols.first, b, v);
+      __syncwarp();
+    }
+  };
+  clear();
   if (item < last) {
     const int64_t r0 = items.first_row(item);
     int left = static_cast<int>(items.first_row(last) - r0);
-    const Cols cols(t, threads, a.hidden);
     RowStream<TX, TR, E, V, 2, 2, STAGES> rows;
     rows.template set<TX>(0, a.x, r0, plan.rows.step[0], cols);
     rows.template set<TX>(1, a.dy, r0, plan.rows.step[1], cols);
@@ -133,30 +159,21 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     int turn = 0;  // of the parts of a sum
     const float2* rstd = reinterpret_cast<const float2*>(a.rstd) + r0;
     float2 next_r = *rstd;  // loaded a row ahead
-    KeptRows kept(TENSOR ? tensor_base : 0u);
-    int64_t seq = r0 / a.rows_per_seq;
+    int64_t seq = static_cast<uint32_t>(r0) / static_cast<uint32_t>(a.rows_per_seq);
     int seq_left = static_cast<int>((seq + 1) * a.rows_per_seq - r0);
     const bool by_seq = (a.branch_weight.seq_stride | a.gate.seq_stride | a.weight.seq_stride) != 0;
     auto params = [&] {
+      F2 c[NB][BP], w[NB][BP];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        F2 f[BP];
-        cols.branch_coefficient(a, seq, b, f);
-        __syncwarp();
-        kept.write(KEPT_C, b, f);
-        cols.param(a.weight, seq, 1.f, b, f);
-        __syncwarp();
-        kept.write(KEPT_W, b, f);
+        cols.branch_coefficient(a, seq, b, c[b]);
+        cols.param(a.weight, seq, 1.f, b, w[b]);
       }
-    };
-    auto clear = [&] {
-      F2 zero[BP];
+      __syncwarp();
 #pragma unroll
-      for (int j = 0; j < BP; ++j) zero[j] = f2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < SUMS; ++i) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b) kept.write(i, b, zero);
+      for (int b = 0; b < NB; ++b) {
+        kept.write(KEPT_C, b, c[b]);
+        kept.write(KEPT_W, b, w[b]);
       }
     };
     uint64_t element = static_cast<uint64_t>(r0) * a.hidden;  // the row's first
@@ -165,7 +182,6 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     const bool sum_branch = plan.partials[SUM_BRANCH] != nullptr, sum_weight = plan.partials[SUM_WEIGHT] != nullptr,
                sum_shift = plan.partials[SUM_SHIFT] != nullptr, normed = a.dy != nullptr;
     params();
-    clear();
     int item_left = static_cast<int>(items.first_row(item + 1) - r0);
     for (;;) {
       const uint32_t bits = a.dropped ? cols.kept(a.drop, key, element) : ~0u;
@@ -264,21 +280,11 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       }
       dx += a.hidden;
       dres += a.hidden;
-      if (--item_left == 0) {
+      if (--item_left == 0 && !plan.joined) {
         kept.settle();
 #pragma unroll
-        for (int i = 0; i < SUMS; ++i) {
-          if (plan.partials[i] == nullptr) continue;
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            F2 v[BP];
-            kept.read(i, b, v);
-            kept.wait();
-            kept.arrived(v);
-            cols.store(plan.partials[i] + item * a.hidden + cols.first, b, v);
-            __syncwarp();
-          }
-        }
+        for (int i = 0; i < SUMS; ++i)
+          if (plan.partials[i] != nullptr) give(i, plan.partials[i] + static_cast<int64_t>(item) * a.hidden);
         clear();
         ++item;
         if (item < last) item_left = static_cast<int>(items.first_row(item + 1) - items.first_row(item));
@@ -292,8 +298,26 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       }
     }
   }
+  kept.settle();
+  if (plan.joined) {
+    // over the ring: no copy is in flight past the last row, and the other groups are done with theirs
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    float* parts = reinterpret_cast<float*>(smem);  // [SUMS][groups][hidden]
+#pragma unroll
+    for (int i = 0; i < SUMS; ++i)
+      if (plan.partials[i] != nullptr) give(i, parts + (i * plan.rows.groups + group) * a.hidden);
+    __syncthreads();
+    for (int i = 0; i < SUMS; ++i) {
+      if (plan.partials[i] == nullptr) continue;
+      for (int c = threadIdx.x; c < a.hidden; c += blockDim.x) {
+        float v = 0.f;
+        for (int g = 0; g < plan.rows.groups; ++g) v += parts[(i * plan.rows.groups + g) * a.hidden + c];
+        plan.partials[i][static_cast<int64_t>(blockIdx.x) * a.hidden + c] = v;
+      }
+    }
+  }
   if constexpr (TENSOR) {
-    tmem_st_wait();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -377,7 +401,7 @@ __global__ void __launch_bounds__(kRowThreads)
   }
 }
 
-// One parameter's gradient: out[o, i] = factor * sum over the output's items of other[sequence, i] * partials[item, i].
+// One parameter's gradient: out[o, i] = factor * sum over the output's partial rows of other[sequence, i] * partials[m, i].
 struct ParamSum {
   const float* partials;
   RowParam out;    // `grad` with dtype; one row for all or (seq_stride not 0) one for each sequence
@@ -387,39 +411,68 @@ struct ParamSum {
 struct ParamSums {
   ParamSum of[4];
   int n;
-  RowItems items;
-  int64_t seqs;
+  uint32_t parts, chunks, seqs;  // partial rows; of a sequence; sequences
   int hidden;
 };
 
-// 32 columns of one output per CTA; `blockDim.y` threads a column take every so manyth item.
-__global__ void residual_param_grad_kernel(const __grid_constant__ ParamSums s) {
-  __shared__ double red[32][33];
+// C neighbouring columns of one output for each lane of a CTA, whose warps take every so manyth partial row, several
+// loads in flight; sums in fp64. Bound by latency: the partial rows come from L2.
+template <int C>
+__global__ void __launch_bounds__(512) residual_param_grad_kernel(const __grid_constant__ ParamSums s) {
+  constexpr int AHEAD = 10;  // 16 warps of them cover a partial row for each SM
+  __shared__ double red[16][32 * C + 1];
   griddep_launch_dependents();
-  griddep_wait();
   const ParamSum& p = s.of[blockIdx.y];
-  const int64_t col_blocks = (s.hidden + 31) / 32;
-  const int64_t outs = p.out.seq_stride != 0 ? s.seqs : 1;
-  for (int64_t job = blockIdx.x; job < outs * col_blocks; job += gridDim.x) {
-    const int64_t o = job / col_blocks;
-    const int i = static_cast<int>(job - o * col_blocks) * 32 + threadIdx.x;
-    const int64_t i0 = p.out.seq_stride != 0 ? o * s.items.chunks : 0;
-    const int64_t i1 = p.out.seq_stride != 0 ? i0 + s.items.chunks : s.items.count();
-    double t = 0.0;
+  const uint32_t col_blocks = (s.hidden + 32 * C - 1) / (32 * C);
+  const bool own = p.out.seq_stride != 0;
+  const uint32_t jobs = (own ? s.seqs : 1u) * col_blocks;
+  const uint32_t warps = blockDim.x / 32, warp = threadIdx.x / 32;
+  const int lane = threadIdx.x & 31;
+  // a factor that differs between the rows of an output goes into the sum, another one behind it
+  const bool inside = p.other.p != nullptr && p.other.seq_stride != 0 && !own;
+  griddep_wait();
+  for (uint32_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+    const uint32_t o = job / col_blocks;
+    const int i = static_cast<int>(job - o * col_blocks) * 32 * C + lane * C;
+    const uint32_t m1 = own ? (o + 1) * s.chunks : s.parts;
+    double t[C] = {};
     if (i < s.hidden) {
-      for (int64_t m = i0 + threadIdx.y; m < i1; m += blockDim.y) {
-        double v = p.partials[m * s.hidden + i];
-        if (p.other.p != nullptr)
-          v *= load_as_float(p.other.p, (m / s.items.chunks) * p.other.seq_stride + i, p.other.dtype);
-        t += v;
+      for (uint32_t m0 = (own ? o * s.chunks : 0u) + warp; m0 < m1; m0 += warps * AHEAD) {
+        float v[AHEAD][C];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const uint32_t m = m0 + k * warps;
+#pragma unroll
+          for (int j = 0; j < C; ++j) v[k][j] = 0.f;
+          if (m < m1) load_floats<C>(p.partials, static_cast<int64_t>(m) * s.hidden + i, F32, v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const uint32_t m = m0 + k * warps;
+#pragma unroll
+          for (int j = 0; j < C; ++j) {
+            double x = v[k][j];
+            if (inside && m < m1)
+              x *= load_as_float(p.other.p, static_cast<int64_t>(m / s.chunks) * p.other.seq_stride + i + j, p.other.dtype);
+            t[j] += x;
+          }
+        }
       }
     }
-    red[threadIdx.y][threadIdx.x] = t;
+#pragma unroll
+    for (int j = 0; j < C; ++j) red[warp][lane * C + j] = t[j];
     __syncthreads();
-    if (threadIdx.y == 0 && i < s.hidden) {
-      for (int y = 1; y < static_cast<int>(blockDim.y); ++y) t += red[y][threadIdx.x];
-      const float v = static_cast<float>(t * p.factor);
-      const int64_t at = o * s.hidden + i;
+    for (int c = threadIdx.x; c < 32 * C; c += blockDim.x) {
+      const int col = i - lane * C + c;
+      if (col >= s.hidden) break;
+      double sum = 0.0;
+#pragma unroll
+      for (int w = 0; w < 16; ++w)
+        if (w < static_cast<int>(warps)) sum += red[w][c];
+      if (p.other.p != nullptr && !inside)
+        sum *= load_as_float(p.other.p, static_cast<int64_t>(own ? o : 0u) * p.other.seq_stride + col, p.other.dtype);
+      const float v = static_cast<float>(sum * p.factor);
+      const int64_t at = static_cast<int64_t>(o) * s.hidden + col;
       if (p.out.dtype == F32) static_cast<float*>(p.out.grad)[at] = v;
       else if (p.out.dtype == F16) static_cast<__half*>(p.out.grad)[at] = __float2half_rn(v);
       else static_cast<__nv_bfloat16*>(p.out.grad)[at] = __float2bfloat16_rn(v);
@@ -442,8 +495,11 @@ struct Shape {
 Shape shape_of(const ResidualArgs& a) {
   const int e = row_chunk(a, true);
   if (e > 1) {
-    // a warp a row as far as 8 columns a thread carry it, then 16 columns a thread
+    // A warp a row as far as 8 columns a thread carry it, then 16 columns a thread; with 4 bytes a column 8 as far
+    // as they go, for which more rows fit into shared memory.
     if (a.hidden <= 256) return {e, 8 / e, 32};
+    if (a.x_dtype == F32)
+      if (const int t = row_threads(a.hidden, e, 8 / e)) return {e, 8 / e, t};
     if (const int t = row_threads(a.hidden, e, 16 / e)) return {e, 16 / e, t};
   } else {
     for (int v = 4; v <= 8; v *= 2)
@@ -462,6 +518,7 @@ RowItems items_of(const ResidualArgs& a, int threads) {
   const int64_t groups = static_cast<int64_t>(num_sms()) * (kRowThreads / threads);
   it.chunks = std::max({groups / it.seqs, (it.seq_rows + kItemRows - 1) / kItemRows, int64_t{1}});
   it.chunks = std::min(it.chunks, it.seq_rows);
+  it.runs = Split::make(it.seq_rows, it.chunks);
   return it;
 }
 
@@ -477,12 +534,18 @@ cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t 
   plan.rows.present = 1 | (a.dy != nullptr ? 2 | 4 : 0) | (a.dh != nullptr ? 8 : 0);  // h serves the norm alone
   plan.rows.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, count / num_sms())));
   const int block = plan.rows.groups * threads;
-  const size_t smem = Stream::kSmemBytes;
+  // the ring, and in its place the groups' sums
+  const size_t smem = std::max(Stream::kSmemBytes, sizeof(float) * SUMS * kRowThreads * E * V);
   const void* fn = reinterpret_cast<const void*>(kernel);
   // at least a little over 48 KB: the sums' static part comes on top
   if (const cudaError_t e = ensure_smem_attr(fn, std::max<size_t>(smem, 49 * 1024)); e != cudaSuccess) return e;
   const int64_t all = static_cast<int64_t>(num_sms()) * std::max(1, cached_occupancy(fn, block, smem));
   const int64_t grid = std::min<int64_t>(all, (count + plan.rows.groups - 1) / plan.rows.groups);
+  plan.rows.share = Split::make(count, grid * plan.rows.groups);
+  if (plan.items.seqs == 1 && count <= grid * plan.rows.groups) {
+    plan.joined = true;
+    plan.parts = grid;
+  }
   note_launch();
   return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a, plan);
 }
@@ -517,6 +580,7 @@ cudaError_t residual_norm_backward_launch(const ResidualArgs& a, void* ws, cudaS
   BackwardPlan plan{};
   plan.rows.threads = sh.threads;
   plan.items = items_of(a, sh.threads);
+  plan.parts = plan.items.count();
   float* at = static_cast<float*>(ws);
   const int64_t count = plan.items.count();
   bool any = false;
@@ -536,8 +600,9 @@ cudaError_t residual_norm_backward_launch(const ResidualArgs& a, void* ws, cudaS
     e = launch_types<float, float>(a, plan, sh, st);
   if (e != cudaSuccess || !any) return e;
   ParamSums s{};
-  s.items = plan.items;
-  s.seqs = a.rows / a.rows_per_seq;
+  s.parts = static_cast<uint32_t>(plan.parts);
+  s.chunks = static_cast<uint32_t>(plan.items.chunks);
+  s.seqs = static_cast<uint32_t>(a.rows / a.rows_per_seq);
   s.hidden = a.hidden;
   const float f = a.dropped ? a.scale * a.drop.scale : a.scale;
   const RowParam none{};
@@ -548,17 +613,17 @@ cudaError_t residual_norm_backward_launch(const ResidualArgs& a, void* ws, cudaS
   add(SUM_BRANCH, a.branch_weight, a.gate, f);
   add(SUM_WEIGHT, a.weight, none, 1.f);
   add(SUM_SHIFT, a.shift, none, 1.f);
-  int64_t outs = 1, most = 1;  // outputs, and items of one
+  int64_t outs = 1, most = 1;  // outputs, and partial rows of one
   for (int i = 0; i < s.n; ++i) {
     const bool own = s.of[i].out.seq_stride != 0;
-    outs = std::max(outs, own ? s.seqs : 1);
-    most = std::max(most, own ? plan.items.chunks : count);
+    outs = std::max<int64_t>(outs, own ? s.seqs : 1);
+    most = std::max(most, own ? plan.items.chunks : plan.parts);
   }
-  int lanes = 1;
-  while (lanes < 32 && lanes < most) lanes *= 2;
+  const int c = a.hidden % 2 == 0 ? 2 : 1;
+  const int warps = static_cast<int>(std::min<int64_t>(16, (most + 1) / 2));  // two loads a lane at least
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(outs * ((a.hidden + 31) / 32), num_sms() * 64ll)), s.n);
-  cfg.blockDim = dim3(32, lanes);
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(outs * ((a.hidden + 32 * c - 1) / (32 * c)), num_sms() * 16ll)), s.n);
+  cfg.blockDim = dim3(std::max(1, warps) * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -566,7 +631,7 @@ cudaError_t residual_norm_backward_launch(const ResidualArgs& a, void* ws, cudaS
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   note_launch();
-  return cudaLaunchKernelEx(&cfg, residual_param_grad_kernel, s);
+  return cudaLaunchKernelEx(&cfg, c == 2 ? residual_param_grad_kernel<2> : residual_param_grad_kernel<1>, s);
 }
 
 }  // namespace tfo
