@@ -13,30 +13,33 @@
 namespace tfo {
 
 struct DropKey {
-  uint32_t k0, k1;      // the seed
-  uint32_t off0, off1;  // the call's offset
+  uint32_t k0[10], k1[10];  // the rounds' keys
+  uint32_t off0, off1;      // the call's offset
   uint32_t threshold;
   __device__ explicit DropKey(const DropoutArgs& d) : threshold(d.threshold) {
     const uint64_t seed = d.seed_ptr != nullptr ? static_cast<uint64_t>(*d.seed_ptr) : d.seed;
-    k0 = static_cast<uint32_t>(seed);
-    k1 = static_cast<uint32_t>(seed >> 32);
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+      k0[i] = static_cast<uint32_t>(seed) + i * 0x9E3779B9u;
+      k1[i] = static_cast<uint32_t>(seed >> 32) + i * 0xBB67AE85u;
+    }
     off0 = static_cast<uint32_t>(d.offset);
     off1 = static_cast<uint32_t>(d.offset >> 32);
   }
-  __device__ uint4 block(uint64_t counter) const {
-    uint32_t a = static_cast<uint32_t>(counter), b = static_cast<uint32_t>(counter >> 32), c = off0, d = off1;
-    uint32_t x = k0, y = k1;
+  __device__ uint4 block(uint32_t counter, uint32_t counter_high) const {
+    uint32_t a = counter, b = counter_high, c = off0, d = off1;
 #pragma unroll
     for (int i = 0; i < 10; ++i) {
       const uint64_t p = static_cast<uint64_t>(0xD2511F53u) * a, q = static_cast<uint64_t>(0xCD9E8D57u) * c;
-      a = static_cast<uint32_t>(q >> 32) ^ b ^ x;
+      a = static_cast<uint32_t>(q >> 32) ^ b ^ k0[i];
       b = static_cast<uint32_t>(q);
-      c = static_cast<uint32_t>(p >> 32) ^ d ^ y;
+      c = static_cast<uint32_t>(p >> 32) ^ d ^ k1[i];
       d = static_cast<uint32_t>(p);
-      x += 0x9E3779B9u;
-      y += 0xBB67AE85u;
     }
     return make_uint4(a, b, c, d);
+  }
+  __device__ uint4 block(uint64_t counter) const {
+    return block(static_cast<uint32_t>(counter), static_cast<uint32_t>(counter >> 32));
   }
   // bits * 2 + (whether an element with this word is kept); the threshold is not 0.
   __device__ uint32_t push(uint32_t bits, uint32_t word) const {
