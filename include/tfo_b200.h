@@ -355,7 +355,14 @@ typedef struct tfo_axes {
   int axes;                    /* 2..4 */
   int64_t pos_stride;          /* elements between the axes' positions */
   const uint8_t* axis_of_pair; /* host memory, one for each pair of columns */
+  void* workspace;             /* heads: tfo_rope_axes_workspace_bytes of scratch, or NULL */
+  size_t workspace_bytes;
 } tfo_axes;
+
+/* Scratch with which calls of many tokens put each token's table row together
+ * first where axes share vectors of columns (without it they are slower).
+ * 16-byte aligned, not shared by calls that may alternate on a stream. */
+TFO_API size_t tfo_rope_axes_workspace_bytes(int64_t tokens, int64_t rotary_dim, int table_dtype);
 
 TFO_API int tfo_rope_tables_axes(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half,
                                  double gain, void* cos, void* sin, int out_dtype, const tfo_axes* axes,

@@ -252,6 +252,7 @@ struct HeadTables {
   int axes;  // 0 or 1: one position
   int64_t pos_stride_axis;
   uint32_t axis_bits[kMaxAxisPairs / 16];  // two bits a pair
+  void* joined;  // room for each token's joined row (axes_workspace_bytes), or NULL
 };
 struct HeadSide {  // the queries or the keys
   const void* x;   // [batch, seq, heads, head_dim]
@@ -275,7 +276,14 @@ struct HeadArgs {
   int dtype;
 };
 cudaError_t qk_rope_launch(const HeadArgs& a, cudaStream_t st);
-cudaError_t qk_rope_axes_launch(const HeadArgs& a, cudaStream_t st);  // qk_rope_axes.cu: a.t.axes > 1
+// a.t.axes > 1 (qk_rope_axes.cu): pairs at their axes' table rows, or rows joined
+// for each token beforehand and the launch of one position.
+cudaError_t qk_rope_axes_launch(const HeadArgs& a, cudaStream_t st);
+size_t axes_workspace_bytes(int64_t tokens, int pairs, int table_dtype);
+// Joins the rows of `a`, if it has room for them and that is the faster way, and makes it a call of one position.
+cudaError_t join_axes(HeadArgs* a, bool backward, cudaStream_t st);
+// Whether the tokens are enough for the streaming kernel (qk_rope.cu).
+bool head_streams(const HeadArgs& a, int elems);
 size_t qk_norm_rope_backward_workspace_bytes(int head_dim);
 cudaError_t qk_norm_rope_backward_launch(const HeadArgs& a, void* ws, cudaStream_t st);
 cudaError_t qk_norm_rope_backward_axes_launch(const HeadArgs& a, void* ws, cudaStream_t st);  // qk_rope_backward_axes.cu

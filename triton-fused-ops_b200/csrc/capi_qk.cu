@@ -55,7 +55,8 @@ int set_heads(HeadArgs* a, const std::string& fn, const void* q, const int64_t* 
   set_side(&a->q, q, q_strides, q_out, q_heads);
   set_side(&a->k, k, k_strides, k_out, k_heads);
   a->t = HeadTables{cos,       sin,       table_stride,     table_rows,     table_dtype,
-                    positions, pos_dtype, pos_stride_batch, pos_stride_seq, 0, 0, {}};
+                    positions, pos_dtype, pos_stride_batch, pos_stride_seq, 0, 0, {}, nullptr};
+  if (pos_dtype == TFO_POS_NONE) a->t.pos_stride_batch = 0;  // the sequences share the table
   a->batch = batch;
   a->seq = seq;
   a->head_dim = static_cast<int>(head_dim);
@@ -83,6 +84,12 @@ int set_axes(HeadArgs* a, const std::string& fn, const tfo_axes* axes) {
   if (st != TFO_OK) return st;
   a->t.axes = axes->axes;
   a->t.pos_stride_axis = axes->pos_stride;
+  const size_t room = axes_workspace_bytes(a->batch * a->seq, a->rotary_dim / 2, a->t.dtype);
+  if (axes->workspace != nullptr) {
+    if (axes->workspace_bytes < room || reinterpret_cast<uintptr_t>(axes->workspace) % 16 != 0)
+      return fail(TFO_ERR_INVALID, fn + ": the axes' workspace is too small or not aligned");
+    a->t.joined = axes->workspace;
+  }
   return TFO_OK;
 }
 
@@ -92,6 +99,11 @@ int set_axes(HeadArgs* a, const std::string& fn, const tfo_axes* axes) {
 using namespace tfo;
 
 extern "C" {
+
+size_t tfo_rope_axes_workspace_bytes(int64_t tokens, int64_t rotary_dim, int table_dtype) {
+  if (tokens <= 0 || rotary_dim <= 0 || rotary_dim > 2 * kMaxAxisPairs || !is_float_dtype(table_dtype)) return 0;
+  return axes_workspace_bytes(tokens, static_cast<int>(rotary_dim / 2), table_dtype);
+}
 
 int tfo_rope_tables_axes(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half,
                          double gain, void* cos, void* sin, int out_dtype, const tfo_axes* axes, void* stream) {

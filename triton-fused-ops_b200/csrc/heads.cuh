@@ -143,11 +143,11 @@ __device__ __forceinline__ LaneCols lane_cols(int p, int lanes, int nvec, int ro
 }
 
 // ---- a token's table row ----------------------------------------------------
-// The position of token (b, s): given, or s itself. A given position outside
+// The position of token (b, s): given, or s itself (s of sequence b's own rows). A given position outside
 // the table is recorded in the device error word and returned as -1 (its
 // rotated columns become NaN; the table is not read).
 __device__ __forceinline__ int64_t token_position(const HeadTables& t, int64_t b, int64_t s, uint32_t* err, bool report) {
-  int64_t pos = s;
+  int64_t pos = b * t.pos_stride_batch + s;  // without positions: rows per sequence, 0 where they share the table
   if (t.pos_dtype == POS_I64) {
     pos = reinterpret_cast<const int64_t*>(t.positions)[b * t.pos_stride_batch + s * t.pos_stride_seq];
   } else if (t.pos_dtype == POS_I32) {
@@ -197,6 +197,30 @@ __device__ __forceinline__ int64_t axis_position(const HeadTables& t, int64_t b,
   return pos;
 }
 
+// H neighbouring pairs of several axes, column by column, all loads in flight.
+template <typename T, int H>
+__device__ __forceinline__ void mixed_table(const HeadTables& t, int64_t b, int64_t s, uint32_t bits, int first, uint32_t* err,
+                                            float* c, float* sn) {
+  int64_t pos[kMaxAxes];
+#pragma unroll
+  for (int i = 0; i < kMaxAxes; ++i) pos[i] = i < t.axes ? axis_position(t, b, s, i, err) : 0;
+  T x[H], y[H];
+#pragma unroll
+  for (int j = 0; j < H; ++j) {
+    const uint32_t axis = bits >> (2 * j) & 3u;
+    const int64_t p = axis == 0 ? pos[0] : axis == 1 ? pos[1] : axis == 2 ? pos[2] : pos[3];
+    const int64_t at = max(p, int64_t{0}) * t.row_stride + first + j;
+    x[j] = static_cast<const T*>(t.cos)[at];
+    y[j] = static_cast<const T*>(t.sin)[at];
+    c[j] = p < 0 ? __int_as_float(0x7fffffff) : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < H; ++j) {
+    sn[j] = c[j] + Ty<T>::to_f(y[j]);  // 0, or NaN for a bad position
+    c[j] += Ty<T>::to_f(x[j]);
+  }
+}
+
 // lane_table for a token with a position on each axis. Pairs of an axis whose position is bad become NaN.
 template <int E, bool PAIRS>
 __device__ __forceinline__ void lane_table_axes(const HeadTables& t, int64_t b, int64_t s, const LaneCols& col,
@@ -221,20 +245,12 @@ __device__ __forceinline__ void lane_table_axes(const HeadTables& t, int64_t b, 
         c[v * H + j] = x[j];
         sn[v * H + j] = y[j];
       }
+    } else if (t.dtype == F32) {
+      mixed_table<float, H>(t, b, s, ax.bits >> (2 * v * H), first, err, c + v * H, sn + v * H);
+    } else if (t.dtype == F16) {
+      mixed_table<__half, H>(t, b, s, ax.bits >> (2 * v * H), first, err, c + v * H, sn + v * H);
     } else {
-      int64_t row[kMaxAxes];  // a bad one is negative
-#pragma unroll
-      for (int i = 0; i < kMaxAxes; ++i) {
-        const int64_t pos = i < t.axes ? axis_position(t, b, s, i, err) : -1;
-        row[i] = pos < 0 ? -1 : pos * t.row_stride;
-      }
-#pragma unroll
-      for (int j = 0; j < H; ++j) {
-        const uint32_t axis = ax.bits >> (2 * (v * H + j)) & 3u;
-        const int64_t at = axis == 0 ? row[0] : axis == 1 ? row[1] : axis == 2 ? row[2] : row[3];
-        c[v * H + j] = at < 0 ? __int_as_float(0x7fffffff) : load_as_float(t.cos, at + first + j, t.dtype);
-        sn[v * H + j] = at < 0 ? __int_as_float(0x7fffffff) : load_as_float(t.sin, at + first + j, t.dtype);
-      }
+      mixed_table<__nv_bfloat16, H>(t, b, s, ax.bits >> (2 * v * H), first, err, c + v * H, sn + v * H);
     }
   }
   if (inverse) {

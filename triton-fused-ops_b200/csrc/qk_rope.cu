@@ -39,6 +39,8 @@ int head_vector_elems(const HeadArgs& a, bool backward) {
   return 0;
 }
 
+bool head_streams(const HeadArgs& a, int elems) { return head_warps4(a, elems) >= static_cast<int64_t>(num_sms()) * 24; }
+
 cudaError_t qk_rope_launch(const HeadArgs& a, cudaStream_t st) {
   return a.t.axes > 1 ? qk_rope_axes_launch(a, st) : launch_rope<false>(a, st);
 }

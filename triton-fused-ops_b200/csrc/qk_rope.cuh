@@ -260,6 +260,12 @@ __global__ void __launch_bounds__(256) qk_rope_any_kernel(const HeadArgs a, int6
 }
 
 namespace {
+// Warps that units of four heads make.
+inline int64_t head_warps4(const HeadArgs& a, int elems) {
+  const int lanes = (a.head_dim / elems + 1) / 2;
+  return a.batch * a.seq * ((a.q.heads + 3) / 4 + (a.k.heads + 3) / 4) / (32 / lanes);
+}
+
 template <typename T, int E, bool PAIRS, bool NORM, int NH, bool AXES>
 cudaError_t launch_units(const HeadArgs& a, int lanes, cudaStream_t st) {
   const uint32_t qc = (a.q.heads + NH - 1) / NH, kc = (a.k.heads + NH - 1) / NH;
@@ -306,9 +312,8 @@ cudaError_t launch_form(const HeadArgs& a, cudaStream_t st) {
   //            65536: 425 / 289 / 214
   // A few tokens want every SM at work, four heads share the table columns and
   // the division of the token index, the stream keeps more loads in flight.
-  const int64_t units4 = a.batch * a.seq * ((a.q.heads + 3) / 4 + (a.k.heads + 3) / 4);
-  const int64_t warps4 = units4 / (32 / lanes);
-  if (warps4 >= static_cast<int64_t>(num_sms()) * 24) return launch_stream<T, E, PAIRS, NORM, 4, 3, AXES>(a, lanes, st);
+  const int64_t warps4 = head_warps4(a, E);
+  if (head_streams(a, E)) return launch_stream<T, E, PAIRS, NORM, 4, 3, AXES>(a, lanes, st);
   if (warps4 >= static_cast<int64_t>(num_sms()) * 8) return launch_units<T, E, PAIRS, NORM, 4, AXES>(a, lanes, st);
   return launch_units<T, E, PAIRS, NORM, 1, AXES>(a, lanes, st);
 }

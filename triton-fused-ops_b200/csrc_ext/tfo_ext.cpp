@@ -247,6 +247,7 @@ struct HeadsCall {  // the C ABI's shared arguments
   int pos_dtype = TFO_POS_NONE;
   int64_t pos_sb = 0, pos_ss = 0, batch, seq, q_heads, k_heads, dim, rot;
   tfo_axes axes_of{};
+  at::Tensor joined;  // scratch of the axes
   HeadsCall(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos, const at::Tensor& pos, const at::Tensor& axes)
       : positions(&pos) {
     if (pos.defined()) {
@@ -254,7 +255,13 @@ struct HeadsCall {  // the C ABI's shared arguments
       pos_sb = q.dim() == 4 ? pos.stride(-2) : 0;
       pos_ss = pos.stride(-1);
     }
-    if (axes.defined()) axes_of = {axis_count(axes), pos.stride(0), axes.data_ptr<uint8_t>()};
+    if (axes.defined()) {
+      joined = scratch(tfo_rope_axes_workspace_bytes(q.numel() / (q.size(-1) * q.size(-2)), cos.size(1),
+                                                     dtype_code(cos.scalar_type())),
+                       q.device());
+      axes_of = {axis_count(axes), pos.stride(0), axes.data_ptr<uint8_t>(), joined.data_ptr(),
+                 static_cast<size_t>(joined.numel())};
+    }
     batch = q.dim() == 4 ? q.size(0) : 1;
     seq = q.size(-3);
     q_heads = q.size(-2);
@@ -462,7 +469,8 @@ py::object rope_tables(const at::Tensor& positions, const at::Tensor& turns, dou
     return py::none();
   std::vector<int64_t> shape(positions.sizes().begin() + (axes.has_value() ? 1 : 0), positions.sizes().end());
   const int64_t rows = axes.has_value() ? positions.numel() / positions.size(0) : positions.numel();
-  const tfo_axes of = axes.has_value() ? tfo_axes{axis_count(*axes), rows, axes->data_ptr<uint8_t>()} : tfo_axes{};
+  const tfo_axes of = axes.has_value() ? tfo_axes{axis_count(*axes), rows, axes->data_ptr<uint8_t>(), nullptr, 0}
+                                          : tfo_axes{};
   shape.push_back(2 * half);
   const auto type = out_code == TFO_DTYPE_F16 ? at::kHalf : out_code == TFO_DTYPE_BF16 ? at::kBFloat16 : at::kFloat;
   at::Tensor cos = fresh(shape, type, positions.device());

@@ -74,7 +74,8 @@ class RowParam(ctypes.Structure):
 class Axes(ctypes.Structure):
     """tfo_axes."""
 
-    _fields_ = [("axes", _c_int), ("pos_stride", _c_i64), ("axis_of_pair", _c_vp)]
+    _fields_ = [("axes", _c_int), ("pos_stride", _c_i64), ("axis_of_pair", _c_vp), ("workspace", _c_vp),
+                ("workspace_bytes", _c_size)]
 
 
 _c_axes = ctypes.POINTER(Axes)
@@ -158,6 +159,7 @@ _SIGNATURES = {
          _c_vp, _c_vp, _c_vp, _c_vp, *_HEADS_SIZES, ctypes.c_double, _c_int, _c_int, _c_int, _c_int, _c_vp, _c_size,
          _c_vp],
     ),
+    "tfo_rope_axes_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_int]),
     "tfo_lora_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
     "tfo_lora": (
         _c_int,

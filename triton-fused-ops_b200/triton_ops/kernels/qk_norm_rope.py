@@ -49,11 +49,12 @@ def _weight_code(w: Optional[torch.Tensor], name: str) -> int:
 def _forward(q, k, qw, kw, cos, sin, positions, eps, interleaved, pair_axes=None):
     q_out, k_out = _empty_like_heads(q), _empty_like_heads(k)
     with _lib.on_device(q):
+        axes, axes_ws = _heads_axes(pair_axes, positions, cos)
         _lib.call("tfo_qk_norm_rope_axes", q.data_ptr(), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(qw), _lib.ptr(kw),
                   *_table_args(cos, sin, positions, q), q_out.data_ptr(), _lib.ptr(k_out),
                   *_size_args(q, k, cos, interleaved), float(eps), _lib.dtype_code(q.dtype, "q"),
                   _weight_code(qw, "q_weight"), _weight_code(kw, "k_weight"), _lib.dtype_code(cos.dtype, "cos"),
-                  _heads_axes(pair_axes, positions), _lib.stream_of(q))
+                  axes, _lib.stream_of(q))
     return q_out, k_out
 
 
@@ -97,6 +98,7 @@ def _backward(ctx, gq, gk):
     dkw = torch.empty_like(kw) if kw is not None and ctx.needs_input_grad[3] else None
     with _lib.on_device(q):
         ws = None
+        axes, axes_ws = _heads_axes(ctx.pair_axes, positions, cos)
         if dqw is not None or dkw is not None:
             ws = _lib.scratch(_lib.load().tfo_qk_norm_rope_backward_workspace_bytes(q.shape[-1]), q.device)
         _lib.call("tfo_qk_norm_rope_backward_axes", gq.data_ptr(), _strides(gq), _lib.ptr(gk), _strides(gk), q.data_ptr(),
@@ -104,7 +106,7 @@ def _backward(ctx, gq, gk):
                   *_table_args(cos, sin, positions, q), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dqw), _lib.ptr(dkw),
                   *_size_args(q, k, cos, ctx.interleaved), float(ctx.eps), _lib.dtype_code(q.dtype, "q"),
                   _weight_code(qw, "q_weight"), _weight_code(kw, "k_weight"), _lib.dtype_code(cos.dtype, "cos"),
-                  _lib.ptr(ws), 0 if ws is None else ws.numel(), _heads_axes(ctx.pair_axes, positions), _lib.stream_of(q))
+                  _lib.ptr(ws), 0 if ws is None else ws.numel(), axes, _lib.stream_of(q))
     return dq, dk, dqw, dkw
 
 

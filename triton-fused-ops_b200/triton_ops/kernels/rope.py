@@ -284,15 +284,21 @@ def _strides(t: Optional[torch.Tensor]):
     return (ctypes.c_int64 * 3)(*(s[:3] if t.dim() == 4 else (0, s[0], s[1])))
 
 
-def _axes_arg(pair_axes: Optional[torch.Tensor], pos_stride: int):
+def _axes_arg(pair_axes: Optional[torch.Tensor], pos_stride: int, ws: Optional[torch.Tensor] = None):
     """The C ABI's axes: NULL for one position."""
     if pair_axes is None:
         return None
-    return ctypes.byref(_lib.Axes(int(pair_axes.max()) + 1, pos_stride, pair_axes.data_ptr()))
+    return ctypes.byref(_lib.Axes(int(pair_axes.max()) + 1, pos_stride, pair_axes.data_ptr(), _lib.ptr(ws),
+                                  0 if ws is None else ws.numel()))
 
 
-def _heads_axes(pair_axes, positions):
-    return _axes_arg(pair_axes, 0 if pair_axes is None else positions.stride(0))
+def _heads_axes(pair_axes, positions, cos):
+    """(the C ABI's axes, their scratch, to be kept until the call is made)."""
+    if pair_axes is None:
+        return None, None
+    ws = _lib.scratch(_lib.load().tfo_rope_axes_workspace_bytes(positions[0].numel(), cos.shape[1], _lib.dtype_code(cos.dtype)),
+                      cos.device)
+    return _axes_arg(pair_axes, positions.stride(0), ws), ws
 
 
 def _table_args(cos, sin, positions, q):
@@ -317,10 +323,10 @@ def _rotate(q, k, cos, sin, positions, interleaved, inverse, pair_axes=None):
     """Launches tfo_rope on checked arguments."""
     q_out, k_out = _empty_like_heads(q), _empty_like_heads(k)
     with _lib.on_device(q):
+        axes, ws = _heads_axes(pair_axes, positions, cos)
         _lib.call("tfo_rope_axes", q.data_ptr(), _strides(q), _lib.ptr(k), _strides(k), *_table_args(cos, sin, positions, q),
                   q_out.data_ptr(), _lib.ptr(k_out), *_size_args(q, k, cos, interleaved), int(inverse),
-                  _lib.dtype_code(q.dtype, "q"), _lib.dtype_code(cos.dtype, "cos"), _heads_axes(pair_axes, positions),
-                  _lib.stream_of(q))
+                  _lib.dtype_code(q.dtype, "q"), _lib.dtype_code(cos.dtype, "cos"), axes, _lib.stream_of(q))
     return q_out, k_out
 
 
