@@ -83,9 +83,8 @@ template <class Cols> struct RowKept<Cols, true> {
 struct BackwardPlan {
   RowPlan rows;
   RowItems items;
-  bool joined;            // a group has one item at most, and a CTA joins its groups' sums into one partial row
-  int64_t parts;          // partial rows: items, or CTAs
-  float* partials[SUMS];  // [parts][hidden], or NULL: not wanted
+  bool joined;            // an item for each CTA, whose groups share its rows and join their sums; else items by group
+  float* partials[SUMS];  // [items][hidden], or NULL: not wanted
 };
 
 template <typename TX, typename TR, int E, int V, int STAGES>
@@ -117,8 +116,19 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   griddep_wait();
   const uint32_t me = blockIdx.x * plan.rows.groups + group;
   const RowItems items = plan.items;
-  uint32_t item = plan.rows.share.first(me);
-  const uint32_t last = plan.rows.share.first(me + 1);
+  uint32_t item = plan.joined ? blockIdx.x : plan.rows.share.first(me);
+  const uint32_t last = plan.joined ? item + 1 : plan.rows.share.first(me + 1);
+  int64_t r0 = 0;
+  int left = 0;
+  if (item < last) {
+    r0 = items.first_row(item);
+    left = static_cast<int>(items.first_row(last) - r0);
+    if (plan.joined) {
+      const int n = plan.rows.groups, from = left * group / n;
+      left = left * (group + 1) / n - from;
+      r0 += from;
+    }
+  }
   const Cols cols(t, threads, a.hidden);
   KeptRows kept(TENSOR ? tensor_base : 0u);
   auto clear = [&] {
@@ -144,9 +154,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     }
   };
   clear();
-  if (item < last) {
-    const int64_t r0 = items.first_row(item);
-    int left = static_cast<int>(items.first_row(last) - r0);
+  if (left > 0) {
     RowStream<TX, TR, E, V, 2, 2, STAGES> rows;
     rows.template set<TX>(0, a.x, r0, plan.rows.step[0], cols);
     rows.template set<TX>(1, a.dy, r0, plan.rows.step[1], cols);
@@ -508,16 +516,23 @@ Shape shape_of(const ResidualArgs& a) {
   return {1, 0, kRowThreads};
 }
 
-// The split: items for every group of a full grid, and short enough for fp32 sums.
-RowItems items_of(const ResidualArgs& a, int threads) {
+// The split. One item for each CTA of a full grid where that leaves few of them without one and the rows of an item are
+// few enough for fp32 sums; else (many sequences, very many rows) items for every group.
+RowItems items_of(const ResidualArgs& a, const Shape& sh, bool* joined) {
   bool by_seq = false;
   for (const RowParam* p : {&a.branch_weight, &a.gate, &a.weight, &a.shift}) by_seq = by_seq || (p->seq_stride != 0);
   RowItems it;
   it.seqs = by_seq ? a.rows / a.rows_per_seq : 1;
   it.seq_rows = by_seq ? a.rows_per_seq : a.rows;
-  const int64_t groups = static_cast<int64_t>(num_sms()) * (kRowThreads / threads);
-  it.chunks = std::max({groups / it.seqs, (it.seq_rows + kItemRows - 1) / kItemRows, int64_t{1}});
-  it.chunks = std::min(it.chunks, it.seq_rows);
+  const int64_t ctas = num_sms(), per_cta = kRowThreads / sh.threads;
+  it.chunks = std::min(std::max<int64_t>(1, ctas / it.seqs), it.seq_rows);
+  const int64_t rows = (it.seq_rows + it.chunks - 1) / it.chunks;
+  *joined = sh.v > 0 && it.count() <= ctas && rows <= kItemRows * std::min(per_cta, rows) &&
+            (it.seqs == 1 || it.count() * 10 >= ctas * 9);
+  if (!*joined) {
+    it.chunks = std::max({ctas * per_cta / it.seqs, (it.seq_rows + kItemRows - 1) / kItemRows, int64_t{1}});
+    it.chunks = std::min(it.chunks, it.seq_rows);
+  }
   it.runs = Split::make(it.seq_rows, it.chunks);
   return it;
 }
@@ -532,7 +547,9 @@ cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t 
   const int64_t step[4] = {a.x_stride * x, a.dy_stride * x, a.res_stride * r, a.dh_stride * r};
   std::copy(step, step + 4, plan.rows.step);
   plan.rows.present = 1 | (a.dy != nullptr ? 2 | 4 : 0) | (a.dh != nullptr ? 8 : 0);  // h serves the norm alone
-  plan.rows.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, count / num_sms())));
+  // groups of a CTA: as many as have rows of their own
+  const int64_t most = plan.joined ? (plan.items.seq_rows + plan.items.chunks - 1) / plan.items.chunks : count / num_sms();
+  plan.rows.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, most)));
   const int block = plan.rows.groups * threads;
   // the ring, and in its place the groups' sums
   const size_t smem = std::max(Stream::kSmemBytes, sizeof(float) * SUMS * kRowThreads * E * V);
@@ -540,12 +557,8 @@ cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t 
   // at least a little over 48 KB: the sums' static part comes on top
   if (const cudaError_t e = ensure_smem_attr(fn, std::max<size_t>(smem, 49 * 1024)); e != cudaSuccess) return e;
   const int64_t all = static_cast<int64_t>(num_sms()) * std::max(1, cached_occupancy(fn, block, smem));
-  const int64_t grid = std::min<int64_t>(all, (count + plan.rows.groups - 1) / plan.rows.groups);
+  const int64_t grid = plan.joined ? count : std::min<int64_t>(all, (count + plan.rows.groups - 1) / plan.rows.groups);
   plan.rows.share = Split::make(count, grid * plan.rows.groups);
-  if (plan.items.seqs == 1 && count <= grid * plan.rows.groups) {
-    plan.joined = true;
-    plan.parts = grid;
-  }
   note_launch();
   return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a, plan);
 }
@@ -572,15 +585,15 @@ size_t residual_norm_backward_workspace_bytes(const ResidualArgs& a) {
   for (int i = 0; i < SUMS; ++i) wanted += wants(a, i);
   if (wanted == 0) return 0;
   const int64_t row = (static_cast<int64_t>(a.hidden) * 4 + 15) / 16 * 16;
-  return static_cast<size_t>(wanted * items_of(a, shape_of(a).threads).count() * row);
+  bool joined;
+  return static_cast<size_t>(wanted * items_of(a, shape_of(a), &joined).count() * row);
 }
 
 cudaError_t residual_norm_backward_launch(const ResidualArgs& a, void* ws, cudaStream_t st) {
   const Shape sh = shape_of(a);
   BackwardPlan plan{};
   plan.rows.threads = sh.threads;
-  plan.items = items_of(a, sh.threads);
-  plan.parts = plan.items.count();
+  plan.items = items_of(a, sh, &plan.joined);
   float* at = static_cast<float*>(ws);
   const int64_t count = plan.items.count();
   bool any = false;
@@ -600,7 +613,7 @@ cudaError_t residual_norm_backward_launch(const ResidualArgs& a, void* ws, cudaS
     e = launch_types<float, float>(a, plan, sh, st);
   if (e != cudaSuccess || !any) return e;
   ParamSums s{};
-  s.parts = static_cast<uint32_t>(plan.parts);
+  s.parts = static_cast<uint32_t>(count);
   s.chunks = static_cast<uint32_t>(plan.items.chunks);
   s.seqs = static_cast<uint32_t>(a.rows / a.rows_per_seq);
   s.hidden = a.hidden;
@@ -617,7 +630,7 @@ cudaError_t residual_norm_backward_launch(const ResidualArgs& a, void* ws, cudaS
   for (int i = 0; i < s.n; ++i) {
     const bool own = s.of[i].out.seq_stride != 0;
     outs = std::max<int64_t>(outs, own ? s.seqs : 1);
-    most = std::max(most, own ? plan.items.chunks : plan.parts);
+    most = std::max(most, own ? plan.items.chunks : count);
   }
   const int c = a.hidden % 2 == 0 ? 2 : 1;
   const int warps = static_cast<int>(std::min<int64_t>(16, (most + 1) / 2));  // two loads a lane at least
