@@ -2,12 +2,16 @@
 // residual_norm_backward.cu): how a row is spread over threads, the stream of
 // rows through shared memory, sums over a row, and the parameters' columns.
 //
-// A row of `hidden` columns is chunks of E columns (16 bytes of the wider of x
-// and the stream, or one column where rows are not whole aligned vectors). T threads (whole
+// A row of `hidden` columns is chunks of E columns: 16 bytes of the wider of x
+// and the stream. Rows need not be whole aligned vectors: if they are not (SHIFTED),
+// a chunk is read as the two aligned vectors that it lies in, and a warp puts its
+// outputs together into aligned vectors. T threads (whole
 // warps) take a row, thread t its chunks t, t + T, ... (V of them): a group.
 // A CTA holds several groups when rows are short, each with rows of its own
 // and a named barrier for its sums.
 #pragma once
+
+#include <initializer_list>
 
 #include "heads.cuh"
 #include "philox.cuh"
@@ -30,7 +34,8 @@ struct Split {
 struct RowPlan {
   int threads;      // T
   int groups;       // of a CTA
-  int64_t step[4];  // bytes between the rows of the streamed tensors
+  const char* base[4];  // the streamed tensors
+  uint32_t step[4];     // bytes between their rows
   int present;      // a bit for each of them that is there (the others are zeros)
   Split share;      // rows (backward: items) of the launch's groups
 };
@@ -80,54 +85,91 @@ __device__ __forceinline__ void row_sum(float (&v)[4], float* red, int warps, in
 }
 
 // ---- chunks -----------------------------------------------------------------
-// E columns of T as pairs of floats at `f`, from and to memory in vectors of 16 or 8 bytes.
+// E columns of T, one vector of 16 or 8 bytes, as pairs of floats.
 template <typename T, int E> struct Chunk {
   static constexpr int kBytes = E * static_cast<int>(sizeof(T));
-  static constexpr int kVecBytes = kBytes < 16 ? 8 : 16;
-  static constexpr int kVecs = kBytes / kVecBytes;
-  static_assert(kVecs * kVecBytes == kBytes, "whole vectors");
-  static constexpr int kVecCols = E / kVecs;
-  using Vec = HeadVec<T, kVecCols>;
-  __device__ static void unpack(const typename Vec::Raw& r, F2* f) {
-    F2 t[kVecCols / 2];
+  static constexpr int kWords = kBytes / 4;
+  static_assert(kBytes == 16 || kBytes == 8, "one vector");
+  using Vec = HeadVec<T, E>;
+  using Raw = typename Vec::Raw;
+  __device__ static void unpack(const Raw& r, F2* f) {
+    F2 t[E / 2];
     Vec::unpack(r, t);
 #pragma unroll
-    for (int i = 0; i < kVecCols / 2; ++i) f[i] = t[i];
+    for (int i = 0; i < E / 2; ++i) f[i] = t[i];
   }
-  __device__ static void store(T* p, const F2* f) {
+  __device__ static Raw pack(const F2* f) {
+    Raw r;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
 #pragma unroll
-    for (int v = 0; v < kVecs; ++v) {
-      F2 t[kVecCols / 2];
-#pragma unroll
-      for (int i = 0; i < kVecCols / 2; ++i) t[i] = f[v * kVecCols / 2 + i];
-      Vec::store(p + v * kVecCols, t);
+    for (int i = 0; i < E / 2; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[2 * i] = __float_as_uint(f[i].x);
+        w[2 * i + 1] = __float_as_uint(f[i].y);
+      } else {
+        w[i] = Pair16<T>::pack(f[i].x, f[i].y);
+      }
     }
+    return r;
+  }
+  // The vector that starts `bytes` (less than a vector) into two of them side by side.
+  __device__ static Raw joined(const Raw& low, const Raw& high, uint32_t bytes) {
+    uint32_t w[2 * kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      w[i] = reinterpret_cast<const uint32_t*>(&low)[i];
+      w[kWords + i] = reinterpret_cast<const uint32_t*>(&high)[i];
+    }
+    if constexpr (kWords == 4) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = bytes & 8 ? w[i + 2] : w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kWords + 1; ++i) w[i] = bytes & 4 ? w[i + 1] : w[i];
+    Raw r;
+    uint32_t* o = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) o[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], (bytes & 3) * 8);
+    return r;
   }
 };
 
 __device__ __forceinline__ float& lane_of(F2* f, int i) { return i & 1 ? f[i >> 1].y : f[i >> 1].x; }
 
 // Which columns this thread takes, in blocks of up to 8 of them (whole chunks).
-template <int E, int V> struct RowCols {
+template <int E, int V, bool SHIFTED> struct RowCols {
   static constexpr int N = E * V;         // columns
   static constexpr int B = N < 8 ? N : 8;  // of a block
   static constexpr int BLOCKS = N / B;
   static constexpr int BP = B / 2;  // pairs of a block
+  static constexpr int BC = B / E;  // chunks of a block
   static_assert(B % 2 == 0 && B % E == 0 && N % B == 0, "whole pairs and chunks");
   int first, step, hidden;
   __device__ RowCols(int t, int threads, int h) : first(t * E), step(threads * E), hidden(h) {}
   __device__ int col(int k) const { return first + k * step; }
   __device__ bool has(int k) const { return col(k) < hidden; }
+  // How many of chunk k's columns there are: all or none but in SHIFTED rows.
+  __device__ int count(int k) const { return min(max(hidden - col(k), 0), E); }
 
   // Block b of p's columns of a sequence (otherwise: of a parameter that is not there, and past the row).
   __device__ void param(const RowParam& p, int64_t seq, float otherwise, int b, F2 (&f)[BP]) const {
 #pragma unroll
-    for (int k = 0; k < B / E; ++k) {
+    for (int k = 0; k < BC; ++k) {
       float v[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) v[j] = otherwise;
-      const int at = b * (B / E) + k;
-      if (p.p != nullptr && has(at)) load_floats<E>(p.p, seq * p.seq_stride + col(at), p.dtype, v);
+      const int at = b * BC + k;
+      if (p.p != nullptr && has(at)) {
+        const int64_t i = seq * p.seq_stride + col(at);
+        if constexpr (SHIFTED) {
+          const int n = count(at);
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (j < n) v[j] = load_as_float(p.p, i + j, p.dtype);
+        } else {
+          load_floats<E>(p.p, i, p.dtype, v);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < E; ++j) lane_of(f, k * E + j) = v[j];
     }
@@ -141,14 +183,51 @@ template <int E, int V> struct RowCols {
 #pragma unroll
     for (int j = 0; j < BP; ++j) c[j] = mul2(mul2(c[j], g[j]), f2(s, s));
   }
-  // Block b to this thread's first column of a row.
-  template <typename T> __device__ void store(T* mine, int b, F2 (&f)[BP]) const {
+  // Block b to a row. The whole warp takes part.
+  template <typename T> __device__ void store(T* row, int b, F2 (&f)[BP]) const {
+    using C = Chunk<T, E>;
 #pragma unroll
-    for (int k = 0; k < B / E; ++k) {
-      const int at = b * (B / E) + k;
+    for (int k = 0; k < BC; ++k) {
+      const int at = b * BC + k;
+      const typename C::Raw own = C::pack(f + k * E / 2);
+      T* to = row + col(at);
+      const uint32_t shift = SHIFTED ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to)) % C::kBytes : 0u;
+      if (!SHIFTED || (shift == 0 && hidden % E == 0)) {
+        if (has(at)) *reinterpret_cast<typename C::Raw*>(to) = own;
+        continue;
+      }
+      // The aligned vector in which this chunk begins: the lane before's last columns and this one's first. A lane
+      // without the columns for it, the warp's first one and the last of the row give theirs one by one.
+      const int lane = threadIdx.x & 31, n = count(at);
+      const int head = static_cast<int>((C::kBytes - shift) / sizeof(T));  // own columns in that vector
+      typename C::Raw before;
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&own);
+      uint32_t* u = reinterpret_cast<uint32_t*>(&before);
+#pragma unroll
+      for (int i = 0; i < C::kWords; ++i) u[i] = __shfl_up_sync(0xffffffffu, w[i], 1);
+      const bool whole = n >= head && (shift == 0 || lane > 0);
+      const bool next = __shfl_down_sync(0xffffffffu, static_cast<int>(whole), 1) && lane < 31;
+      if (whole)
+        *reinterpret_cast<typename C::Raw*>(reinterpret_cast<char*>(to) - shift) =
+            shift == 0 ? own : C::joined(before, own, C::kBytes - shift);
+      if (!whole || !next) {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (j < n && (j < head ? !whole : !next)) to[j] = Ty<T>::from_f(lane_of(f, k * E + j));
+      }
+      __syncwarp();
+    }
+  }
+  // Block b to a row of floats (aligned rows).
+  __device__ void store_floats(float* row, int b, const F2 (&f)[BP]) const {
+#pragma unroll
+    for (int k = 0; k < BC; ++k) {
+      const int at = b * BC + k;
       if (!has(at)) continue;
-      if constexpr (E == 1) mine[at * step] = Ty<T>::from_f(lane_of(f, k));
-      else Chunk<T, E>::store(mine + at * step, f + k * E / 2);
+#pragma unroll
+      for (int j = 0; j < E / 4; ++j)
+        reinterpret_cast<float4*>(row + col(at))[j] =
+            make_float4(f[k * E / 2 + 2 * j].x, f[k * E / 2 + 2 * j].y, f[k * E / 2 + 2 * j + 1].x, f[k * E / 2 + 2 * j + 1].y);
     }
   }
   // Which of this thread's columns are kept in the row whose first element has this index.
@@ -156,7 +235,12 @@ template <int E, int V> struct RowCols {
     if (d.all) return 0u;
     uint32_t bits = 0;
 #pragma unroll
-    for (int k = 0; k < V; ++k) bits |= key.kept<E>(row + static_cast<uint32_t>(col(k))) << (k * E);
+    for (int k = 0; k < V; ++k) {
+      const uint64_t i = row + static_cast<uint32_t>(col(k));
+      // whole blocks of words, of which the chunk begins in the first one
+      if constexpr (SHIFTED) bits |= (key.kept<E + 4>(i & ~uint64_t{3}) >> (i & 3) & ((1u << E) - 1)) << (k * E);
+      else bits |= key.kept<E>(i) << (k * E);
+    }
     return bits;
   }
   __device__ static void drop(uint32_t bits, int b, F2 (&f)[BP]) {
@@ -169,145 +253,131 @@ template <int E, int V> struct RowCols {
 };
 
 // ---- a group's stream of rows -----------------------------------------------
-// A thread's chunks of the rows ahead, of NX tensors of TX and NR of TR. Whole
-// 16-byte vectors (E > 1) go through a ring in shared memory by cp.async, each
-// thread writing and reading its own slots: no barrier, and the loads in flight
-// cost no registers. Single columns (E == 1) are held in registers, a row ahead.
-template <typename TX, typename TR, int E, int V, int NX, int NR, int STAGES>
+// A thread's chunks of the rows ahead, of NX tensors of TX and NR of TR, through a
+// ring in shared memory by cp.async, each thread writing and reading its own
+// slots: no barrier, and the loads in flight cost no registers. SHIFTED: two
+// aligned vectors for each chunk, of which only those are read that hold a column
+// of it (so none lies outside the row's first and last aligned vector).
+template <typename TX, typename TR, int E, int V, bool SHIFTED, int NX, int NR, int STAGES>
 struct RowStream {
+  using Cols = RowCols<E, V, SHIFTED>;
   static constexpr int kTensors = NX + NR;
-  using ChunkX = Chunk<TX, E == 1 ? 16 : E>;
-  using ChunkR = Chunk<TR, E == 1 ? 16 : E>;
-  static constexpr int kBytesX = V * ChunkX::kBytes, kBytesR = V * ChunkR::kBytes;  // of a thread and row
-  static constexpr int kRowBytes = E == 1 ? 0 : NX * kBytesX + NR * kBytesR;
+  static constexpr int VECS = SHIFTED ? 2 : 1;  // of a chunk
+  using ChunkX = Chunk<TX, E>;
+  using ChunkR = Chunk<TR, E>;
+  static constexpr int kBytesX = V * VECS * ChunkX::kBytes, kBytesR = V * VECS * ChunkR::kBytes;  // of a thread and row
+  static constexpr int kRowBytes = NX * kBytesX + NR * kBytesR;
   // Slots lie as for a full CTA, so that all but the stage of an address is known when this is compiled.
   static constexpr uint32_t kStageBytes = kRowBytes * kRowThreads;
   static constexpr size_t kSmemBytes = static_cast<size_t>(STAGES) * kStageBytes;
+  template <int I> using ChunkOf = std::conditional_t<(I < NX), ChunkX, ChunkR>;
 
-  const char* at[kTensors];  // this thread's first column of the next row to load
-  int left;                  // rows to load
+  uint32_t next, end;          // rows to load
   uint32_t ring, write, read;  // shared memory: all stages, and the stages to fill and to read
-  float ahead[E == 1 ? kTensors * V : 1], now[E == 1 ? kTensors * V : 1];
 
   // Vector v of tensor i in a stage: the CTA's threads side by side.
   static __device__ constexpr uint32_t offset(int i, int v, int vec_bytes) {
     return ((i < NX ? i * kBytesX : NX * kBytesX + (i - NX) * kBytesR) + v * vec_bytes) * kRowThreads;
   }
 
-  template <typename T> __device__ void set(int i, const void* base, int64_t row, int64_t step, const RowCols<E, V>& cols) {
-    at[i] = static_cast<const char*>(base) + row * step + cols.first * static_cast<int>(sizeof(T));
-  }
-  // After set() of each tensor: `rows` rows from there.
-  __device__ void start(const RowCols<E, V>& cols, const RowPlan& plan, void* smem, int rows) {
-    left = rows;
-    if constexpr (E > 1) {
-      ring = write = smem_u32(smem);
-      read = ring + (STAGES - 1) * kStageBytes;
-      // what no copy ever fills stays zero
+  // Rows from `first` on, `rows` of them.
+  __device__ void start(const Cols& cols, const RowPlan& plan, void* smem, uint32_t first, uint32_t rows) {
+    next = first;
+    end = first + rows;
+    ring = write = smem_u32(smem);
+    read = ring + (STAGES - 1) * kStageBytes;
+    // what no copy ever fills stays zero
 #pragma unroll
-      for (int i = 0; i < kTensors; ++i) {
-        if (cols.has(V - 1) && (plan.present >> i & 1)) continue;
-        if (i < NX) clear<ChunkX>(i);
-        else clear<ChunkR>(i);
-      }
-#pragma unroll 1
-      for (int i = 0; i < STAGES - 1; ++i) load(cols, plan);
-    } else {
-      load(cols, plan);
+    for (int i = 0; i < kTensors; ++i) {
+      if (cols.has(V - 1) && (plan.present >> i & 1)) continue;
+      if (i < NX) clear<ChunkX>(i);
+      else clear<ChunkR>(i);
     }
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; ++i) load(cols, plan);
   }
   // The next row: its values are there for get(), and the loads of a later one are under way.
-  __device__ void advance(const RowCols<E, V>& cols, const RowPlan& plan) {
-    if constexpr (E > 1) {
-      load(cols, plan);
-      read = next_stage(read);
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-    } else {
-#pragma unroll
-      for (int i = 0; i < kTensors * V; ++i) now[i] = ahead[i];
-      load(cols, plan);
-    }
+  __device__ void advance(const Cols& cols, const RowPlan& plan) {
+    load(cols, plan);
+    read = next_stage(read);
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
   }
-  // Block b of tensor I.
-  template <int I> __device__ void get(int b, F2 (&f)[RowCols<E, V>::BP]) const {
-    constexpr int CHUNKS = RowCols<E, V>::B / E;
-    if constexpr (E > 1) {
-      using C = std::conditional_t<(I < NX), ChunkX, ChunkR>;
-      const uint32_t mine = read + threadIdx.x * C::kVecBytes;
+  // Block b of tensor I of `row`, the one that advance() has brought.
+  template <int I> __device__ void get(const Cols& cols, const RowPlan& plan, uint32_t row, int b, F2 (&f)[Cols::BP]) const {
+    using C = ChunkOf<I>;
+    // bytes into the first of a chunk's aligned vectors, the same for all chunks
+    const uint32_t shift =
+        SHIFTED ? (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(plan.base[I])) + row * plan.step[I]) % C::kBytes : 0u;
+    const uint32_t mine = read + threadIdx.x * C::kBytes;
 #pragma unroll
-      for (int v = 0; v < CHUNKS * C::kVecs; ++v) {
-        typename C::Vec::Raw r;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&r);
-        const uint32_t from = mine + offset(I, b * CHUNKS * C::kVecs + v, C::kVecBytes);
-        if constexpr (C::kVecBytes == 16)
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(from));
-        else
-          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from));
-        C::unpack(r, f + v * C::kVecCols / 2);
+    for (int k = 0; k < Cols::BC; ++k) {
+      const int at_chunk = b * Cols::BC + k;
+      typename C::Raw r = fetch<C>(mine + offset(I, at_chunk * VECS, C::kBytes));
+      if constexpr (SHIFTED) {
+        r = C::joined(r, fetch<C>(mine + offset(I, at_chunk * VECS + 1, C::kBytes)), shift);
+        C::unpack(r, f + k * E / 2);
+        const int n = cols.count(at_chunk);
+        if (n < E) {  // the next row's columns, or nobody's
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (j >= n) lane_of(f, k * E + j) = 0.f;
+        }
+      } else {
+        C::unpack(r, f + k * E / 2);
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < CHUNKS; ++k) lane_of(f, k) = now[I * V + b * CHUNKS + k];
     }
   }
 
  private:
+  template <class C> static __device__ typename C::Raw fetch(uint32_t from) {
+    typename C::Raw r;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+    if constexpr (C::kBytes == 16)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from));
+    else
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(from));
+    return r;
+  }
   __device__ uint32_t next_stage(uint32_t st) const {
     return st == ring + (STAGES - 1) * kStageBytes ? ring : st + kStageBytes;
   }
-  __device__ void load(const RowCols<E, V>& cols, const RowPlan& plan) {
-    if (left > 0) {
+  __device__ void load(const Cols& cols, const RowPlan& plan) {
+    if (next < end) {
 #pragma unroll
       for (int i = 0; i < kTensors; ++i) {
-        if (!(plan.present >> i & 1)) {
-          if constexpr (E == 1) {
-#pragma unroll
-            for (int k = 0; k < V; ++k) ahead[i * V + k] = 0.f;
-          }
-          continue;
-        }
-        if (i < NX) copy<TX, ChunkX>(cols, i);
-        else copy<TR, ChunkR>(cols, i);
-        at[i] += plan.step[i];
+        if (!(plan.present >> i & 1)) continue;
+        const char* at = plan.base[i] + static_cast<uint64_t>(next) * plan.step[i];
+        if (i < NX) copy<TX, ChunkX>(cols, i, at);
+        else copy<TR, ChunkR>(cols, i, at);
       }
     }
-    --left;
-    if constexpr (E > 1) {
-      write = next_stage(write);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    ++next;
+    write = next_stage(write);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  template <typename T, class C> __device__ void copy(const RowCols<E, V>& cols, int i) {
-    const T* from = reinterpret_cast<const T*>(at[i]);
-    const uint32_t to = write + threadIdx.x * C::kVecBytes;
+  template <class C> static __device__ void copy_vector(uint32_t to, const void* from) {
+    if constexpr (C::kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+  }
+  template <typename T, class C> __device__ void copy(const Cols& cols, int i, const char* row) {
+    const uint32_t to = write + threadIdx.x * C::kBytes;
+    const uint32_t into = SHIFTED ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row)) % C::kBytes : 0u;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      if constexpr (E == 1) {
-        ahead[i * V + k] = cols.has(k) ? Ty<T>::to_f(from[k * cols.step]) : 0.f;
-      } else if (cols.has(k)) {
-#pragma unroll
-        for (int v = 0; v < C::kVecs; ++v) {
-          if constexpr (C::kVecBytes == 16)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + offset(i, k * C::kVecs + v, 16)),
-                         "l"(from + k * cols.step + v * C::kVecCols)
-                         : "memory");
-          else
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to + offset(i, k * C::kVecs + v, 8)),
-                         "l"(from + k * cols.step + v * C::kVecCols)
-                         : "memory");
-        }
-      }
+      if (!cols.has(k)) continue;
+      const T* from = reinterpret_cast<const T*>(row - into) + cols.col(k);
+      copy_vector<C>(to + offset(i, k * VECS, C::kBytes), from);
+      if (SHIFTED && into + cols.count(k) * static_cast<int>(sizeof(T)) > C::kBytes)
+        copy_vector<C>(to + offset(i, k * VECS + 1, C::kBytes), from + E);
     }
   }
   template <class C> __device__ void clear(int i) const {
 #pragma unroll 1
     for (int st = 0; st < STAGES; ++st) {
-      const uint32_t mine = ring + st * kStageBytes + threadIdx.x * C::kVecBytes;
+      const uint32_t mine = ring + st * kStageBytes + threadIdx.x * C::kBytes;
 #pragma unroll
-      for (int v = 0; v < V * C::kVecs; ++v) {
-        if constexpr (C::kVecBytes == 16)
+      for (int v = 0; v < V * VECS; ++v) {
+        if constexpr (C::kBytes == 16)
           asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(mine + offset(i, v, 16)), "r"(0u) : "memory");
         else
           asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(mine + offset(i, v, 8)), "r"(0u) : "memory");
@@ -317,18 +387,29 @@ struct RowStream {
 };
 
 // Rows ahead in shared memory: as many as a full CTA has room for, four at most.
-template <typename TX, typename TR> constexpr int row_stages(int cols, int nx, int nr) {
-  const int row = cols * (nx * static_cast<int>(sizeof(TX)) + nr * static_cast<int>(sizeof(TR))) * kRowThreads;
+template <typename TX, typename TR> constexpr int row_stages(int cols, int nx, int nr, bool shifted) {
+  const int row = (shifted ? 2 : 1) * cols * (nx * static_cast<int>(sizeof(TX)) + nr * static_cast<int>(sizeof(TR))) * kRowThreads;
   const int n = 208 * 1024 / row;
   return n < 1 ? 1 : n > 4 ? 4 : n;
 }
 
 // ---- host: which rows are whole aligned vectors ------------------------------
 inline int row_elem_bytes(int dtype) { return dtype == F32 ? 4 : 2; }
-// Columns of a vector chunk: 16 bytes of the wider type.
+// Columns of a chunk: 16 bytes of the wider type.
 template <typename TX, typename TR> constexpr int kRowChunk = 16 / (sizeof(TX) > sizeof(TR) ? sizeof(TX) : sizeof(TR));
-// Columns of a chunk with which the kernels can take these rows: kRowChunk, or 1.
-inline int row_chunk(const ResidualArgs& a, bool backward) {
+// The streamed tensors of a launch: their steps have to be 32-bit numbers of bytes.
+inline bool set_tensors(RowPlan* plan, std::initializer_list<std::pair<const void*, int64_t>> tensors) {
+  int i = 0;
+  for (const auto& [p, step] : tensors) {
+    if (p != nullptr && step > UINT32_MAX) return false;
+    plan->base[i] = static_cast<const char*>(p);
+    plan->step[i] = static_cast<uint32_t>(step);
+    plan->present |= (p != nullptr ? 1 : 0) << i++;
+  }
+  return true;
+}
+// Whether rows and parameters are whole aligned vectors of chunks.
+inline bool rows_aligned(const ResidualArgs& a, bool backward) {
   const int e = 16 / std::max(row_elem_bytes(a.x_dtype), row_elem_bytes(a.res_dtype));
   bool ok = a.hidden % e == 0;
   auto aligned = [&](const void* p, int64_t stride, int dtype) {
@@ -349,7 +430,7 @@ inline int row_chunk(const ResidualArgs& a, bool backward) {
   for (const RowParam* p : {&a.branch_weight, &a.gate, &a.weight, &a.shift})
     ok = ok && (p->p == nullptr || (reinterpret_cast<uintptr_t>(p->p) % 16 == 0 &&
                                     p->seq_stride * row_elem_bytes(p->dtype) % std::min(16, e * row_elem_bytes(p->dtype)) == 0));
-  return ok ? e : 1;
+  return ok;
 }
 // T for V chunks of E columns a thread (0: the row does not fit).
 inline int row_threads(int hidden, int e, int v) {

@@ -20,10 +20,10 @@ namespace tfo {
 // Parameters stay in registers up to this many columns a thread; above it they are read again for every row.
 constexpr int kParamCols = 16;
 
-template <typename TX, typename TR, int E, int V, int STAGES>
+template <typename TX, typename TR, int E, int V, bool SHIFTED, int STAGES>
 __global__ void __launch_bounds__(kRowThreads, 1)
     residual_norm_kernel(const __grid_constant__ ResidualArgs a, const __grid_constant__ RowPlan plan) {
-  using Cols = RowCols<E, V>;
+  using Cols = RowCols<E, V, SHIFTED>;
   constexpr int NB = Cols::BLOCKS, BP = Cols::BP;
   constexpr bool KEEP_PARAMS = Cols::N <= kParamCols;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -36,25 +36,19 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   __syncthreads();
   griddep_wait();
   const uint32_t me = blockIdx.x * plan.groups + group;
-  const int64_t r0 = plan.share.first(me);
-  int left = static_cast<int>(plan.share.first(me + 1) - r0);
-  if (left == 0) return;
+  uint32_t row = plan.share.first(me);
+  const uint32_t end = plan.share.first(me + 1);
+  if (row == end) return;
   const Cols cols(t, plan.threads, a.hidden);
-  RowStream<TX, TR, E, V, 1, 1, STAGES> rows;
-  rows.template set<TX>(0, a.x, r0, plan.step[0], cols);
-  rows.template set<TR>(1, a.res, r0, plan.step[1], cols);
-  rows.start(cols, plan, smem, left);
+  RowStream<TX, TR, E, V, SHIFTED, 1, 1, STAGES> rows;
+  rows.start(cols, plan, smem, row, end - row);
   const DropKey key(a.drop);
   const float inv_h = 1.f / static_cast<float>(a.hidden);
   const int bar = 1 + group;
   int turn = 0;  // of the parts of a sum
-  int64_t seq = static_cast<uint32_t>(r0) / static_cast<uint32_t>(a.rows_per_seq);
-  int seq_left = static_cast<int>((seq + 1) * a.rows_per_seq - r0);
+  const uint32_t per = static_cast<uint32_t>(a.rows_per_seq);
+  uint32_t seq = row / per, seq_end = (seq + 1) * per;
   const bool by_seq = (a.branch_weight.seq_stride | a.gate.seq_stride | a.weight.seq_stride) != 0;
-  uint64_t element = static_cast<uint64_t>(r0) * a.hidden;  // the row's first
-  TR* h_out = static_cast<TR*>(a.h) + element + cols.first;
-  TX* y_out = static_cast<TX*>(a.y) + element + cols.first;
-  float* rstd = a.rstd + 2 * r0;
   F2 c[KEEP_PARAMS ? NB : 1][BP], w[KEEP_PARAMS ? NB : 1][BP];
   auto params = [&] {
 #pragma unroll
@@ -65,6 +59,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   };
   if constexpr (KEEP_PARAMS) params();
   for (;;) {
+    const uint64_t element = static_cast<uint64_t>(row) * static_cast<uint32_t>(a.hidden);  // the row's first
     const uint32_t bits = a.dropped ? cols.kept(a.drop, key, element) : ~0u;
     rows.advance(cols, plan);
     F2 h[NB][BP];
@@ -73,7 +68,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       F2 s2 = f2(0.f, 0.f);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        rows.template get<0>(b, h[b]);
+        rows.template get<0>(cols, plan, row, b, h[b]);
 #pragma unroll
         for (int j = 0; j < BP; ++j) s2 = fma2(h[b][j], h[b][j], s2);
       }
@@ -85,8 +80,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       F2 res[BP];
-      if (!a.branch_norm) rows.template get<0>(b, h[b]);
-      rows.template get<1>(b, res);
+      if (!a.branch_norm) rows.template get<0>(cols, plan, row, b, h[b]);
+      rows.template get<1>(cols, plan, row, b, res);
       F2(&cb)[BP] = c[KEEP_PARAMS ? b : 0];
       if constexpr (!KEEP_PARAMS) cols.branch_coefficient(a, seq, b, cb);
 #pragma unroll
@@ -97,9 +92,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         h[b][j] = add2(res[j], h[b][j]);
         s2 = fma2(h[b][j], h[b][j], s2);
       }
-      cols.store(h_out, b, h[b]);
+      cols.store(static_cast<TR*>(a.h) + element, b, h[b]);
     }
-    h_out += a.hidden;
     float r_sum = 1.f;
     if (a.y != nullptr) {
       float s[1] = {s2.x + s2.y};
@@ -117,19 +111,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
           for (int j = 0; j < BP; ++j) h[b][j] = add2(h[b][j], sh[j]);
         }
-        cols.store(y_out, b, h[b]);
+        cols.store(static_cast<TX*>(a.y) + element, b, h[b]);
       }
-      y_out += a.hidden;
     }
-    if (a.rstd != nullptr) {
-      if (t == 0) *reinterpret_cast<float2*>(rstd) = make_float2(r_branch, r_sum);
-      rstd += 2;
-    }
-    if (--left == 0) return;
-    element += a.hidden;
-    if (--seq_left == 0) {
+    if (a.rstd != nullptr && t == 0) reinterpret_cast<float2*>(a.rstd)[row] = make_float2(r_branch, r_sum);
+    if (++row == end) return;
+    if (row == seq_end) {
       ++seq;
-      seq_left = static_cast<int>(a.rows_per_seq);
+      seq_end += per;
       if (KEEP_PARAMS && by_seq) params();
     }
   }
@@ -187,11 +176,11 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_any_kernel(const __
 }
 
 namespace {
-template <typename TX, typename TR, int E, int V>
-cudaError_t launch_rows(const ResidualArgs& a, int threads, cudaStream_t st) {
-  constexpr int STAGES = row_stages<TX, TR>(E * V, 1, 1);
-  auto* kernel = residual_norm_kernel<TX, TR, E, V, STAGES>;
-  using Stream = RowStream<TX, TR, E, V, 1, 1, STAGES>;
+template <typename TX, typename TR, int V, bool SHIFTED>
+cudaError_t launch_rows(const ResidualArgs& a, RowPlan plan, int threads, cudaStream_t st) {
+  constexpr int E = kRowChunk<TX, TR>, STAGES = row_stages<TX, TR>(E * V, 1, 1, SHIFTED);
+  auto* kernel = residual_norm_kernel<TX, TR, E, V, SHIFTED, STAGES>;
+  using Stream = RowStream<TX, TR, E, V, SHIFTED, 1, 1, STAGES>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   // as many groups a CTA as still leave every SM a row
   const int groups =
@@ -202,26 +191,36 @@ cudaError_t launch_rows(const ResidualArgs& a, int threads, cudaStream_t st) {
   if (const cudaError_t e = ensure_smem_attr(fn, std::max<size_t>(smem, 49 * 1024)); e != cudaSuccess) return e;
   const int64_t all = static_cast<int64_t>(num_sms()) * std::max(1, cached_occupancy(fn, block, smem));
   const int64_t grid = std::min<int64_t>(all, (a.rows + groups - 1) / groups);
+  plan.threads = threads;
+  plan.groups = groups;
+  plan.share = Split::make(a.rows, grid * groups);
   note_launch();
-  return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a,
-                          RowPlan{threads, groups, {a.x_stride * static_cast<int64_t>(sizeof(TX)),
-                                                    a.res_stride * static_cast<int64_t>(sizeof(TR))}, 3,
-                                  Split::make(a.rows, grid * groups)});
+  return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a, plan);
+}
+
+// A warp a row as far as 16 columns a thread carry it, then 16 columns a thread, then (aligned rows) 32.
+template <typename TX, typename TR, bool SHIFTED>
+cudaError_t launch_width(const ResidualArgs& a, const RowPlan& plan, cudaStream_t st, bool* done) {
+  constexpr int E = kRowChunk<TX, TR>, FULL = 16 / E;
+  *done = true;
+  if (a.hidden <= 32 * E) return launch_rows<TX, TR, 1, SHIFTED>(a, plan, 32, st);
+  if (FULL > 2 && a.hidden <= 64 * E) return launch_rows<TX, TR, 2, SHIFTED>(a, plan, 32, st);
+  if (const int t = row_threads(a.hidden, E, FULL)) return launch_rows<TX, TR, FULL, SHIFTED>(a, plan, t, st);
+  if constexpr (!SHIFTED) {
+    if (const int t = row_threads(a.hidden, E, 2 * FULL)) return launch_rows<TX, TR, 2 * FULL, SHIFTED>(a, plan, t, st);
+  }
+  *done = false;
+  return cudaSuccess;
 }
 
 template <typename TX, typename TR>
 cudaError_t launch_types(const ResidualArgs& a, cudaStream_t st) {
-  constexpr int E = kRowChunk<TX, TR>;
-  if (row_chunk(a, false) == E) {
-    // A warp a row as far as 16 columns a thread carry it, then 16 columns a thread.
-    constexpr int FULL = 16 / E;
-    if (a.hidden <= 32 * E) return launch_rows<TX, TR, E, 1>(a, 32, st);
-    if (FULL > 2 && a.hidden <= 64 * E) return launch_rows<TX, TR, E, 2>(a, 32, st);
-    if (const int t = row_threads(a.hidden, E, FULL)) return launch_rows<TX, TR, E, FULL>(a, t, st);
-    if (const int t = row_threads(a.hidden, E, 2 * FULL)) return launch_rows<TX, TR, E, 2 * FULL>(a, t, st);
-  } else {
-    if (const int t = row_threads(a.hidden, 1, 4)) return launch_rows<TX, TR, 1, 4>(a, t, st);
-    if (const int t = row_threads(a.hidden, 1, 8)) return launch_rows<TX, TR, 1, 8>(a, t, st);
+  RowPlan plan{};
+  if (set_tensors(&plan, {{a.x, a.x_stride * static_cast<int64_t>(sizeof(TX))}, {a.res, a.res_stride * static_cast<int64_t>(sizeof(TR))}})) {
+    bool done = false;
+    const cudaError_t e = rows_aligned(a, false) ? launch_width<TX, TR, false>(a, plan, st, &done)
+                                                 : launch_width<TX, TR, true>(a, plan, st, &done);
+    if (done) return e;
   }
   note_launch();
   return launch_dependent(residual_norm_any_kernel<TX, TR>, static_cast<int>(std::min<int64_t>(a.rows, num_sms() * 4ll)),

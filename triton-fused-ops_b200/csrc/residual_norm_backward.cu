@@ -34,9 +34,9 @@ struct RowItems {
   int64_t seqs, seq_rows, chunks;
   Split runs;  // a sequence's rows over its items
   __host__ __device__ int64_t count() const { return seqs * chunks; }
-  __device__ int64_t first_row(uint32_t item) const {
+  __device__ uint32_t first_row(uint32_t item) const {
     const uint32_t b = item / static_cast<uint32_t>(chunks), c = item - b * static_cast<uint32_t>(chunks);
-    return b * seq_rows + runs.first(c);
+    return b * static_cast<uint32_t>(seq_rows) + runs.first(c);
   }
 };
 
@@ -87,10 +87,10 @@ struct BackwardPlan {
   float* partials[SUMS];  // [items][hidden], or NULL: not wanted
 };
 
-template <typename TX, typename TR, int E, int V, int STAGES>
+template <typename TX, typename TR, int E, int V, bool SHIFTED, int STAGES>
 __global__ void __launch_bounds__(kRowThreads, 1)
     residual_norm_backward_kernel(const __grid_constant__ ResidualArgs a, const __grid_constant__ BackwardPlan plan) {
-  using Cols = RowCols<E, V>;
+  using Cols = RowCols<E, V, SHIFTED>;
   constexpr int NB = Cols::BLOCKS, BP = Cols::BP;
   constexpr bool TENSOR = Cols::N == 16;
   using KeptRows = RowKept<Cols, TENSOR>;
@@ -118,15 +118,14 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   const RowItems items = plan.items;
   uint32_t item = plan.joined ? blockIdx.x : plan.rows.share.first(me);
   const uint32_t last = plan.joined ? item + 1 : plan.rows.share.first(me + 1);
-  int64_t r0 = 0;
-  int left = 0;
+  uint32_t row = 0, end = 0;
   if (item < last) {
-    r0 = items.first_row(item);
-    left = static_cast<int>(items.first_row(last) - r0);
+    row = items.first_row(item);
+    end = items.first_row(last);
     if (plan.joined) {
-      const int n = plan.rows.groups, from = left * group / n;
-      left = left * (group + 1) / n - from;
-      r0 += from;
+      const uint32_t n = plan.rows.groups, rows = end - row;
+      end = row + rows * (group + 1) / n;
+      row += rows * group / n;
     }
   }
   const Cols cols(t, threads, a.hidden);
@@ -142,33 +141,37 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     }
   };
   // This thread's columns of the sums to a partial row.
-  auto give = [&](int i, float* row) {
+  auto give = [&](int i, float* to) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       F2 v[BP];
       kept.read(i, b, v);
       kept.wait();
       kept.arrived(v);
-      cols.store(row + cols.first, b, v);
+      if constexpr (SHIFTED) {
+#pragma unroll
+        for (int j = 0; j < Cols::B; ++j) {
+          const int k = b * Cols::BC + j / E;
+          if (j % E < cols.count(k)) to[cols.col(k) + j % E] = lane_of(v, j);
+        }
+      } else {
+        cols.store_floats(to, b, v);
+      }
       __syncwarp();
     }
   };
   clear();
-  if (left > 0) {
-    RowStream<TX, TR, E, V, 2, 2, STAGES> rows;
-    rows.template set<TX>(0, a.x, r0, plan.rows.step[0], cols);
-    rows.template set<TX>(1, a.dy, r0, plan.rows.step[1], cols);
-    rows.template set<TR>(2, a.res, r0, plan.rows.step[2], cols);
-    rows.template set<TR>(3, a.dh, r0, plan.rows.step[3], cols);
-    rows.start(cols, plan.rows, smem, left);
+  if (row < end) {
+    RowStream<TX, TR, E, V, SHIFTED, 2, 2, STAGES> rows;
+    rows.start(cols, plan.rows, smem, row, end - row);
     const DropKey key(a.drop);
     const float inv_h = 1.f / static_cast<float>(a.hidden);
     const int bar = 1 + group;
     int turn = 0;  // of the parts of a sum
-    const float2* rstd = reinterpret_cast<const float2*>(a.rstd) + r0;
-    float2 next_r = *rstd;  // loaded a row ahead
-    int64_t seq = static_cast<uint32_t>(r0) / static_cast<uint32_t>(a.rows_per_seq);
-    int seq_left = static_cast<int>((seq + 1) * a.rows_per_seq - r0);
+    const float2* rstd = reinterpret_cast<const float2*>(a.rstd);
+    float2 next_r = rstd[row];  // loaded a row ahead
+    const uint32_t per = static_cast<uint32_t>(a.rows_per_seq);
+    uint32_t seq = row / per, seq_end = (seq + 1) * per;
     const bool by_seq = (a.branch_weight.seq_stride | a.gate.seq_stride | a.weight.seq_stride) != 0;
     auto params = [&] {
       F2 c[NB][BP], w[NB][BP];
@@ -184,17 +187,15 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         kept.write(KEPT_W, b, w[b]);
       }
     };
-    uint64_t element = static_cast<uint64_t>(r0) * a.hidden;  // the row's first
-    TX* dx = static_cast<TX*>(a.dx) + element + cols.first;
-    TR* dres = static_cast<TR*>(a.dres) + element + cols.first;
     const bool sum_branch = plan.partials[SUM_BRANCH] != nullptr, sum_weight = plan.partials[SUM_WEIGHT] != nullptr,
                sum_shift = plan.partials[SUM_SHIFT] != nullptr, normed = a.dy != nullptr;
     params();
-    int item_left = static_cast<int>(items.first_row(item + 1) - r0);
+    uint32_t item_end = plan.joined ? 0u : static_cast<uint32_t>(items.first_row(item + 1));
     for (;;) {
+      const uint64_t element = static_cast<uint64_t>(row) * static_cast<uint32_t>(a.hidden);  // the row's first
       const uint32_t bits = a.dropped ? cols.kept(a.drop, key, element) : ~0u;
       const float2 rs = next_r;
-      if (left > 1) next_r = *++rstd;
+      if (row + 1 < end) next_r = rstd[row + 1];
       rows.advance(cols, plan.rows);
       kept.settle();
       F2 x[NB][BP], q[NB][BP], hat[NB][BP];  // x', dH and what it is made of, h'
@@ -203,8 +204,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       for (int b = 0; b < NB; ++b) {
         F2 u[BP], c[BP];
         kept.read(KEPT_C, b, c);
-        rows.template get<0>(b, x[b]);
-        rows.template get<3>(b, q[b]);
+        rows.template get<0>(cols, plan.rows, row, b, x[b]);
+        rows.template get<3>(cols, plan.rows, row, b, q[b]);
         kept.wait();
         kept.arrived(c);
 #pragma unroll
@@ -219,8 +220,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           F2 dy[BP], w[BP], sum[BP];
           kept.read(KEPT_W, b, w);
           kept.read(SUM_WEIGHT, b, sum);
-          rows.template get<1>(b, dy);
-          rows.template get<2>(b, hat[b]);
+          rows.template get<1>(cols, plan.rows, row, b, dy);
+          rows.template get<2>(cols, plan.rows, row, b, hat[b]);
           kept.wait();
           kept.arrived(w);
           kept.arrived(sum);
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         kept.wait();
         kept.arrived(c);
         kept.arrived(sum);
-        if (a.dres != nullptr) cols.store(dres, b, q[b]);
+        if (a.dres != nullptr) cols.store(static_cast<TR*>(a.dres) + element, b, q[b]);
         if (a.dropped) Cols::drop(bits, b, q[b]);
         if (sum_branch) {
 #pragma unroll
@@ -282,26 +283,24 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 #pragma unroll
             for (int j = 0; j < BP; ++j) q[b][j] = mul2(fma2(x[b][j], f2(m1, m1), q[b][j]), f2(rs.x, rs.x));
           }
-          cols.store(dx, b, q[b]);
+          cols.store(static_cast<TX*>(a.dx) + element, b, q[b]);
         }
         __syncwarp();
       }
-      dx += a.hidden;
-      dres += a.hidden;
-      if (--item_left == 0 && !plan.joined) {
+      ++row;
+      if (row == item_end) {
         kept.settle();
 #pragma unroll
         for (int i = 0; i < SUMS; ++i)
           if (plan.partials[i] != nullptr) give(i, plan.partials[i] + static_cast<int64_t>(item) * a.hidden);
         clear();
         ++item;
-        if (item < last) item_left = static_cast<int>(items.first_row(item + 1) - items.first_row(item));
+        if (item < last) item_end = items.first_row(item + 1);
       }
-      if (--left == 0) break;
-      element += a.hidden;
-      if (--seq_left == 0) {
+      if (row == end) break;
+      if (row == seq_end) {
         ++seq;
-        seq_left = static_cast<int>(a.rows_per_seq);
+        seq_end += per;
         if (by_seq) params();
       }
     }
@@ -313,10 +312,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     __syncthreads();
     float* parts = reinterpret_cast<float*>(smem);  // [SUMS][groups][hidden]
 #pragma unroll
-    for (int i = 0; i < SUMS; ++i)
-      if (plan.partials[i] != nullptr) give(i, parts + (i * plan.rows.groups + group) * a.hidden);
-    __syncthreads();
     for (int i = 0; i < SUMS; ++i) {
+      if (plan.partials[i] == nullptr) continue;
+      give(i, plan.rows.groups > 1 ? parts + (i * plan.rows.groups + group) * a.hidden
+                                   : plan.partials[i] + static_cast<int64_t>(blockIdx.x) * a.hidden);
+    }
+    if (plan.rows.groups > 1) __syncthreads();
+    for (int i = 0; i < SUMS && plan.rows.groups > 1; ++i) {
       if (plan.partials[i] == nullptr) continue;
       for (int c = threadIdx.x; c < a.hidden; c += blockDim.x) {
         float v = 0.f;
@@ -498,22 +500,22 @@ bool wants(const ResidualArgs& a, int sum) {
 }
 
 struct Shape {
-  int e, v, threads;  // v 0: any
+  int cols, threads;  // columns a thread; 0: any
+  bool shifted;
 };
 Shape shape_of(const ResidualArgs& a) {
-  const int e = row_chunk(a, true);
-  if (e > 1) {
-    // A warp a row as far as 8 columns a thread carry it, then 16 columns a thread; with 4 bytes a column 8 as far
-    // as they go, for which more rows fit into shared memory.
-    if (a.hidden <= 256) return {e, 8 / e, 32};
-    if (a.x_dtype == F32)
-      if (const int t = row_threads(a.hidden, e, 8 / e)) return {e, 8 / e, t};
-    if (const int t = row_threads(a.hidden, e, 16 / e)) return {e, 16 / e, t};
-  } else {
-    for (int v = 4; v <= 8; v *= 2)
-      if (const int t = row_threads(a.hidden, 1, v)) return {1, v, t};
-  }
-  return {1, 0, kRowThreads};
+  const int e = 16 / std::max(row_elem_bytes(a.x_dtype), row_elem_bytes(a.res_dtype));
+  const bool shifted = !rows_aligned(a, true);
+  // A warp a row as far as 8 columns a thread carry it, then 16 columns a thread; with 4 bytes a column, or two vectors
+  // for each chunk, 8 as far as they go, for which more rows fit into shared memory.
+  for (const auto& [stride, dtype] : {std::pair<int64_t, int>{a.x_stride, a.x_dtype}, {a.dy_stride, a.x_dtype},
+                                      {a.res_stride, a.res_dtype}, {a.dh_stride, a.res_dtype}})
+    if (stride * row_elem_bytes(dtype) > UINT32_MAX) return {0, kRowThreads, shifted};
+  if (a.hidden <= 256) return {8, 32, shifted};
+  if (a.x_dtype == F32 || shifted)
+    if (const int t = row_threads(a.hidden, e, 8 / e)) return {8, t, shifted};
+  if (const int t = row_threads(a.hidden, e, 16 / e); t != 0 && !(shifted && a.res_dtype == F32)) return {16, t, shifted};
+  return {0, kRowThreads, shifted};
 }
 
 // The split. One item for each CTA of a full grid where that leaves few of them without one and the rows of an item are
@@ -527,7 +529,7 @@ RowItems items_of(const ResidualArgs& a, const Shape& sh, bool* joined) {
   const int64_t ctas = num_sms(), per_cta = kRowThreads / sh.threads;
   it.chunks = std::min(std::max<int64_t>(1, ctas / it.seqs), it.seq_rows);
   const int64_t rows = (it.seq_rows + it.chunks - 1) / it.chunks;
-  *joined = sh.v > 0 && it.count() <= ctas && rows <= kItemRows * std::min(per_cta, rows) &&
+  *joined = sh.cols > 0 && it.count() <= ctas && rows <= kItemRows * std::min(per_cta, rows) &&
             (it.seqs == 1 || it.count() * 10 >= ctas * 9);
   if (!*joined) {
     it.chunks = std::max({ctas * per_cta / it.seqs, (it.seq_rows + kItemRows - 1) / kItemRows, int64_t{1}});
@@ -537,16 +539,13 @@ RowItems items_of(const ResidualArgs& a, const Shape& sh, bool* joined) {
   return it;
 }
 
-template <typename TX, typename TR, int E, int V>
+template <typename TX, typename TR, int V, bool SHIFTED>
 cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t st) {
-  constexpr int STAGES = row_stages<TX, TR>(E * V, 2, 2);
-  auto* kernel = residual_norm_backward_kernel<TX, TR, E, V, STAGES>;
-  using Stream = RowStream<TX, TR, E, V, 2, 2, STAGES>;
+  constexpr int E = kRowChunk<TX, TR>, STAGES = row_stages<TX, TR>(E * V, 2, 2, SHIFTED);
+  auto* kernel = residual_norm_backward_kernel<TX, TR, E, V, SHIFTED, STAGES>;
+  using Stream = RowStream<TX, TR, E, V, SHIFTED, 2, 2, STAGES>;
   const int threads = plan.rows.threads;
-  const int64_t count = plan.items.count(), x = sizeof(TX), r = sizeof(TR);
-  const int64_t step[4] = {a.x_stride * x, a.dy_stride * x, a.res_stride * r, a.dh_stride * r};
-  std::copy(step, step + 4, plan.rows.step);
-  plan.rows.present = 1 | (a.dy != nullptr ? 2 | 4 : 0) | (a.dh != nullptr ? 8 : 0);  // h serves the norm alone
+  const int64_t count = plan.items.count();
   // groups of a CTA: as many as have rows of their own
   const int64_t most = plan.joined ? (plan.items.seq_rows + plan.items.chunks - 1) / plan.items.chunks : count / num_sms();
   plan.rows.groups = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, most)));
@@ -565,14 +564,15 @@ cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t 
 
 template <typename TX, typename TR>
 cudaError_t launch_types(const ResidualArgs& a, BackwardPlan& plan, const Shape& sh, cudaStream_t st) {
-  constexpr int E = kRowChunk<TX, TR>;
-  if (sh.e == E) {
-    constexpr int HALF = 8 / E;  // chunks of 8 columns
-    if (sh.v == HALF) return launch_rows<TX, TR, E, HALF>(a, plan, st);
-    if (sh.v == 2 * HALF) return launch_rows<TX, TR, E, 2 * HALF>(a, plan, st);
-  } else {
-    if (sh.v == 4) return launch_rows<TX, TR, 1, 4>(a, plan, st);
-    if (sh.v == 8) return launch_rows<TX, TR, 1, 8>(a, plan, st);
+  constexpr int HALF = 8 / kRowChunk<TX, TR>;  // chunks of 8 columns
+  constexpr int64_t x = sizeof(TX), r = sizeof(TR);
+  set_tensors(&plan.rows, {{a.x, a.x_stride * x}, {a.dy, a.dy_stride * x}, {a.dy ? a.res : nullptr, a.res_stride * r},  // h serves the norm
+                           {a.dh, a.dh_stride * r}});
+  if (sh.cols == 8) return sh.shifted ? launch_rows<TX, TR, HALF, true>(a, plan, st) : launch_rows<TX, TR, HALF, false>(a, plan, st);
+  if (sh.cols == 16) {
+    if (!sh.shifted) return launch_rows<TX, TR, 2 * HALF, false>(a, plan, st);
+    // two vectors a chunk of 4 bytes a column: more than shared memory holds
+    if constexpr (sizeof(TR) == 2) return launch_rows<TX, TR, 2 * HALF, true>(a, plan, st);
   }
   note_launch();
   return launch_dependent(residual_norm_backward_any_kernel<TX, TR>,
