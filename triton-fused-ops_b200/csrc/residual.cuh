@@ -37,7 +37,10 @@ struct RowPlan {
   const char* base[4];  // the streamed tensors
   uint32_t step[4];     // bytes between their rows
   int present;      // a bit for each of them that is there (the others are zeros)
-  Split share;      // rows (backward: items) of the launch's groups
+  // The rows (backward: items) of the launch's groups: a run for each or, with a stride, every so manyth one, so that all
+  // groups read side by side (8192 x 4096: bf16 forward 49 -> 45 us, fp32 backward 74 -> 69 of half the rows).
+  Split share;
+  uint32_t stride;  // 0: runs
 };
 
 // ---- sums over a row --------------------------------------------------------
@@ -272,7 +275,7 @@ struct RowStream {
   static constexpr size_t kSmemBytes = static_cast<size_t>(STAGES) * kStageBytes;
   template <int I> using ChunkOf = std::conditional_t<(I < NX), ChunkX, ChunkR>;
 
-  uint32_t next, end;          // rows to load
+  uint32_t next, end, by;      // rows to load
   // Two tensors' next rows as pointers that walk on; with four they would cost registers that the rest needs, and are
   // made from the row's index (forward with dropout 65 us walking, 70 not; backward 84 -> 75 us in fp32).
   static constexpr bool WALK = kTensors == 2;
@@ -284,10 +287,11 @@ struct RowStream {
     return ((i < NX ? i * kBytesX : NX * kBytesX + (i - NX) * kBytesR) + v * vec_bytes) * kRowThreads;
   }
 
-  // Rows from `first` on, `rows` of them.
-  __device__ void start(const Cols& cols, const RowPlan& plan, void* smem, uint32_t first, uint32_t rows) {
+  // Rows from `first` on, before `last`, `step` apart.
+  __device__ void start(const Cols& cols, const RowPlan& plan, void* smem, uint32_t first, uint32_t last, uint32_t step) {
     next = first;
-    end = first + rows;
+    end = last;
+    by = step;
     if constexpr (WALK) {
 #pragma unroll
       for (int i = 0; i < kTensors; ++i)
@@ -358,7 +362,7 @@ struct RowStream {
         const char* from;
         if constexpr (WALK) {
           from = at[i];
-          at[i] += plan.step[i];
+          at[i] += static_cast<uint64_t>(plan.step[i]) * by;
         } else {
           from = plan.base[i] + static_cast<uint64_t>(next) * plan.step[i] + cols.first * (i < NX ? sizeof(TX) : sizeof(TR));
         }
@@ -366,7 +370,7 @@ struct RowStream {
         else copy<TR, ChunkR>(cols, i, from);
       }
     }
-    ++next;
+    next += by;
     write = next_stage(write);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }

@@ -36,12 +36,13 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   __syncthreads();
   griddep_wait();
   const uint32_t me = blockIdx.x * plan.groups + group;
-  uint32_t row = plan.share.first(me);
-  const uint32_t end = plan.share.first(me + 1);
-  if (row == end) return;
+  const uint32_t by = plan.stride != 0 ? plan.stride : 1u;
+  uint32_t row = plan.stride != 0 ? me : plan.share.first(me);
+  const uint32_t end = plan.stride != 0 ? static_cast<uint32_t>(a.rows) : plan.share.first(me + 1);
+  if (row >= end) return;
   const Cols cols(t, plan.threads, a.hidden);
   RowStream<TX, TR, E, V, SHIFTED, 1, 1, STAGES> rows;
-  rows.start(cols, plan, smem, row, end - row);
+  rows.start(cols, plan, smem, row, end, by);
   const DropKey key(a.drop);
   const float inv_h = 1.f / static_cast<float>(a.hidden);
   const int bar = 1 + group;
@@ -115,8 +116,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       }
     }
     if (a.rstd != nullptr && t == 0) reinterpret_cast<float2*>(a.rstd)[row] = make_float2(r_branch, r_sum);
-    if (++row == end) return;
-    if (row == seq_end) {
+    row += by;
+    if (row >= end) return;
+    if (row == seq_end) {  // (runs: with a stride no parameter differs between sequences)
       ++seq;
       seq_end += per;
       if (KEEP_PARAMS && by_seq) params();
@@ -194,6 +196,8 @@ cudaError_t launch_rows(const ResidualArgs& a, RowPlan plan, int threads, cudaSt
   plan.threads = threads;
   plan.groups = groups;
   plan.share = Split::make(a.rows, grid * groups);
+  const bool by_seq = (a.branch_weight.seq_stride | a.gate.seq_stride | a.weight.seq_stride | a.shift.seq_stride) != 0;
+  plan.stride = by_seq ? 0 : static_cast<uint32_t>(grid * groups);
   note_launch();
   return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a, plan);
 }

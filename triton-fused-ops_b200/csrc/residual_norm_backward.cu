@@ -118,8 +118,12 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   const RowItems items = plan.items;
   uint32_t item = plan.joined ? blockIdx.x : plan.rows.share.first(me);
   const uint32_t last = plan.joined ? item + 1 : plan.rows.share.first(me + 1);
-  uint32_t row = 0, end = 0;
-  if (item < last) {
+  uint32_t row = 0, end = 0, by = 1;
+  if (plan.rows.stride != 0) {
+    row = me;
+    end = static_cast<uint32_t>(a.rows);
+    by = plan.rows.stride;
+  } else if (item < last) {
     row = items.first_row(item);
     end = items.first_row(last);
     if (plan.joined) {
@@ -163,7 +167,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
   clear();
   if (row < end) {
     RowStream<TX, TR, E, V, SHIFTED, 2, 2, STAGES> rows;
-    rows.start(cols, plan.rows, smem, row, end - row);
+    rows.start(cols, plan.rows, smem, row, end, by);
     const DropKey key(a.drop);
     const float inv_h = 1.f / static_cast<float>(a.hidden);
     const int bar = 1 + group;
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
       const uint64_t element = static_cast<uint64_t>(row) * static_cast<uint32_t>(a.hidden);  // the row's first
       const uint32_t bits = a.dropped ? cols.kept(a.drop, key, element) : ~0u;
       const float2 rs = next_r;
-      if (row + 1 < end) next_r = rstd[row + 1];
+      if (row + by < end) next_r = rstd[row + by];
       rows.advance(cols, plan.rows);
       kept.settle();
       F2 x[NB][BP], q[NB][BP], hat[NB][BP];  // x', dH and what it is made of, h'
@@ -287,7 +291,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         }
         __syncwarp();
       }
-      ++row;
+      row += by;
       if (row == item_end) {
         kept.settle();
 #pragma unroll
@@ -297,7 +301,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         ++item;
         if (item < last) item_end = items.first_row(item + 1);
       }
-      if (row == end) break;
+      if (row >= end) break;
       if (row == seq_end) {
         ++seq;
         seq_end += per;
@@ -558,6 +562,7 @@ cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t 
   const int64_t all = static_cast<int64_t>(num_sms()) * std::max(1, cached_occupancy(fn, block, smem));
   const int64_t grid = plan.joined ? count : std::min<int64_t>(all, (count + plan.rows.groups - 1) / plan.rows.groups);
   plan.rows.share = Split::make(count, grid * plan.rows.groups);
+  plan.rows.stride = plan.joined && plan.items.seqs == 1 ? static_cast<uint32_t>(grid * plan.rows.groups) : 0;
   note_launch();
   return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a, plan);
 }
