@@ -93,8 +93,9 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         h[b][j] = add2(res[j], h[b][j]);
         s2 = fma2(h[b][j], h[b][j], s2);
       }
-      cols.store(static_cast<TR*>(a.h) + element, b, h[b]);
     }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) cols.store(static_cast<TR*>(a.h) + element, b, h[b]);
     float r_sum = 1.f;
     if (a.y != nullptr) {
       float s[1] = {s2.x + s2.y};
@@ -178,15 +179,12 @@ __global__ void __launch_bounds__(kRowThreads) residual_norm_any_kernel(const __
 }
 
 namespace {
-template <typename TX, typename TR, int V, bool SHIFTED>
-cudaError_t launch_rows(const ResidualArgs& a, RowPlan plan, int threads, cudaStream_t st) {
-  constexpr int E = kRowChunk<TX, TR>, STAGES = row_stages<TX, TR>(E * V, 1, 1, SHIFTED);
+template <typename TX, typename TR, int V, bool SHIFTED, int STAGES>
+cudaError_t launch_groups(const ResidualArgs& a, RowPlan plan, int threads, int groups, cudaStream_t st) {
+  constexpr int E = kRowChunk<TX, TR>;
   auto* kernel = residual_norm_kernel<TX, TR, E, V, SHIFTED, STAGES>;
   using Stream = RowStream<TX, TR, E, V, SHIFTED, 1, 1, STAGES>;
   const void* fn = reinterpret_cast<const void*>(kernel);
-  // as many groups a CTA as still leave every SM a row
-  const int groups =
-      static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, a.rows / num_sms())));
   const int block = groups * threads;
   const size_t smem = Stream::kSmemBytes;
   // at least a little over 48 KB: the sums' static part comes on top
@@ -200,6 +198,25 @@ cudaError_t launch_rows(const ResidualArgs& a, RowPlan plan, int threads, cudaSt
   plan.stride = by_seq ? 0 : static_cast<uint32_t>(grid * groups);
   note_launch();
   return launch_gemm_grid(kernel, block, static_cast<int>(grid), 1, smem, st, a, plan);
+}
+
+template <typename TX, typename TR, int V, bool SHIFTED>
+cudaError_t launch_rows(const ResidualArgs& a, const RowPlan& plan, int threads, cudaStream_t st) {
+  constexpr int COLS = kRowChunk<TX, TR> * V, MOST = row_stages<TX, TR>(COLS, 1, 1, SHIFTED);
+  // as many groups a CTA as still leave every SM a row
+  const int groups =
+      static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowThreads / threads, a.rows / num_sms())));
+  // One row ahead is enough where a CTA's groups wait for different rows, and reads and writes lie closer together in
+  // memory than with two or three: bf16 65536 x 4096 356 -> 331 us, 65536 x 2048 186 -> 165, with an fp32 stream
+  // 16384 x 4096 137 -> 130. A group alone needs more (8192 x 8192 93 us, with two ahead 87), and the first rows come
+  // faster with more, which tells where a group has few of them (bf16 8192 x 4096 47 us, with three ahead 46; one row
+  // ahead is only 32 KB an SM there, and 48 or 64 with a type of 32 bits).
+  if constexpr (!SHIFTED && COLS == 16 && MOST > 2) {
+    const int64_t many = sizeof(TX) + sizeof(TR) > 4 ? 24 : 96;
+    if (groups > 2 || (groups == 2 && a.rows / (num_sms() * groups) >= many))
+      return launch_groups<TX, TR, V, SHIFTED, 2>(a, plan, threads, groups, st);
+  }
+  return launch_groups<TX, TR, V, SHIFTED, MOST>(a, plan, threads, groups, st);
 }
 
 // A warp a row as far as 16 columns a thread carry it, then 16 columns a thread, then (aligned rows) 32.
