@@ -111,6 +111,17 @@ def test_c_abi_refusals():
     assert forward(norm=0, p=params(branch_weight=_lib.RowParam(16, 0, 2, None))) == _lib.ERR_INVALID
     assert backward(rstd=None) == backward(rstd=4) == backward(per=3) == _lib.ERR_INVALID
 
+    def strided(x=8, res=8):
+        return lib.tfo_residual_rmsnorm(16, x, 16, res, params(), 16, None, None, 4, 2, 8, 1, 1.0, 1e-6, None, 0, 0, None)
+
+    def strided_backward(x=8, res=8, dh=8, dy=8):
+        return lib.tfo_residual_rmsnorm_backward(16, dh, 16, dy, 16, x, 16, res, params(), 16, 16, 16, 4, 2, 8, 1, 1.0, None, 0, 0,
+                                                 None, 0, None)
+
+    assert strided(x=-8) == strided(res=-1) == _lib.ERR_INVALID
+    for wrong in (dict(x=-8), dict(res=-8), dict(dh=-8), dict(dy=-8)):
+        assert strided_backward(**wrong) == _lib.ERR_INVALID
+
     def heads(axes):
         s = (ctypes.c_int64 * 3)(64, 64, 8)
         return lib.tfo_rope_axes(16, s, None, None, 16, 16, 8, 4, 16, _lib.POS_I64, 4, 1, 16, None, 1, 4, 1, 0, 8, 8, 0, 0, 0, 2, axes,

@@ -47,6 +47,7 @@ int set_rows(ResidualArgs* a, const std::string& fn, const void* x, int64_t x_st
   if (rows < 0 || rows > INT32_MAX) return fail(TFO_ERR_INVALID, fn + ": rows must be in 0..2^31 - 1");
   if (rows > 0 && (rows_per_seq <= 0 || rows % rows_per_seq != 0))
     return fail(TFO_ERR_INVALID, fn + ": rows_per_seq must divide rows");
+  if (x_stride < 0 || res_stride < 0) return fail(TFO_ERR_INVALID, fn + ": negative row stride");
   if (params == nullptr || (rows > 0 && (x == nullptr || res == nullptr)))
     return fail(TFO_ERR_INVALID, fn + ": NULL pointer");
   RowParam* to[4] = {&a->branch_weight, &a->gate, &a->weight, &a->shift};
@@ -161,6 +162,7 @@ int tfo_residual_rmsnorm_backward(const void* dh, int64_t dh_stride, const void*
   a.rstd = const_cast<float*>(rstd);
   a.scale = static_cast<float>(scale);
   set_grads(&a, dh, dh_stride, dy, dy_stride, dx, dresidual);
+  if (dh_stride < 0 || dy_stride < 0) return fail(TFO_ERR_INVALID, std::string(fn) + ": negative row stride");
   const size_t need = residual_norm_backward_workspace_bytes(a);
   if (need > 0 && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))
     return fail(TFO_ERR_INVALID, std::string(fn) + ": workspace too small or not aligned");
