@@ -328,6 +328,88 @@ def test_values_at_the_borders(cuda, hidden):
     assert (got["h"] == 0).all() and (got["y"] == 0).all()
 
 
+@pytest.mark.parametrize("hidden", [200, 512, 777, 4400, 20000])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_dropped_infinities_leave_no_trace(cuda, dtype, hidden):
+    """Without the branch norm what lies at dropped places changes nothing, the gate's gradient included."""
+    shape, p, seed = (2, 30, hidden), 0.5, 5
+    t = make(shape, dtype, dtype, gate="f32", shift="f32")
+    dropped = ~dropout_keep_reference(shape, p, seed, 0, "cuda")
+    gh, gy = randn(shape, dtype, 11), randn(shape, dtype, 12)
+    want = run(t, False, 0.7, p, seed, gh, gy)
+    t["x"] = torch.where(dropped, torch.tensor([float("inf"), float("nan")] * (hidden // 2) + [-1.0] * (hidden % 2), device="cuda"),
+                         t["x"]).to(DT[dtype])
+    got = run(t, False, 0.7, p, seed, gh, gy)
+    assert all(torch.equal(got[k], want[k]) for k in want if want[k] is not None)
+
+
+@pytest.mark.parametrize("dtype,stream,hidden", [
+    ("bf16", "bf16", 33), ("f16", "f16", 1001), ("f16", "f32", 1001), ("f32", "f32", 1002), ("bf16", "bf16", 4101),
+    ("bf16", "f32", 4101), ("f32", "f32", 4103), ("f16", "f16", 6001), ("bf16", "bf16", 8192), ("f32", "f32", 8000),
+])
+def test_every_alignment(cuda, dtype, stream, hidden):
+    """Rows that start anywhere in a vector, x and the stream at different places of theirs."""
+    from triton_ops import fused_residual_rmsnorm
+
+    shape = (2, 9, hidden)
+    params = make(shape, dtype, stream, branch_weight="f32", gate="bf16", shift="f32", per="gate")
+    keep = dropout_keep_reference(shape, 0.2, 7, 0, "cuda")
+    for start in range(8):
+        t = {**params, "x": randn(shape, dtype, 1, start), "residual": randn(shape, stream, 2, (3 * start + 1) % 8)}
+        gh, gy = randn(shape, stream, 11, (5 * start + 2) % 8), randn(shape, dtype, 12, 7 - start)
+        got = run(t, True, 0.7, 0.2, 7, gh, gy)
+        compare(t, got, formulas(t, True, 0.7, keep, 0.2, gh, gy), f"start {start}")
+        with torch.no_grad():  # a tensor beside the rows is not written
+            h, y = fused_residual_rmsnorm(t["x"], t["residual"], t["weight"], t["gate"], branch_norm=True, scale=0.7, eps=EPS,
+                                          branch_weight=t["branch_weight"], shift=t["shift"], dropout_p=0.2, seed=7)
+        assert torch.equal(h, got["h"]) and torch.equal(y, got["y"])
+
+
+@pytest.mark.parametrize("dtype,stream,rows,hidden", [
+    ("bf16", "bf16", 30000, 4096), ("bf16", "f32", 8000, 4096), ("f32", "f32", 7500, 2560), ("f16", "f16", 3000, 1024),
+])
+def test_groups_with_many_rows(cuda, dtype, stream, rows, hidden):
+    t = make((rows, hidden), dtype, stream, branch_weight="f32")
+    at = torch.cat([torch.arange(200), torch.arange(rows // 2, rows // 2 + 200), torch.arange(rows - 900, rows)]).cuda()
+    part = {k: v if v is None or v.dim() == 1 else v[at] for k, v in t.items()}
+    got = run(t, True)
+    compare(part, {k: v[at] for k, v in got.items()}, formulas(part, True, 1.0), "many rows")
+
+
+def test_captured_beside_an_eager_graph(cuda):
+    """A step captured, through leaves of its own, while an eager graph of the same memory waits for its backward pass.
+
+    (torch itself refuses the capture of a backward pass whose leaves an eager graph holds.)
+    """
+    from triton_ops import fused_dropout, fused_residual_rmsnorm
+
+    x, res = (randn((64, 520), "bf16", i).requires_grad_() for i in (1, 2))
+    w = torch.ones(520, device="cuda", requires_grad=True)
+    seed = torch.tensor([3], device="cuda")
+    eager_leaves = (x, res, w)
+
+    def loss(x, res, w):
+        h, y = fused_residual_rmsnorm(x, res, w, branch_norm=True, dropout_p=0.1, seed=seed)
+        return fused_dropout(y, 0.2, seed, offset=1, residual=h).float().sum()
+
+    want = torch.autograd.grad(loss(*eager_leaves), eager_leaves)
+    eager = loss(*eager_leaves)
+    leaves = [t.detach().requires_grad_() for t in eager_leaves]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            torch.autograd.grad(loss(*leaves), leaves)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        captured = torch.autograd.grad(loss(*leaves), leaves)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(captured, want))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(eager, eager_leaves), want))
+
+
 def test_gradients_against_differences(cuda):
     """Central differences of the fp32 op's own formula in 64 bits, along random directions."""
     from triton_ops.kernels.residual import residual_rmsnorm_reference

@@ -193,6 +193,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
     };
     const bool sum_branch = plan.partials[SUM_BRANCH] != nullptr, sum_weight = plan.partials[SUM_WEIGHT] != nullptr,
                sum_shift = plan.partials[SUM_SHIFT] != nullptr, normed = a.dy != nullptr;
+    // a branch that is not normed is dropped itself, so that infinities there stay out of the sum of A
+    const bool drop_x = a.dropped && !a.branch_norm, drop_u = a.dropped && a.branch_norm;
     params();
     uint32_t item_end = plan.joined ? 0u : static_cast<uint32_t>(items.first_row(item + 1));
     for (;;) {
@@ -210,6 +212,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
         kept.read(KEPT_C, b, c);
         rows.template get<0>(cols, plan.rows, row, b, x[b]);
         rows.template get<3>(cols, plan.rows, row, b, q[b]);
+        if (drop_x) Cols::drop(bits, b, x[b]);
         kept.wait();
         kept.arrived(c);
 #pragma unroll
@@ -217,7 +220,7 @@ __global__ void __launch_bounds__(kRowThreads, 1)
           x[b][j] = mul2(x[b][j], f2(rs.x, rs.x));
           u[j] = mul2(x[b][j], c[j]);
         }
-        if (a.dropped) Cols::drop(bits, b, u);
+        if (drop_u) Cols::drop(bits, b, u);
 #pragma unroll
         for (int j = 0; j < BP; ++j) s1 = fma2(u[j], q[b][j], s1);
         if (normed) {
@@ -403,7 +406,7 @@ __global__ void __launch_bounds__(kRowThreads)
           const float b = e * v.c;
           static_cast<TX*>(a.dx)[r * a.hidden + i] = Ty<TX>::from_f(a.branch_norm ? rs.x * (b - v.x * m1) : b);
         }
-        const float add[SUMS] = {e * v.x, v.dy * v.hat, v.dy};
+        const float add[SUMS] = {v.keep ? e * v.x : 0.f, v.dy * v.hat, v.dy};
 #pragma unroll
         for (int p = 0; p < SUMS; ++p) {
           if (plan.partials[p] == nullptr) continue;
@@ -548,6 +551,9 @@ cudaError_t launch_rows(const ResidualArgs& a, BackwardPlan& plan, cudaStream_t 
   constexpr int E = kRowChunk<TX, TR>, STAGES = row_stages<TX, TR>(E * V, 2, 2, SHIFTED);
   auto* kernel = residual_norm_backward_kernel<TX, TR, E, V, SHIFTED, STAGES>;
   using Stream = RowStream<TX, TR, E, V, SHIFTED, 2, 2, STAGES>;
+  // A launch before it may let this one start before its own CTAs have their tensor memory: none of those (120 KB and
+  // more of shared memory) shares an SM with a CTA of this one, whose allocation would keep theirs waiting.
+  static_assert(E * V != 16 || Stream::kSmemBytes >= 120 * 1024, "alone on its SM beside kernels with tensor memory");
   const int threads = plan.rows.threads;
   const int64_t count = plan.items.count();
   // groups of a CTA: as many as have rows of their own
