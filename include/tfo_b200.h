@@ -428,7 +428,8 @@ typedef struct tfo_dropout_params {
  * is NULL; n contiguous elements, fp32 with one rounding. residual and out
  * have out_dtype: x_dtype; or F32 for a 16-bit x with a residual; or a 16-bit
  * type for an F32 x without one (the gradient of the former). The gradient of
- * x is the same call on out's gradient, without a residual. */
+ * x is the same call on out's gradient, without a residual. out overlaps
+ * neither input. */
 TFO_API int tfo_dropout(const void* x, const void* residual, void* out, int64_t n, const tfo_dropout_params* dropout,
                         int x_dtype, int out_dtype, void* stream);
 
@@ -450,7 +451,8 @@ typedef struct tfo_row_param {
  * x and residual have rows x_stride / residual_stride elements apart (innermost
  * stride 1), h and y are contiguous. rows_per_seq divides rows. residual_dtype:
  * x_dtype or F32. dropout NULL: none; element i of row r counts as r * hidden + i.
- * rstd: [rows, 2] fp32 for the backward pass, or NULL. */
+ * rstd: [rows, 2] fp32 for the backward pass, or NULL. No output overlaps an
+ * input. */
 TFO_API int tfo_residual_rmsnorm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                                  const tfo_row_param* params, void* h, void* y, float* rstd, int64_t rows,
                                  int64_t rows_per_seq, int64_t hidden, int branch_norm, double scale, double eps,
@@ -460,7 +462,8 @@ TFO_API int tfo_residual_rmsnorm(const void* x, int64_t x_stride, const void* re
  * dh (residual_dtype) and dy (x_dtype) of its outputs (either may be NULL:
  * zeros). dx and dresidual are contiguous (NULL: not wanted), the parameters'
  * go to their `grad`. Sums over rows are fp32 within runs of at most 2048 rows
- * and fp64 over those, in a fixed order (no atomics). No rows: nothing is
+ * and the up to 16 runs of a CTA, and fp64 over those, in a fixed order (no
+ * atomics). No rows: nothing is
  * written. The workspace (16-byte aligned) is needed for the parameters'
  * gradients and not shared by calls that may alternate on a stream; its size
  * depends on the same arguments. */
