@@ -199,8 +199,7 @@ template <int E, int V, bool SHIFTED> struct RowCols {
         if (has(at)) *reinterpret_cast<typename C::Raw*>(to) = own;
         continue;
       }
-      // The aligned vector in which this chunk begins: the lane before's last columns and this one's first. A lane
-      // without the columns for it, the warp's first one and the last of the row give theirs one by one.
+      // The aligned vector in which this chunk begins: the lane before's last columns and this one's first.
       const int lane = threadIdx.x & 31, n = count(at);
       const int head = static_cast<int>((C::kBytes - shift) / sizeof(T));  // own columns in that vector
       typename C::Raw before;
@@ -208,11 +207,32 @@ template <int E, int V, bool SHIFTED> struct RowCols {
       uint32_t* u = reinterpret_cast<uint32_t*>(&before);
 #pragma unroll
       for (int i = 0; i < C::kWords; ++i) u[i] = __shfl_up_sync(0xffffffffu, w[i], 1);
+      const typename C::Raw joined = shift == 0 ? own : C::joined(before, own, C::kBytes - shift);
+      auto* vector = reinterpret_cast<typename C::Raw*>(reinterpret_cast<char*>(to) - shift);
+      if (col(at) - lane * E + 32 * E <= hidden) {
+        // Whole chunks in all lanes. The E columns that are left, the first lane's first ones and the last lane's last
+        // ones, by a lane each.
+        if (shift == 0 || lane > 0) *vector = joined;
+        const int from = lane < head ? 0 : 31;
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < C::kWords; ++i) {
+          const uint32_t got = __shfl_sync(0xffffffffu, w[i], from);
+          if (lane * static_cast<int>(sizeof(T)) / 4 == i) word = got;
+        }
+        if (shift != 0 && lane < E) {
+          T* one = to + (from - lane) * E + lane;
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(one) = word;
+          else *reinterpret_cast<uint16_t*>(one) = static_cast<uint16_t>(lane & 1 ? word >> 16 : word);
+        }
+        __syncwarp();
+        continue;
+      }
+      // The row's end: a lane without the columns for its vector, the first one and the last of the row give theirs one by
+      // one.
       const bool whole = n >= head && (shift == 0 || lane > 0);
       const bool next = __shfl_down_sync(0xffffffffu, static_cast<int>(whole), 1) && lane < 31;
-      if (whole)
-        *reinterpret_cast<typename C::Raw*>(reinterpret_cast<char*>(to) - shift) =
-            shift == 0 ? own : C::joined(before, own, C::kBytes - shift);
+      if (whole) *vector = joined;
       if (!whole || !next) {
 #pragma unroll
         for (int j = 0; j < E; ++j)
