@@ -10,7 +10,9 @@
 // takes units of 8 neighbouring elements, two at a time: four generator blocks
 // side by side, 16-byte accesses. The rounds' keys stay in registers, and the
 // counter's upper half is the same for the whole launch (2^34 elements), so that
-// what it leads to in the first two rounds is made once for a thread.
+// what it leads to in the first two rounds is made once for a thread. Measured for
+// 8192 x 4096: bf16 35.7 us (57 % of the copy rate at 61 % of the issue slots), with
+// a residual 39.6 (78 %); fp32 43 (95 %), with one 62 (99 %).
 #include "heads.cuh"
 #include "philox.cuh"
 
@@ -160,7 +162,7 @@ cudaError_t launch(const void* x, const void* residual, void* out, int64_t n, co
   const auto* rs = static_cast<const TO*>(residual);
   auto* os = static_cast<TO*>(out);
   // Walking on or done at once, by the bytes that a unit has in flight. Measured for 8192 x 4096 elements, us walking /
-  // at once: bf16 35 / 40, with a residual 38 / 51; fp32 54 / 43, with a residual 66 / 62.
+  // at once: bf16 36 / 40, with a residual 40 / 51; fp32 54 / 43, with a residual 66 / 62.
   constexpr bool WALK = sizeof(TX) + sizeof(TO) < 8;
   if (d.none || d.all) {
     note_launch();

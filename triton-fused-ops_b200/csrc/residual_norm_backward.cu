@@ -21,6 +21,10 @@
 // parameter's factor. No atomics: the results do not depend on scheduling.
 //
 // Floor: HBM (x, residual, dy and dh read, dx and dresidual written).
+// Measured, of the copy rate, with the second kernel (4 us): bf16 32768 x 4096 266
+// us (92 %), 8192 x 4096 82 (75 %: the start with its parameters, the end with its
+// sums), 8192 x 8192 149 (82 %), fp32 4096 x 4096 69 (88 %), with dropout 8192 x
+// 4096 bf16 103 (60 %).
 #include "residual.cuh"
 
 namespace tfo {
