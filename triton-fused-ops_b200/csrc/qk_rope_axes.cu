@@ -63,6 +63,7 @@ cudaError_t join(const HeadArgs& a, void* cos, void* sin, cudaStream_t st) {
 cudaError_t join_axes(HeadArgs* a, bool backward, cudaStream_t st) {
   const int elems = head_vector_elems(*a, backward);
   if (a->t.joined == nullptr || elems == 0 || !head_streams(*a, elems) || !mixed(*a, elems)) return cudaSuccess;
+  if (a->batch * a->seq > INT32_MAX) return cudaSuccess;  // tokens are 32-bit numbers there
   const int pairs = a->rotary_dim / 2;
   void* cos = a->t.joined;
   void* sin = static_cast<char*>(cos) + axes_workspace_bytes(a->batch * a->seq, pairs, a->t.dtype) / 2;
