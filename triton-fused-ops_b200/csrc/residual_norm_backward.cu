@@ -49,6 +49,9 @@ struct RowItems {
 // memory: a block of 8 is read or written by one instruction, and the registers
 // are free for the row. Warp w of the CTA uses the lanes of its sub-partition
 // (w % 4) and columns of its own. With 8 columns or less they are registers.
+// These instructions take a warp whose lanes are together; what stands before them
+// parts the lanes where a row ends inside the warp (its copies, the columns past its
+// end, its stores). Each of them therefore joins the lanes first.
 enum Kept : int { KEPT_C = SUMS, KEPT_W = SUMS + 1, KEPT = SUMS + 2 };
 template <class Cols, bool TENSOR> struct RowKept {
   F2 v[KEPT][Cols::BLOCKS][Cols::BP];
@@ -74,14 +77,24 @@ template <class Cols> struct RowKept<Cols, true> {
     mine = base + ((w & 3u) << 21) + (w >> 2) * (KEPT * 16);  // lane 32 * (w % 4) in the upper half
   }
   // Between a write and a read of the same values.
-  __device__ void settle() { tmem_st_wait(); }
+  __device__ void settle() {
+    __syncwarp();
+    tmem_st_wait();
+  }
   // Asks for a block; it is there after wait() and arrived() of it.
   __device__ void read(int i, int b, F2 (&out)[4]) const {
+    __syncwarp();
     tmem_ld8(mine + 16 * i + 8 * b, *reinterpret_cast<uint32_t(*)[8]>(&out));
   }
-  __device__ void wait() { tmem_ld_wait(); }
+  __device__ void wait() {
+    __syncwarp();
+    tmem_ld_wait();
+  }
   __device__ void arrived(F2 (&out)[4]) const { tmem_ld_fence(*reinterpret_cast<uint32_t(*)[8]>(&out)); }
-  __device__ void write(int i, int b, const F2 (&in)[4]) { tmem_st8(mine + 16 * i + 8 * b, *reinterpret_cast<const uint32_t(*)[8]>(&in)); }
+  __device__ void write(int i, int b, const F2 (&in)[4]) {
+    __syncwarp();
+    tmem_st8(mine + 16 * i + 8 * b, *reinterpret_cast<const uint32_t(*)[8]>(&in));
+  }
 };
 
 struct BackwardPlan {
