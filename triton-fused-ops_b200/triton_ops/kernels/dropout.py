@@ -119,30 +119,58 @@ def fused_dropout(
     return _FusedDropout.apply(x, residual, float(p), seed, offset, dtype)
 
 
+def module_seed(module: torch.nn.Module, device: torch.device) -> torch.Tensor:
+    """The seed of one training call of a module with dropout, on `device` (the backward pass reads it again).
+
+    Drawn from torch's generator of the device or, where the module was given a
+    seed, the number in its buffer, which goes up by one on the device. A call in
+    a backward pass is a forward pass made again for its activations: torch's
+    generators are put back for it, the buffer is not, so that it is refused.
+    """
+    if not module.seed_given:
+        return torch.empty(1, dtype=torch.int64, device=device).random_()
+    if torch._C._current_graph_task_id() != -1:
+        raise RuntimeError("a dropout module with a seed of its own numbers its calls and cannot make one again in a backward "
+                           "pass (activation checkpointing): leave its seed out, so that torch's generators give it")
+    mine = module.seed.clone()
+    module.seed.add_(1)
+    return mine
+
+
 class FusedDropout(torch.nn.Module):
-    """Module form: a seed in a buffer, which every training call advances on the device.
+    """Module form: each training call drops other elements.
+
+    Args:
+        p: probability that an element is dropped
+        seed: None: every call draws its seed on the device from torch's generator,
+            as ``torch.nn.Dropout`` draws its mask: ``torch.manual_seed`` governs it,
+            activation checkpointing makes the same mask again, modules and ranks
+            with generators of their own are independent. An int: calls are
+            numbered from it in a buffer of the module, whatever torch's generators
+            do; modules whose numbers meet drop the same elements (seeds further
+            apart than there are calls do not), and a call in a backward pass
+            (checkpointing) raises
 
     Calls in evaluation mode return x (plus the residual). A captured training
-    step advances the seed with each replay.
+    step takes another seed with each replay.
     """
 
-    def __init__(self, p: float, seed: int = 0):
+    def __init__(self, p: float, seed: Optional[int] = None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"the dropout probability must be in 0..1, got {p}")
         self.p = p
-        self.register_buffer("seed", torch.tensor([seed], dtype=torch.int64))
+        self.seed_given = seed is not None
+        self.register_buffer("seed", torch.tensor([seed or 0], dtype=torch.int64))
 
-    def next_seed(self) -> torch.Tensor:
-        """This call's seed, a copy of its own (the backward pass reads it again)."""
-        mine = self.seed.clone()
-        self.seed.add_(1)
-        return mine
+    def next_seed(self, device: Optional[torch.device] = None) -> torch.Tensor:
+        """This call's seed, a tensor of its own on `device` (default: that of the module's buffer)."""
+        return module_seed(self, self.seed.device if device is None else device)
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if not self.training or self.p == 0:
             return x if residual is None else x + residual
-        return fused_dropout(x, self.p, self.next_seed(), residual=residual)
+        return fused_dropout(x, self.p, self.next_seed(x.device), residual=residual)
 
 
 def dropout_keep_reference(shape, p: float, seed: int, offset: int = 0, device="cpu") -> torch.Tensor:

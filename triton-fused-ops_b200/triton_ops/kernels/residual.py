@@ -18,7 +18,7 @@ import torch
 
 from triton_ops import _lib
 from triton_ops.kernels._native import NativeKernel
-from triton_ops.kernels.dropout import Seed, dropout_params, split_seed
+from triton_ops.kernels.dropout import Seed, dropout_params, module_seed, split_seed
 from triton_ops.validation import refuse_tangents, validate_residual_inputs
 
 fused_residual_rmsnorm_kernel = NativeKernel(
@@ -237,15 +237,16 @@ def residual_rmsnorm_reference(
 
 
 class FusedResidualRMSNorm(torch.nn.Module):
-    """Module form: holds the fp32 norm weights (ones), with ``layer_scale`` a gate of its own, and a dropout seed.
+    """Module form: holds the fp32 norm weights (ones) and, with ``layer_scale``, a gate of its own.
 
     With ``branch_norm`` a block has norms on both sides. In training with
-    ``dropout`` > 0 each call advances the seed on the device, as
+    ``dropout`` > 0 each call has a seed of its own: drawn from torch's generator
+    or, with a ``dropout_seed``, numbered from it, as
     :class:`~triton_ops.kernels.dropout.FusedDropout` does.
     """
 
     def __init__(self, hidden_dim: int, eps: float = 1e-6, *, branch_norm: bool = False, scale: float = 1.0,
-                 layer_scale: Optional[float] = None, dropout: float = 0.0, dropout_seed: int = 0):
+                 layer_scale: Optional[float] = None, dropout: float = 0.0, dropout_seed: Optional[int] = None):
         super().__init__()
         if not 0.0 <= dropout <= 1.0:
             raise ValueError(f"the dropout probability must be in 0..1, got {dropout}")
@@ -253,7 +254,8 @@ class FusedResidualRMSNorm(torch.nn.Module):
         self.weight = torch.nn.Parameter(torch.ones(hidden_dim))
         self.branch_weight = torch.nn.Parameter(torch.ones(hidden_dim)) if branch_norm else None
         self.gate = torch.nn.Parameter(torch.full((hidden_dim,), float(layer_scale))) if layer_scale is not None else None
-        self.register_buffer("seed", torch.tensor([dropout_seed], dtype=torch.int64))
+        self.seed_given = dropout_seed is not None
+        self.register_buffer("seed", torch.tensor([dropout_seed or 0], dtype=torch.int64))
 
     def forward(
         self,
@@ -263,10 +265,8 @@ class FusedResidualRMSNorm(torch.nn.Module):
         shift: Optional[torch.Tensor] = None,
     ) -> Tuple[torch.Tensor, torch.Tensor]:
         """(h, y); `gate` takes the place of the module's own."""
-        p, seed = (self.dropout, None) if self.training else (0.0, None)
-        if p > 0:
-            seed = self.seed.clone()  # read again by the backward pass
-            self.seed.add_(1)
+        p = self.dropout if self.training else 0.0
+        seed = module_seed(self, x.device) if p > 0 else None
         return fused_residual_rmsnorm(x, residual, self.weight, self.gate if gate is None else gate,
                                       branch_norm=self.branch_norm, branch_weight=self.branch_weight, shift=shift,
                                       scale=self.scale, eps=self.eps, dropout_p=p, seed=seed)
