@@ -355,14 +355,20 @@ typedef struct tfo_axes {
   int axes;                    /* 2..4 */
   int64_t pos_stride;          /* elements between the axes' positions */
   const uint8_t* axis_of_pair; /* host memory, one for each pair of columns */
-  void* workspace;             /* heads: tfo_rope_axes_workspace_bytes of scratch, or NULL */
+  void* workspace;             /* heads: tfo_rope_axes_workspace_bytes of scratch, or NULL; else not read */
   size_t workspace_bytes;
 } tfo_axes;
 
 /* Scratch with which calls of many tokens put each token's table row together
  * first where axes share vectors of columns (without it they are slower).
- * 16-byte aligned, not shared by calls that may alternate on a stream. */
+ * 16-byte aligned, not shared by calls that may alternate on a stream. The call's
+ * own figure is the same, or 0 where heads of its sizes on the current device make no
+ * use of it (few tokens, axes whose sections are whole vectors of columns); of its
+ * axes, workspace and pos_stride are not read. Errors: 0. */
 TFO_API size_t tfo_rope_axes_workspace_bytes(int64_t tokens, int64_t rotary_dim, int table_dtype);
+TFO_API size_t tfo_rope_axes_call_workspace_bytes(int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads,
+                                                  int64_t head_dim, int64_t rotary_dim, int interleaved, int dtype,
+                                                  int table_dtype, const tfo_axes* axes);
 
 TFO_API int tfo_rope_tables_axes(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half,
                                  double gain, void* cos, void* sin, int out_dtype, const tfo_axes* axes,

@@ -280,6 +280,8 @@ cudaError_t qk_rope_launch(const HeadArgs& a, cudaStream_t st);
 // for each token beforehand and the launch of one position.
 cudaError_t qk_rope_axes_launch(const HeadArgs& a, cudaStream_t st);
 size_t axes_workspace_bytes(int64_t tokens, int pairs, int table_dtype);
+// Whether join_axes would use that room, had `a` a fitting alignment.
+bool axes_may_join(const HeadArgs& a);
 // Joins the rows of `a`, if it has room for them and that is the faster way, and makes it a call of one position.
 cudaError_t join_axes(HeadArgs* a, bool backward, cudaStream_t st);
 // Whether the tokens are enough for the streaming kernel (qk_rope.cu).
@@ -287,6 +289,8 @@ bool head_streams(const HeadArgs& a, int elems);
 size_t qk_norm_rope_backward_workspace_bytes(int head_dim);
 cudaError_t qk_norm_rope_backward_launch(const HeadArgs& a, void* ws, cudaStream_t st);
 cudaError_t qk_norm_rope_backward_axes_launch(const HeadArgs& a, void* ws, cudaStream_t st);  // qk_rope_backward_axes.cu
+// Whether heads of these sizes are whole vectors of `elems` elements.
+bool head_vectors_fit(const HeadArgs& a, int elems);
 // Elements per vector with which the vector kernels can take these heads (0: they cannot).
 int head_vector_elems(const HeadArgs& a, bool backward);
 

@@ -105,6 +105,24 @@ size_t tfo_rope_axes_workspace_bytes(int64_t tokens, int64_t rotary_dim, int tab
   return axes_workspace_bytes(tokens, static_cast<int>(rotary_dim / 2), table_dtype);
 }
 
+size_t tfo_rope_axes_call_workspace_bytes(int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t head_dim,
+                                          int64_t rotary_dim, int interleaved, int dtype, int table_dtype,
+                                          const tfo_axes* axes) {
+  // (addresses that only have to be there: no head is read)
+  const void* any = axes;
+  void* out = const_cast<tfo_axes*>(axes);
+  const int64_t strides[3] = {};
+  HeadArgs a{};
+  bool empty = false;
+  const std::string fn = "tfo_rope_axes_call_workspace_bytes";
+  if (axes == nullptr ||
+      set_heads(&a, fn, any, strides, any, strides, any, any, rotary_dim, 1, any, TFO_POS_I64, 0, 0, out, out, batch, seq,
+                q_heads, k_heads, head_dim, rotary_dim, interleaved, dtype, table_dtype, &empty) != TFO_OK ||
+      empty || check_axes(fn, *axes, rotary_dim / 2, TFO_POS_I64, a.t.axis_bits) != TFO_OK || !axes_may_join(a))
+    return 0;
+  return axes_workspace_bytes(batch * seq, static_cast<int>(rotary_dim / 2), table_dtype);
+}
+
 int tfo_rope_tables_axes(const void* positions, int pos_dtype, int64_t n, const double* turns, int64_t half,
                          double gain, void* cos, void* sin, int out_dtype, const tfo_axes* axes, void* stream) {
   const char* fn = axes != nullptr ? "tfo_rope_tables_axes" : "tfo_rope_tables";

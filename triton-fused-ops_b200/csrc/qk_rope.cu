@@ -13,14 +13,16 @@ bool rows_aligned(const void* x, const HeadArgs& a, int heads, int64_t sb, int64
 }
 }  // namespace
 
+bool head_vectors_fit(const HeadArgs& a, int e) {
+  if (a.batch * a.seq * (a.q.heads + a.k.heads) >= (1ll << 31) - (1 << 20)) return false;  // units are counted in 32 bits
+  return a.head_dim % e == 0 && a.head_dim / e <= 64 && (a.pairs ? a.rotary_dim : a.rotary_dim / 2) % e == 0;
+}
+
 int head_vector_elems(const HeadArgs& a, bool backward) {
   const int esz = a.dtype == F32 ? 4 : 2;
-  const int64_t tokens = a.batch * a.seq;
-  if (tokens * (a.q.heads + a.k.heads) >= (1ll << 31) - (1 << 20)) return 0;  // units are counted in 32 bits
   for (int bytes = 16; bytes >= 8; bytes /= 2) {
     const int e = bytes / esz;
-    if (a.head_dim % e != 0 || a.head_dim / e > 64) continue;
-    if (a.pairs ? a.rotary_dim % e != 0 : (a.rotary_dim / 2) % e != 0) continue;
+    if (!head_vectors_fit(a, e)) continue;
     const int tsz = a.t.dtype == F32 ? 4 : 2;
     const int tb = std::min(16, (a.pairs ? e / 2 : e) * tsz);
     if (!aligned(a.t.cos, tb) || !aligned(a.t.sin, tb) || (a.t.rows > 1 && a.t.row_stride * tsz % tb != 0)) continue;

@@ -49,6 +49,11 @@ bool mixed(const HeadArgs& a, int elems) {
   return false;
 }
 
+// With vectors of `elems` elements: whether joining the rows is the faster way.
+bool joins(const HeadArgs& a, int elems) {
+  return a.batch * a.seq <= INT32_MAX /* tokens are 32-bit numbers there */ && head_streams(a, elems) && mixed(a, elems);
+}
+
 template <typename T>
 cudaError_t join(const HeadArgs& a, void* cos, void* sin, cudaStream_t st) {
   const int pairs = a.rotary_dim / 2;
@@ -60,10 +65,16 @@ cudaError_t join(const HeadArgs& a, void* cos, void* sin, cudaStream_t st) {
 }
 }  // namespace
 
+bool axes_may_join(const HeadArgs& a) {
+  const int esz = a.dtype == F32 ? 4 : 2;
+  for (const int elems : {16 / esz, 8 / esz})
+    if (head_vectors_fit(a, elems) && joins(a, elems)) return true;
+  return false;
+}
+
 cudaError_t join_axes(HeadArgs* a, bool backward, cudaStream_t st) {
   const int elems = head_vector_elems(*a, backward);
-  if (a->t.joined == nullptr || elems == 0 || !head_streams(*a, elems) || !mixed(*a, elems)) return cudaSuccess;
-  if (a->batch * a->seq > INT32_MAX) return cudaSuccess;  // tokens are 32-bit numbers there
+  if (a->t.joined == nullptr || elems == 0 || !joins(*a, elems)) return cudaSuccess;
   const int pairs = a->rotary_dim / 2;
   void* cos = a->t.joined;
   void* sin = static_cast<char*>(cos) + axes_workspace_bytes(a->batch * a->seq, pairs, a->t.dtype) / 2;

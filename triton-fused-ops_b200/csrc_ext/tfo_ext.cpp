@@ -248,19 +248,13 @@ struct HeadsCall {  // the C ABI's shared arguments
   int64_t pos_sb = 0, pos_ss = 0, batch, seq, q_heads, k_heads, dim, rot;
   tfo_axes axes_of{};
   at::Tensor joined;  // scratch of the axes
-  HeadsCall(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos, const at::Tensor& pos, const at::Tensor& axes)
+  HeadsCall(const at::Tensor& q, const at::Tensor& k, const at::Tensor& cos, const at::Tensor& pos, bool interleaved,
+            const at::Tensor& axes)
       : positions(&pos) {
     if (pos.defined()) {
       pos_dtype = pos_code(pos.scalar_type());
       pos_sb = q.dim() == 4 ? pos.stride(-2) : 0;
       pos_ss = pos.stride(-1);
-    }
-    if (axes.defined()) {
-      joined = scratch(tfo_rope_axes_workspace_bytes(q.numel() / (q.size(-1) * q.size(-2)), cos.size(1),
-                                                     dtype_code(cos.scalar_type())),
-                       q.device());
-      axes_of = {axis_count(axes), pos.stride(0), axes.data_ptr<uint8_t>(), joined.data_ptr(),
-                 static_cast<size_t>(joined.numel())};
     }
     batch = q.dim() == 4 ? q.size(0) : 1;
     seq = q.size(-3);
@@ -268,6 +262,16 @@ struct HeadsCall {  // the C ABI's shared arguments
     k_heads = k.defined() ? k.size(-2) : 0;
     dim = q.size(-1);
     rot = cos.size(1);
+    if (axes.defined()) {
+      axes_of = {axis_count(axes), pos.stride(0), axes.data_ptr<uint8_t>(), nullptr, 0};
+      joined = scratch(tfo_rope_axes_call_workspace_bytes(batch, seq, q_heads, k_heads, dim, rot, interleaved,
+                                                          dtype_code(q.scalar_type()), dtype_code(cos.scalar_type()), &axes_of),
+                       q.device());
+      if (joined.defined()) {
+        axes_of.workspace = joined.data_ptr();
+        axes_of.workspace_bytes = static_cast<size_t>(joined.numel());
+      }
+    }
   }
   const void* pos_ptr() const { return positions->defined() ? positions->data_ptr() : nullptr; }
   const tfo_axes* axes() const { return axes_of.axis_of_pair != nullptr ? &axes_of : nullptr; }
@@ -287,7 +291,7 @@ std::array<at::Tensor, 2> rope_call(const at::Tensor& q, const at::Tensor& k, co
                                     const at::Tensor& sin, const at::Tensor& positions, bool interleaved, bool inverse,
                                     const at::Tensor& axes) {
   const c10::cuda::CUDAGuard guard(q.device());
-  const HeadsCall h(q, k, cos, positions, axes);
+  const HeadsCall h(q, k, cos, positions, interleaved, axes);
   std::array<at::Tensor, 2> out{empty_heads(q), empty_heads(k)};
   const Strides3 qs = strides_of(q), ks = k.defined() ? strides_of(k) : Strides3{};
   check(tfo_rope_axes(q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(), cos.data_ptr(), sin.data_ptr(), cos.stride(0),
@@ -304,7 +308,7 @@ std::array<at::Tensor, 2> qk_norm_call(const at::Tensor& q, const at::Tensor& k,
                                        const at::Tensor& positions, double eps, bool interleaved,
                                        const at::Tensor& axes) {
   const c10::cuda::CUDAGuard guard(q.device());
-  const HeadsCall h(q, k, cos, positions, axes);
+  const HeadsCall h(q, k, cos, positions, interleaved, axes);
   std::array<at::Tensor, 2> out{empty_heads(q), empty_heads(k)};
   const Strides3 qs = strides_of(q), ks = k.defined() ? strides_of(k) : Strides3{};
   check(tfo_qk_norm_rope_axes(q.data_ptr(), qs.data(), ptr_or_null(k), ks.data(), ptr_or_null(qw), ptr_or_null(kw),
@@ -406,7 +410,7 @@ struct QKNormRopeNode : public torch::autograd::Function<QKNormRopeNode> {
     const at::Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3], &cos = saved[4], &sin = saved[5];
     const c10::cuda::CUDAGuard guard(q.device());
     const auto st = at::cuda::getCurrentCUDAStream(q.device().index()).stream();
-    const HeadsCall h(q, k, cos, saved[6], saved_axes(ctx));
+    const HeadsCall h(q, k, cos, saved[6], ctx->saved_data["interleaved"].toBool(), saved_axes(ctx));
     const at::Tensor gq = dense_heads(grads[0]), gk = k.defined() ? dense_heads(grads[1]) : at::Tensor();
     const at::Tensor dq = empty_heads(q), dk = empty_heads(k);
     at::Tensor dqw, dkw, ws;

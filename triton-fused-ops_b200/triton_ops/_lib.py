@@ -160,6 +160,7 @@ _SIGNATURES = {
          _c_vp],
     ),
     "tfo_rope_axes_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_int]),
+    "tfo_rope_axes_call_workspace_bytes": (_c_size, [*_HEADS_SIZES, _c_int, _c_int, _c_axes]),
     "tfo_lora_workspace_bytes": (_c_size, [_c_i64, _c_i64]),
     "tfo_lora": (
         _c_int,

@@ -49,7 +49,7 @@ def _weight_code(w: Optional[torch.Tensor], name: str) -> int:
 def _forward(q, k, qw, kw, cos, sin, positions, eps, interleaved, pair_axes=None):
     q_out, k_out = _empty_like_heads(q), _empty_like_heads(k)
     with _lib.on_device(q):
-        axes, axes_ws = _heads_axes(pair_axes, positions, cos)
+        axes, axes_ws = _heads_axes(pair_axes, positions, q, k, cos, interleaved)
         _lib.call("tfo_qk_norm_rope_axes", q.data_ptr(), _strides(q), _lib.ptr(k), _strides(k), _lib.ptr(qw), _lib.ptr(kw),
                   *_table_args(cos, sin, positions, q), q_out.data_ptr(), _lib.ptr(k_out),
                   *_size_args(q, k, cos, interleaved), float(eps), _lib.dtype_code(q.dtype, "q"),
@@ -98,7 +98,7 @@ def _backward(ctx, gq, gk):
     dkw = torch.empty_like(kw) if kw is not None and ctx.needs_input_grad[3] else None
     with _lib.on_device(q):
         ws = None
-        axes, axes_ws = _heads_axes(ctx.pair_axes, positions, cos)
+        axes, axes_ws = _heads_axes(ctx.pair_axes, positions, q, k, cos, ctx.interleaved)
         if dqw is not None or dkw is not None:
             ws = _lib.scratch(_lib.load().tfo_qk_norm_rope_backward_workspace_bytes(q.shape[-1]), q.device)
         _lib.call("tfo_qk_norm_rope_backward_axes", gq.data_ptr(), _strides(gq), _lib.ptr(gk), _strides(gk), q.data_ptr(),

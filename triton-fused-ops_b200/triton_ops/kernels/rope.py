@@ -293,12 +293,13 @@ def _axes_arg(pair_axes: Optional[torch.Tensor], pos_stride: int, ws: Optional[t
                                   0 if ws is None else ws.numel()))
 
 
-def _heads_axes(pair_axes, positions, cos):
+def _heads_axes(pair_axes, positions, q, k, cos, interleaved):
     """(the C ABI's axes, their scratch, to be kept until the call is made)."""
     if pair_axes is None:
         return None, None
-    ws = _lib.scratch(_lib.load().tfo_rope_axes_workspace_bytes(positions[0].numel(), cos.shape[1], _lib.dtype_code(cos.dtype)),
-                      cos.device)
+    size = _lib.load().tfo_rope_axes_call_workspace_bytes(*_size_args(q, k, cos, interleaved), _lib.dtype_code(q.dtype, "q"),
+                                                          _lib.dtype_code(cos.dtype, "cos"), _axes_arg(pair_axes, 0))
+    ws = _lib.scratch(size, cos.device)
     return _axes_arg(pair_axes, positions.stride(0), ws), ws
 
 
@@ -324,7 +325,7 @@ def _rotate(q, k, cos, sin, positions, interleaved, inverse, pair_axes=None):
     """Launches tfo_rope on checked arguments."""
     q_out, k_out = _empty_like_heads(q), _empty_like_heads(k)
     with _lib.on_device(q):
-        axes, ws = _heads_axes(pair_axes, positions, cos)
+        axes, ws = _heads_axes(pair_axes, positions, q, k, cos, interleaved)
         _lib.call("tfo_rope_axes", q.data_ptr(), _strides(q), _lib.ptr(k), _strides(k), *_table_args(cos, sin, positions, q),
                   q_out.data_ptr(), _lib.ptr(k_out), *_size_args(q, k, cos, interleaved), int(inverse),
                   _lib.dtype_code(q.dtype, "q"), _lib.dtype_code(cos.dtype, "cos"), axes, _lib.stream_of(q))
