@@ -135,7 +135,6 @@ class RoPEAxes(_Axes):
 
 
 @lru_cache(maxsize=64)
-@lru_cache(maxsize=64)
 def _pair_axes(axes: RoPEAxes) -> torch.Tensor:
     """The axis of each pair in host memory, as the library reads it (made once for an order of axes, not changed)."""
     return torch.tensor(axes.axis_of_pairs(), dtype=torch.uint8, device="cpu")
