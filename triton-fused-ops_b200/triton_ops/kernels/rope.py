@@ -148,7 +148,7 @@ def _check_axes(axes: RoPEAxes, rotary_dim: int) -> None:
                                  tensor_name="cos")
 
 
-@lru_cache(maxsize=64)
+@lru_cache(maxsize=64, typed=True)  # a tuple equals the named one that was checked
 def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[RoPEScaling] = None,
                      axes: Optional[RoPEAxes] = None) -> Tuple[tuple, float]:
     """(angle per position of each pair, factor on cos and sin), in double precision on the host."""
@@ -192,7 +192,7 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[R
     return tuple(freq), gain
 
 
-@lru_cache(maxsize=64)
+@lru_cache(maxsize=64, typed=True)  # a tuple equals the named one that was checked
 def _turns(rotary_dim: int, base: float, scaling: Optional[RoPEScaling], axes: Optional[RoPEAxes] = None):
     """The frequencies as host arrays of turns per position (what the kernel takes; torch's default device may be another
     one), and the gain."""
