@@ -22,8 +22,8 @@
 //
 // Floor: HBM (x, residual, dy and dh read, dx and dresidual written).
 // Measured, of the copy rate, with the second kernel (4 us): bf16 32768 x 4096 266
-// us (92 %), 8192 x 4096 82 (75 %: the start with its parameters, the end with its
-// sums), 8192 x 8192 149 (82 %), fp32 4096 x 4096 69 (88 %), with dropout 8192 x
+// us (92 %), 8192 x 4096 83 (74 %: the start with its parameters, the end with its
+// sums), 8192 x 8192 150 (82 %), fp32 4096 x 4096 69 (88 %), with dropout 8192 x
 // 4096 bf16 103 (60 %).
 #include "residual.cuh"
 
@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(kRowThreads, 1)
 }
 
 // Rows of any width: a CTA for each, which reads it again for the results (from L1 and L2); a CTA's items' sums are
-// added up in the partial rows themselves, each column by one thread.
+// added up in the partial rows themselves, each column by one thread. Slow: it waits for its loads of one column and for the
+// partial rows (4096 x 12288 bf16 2237 us, 4 % of the copy rate; 4096 x 5329 fp32 692 us, 12 %).
 template <typename TX, typename TR>
 __global__ void __launch_bounds__(kRowThreads)
     residual_norm_backward_any_kernel(const __grid_constant__ ResidualArgs a, const __grid_constant__ BackwardPlan plan) {
